@@ -36,11 +36,16 @@ _load_ops()
 from .attention import (  # noqa: E402
     apply_rotary_pos_emb,
     dvattn_fused,
+    dvattn_kv_select,
+    dvattn_paged_key_mass,
     dvattn_paged_kv_append,
+    dvattn_paged_kv_compact,
     dvattn_paged_sdpa,
     dvattn_rope,
     dvattn_sdpa,
     dvattn_sdpa_pt,
+    dvattn_tree_metadata,
+    dvattn_tree_paged_sdpa,
     dvattn_varlen_paged_sdpa,
     dvattn_varlen_rope,
     dvattn_view_metadata,
@@ -51,11 +56,16 @@ from .attention import (  # noqa: E402
 __all__ = [
     "apply_rotary_pos_emb",
     "dvattn_fused",
+    "dvattn_kv_select",
+    "dvattn_paged_key_mass",
     "dvattn_paged_kv_append",
+    "dvattn_paged_kv_compact",
     "dvattn_paged_sdpa",
     "dvattn_rope",
     "dvattn_sdpa",
     "dvattn_sdpa_pt",
+    "dvattn_tree_metadata",
+    "dvattn_tree_paged_sdpa",
     "dvattn_varlen_paged_sdpa",
     "dvattn_varlen_rope",
     "dvattn_view_metadata",

@@ -152,6 +152,114 @@ def dvattn_view_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, nu
     return loc, cos, sin
 
 
+def dvattn_tree_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, parents: torch.Tensor,
+                         inv_freq: torch.Tensor, attention_scaling: float = 1.0,
+                         round_to: Optional[torch.dtype] = None):
+    """Metadata of a step in which every sequence drafts a tree of up to S tokens:
+    ``dvattn_view_metadata`` with positions that follow the nodes' depths.
+
+    parents ``[W,S]`` int32: -1 for a child of the committed tokens, the index of
+    an earlier node (``0 .. s-1``), or anything else (-2, say) for an absent node:
+    the padding of a smaller tree; nodes below an absent one are absent too.  The
+    drafted rows are the last S of each sequence's own view (the last of its
+    ``order [W,F]``): fragment_lengths ``[F]`` count them.  Returns
+
+    * ``locations [F,W,S]``: the committed keys of each view, -1 for absent nodes;
+    * ``cosines``, ``sines`` ``[F,W,S,R]`` at the position (committed tokens from the
+      view to the end of the sequence's order) + (the node's depth);
+    * ``tree_views [W]``, ``tree_rows [W]``: each sequence's own view, and the row of
+      its page stream that holds node 0 (node s is appended at ``tree_rows + s``).
+
+    The last four and the first are ``dvattn_tree_paged_sdpa``'s arguments.  Another
+    sequence's drafted nodes are neither seen nor counted.  S and F are at most 4096.
+    """
+    F = fragment_lengths.numel()
+    W, S = parents.shape
+    R = 2 * inv_freq.numel()
+    dev = fragment_lengths.device
+    loc = torch.empty((F, W, S), dtype=torch.int32, device=dev)
+    cos = torch.empty((F, W, S, R), dtype=torch.float32, device=dev)
+    sin = torch.empty_like(cos)
+    views = torch.empty((W,), dtype=torch.int32, device=dev)
+    rows = torch.empty_like(views)
+    torch.ops.libdvatt.dvattn_tree_metadata(loc, cos, sin, views, rows, fragment_lengths, order, parents, inv_freq,
+                                            float(attention_scaling), round_to)
+    return loc, cos, sin, views, rows
+
+
+def dvattn_tree_paged_sdpa(queries: torch.Tensor, locations: torch.Tensor, cosines: torch.Tensor,
+                           sines: torch.Tensor, fragment_lengths: torch.Tensor, k_cache: torch.Tensor,
+                           v_cache: torch.Tensor, block_tables: torch.Tensor, parents: torch.Tensor,
+                           tree_views: torch.Tensor, tree_rows: torch.Tensor, scale: float,
+                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dvattn_paged_sdpa`` for the nodes of drafted token trees.  Node s of sequence
+    w (queries ``[W,Hq,S,E]``) sees the keys its ``locations`` allow and, in view
+    ``tree_views[w]``, the rows ``tree_rows[w] + j`` of the page stream for j = s and
+    its ancestors by ``parents [W,S]`` (see ``dvattn_tree_metadata``).  Absent nodes
+    give zeros.  Out ``[W,Hq,S,Ev]``."""
+    if out is None:
+        out = torch.empty(tuple(queries.shape[:3]) + (v_cache.size(-1),), dtype=queries.dtype,
+                          device=queries.device)
+    torch.ops.libdvatt.dvattn_tree_paged_sdpa(out, scale, locations, queries, cosines, sines, fragment_lengths,
+                                              k_cache, v_cache, block_tables, parents, tree_views, tree_rows)
+    return out
+
+
+def dvattn_paged_key_mass(mass: Optional[torch.Tensor], queries: torch.Tensor, locations: torch.Tensor,
+                          cosines: torch.Tensor, sines: torch.Tensor, fragment_lengths: torch.Tensor,
+                          k_cache: torch.Tensor, block_tables: torch.Tensor, scale: float, decay: float = 1.0,
+                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention weight that every cached key receives: ``out = decay * mass +`` the
+    softmax weights of ``dvattn_paged_sdpa`` on the same arguments, summed over the
+    tokens and the 16 query heads of each KV head.
+
+    mass ``[W,Hkv,capacity]`` float32, by row of each sequence's page stream (views
+    one after the other); ``out`` defaults to ``mass`` itself (accumulation in place).
+    With ``decay=0`` mass is not read and may be None if ``out`` is given.  Rows at or
+    past the capacity take part in the softmax and are not stored."""
+    if out is None:
+        out = mass
+    if out is None:
+        raise ValueError("dvattn_paged_key_mass: mass or out must be given")
+    torch.ops.libdvatt.dvattn_paged_key_mass(out, mass, float(decay), scale, locations, queries, cosines, sines,
+                                             fragment_lengths, k_cache, block_tables)
+    return out
+
+
+def dvattn_kv_select(mass: torch.Tensor, first_rows: torch.Tensor, lengths: torch.Tensor, budget: int,
+                     keep_first: int = 0, keep_last: int = 0, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The rows of a cache worth keeping, ``[W,Hkv,budget]`` int32, ascending and
+    relative to ``first_rows [W]``: of the ``lengths[w]`` rows from there on all if
+    they fit the budget (then -1), else the first ``keep_first``, the last
+    ``keep_last`` and the heaviest others by ``mass [W,Hkv,capacity]`` (ties to the
+    lowest row, NaN lightest).  ``dvattn_paged_kv_compact`` moves them together."""
+    if rows is None:
+        rows = torch.empty(tuple(mass.shape[:2]) + (budget,), dtype=torch.int32, device=mass.device)
+    elif rows.size(-1) != budget:
+        raise ValueError(f"dvattn_kv_select: rows hold {rows.size(-1)} entries, budget {budget}")
+    torch.ops.libdvatt.dvattn_kv_select(rows, mass, first_rows, lengths, keep_first, keep_last)
+    return rows
+
+
+def dvattn_paged_kv_compact(rows: torch.Tensor, first_rows: torch.Tensor, k_cache: torch.Tensor,
+                            v_cache: torch.Tensor, block_tables: torch.Tensor, mass: Optional[torch.Tensor] = None,
+                            lengths: Optional[torch.Tensor] = None):
+    """Move kept rows of a paged cache together, in place: row ``first_rows[w] + i``
+    takes the keys and values of row ``first_rows[w] + rows[w,h,i]`` wherever
+    ``rows[w,h,i] >= i`` (and ``< lengths[w]`` if given); other rows stay.
+
+    rows ``[W,Hkv,N]`` int32 (``dvattn_kv_select``), or ``[W,1,N]`` for all KV heads
+    alike: the accepted path of a drafted tree, with ``first_rows = tree_rows``.
+    ``mass [W,Hkv,capacity]`` moves along (needs lengths); entries of the range's
+    rows that nothing moves into become 0.  The caches may be strided views as in
+    ``dvattn_paged_kv_append``.  The moved rows' pages must not be named twice in
+    ``block_tables``: pages that sequences or segments share lie before first_rows.
+    Positions of the kept keys do not change (their rotation stays valid); the
+    caller's locations and lengths count rows from here on."""
+    torch.ops.libdvatt.dvattn_paged_kv_compact(k_cache, v_cache, block_tables, rows, first_rows, lengths, mass)
+    return k_cache, v_cache
+
+
 def dvattn_sdpa_pt(queries: torch.Tensor, locations: torch.Tensor, keys: list, values: list,
                    scale: float, return_intermediate_results: bool = False):
     """Pure-PyTorch attention over already-rotated queries and contiguous views,
@@ -222,5 +330,6 @@ def apply_rotary_pos_emb(x, cos, sin, unsqueeze_dim=1):
 __all__ = [
     "dvattn_fused", "dvattn_sdpa", "dvattn_rope", "dvattn_varlen_rope", "dvattn_paged_sdpa",
     "dvattn_varlen_paged_sdpa", "dvattn_sdpa_pt", "rotate_half", "apply_rotary_pos_emb",
-    "dvattn_paged_kv_append", "merge_caches_paged", "dvattn_view_metadata",
+    "dvattn_paged_kv_append", "merge_caches_paged", "dvattn_view_metadata", "dvattn_tree_metadata",
+    "dvattn_tree_paged_sdpa", "dvattn_paged_key_mass", "dvattn_kv_select", "dvattn_paged_kv_compact",
 ]

@@ -29,6 +29,9 @@ EXPORTED = [
     "dvattn_sdpa_workspace_size", "dvattn_sdpa", "dvattn_fused",
     "dvattn_rope", "dvattn_varlen_rope",
     "dvattn_paged_kv_append", "dvattn_view_metadata",
+    "dvattn_tree_metadata", "dvattn_tree_paged_sdpa_workspace_size", "dvattn_tree_paged_sdpa",
+    "dvattn_paged_key_mass_workspace_size", "dvattn_paged_key_mass", "dvattn_kv_select",
+    "dvattn_paged_kv_compact",
 ]
 
 
@@ -57,6 +60,7 @@ _VP = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_LL = ctypes.c_longlong
 _SP = ctypes.POINTER(Shape)
 
 _lib = None
@@ -73,7 +77,8 @@ def lib() -> ctypes.CDLL:
         L.dvattn_abi_version.restype = _I
         L.dvattn_abi_version.argtypes = []
         for n in ("dvattn_paged_sdpa_workspace_size", "dvattn_varlen_paged_sdpa_workspace_size",
-                  "dvattn_sdpa_workspace_size"):
+                  "dvattn_sdpa_workspace_size", "dvattn_tree_paged_sdpa_workspace_size",
+                  "dvattn_paged_key_mass_workspace_size"):
             getattr(L, n).restype = _SZ
             getattr(L, n).argtypes = [_I, _SP, _I]
         L.dvattn_paged_sdpa.restype = _I
@@ -97,6 +102,17 @@ def lib() -> ctypes.CDLL:
                                              ctypes.POINTER(KvLayout), _VP]
         L.dvattn_view_metadata.restype = _I
         L.dvattn_view_metadata.argtypes = [_VP, _VP, _VP, _VP, _VP, _VP, _F, _I, _I, _I, _I, _I, _VP]
+        L.dvattn_tree_metadata.restype = _I
+        L.dvattn_tree_metadata.argtypes = [_VP] * 9 + [_F, _I, _I, _I, _I, _I, _VP]
+        L.dvattn_tree_paged_sdpa.restype = _I
+        L.dvattn_tree_paged_sdpa.argtypes = [_I, _VP, _F] + [_VP] * 11 + [_SP, _VP, _SZ, _VP]
+        L.dvattn_paged_key_mass.restype = _I
+        L.dvattn_paged_key_mass.argtypes = [_I, _VP, _VP, _F, _LL, _F] + [_VP] * 7 + [_SP, _VP, _SZ, _VP]
+        L.dvattn_kv_select.restype = _I
+        L.dvattn_kv_select.argtypes = [_VP, _VP, _VP, _VP, _LL, _I, _I, _I, _I, _I, _VP]
+        L.dvattn_paged_kv_compact.restype = _I
+        L.dvattn_paged_kv_compact.argtypes = [_I, _VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _LL, _SP,
+                                              ctypes.POINTER(KvLayout), _VP]
         L.dvattn_set_option.restype = _I
         L.dvattn_set_option.argtypes = [ctypes.c_char_p, _I]
         L.dvattn_get_option.restype = _I
@@ -283,3 +299,64 @@ def view_metadata(locations, cosines, sines, fragment_lengths, order, inv_freq, 
                                       _ptr(order), _ptr(inv_freq), attention_scaling, rd, F, W, S,
                                       cosines.shape[3], _stream(locations)))
     return locations, cosines, sines
+
+
+def tree_metadata(locations, cosines, sines, tree_views, tree_rows, fragment_lengths, order, parents, inv_freq,
+                  attention_scaling=1.0, round_to=None):
+    """dvattn_tree_metadata: locations [F,W,S] i32, cos/sin [F,W,S,R] f32, tree_views/tree_rows [W] i32."""
+    F, W, S = locations.shape
+    rd = -1 if round_to in (None, torch.float32) else dtype_code(round_to)
+    _check(lib().dvattn_tree_metadata(_ptr(locations), _ptr(cosines), _ptr(sines), _ptr(tree_views), _ptr(tree_rows),
+                                      _ptr(fragment_lengths), _ptr(order), _ptr(parents), _ptr(inv_freq),
+                                      attention_scaling, rd, F, W, S, cosines.shape[3], _stream(locations)))
+    return locations, cosines, sines, tree_views, tree_rows
+
+
+def tree_paged_sdpa(out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, block_tables,
+                    parents, tree_views, tree_rows, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    L = lib()
+    s = paged_shape(queries, locations, cosines, k_cache, v_cache, block_tables)
+    dt = dtype_code(out.dtype)
+    need = L.dvattn_tree_paged_sdpa_workspace_size(dt, ctypes.byref(s), out.device.index or 0)
+    ws = workspace if workspace is not None and workspace.numel() >= need else _workspace(need, out)
+    _check(L.dvattn_tree_paged_sdpa(dt, _ptr(out), scale, _ptr(locations), _ptr(queries), _ptr(cosines), _ptr(sines),
+                                    _ptr(fragment_lengths), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
+                                    _ptr(parents), _ptr(tree_views), _ptr(tree_rows), ctypes.byref(s), _ptr(ws),
+                                    ws.numel(), _stream(out)))
+    return out
+
+
+def paged_key_mass(out, mass, decay, scale, locations, queries, cosines, sines, fragment_lengths, k_cache,
+                   block_tables, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    L = lib()
+    s = paged_shape(queries, locations, cosines, k_cache, k_cache, block_tables)
+    dt = dtype_code(queries.dtype)
+    need = L.dvattn_paged_key_mass_workspace_size(dt, ctypes.byref(s), out.device.index or 0)
+    ws = workspace if workspace is not None and workspace.numel() >= need else _workspace(need, out)
+    _check(L.dvattn_paged_key_mass(dt, _ptr(out), _ptr(mass), decay, out.shape[2], scale, _ptr(locations),
+                                   _ptr(queries), _ptr(cosines), _ptr(sines), _ptr(fragment_lengths), _ptr(k_cache),
+                                   _ptr(block_tables), ctypes.byref(s), _ptr(ws), ws.numel(), _stream(out)))
+    return out
+
+
+def kv_select(rows, mass, first_rows, lengths, keep_first=0, keep_last=0):
+    W, Hkv, capacity = mass.shape
+    _check(lib().dvattn_kv_select(_ptr(rows), _ptr(mass), _ptr(first_rows), _ptr(lengths), capacity, W, Hkv,
+                                  rows.shape[2], keep_first, keep_last, _stream(rows)))
+    return rows
+
+
+def kv_compact(k_cache, v_cache, block_tables, rows, first_rows, lengths=None, mass=None):
+    """dvattn_paged_kv_compact: caches [P,bs,Hkv,E] (strided views allowed), rows [W,Hkv|1,N]."""
+    P, bs, Hkv, E = k_cache.shape
+    s = Shape(F=0, W=rows.shape[0], Hq=0, Hkv=Hkv, E=E, Ev=v_cache.shape[3], S=0, block_size=bs,
+              max_blocks_per_seq=block_tables.shape[1], total_q_tokens=0, num_blocks=P, rotary_dim=0)
+    lay = KvLayout()
+    for i in range(3):
+        lay.k_cache_strides[i] = k_cache.stride(i)
+        lay.v_cache_strides[i] = v_cache.stride(i)
+    _check(lib().dvattn_paged_kv_compact(dtype_code(k_cache.dtype), _ptr(k_cache), _ptr(v_cache), _ptr(block_tables),
+                                         _ptr(rows), rows.shape[1], rows.shape[2], _ptr(first_rows), _ptr(lengths),
+                                         _ptr(mass), 0 if mass is None else mass.shape[2], ctypes.byref(s),
+                                         ctypes.byref(lay), _stream(k_cache)))
+    return k_cache, v_cache

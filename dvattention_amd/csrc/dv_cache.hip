@@ -9,7 +9,9 @@
 //    cos/sin on the device (attention.py:158-186: suffix sums of the segment
 //    lengths in each sequence's segment order, then the model's rotary
 //    embedding at those positions).
-// Both are elementwise and HBM- or launch-bound; one thread per 16-byte run.
+//  * dv_tree_meta -- the same for a step that drafts a token tree per sequence:
+//    positions follow a node's depth, and the drafted rows' places.
+// All are elementwise and HBM- or launch-bound; one thread per 16-byte run.
 #include "dv_common.h"
 #include "dv_device.h"
 
@@ -253,6 +255,138 @@ hipError_t launch_view_meta(const MetaParams& p, hipStream_t stream) {
     if (n == 0) return hipSuccess;
     const long long blocks = (n + 255) / 256;
     hipLaunchKernelGGL(dv_view_meta, dim3((unsigned)blocks), dim3(256), 0, stream, p, n, rh);
+    return hipGetLastError();
+}
+
+// A step that drafts a tree of S nodes per sequence.  With c(g) the committed tokens
+// of view g -- fl[g] less the S drafted rows where g is some sequence's own (last)
+// view -- and d(s) the depth of node s (0: child of the committed tokens),
+//   position[f, w, s] = sum of c over w's segments from f's place in its order to the
+//                       last one, plus d(s),
+//   location[f, w, s] = c(f) - 1 (the drafted rows are seen through the tree alone),
+//   cos / sin         = cos / sin(fp32(position) * inv_freq[i]) * scaling, as dv_view_meta.
+// An absent node (parent neither -1 nor an earlier node, or below such a node) and a
+// view missing from the order get location -1 and the identity rotation.
+//
+// Bound by its writes (F W S (4 + 8 R) bytes) and, for small calls, by the launch.
+// Block (f, w, tile of kTreeTile nodes): which views are drafted, the order's sum and
+// the nodes' depths cost one round of loads each for the whole block and are shared
+// in LDS; then thread = RUN rotary pairs of a node, 16-byte stores.
+constexpr int kTreeTile = 64;
+template <int RUN>
+__global__ __launch_bounds__(256) void dv_tree_meta(const TreeMetaParams tp, int tiles) {
+    const MetaParams& p = tp.m;
+    extern __shared__ int s_meta[];
+    int* s_drafted = s_meta;               // [F]: view is some sequence's own
+    int* s_par = s_drafted + p.F;          // [S]
+    int* s_depth = s_par + p.S;            // [kTreeTile]
+    __shared__ int s_place;
+    __shared__ long long s_sum;
+    const int tid = threadIdx.x;
+    const int tile = blockIdx.x % tiles;
+    const int fw = blockIdx.x / tiles;
+    const int f = fw / p.W, w = fw - (fw / p.W) * p.W;
+    const int* ord = p.order + (long long)w * p.F;
+
+    for (int i = tid; i < p.F; i += 256) s_drafted[i] = 0;
+    for (int i = tid; i < p.S; i += 256) s_par[i] = tp.parents[(long long)w * p.S + i];
+    if (tid == 0) {
+        s_place = p.F;
+        s_sum = 0;
+    }
+    __syncthreads();
+    for (int v = tid; v < p.W; v += 256) {
+        const int g = p.order[(long long)v * p.F + p.F - 1];
+        if (g >= 0 && g < p.F) s_drafted[g] = 1;
+    }
+    // f's first place in the order (integers: the order of the updates does not matter)
+    for (int j = tid; j < p.F; j += 256)
+        if (ord[j] == f) atomicMin(&s_place, j);
+    __syncthreads();
+    auto committed = [&](int g) {
+        const long long c = (long long)p.fl[g] - (s_drafted[g] ? p.S : 0);
+        return c > 0 ? c : 0ll;
+    };
+    const int place = s_place;
+    long long mine = 0;
+    for (int j = tid; j < p.F; j += 256) {
+        const int g = ord[j];
+        if (j >= place && g >= 0 && g < p.F) mine += committed(g);
+    }
+    if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(&s_sum), (unsigned long long)mine);
+    const int s0 = tile * kTreeTile;
+    const int ns = p.S - s0 < kTreeTile ? p.S - s0 : kTreeTile;
+    if (tid < ns) {
+        // every step goes to an earlier node, so the walk ends
+        int j = s0 + tid, dep = 0;
+        for (;;) {
+            const int up = s_par[j];
+            if (up == -1) break;
+            if (up < -1 || up >= j) {
+                dep = -1;
+                break;
+            }
+            j = up;
+            ++dep;
+        }
+        s_depth[tid] = dep;
+    }
+    __syncthreads();
+    const bool found = place < p.F;
+    if (f == 0 && tile == 0 && tid == 0) {
+        // the drafted rows: w's own view, and the stream row of node 0
+        const int own = p.F > 0 ? ord[p.F - 1] : -1;
+        const bool ok = own >= 0 && own < p.F;
+        long long row = 0;
+        for (int g = 0; ok && g < own; ++g) row += p.fl[g];
+        tp.tree_views[w] = ok ? own : -1;
+        tp.tree_rows[w] = ok ? (int)(row + committed(own)) : 0;
+    }
+    const long long t0 = ((long long)f * p.W + w) * p.S + s0;
+    if (tid < ns) p.loc[t0 + tid] = found && s_depth[tid] >= 0 ? (int)committed(f) - 1 : -1;
+    const int rh = p.R >> 1;
+    const int runs = rh / RUN;
+    const long long base = s_sum;
+    for (int k = tid; k < ns * runs; k += 256) {
+        const int t = k / runs;
+        const int i = (k - t * runs) * RUN;
+        const int dep = s_depth[t];
+        float c[RUN], sn[RUN];
+#pragma unroll
+        for (int e = 0; e < RUN; ++e) {
+            c[e] = 1.0f;
+            sn[e] = 0.0f;
+            if (found && dep >= 0) {
+                const float ang = (float)(int)(base + dep) * p.inv_freq[i + e];
+                c[e] = cosf(ang) * p.scaling;
+                sn[e] = sinf(ang) * p.scaling;
+            }
+            if (p.round_dt == kBF16) {
+                c[e] = round_to<kBF16>(c[e]);
+                sn[e] = round_to<kBF16>(sn[e]);
+            } else if (p.round_dt == kF16) {
+                c[e] = round_to<kF16>(c[e]);
+                sn[e] = round_to<kF16>(sn[e]);
+            }
+        }
+        const long long o = (t0 + t) * p.R + i;
+        store_run<float, RUN>(p.cosv + o, c);
+        store_run<float, RUN>(p.cosv + o + rh, c);
+        store_run<float, RUN>(p.sinv + o, sn);
+        store_run<float, RUN>(p.sinv + o + rh, sn);
+    }
+}
+
+hipError_t launch_tree_meta(const TreeMetaParams& p, hipStream_t stream) {
+    const int tiles = (p.m.S + kTreeTile - 1) / kTreeTile;
+    const long long blocks = (long long)p.m.F * p.m.W * tiles;
+    if (blocks == 0) return hipSuccess;
+    if (blocks >= (1ll << 31)) return hipErrorInvalidValue;  // the C ABI rejects such calls first
+    const size_t lds = (size_t)(p.m.F + p.m.S + kTreeTile) * sizeof(int);
+    auto al = [](const void* ptr) { return ((uintptr_t)ptr & 15) == 0; };
+    const bool vec = (p.m.R / 2) % 4 == 0 && al(p.m.cosv) && al(p.m.sinv);
+    if (vec) hipLaunchKernelGGL(dv_tree_meta<4>, dim3((unsigned)blocks), dim3(256), lds, stream, p, tiles);
+    else hipLaunchKernelGGL(dv_tree_meta<1>, dim3((unsigned)blocks), dim3(256), lds, stream, p, tiles);
     return hipGetLastError();
 }
 

@@ -809,4 +809,285 @@ dvattn_status dvattn_view_metadata(int* locations, float* cosines, float* sines,
     return ok();
 }
 
+// ---------------------------------------------------------------------------
+dvattn_status dvattn_tree_metadata(int* locations, float* cosines, float* sines, int* tree_views, int* tree_rows,
+                                   const int* fragment_lengths, const int* order, const int* parents,
+                                   const float* inv_freq, float attention_scaling, int round_dtype, int F, int W,
+                                   int S, int rotary_dim, void* stream) {
+    if (F < 0 || W < 0 || S < 0) return fail(DVATTN_ERR_INVALID, "negative F/W/S");
+    if (rotary_dim < 0 || (rotary_dim & 1))
+        return fail(DVATTN_ERR_UNSUPPORTED, "rotary_dim must be even and >= 0 (got %d)", rotary_dim);
+    if (round_dtype != -1 && !valid_dtype(round_dtype))
+        return fail(DVATTN_ERR_UNSUPPORTED, "unsupported round_dtype code %d", round_dtype);
+    if (S > dv::kMaxTreeNodes || F > dv::kMaxTreeViews)
+        return fail(DVATTN_ERR_UNSUPPORTED, "at most %d drafted nodes and %d views (S=%d, F=%d)", dv::kMaxTreeNodes,
+                    dv::kMaxTreeViews, S, F);
+    if ((long long)F * W * S == 0) return ok();
+    if ((long long)F * W * S >= (1ll << 31))
+        return fail(DVATTN_ERR_UNSUPPORTED, "%lld (view, node) pairs in one call exceed 2^31", (long long)F * W * S);
+    if (!locations || !tree_views || !tree_rows || !fragment_lengths || !order || !parents ||
+        (rotary_dim > 0 && (!cosines || !sines || !inv_freq)))
+        return fail(DVATTN_ERR_INVALID, "null pointer");
+    const dvattn_status st = check_aligned({{locations, "locations", 4}, {cosines, "cosines", 4}, {sines, "sines", 4},
+                                            {tree_views, "tree_views", 4}, {tree_rows, "tree_rows", 4},
+                                            {fragment_lengths, "fragment_lengths", 4}, {order, "order", 4},
+                                            {parents, "parents", 4}, {inv_freq, "inv_freq", 4}});
+    if (st != DVATTN_OK) return st;
+    dv::TreeMetaParams p;
+    memset(&p, 0, sizeof(p));
+    p.m.loc = locations;
+    p.m.cosv = cosines;
+    p.m.sinv = sines;
+    p.m.fl = fragment_lengths;
+    p.m.order = order;
+    p.m.inv_freq = inv_freq;
+    p.m.scaling = attention_scaling;
+    p.m.round_dt = round_dtype == DVATTN_F32 ? -1 : round_dtype;
+    p.m.F = F;
+    p.m.W = W;
+    p.m.S = S;
+    p.m.R = rotary_dim;
+    p.parents = parents;
+    p.tree_views = tree_views;
+    p.tree_rows = tree_rows;
+    const hipError_t e = dv::launch_tree_meta(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "dvattn_tree_metadata launch");
+    return ok();
+}
+
+// ---------------------------------------------------------------------------
+size_t dvattn_tree_paged_sdpa_workspace_size(int dtype, const dvattn_shape* s, int device) {
+    if (!s || !valid_dtype(dtype)) return 0;
+    return dv::chunk_workspace_bytes(s->W, s->S, s->Hkv, current_device(device));
+}
+
+dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scale, const int* locations, const void* queries,
+                                     const float* cosines, const float* sines, const int* fragment_lengths,
+                                     const void* k_cache, const void* v_cache, const int* block_tables,
+                                     const int* parents, const int* tree_views, const int* tree_rows,
+                                     const dvattn_shape* s, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!s) return fail(DVATTN_ERR_INVALID, "shape is null");
+    if (!valid_dtype(dtype)) return fail(DVATTN_ERR_UNSUPPORTED, "unsupported dtype code %d", dtype);
+    if (s->F < 0 || s->W < 0 || s->S < 0) return fail(DVATTN_ERR_INVALID, "negative F/W/S");
+    if ((long long)s->W * s->S == 0 || s->Hkv == 0) return ok();
+    dvattn_status st;
+    if ((st = check_heads(s)) != DVATTN_OK) return st;
+    if ((st = check_rotary(s->rotary_dim, s->E)) != DVATTN_OK) return st;
+    if ((st = check_pages(s)) != DVATTN_OK) return st;
+    if (s->S > dv::kMaxTreeNodes)
+        return fail(DVATTN_ERR_UNSUPPORTED, "at most %d drafted nodes per sequence (S=%d)", dv::kMaxTreeNodes, s->S);
+    if (!out || !queries || !parents || !tree_views || !tree_rows)
+        return fail(DVATTN_ERR_INVALID, "null output, query, parents, tree_views or tree_rows pointer");
+    if (s->F > 0 && (!locations || !fragment_lengths || ((!cosines || !sines) && s->rotary_dim > 0)))
+        return fail(DVATTN_ERR_INVALID, "null locations / fragment_lengths / cos / sin pointer");
+    if (s->num_blocks > 0 && (!k_cache || !v_cache)) return fail(DVATTN_ERR_INVALID, "null k/v cache pointer");
+    if (s->max_blocks_per_seq > 0 && !block_tables) return fail(DVATTN_ERR_INVALID, "null block_tables pointer");
+    if ((st = check_aligned({{out, "out", 16}, {queries, "queries", 16}, {k_cache, "k_cache", 16},
+                             {v_cache, "v_cache", 16}, {workspace, "workspace", 16}, {locations, "locations", 4},
+                             {fragment_lengths, "fragment_lengths", 4}, {cosines, "cosines", 4},
+                             {sines, "sines", 4}, {block_tables, "block_tables", 4}, {parents, "parents", 4},
+                             {tree_views, "tree_views", 4}, {tree_rows, "tree_rows", 4}})) != DVATTN_OK)
+        return st;
+    const size_t need = dvattn_tree_paged_sdpa_workspace_size(dtype, s, -1);
+    if (workspace_bytes < need || (need && !workspace))
+        return fail(DVATTN_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
+
+    dv::DecodeParams p;
+    memset(&p, 0, sizeof(p));
+    p.out = out;
+    p.loc = locations;
+    p.q = queries;
+    p.cosv = cosines;
+    p.sinv = sines;
+    p.fl = fragment_lengths;
+    p.kc = k_cache;
+    p.vc = v_cache;
+    p.bt = block_tables;
+    p.parents = parents;
+    p.tree_views = tree_views;
+    p.tree_rows = tree_rows;
+    p.keep_parts = 1;
+    p.l2scale = scale * 1.4426950408889634f;
+    p.F = s->F;
+    p.W = s->W;
+    p.S = s->S;
+    p.Hq = s->Hq;
+    p.Hkv = s->Hkv;
+    p.R = s->rotary_dim;
+    p.bs = s->block_size;
+    p.bs_shift = log2_exact(s->block_size);
+    p.maxB = s->max_blocks_per_seq;
+    p.nblocks = s->num_blocks;
+    p.min_keys = 256;
+    const long long max_keys = (long long)s->max_blocks_per_seq * s->block_size;
+    const hipError_t e = dv::launch_chunk(dtype, dv::kQRotFull, dv::kKvPaged, p, max_keys, workspace, workspace_bytes,
+                                          (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "dvattn_tree_paged_sdpa launch");
+    return ok();
+}
+
+// ---------------------------------------------------------------------------
+size_t dvattn_paged_key_mass_workspace_size(int dtype, const dvattn_shape* s, int device) {
+    if (!s || !valid_dtype(dtype)) return 0;
+    return dv::mass_workspace_bytes(dtype, s->F, s->W, s->S, s->Hkv,
+                                    (long long)s->max_blocks_per_seq * s->block_size, current_device(device));
+}
+
+dvattn_status dvattn_paged_key_mass(int dtype, float* out, const float* mass, float decay, long long capacity,
+                                    float scale, const int* locations, const void* queries, const float* cosines,
+                                    const float* sines, const int* fragment_lengths, const void* k_cache,
+                                    const int* block_tables, const dvattn_shape* s, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+    if (!s) return fail(DVATTN_ERR_INVALID, "shape is null");
+    if (!valid_dtype(dtype)) return fail(DVATTN_ERR_UNSUPPORTED, "unsupported dtype code %d", dtype);
+    if (s->F < 0 || s->W < 0 || s->S < 0) return fail(DVATTN_ERR_INVALID, "negative F/W/S");
+    if (capacity < 0) return fail(DVATTN_ERR_INVALID, "negative capacity");
+    if (s->W == 0 || s->Hkv == 0 || capacity == 0) return ok();
+    dvattn_status st;
+    if ((st = check_heads(s)) != DVATTN_OK) return st;
+    if ((st = check_rotary(s->rotary_dim, s->E)) != DVATTN_OK) return st;
+    if ((st = check_pages(s)) != DVATTN_OK) return st;
+    const long long max_rows = (long long)s->max_blocks_per_seq * s->block_size;
+    const long long rows = max_rows > capacity ? max_rows : capacity;
+    // one block per 128 rows at least
+    if ((long long)s->W * s->Hkv * (rows / 128 + 1) >= (1ll << 31) ||
+        (long long)s->W * s->Hkv * s->S >= (1ll << 31))
+        return fail(DVATTN_ERR_UNSUPPORTED, "W=%d, Hkv=%d, S=%d, %lld rows: too many blocks for one launch", s->W,
+                    s->Hkv, s->S, rows);
+    if (!out || (s->S > 0 && !queries) || (decay != 0.0f && !mass))
+        return fail(DVATTN_ERR_INVALID, "null out, mass or query pointer");
+    if (s->F > 0 && (!fragment_lengths || (s->S > 0 && (!locations || ((!cosines || !sines) && s->rotary_dim > 0)))))
+        return fail(DVATTN_ERR_INVALID, "null locations / fragment_lengths / cos / sin pointer");
+    if (s->num_blocks > 0 && !k_cache) return fail(DVATTN_ERR_INVALID, "null k cache pointer");
+    if (s->max_blocks_per_seq > 0 && !block_tables) return fail(DVATTN_ERR_INVALID, "null block_tables pointer");
+    if ((st = check_aligned({{out, "out", 4}, {mass, "mass", 4}, {queries, "queries", 16}, {k_cache, "k_cache", 16},
+                             {workspace, "workspace", 16}, {locations, "locations", 4},
+                             {fragment_lengths, "fragment_lengths", 4}, {cosines, "cosines", 4},
+                             {sines, "sines", 4}, {block_tables, "block_tables", 4}})) != DVATTN_OK)
+        return st;
+    const size_t need = dvattn_paged_key_mass_workspace_size(dtype, s, -1);
+    if (workspace_bytes < need || (need && !workspace))
+        return fail(DVATTN_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
+
+    dv::MassParams p;
+    memset(&p, 0, sizeof(p));
+    p.out = out;
+    p.mass = mass;
+    p.decay = decay;
+    p.C = capacity;
+    p.loc = locations;
+    p.q = queries;
+    p.cosv = cosines;
+    p.sinv = sines;
+    p.fl = fragment_lengths;
+    p.kc = k_cache;
+    p.bt = block_tables;
+    p.l2scale = scale * 1.4426950408889634f;
+    p.F = s->F;
+    p.W = s->W;
+    p.S = s->S;
+    p.Hq = s->Hq;
+    p.Hkv = s->Hkv;
+    p.R = s->rotary_dim;
+    p.bs = s->block_size;
+    p.bs_shift = log2_exact(s->block_size);
+    p.maxB = s->max_blocks_per_seq;
+    p.nblocks = s->num_blocks;
+    const hipError_t e = dv::launch_key_mass(dtype, p, workspace, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "dvattn_paged_key_mass launch");
+    return ok();
+}
+
+// ---------------------------------------------------------------------------
+dvattn_status dvattn_kv_select(int* rows, const float* mass, const int* first_rows, const int* lengths,
+                               long long capacity, int W, int Hkv, int budget, int keep_first, int keep_last,
+                               void* stream) {
+    if (W < 0 || Hkv < 0 || capacity < 0 || budget < 0 || keep_first < 0 || keep_last < 0)
+        return fail(DVATTN_ERR_INVALID, "negative W/Hkv/capacity/budget/keep_first/keep_last");
+    if ((long long)keep_first + keep_last > budget)
+        return fail(DVATTN_ERR_INVALID, "keep_first %d and keep_last %d exceed the budget %d", keep_first, keep_last,
+                    budget);
+    if (capacity > (1ll << 30)) return fail(DVATTN_ERR_UNSUPPORTED, "capacity %lld exceeds 2^30 rows", capacity);
+    if (budget > (1 << 30)) return fail(DVATTN_ERR_UNSUPPORTED, "budget %d exceeds 2^30 rows", budget);
+    if ((long long)W * Hkv >= (1ll << 31))
+        return fail(DVATTN_ERR_UNSUPPORTED, "%lld (sequence, KV head) pairs exceed 2^31", (long long)W * Hkv);
+    if ((long long)W * Hkv == 0 || budget == 0) return ok();
+    if (!rows || !first_rows || !lengths || (capacity > 0 && !mass)) return fail(DVATTN_ERR_INVALID, "null pointer");
+    const dvattn_status st = check_aligned({{rows, "rows", 4}, {mass, "mass", 4}, {first_rows, "first_rows", 4},
+                                            {lengths, "lengths", 4}});
+    if (st != DVATTN_OK) return st;
+    dv::SelectParams p;
+    memset(&p, 0, sizeof(p));
+    p.rows = rows;
+    p.mass = mass;
+    p.first = first_rows;
+    p.lengths = lengths;
+    p.C = capacity;
+    p.W = W;
+    p.Hkv = Hkv;
+    p.budget = budget;
+    p.keep_first = keep_first;
+    p.keep_last = keep_last;
+    const hipError_t e = dv::launch_kv_select(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "dvattn_kv_select launch");
+    return ok();
+}
+
+dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, const int* block_tables,
+                                      const int* rows, int row_heads, int N, const int* first_rows,
+                                      const int* lengths, float* mass, long long capacity, const dvattn_shape* s,
+                                      const dvattn_kv_layout* lay, void* stream) {
+    if (!s || !lay) return fail(DVATTN_ERR_INVALID, "shape or layout is null");
+    if (!valid_dtype(dtype)) return fail(DVATTN_ERR_UNSUPPORTED, "unsupported dtype code %d", dtype);
+    if (s->W < 0 || s->Hkv < 0 || s->E < 0 || s->Ev < 0 || N < 0 || capacity < 0)
+        return fail(DVATTN_ERR_INVALID, "negative W/Hkv/E/Ev/N/capacity");
+    if ((long long)s->W * s->Hkv == 0) return ok();
+    if (row_heads != 1 && row_heads != s->Hkv)
+        return fail(DVATTN_ERR_INVALID, "rows must hold 1 or Hkv=%d heads (got %d)", s->Hkv, row_heads);
+    if (s->block_size <= 0) return fail(DVATTN_ERR_INVALID, "block_size must be positive (got %d)", s->block_size);
+    if (s->max_blocks_per_seq < 0 || s->num_blocks < 0)
+        return fail(DVATTN_ERR_INVALID, "max_blocks_per_seq / num_blocks must be >= 0");
+    if (s->E > 8192 || s->Ev > 8192)
+        return fail(DVATTN_ERR_UNSUPPORTED, "head dims up to 8192 (E=%d, Ev=%d)", s->E, s->Ev);
+    if ((long long)s->W * s->Hkv >= (1ll << 24) || N > (1 << 30))
+        return fail(DVATTN_ERR_UNSUPPORTED, "W * Hkv = %lld and N = %d: at most 2^24 and 2^30",
+                    (long long)s->W * s->Hkv, N);
+    if (mass && !lengths) return fail(DVATTN_ERR_INVALID, "mass needs lengths");
+    if (N == 0 && !mass) return ok();
+    if (!first_rows || (N > 0 && !rows) || (s->max_blocks_per_seq > 0 && !block_tables) ||
+        (s->num_blocks > 0 && ((s->E > 0 && !k_cache) || (s->Ev > 0 && !v_cache))))
+        return fail(DVATTN_ERR_INVALID, "null pointer");
+    const dvattn_status st = check_aligned({{k_cache, "k_cache", elem_bytes(dtype)},
+                                            {v_cache, "v_cache", elem_bytes(dtype)}, {rows, "rows", 4},
+                                            {block_tables, "block_tables", 4}, {first_rows, "first_rows", 4},
+                                            {lengths, "lengths", 4}, {mass, "mass", 4}});
+    if (st != DVATTN_OK) return st;
+    dv::CompactParams p;
+    memset(&p, 0, sizeof(p));
+    p.kc = k_cache;
+    p.vc = v_cache;
+    for (int i = 0; i < 3; ++i) {
+        p.kcs[i] = lay->k_cache_strides[i];
+        p.vcs[i] = lay->v_cache_strides[i];
+    }
+    p.bt = block_tables;
+    p.rows = rows;
+    p.first = first_rows;
+    p.lengths = lengths;
+    p.mass = mass;
+    p.C = capacity;
+    p.W = s->W;
+    p.Hkv = s->Hkv;
+    p.heads = row_heads;
+    p.N = N;
+    p.E = s->E;
+    p.Ev = s->Ev;
+    p.bs = s->block_size;
+    p.maxB = s->max_blocks_per_seq;
+    p.nblocks = s->num_blocks;
+    const hipError_t e = dv::launch_kv_compact(dtype, p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "dvattn_paged_kv_compact launch");
+    return ok();
+}
+
 }  // extern "C"

@@ -854,6 +854,7 @@ hipError_t launch1(DecodeParams p, int device, int cus, long long cap, hipStream
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int ntb = max_group_tokens<RM>(p);
+    if (p.parents) return launch_merge_tree(DT, p, ntb, stream);
     hipLaunchKernelGGL((dv_merge_chunk<DT, RM>), dim3(p.nrows * p.Hkv * ntb), dim3(256), 0, stream, p, ntb);
     return hipGetLastError();
 }

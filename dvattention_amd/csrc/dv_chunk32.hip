@@ -330,6 +330,7 @@ hipError_t launch1_f32(DecodeParams p, int device, int cus, long long cap, hipSt
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const int ntb = max_group_tokens<RM>(p);
+    if (p.parents) return launch_merge_tree(kF32, p, ntb, stream);
     hipLaunchKernelGGL((dv_merge_chunk<kF32, RM>), dim3(p.nrows * p.Hkv * ntb), dim3(256), 0, stream, p, ntb);
     return hipGetLastError();
 }

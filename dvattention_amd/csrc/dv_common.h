@@ -76,6 +76,11 @@ struct DecodeParams {
     int piece_cost;       // fixed cost of starting a segment, in keys (charged in the work split)
     int skew_pm;          // per mille of a chunk moved from each odd workgroup to the even one before it
     int slot_floats;      // floats per partial slot
+    int keep_parts;       // 1: every piece goes to a partial slot, none is final (the merge adds more keys)
+    // drafted trees (dv_merge_tree): parents [W, S], each sequence's view and stream row of node 0
+    const int* parents;
+    const int* tree_views;
+    const int* tree_rows;
     FragDesc frags[kMaxFragArgs];
 };
 
@@ -139,6 +144,66 @@ struct MetaParams {
     int F, W, S, R;
 };
 
+// Metadata of a step that drafts a token tree per sequence (dv_tree_meta).
+constexpr int kMaxTreeNodes = 4096;  // drafted nodes of a sequence (parents and ancestors live in LDS)
+constexpr int kMaxTreeViews = 4096;  // views of a tree metadata call (flags and order live in LDS)
+struct TreeMetaParams {
+    MetaParams m;             // outputs and inputs shared with dv_view_meta
+    const int* parents;       // [W, S]
+    int* tree_views;          // [W]
+    int* tree_rows;           // [W]
+};
+
+// Accumulated attention weight of cached keys (dv_mass.hip).
+struct MassParams {
+    float* out;               // [W, Hkv, C]
+    const float* mass;        // [W, Hkv, C], may be out
+    float decay;
+    long long C;              // rows per (sequence, KV head) of mass and out
+    const int* loc;           // [F, W, S]
+    const void* q;            // queries [W, Hq, S, E]
+    const float* cosv;        // [F, W, S, R]
+    const float* sinv;
+    const int* fl;            // [F]
+    const void* kc;           // [num_blocks, block_size, Hkv, E]
+    const int* bt;            // [W, maxB]
+    float l2scale;
+    int F, W, S, Hq, Hkv, R;
+    int bs, bs_shift, maxB, nblocks;
+    // set by the launcher
+    void* rq;                 // rotated queries [F, W, Hq, S, E] (S > 1)
+    float* part;              // (max, sum) of each row over one workgroup's or wave's keys
+    float* lse;               // minus the base-2 log-sum-exp of each (sequence, KV head, token, head) (S > 1)
+    float* scores;            // base-2 scores, tile by tile (S = 1)
+    int nchunks;              // workgroups along the keys of one (sequence, KV head)
+    int s0, ns;               // tokens of this launch
+};
+
+// Rows of a cache worth keeping, and the move of kept rows (dv_evict.hip).
+struct SelectParams {
+    int* rows;                // [W, Hkv, budget]
+    const float* mass;        // [W, Hkv, C]
+    const int* first;         // [W]
+    const int* lengths;       // [W]
+    long long C;
+    int W, Hkv, budget, keep_first, keep_last;
+};
+
+struct CompactParams {
+    void* kc;                 // caches, element strides (page, row, head), last dim contiguous
+    void* vc;
+    long long kcs[3], vcs[3];
+    const int* bt;            // [W, maxB]
+    const int* rows;          // [W, heads, N], heads = Hkv or 1
+    const int* first;         // [W]
+    const int* lengths;       // [W] or null
+    float* mass;              // [W, Hkv, C] or null
+    long long C;
+    int W, Hkv, heads, N, E, Ev;
+    int bs, maxB, nblocks;
+    int slices;               // column slices of a row, a workgroup each
+};
+
 // CU count of a device, queried once per device (thread-safe; 256 if unknown).
 inline int device_cu_count(int device) {
     static std::atomic<int> cache[64];
@@ -193,6 +258,20 @@ hipError_t launch_rope(int dtype, const RopeParams& p, hipStream_t stream);
 // rope_dtype: kF32, or the storage dtype (cos/sin in the model's dtype).
 hipError_t launch_kv_append(int dtype, int rope_dtype, const AppendParams& p, hipStream_t stream);
 hipError_t launch_view_meta(const MetaParams& p, hipStream_t stream);
+hipError_t launch_tree_meta(const TreeMetaParams& p, hipStream_t stream);
+
+// Tree attention: the committed keys through the chunk path (keep_parts), the
+// drafted ones in the merge.  launch_merge_tree merges the segments of a launch
+// of launch_chunk whose parameters carry parents.
+hipError_t launch_merge_tree(int dtype, const DecodeParams& p, int ntb, hipStream_t stream);
+
+// Key mass: workspace of a call with at most max_rows stream rows per sequence, and
+// its launches.
+size_t mass_workspace_bytes(int dtype, int F, int W, int S, int Hkv, long long max_rows, int device);
+hipError_t launch_key_mass(int dtype, const MassParams& p, void* workspace, hipStream_t stream);
+
+hipError_t launch_kv_select(const SelectParams& p, hipStream_t stream);
+hipError_t launch_kv_compact(int dtype, const CompactParams& p, hipStream_t stream);
 
 // Multi-query path (S >= 2 tokens per sequence; dv_chunk for 16-bit types,
 // dv_chunk32 for fp32): K/V read once per block of 16 tokens.  Rows of

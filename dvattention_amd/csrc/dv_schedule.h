@@ -151,7 +151,7 @@ __device__ inline void split_chunks(const DecodeParams& p, int NHG, long long to
             // the segment has no other piece iff its first and last keys both lie
             // in this chunk (chunk_of(ka) == chunk_of(segc + D - 1) == gidx, without
             // the divisions)
-            const bool fin = ka >= u0 && segc + D - 1 < uend;
+            const bool fin = ka >= u0 && segc + D - 1 < uend && !p.keep_parts;
             const int slot = sg + gidx;  // = first slot of the segment (chunk_of(ka) + sg) + piece index
             // cuts inside a segment move down to a multiple of kAlign keys (both
             // neighbours use the same rule; a piece may be left without keys)

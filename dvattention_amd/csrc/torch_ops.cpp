@@ -6,6 +6,7 @@
 // libdvattn_amd.so on the tensors' current HIP stream.  Unsupported dtypes and
 // shapes raise instead of silently doing nothing.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/library.h>
@@ -68,6 +69,57 @@ hipStream_t stream_of(const at::Tensor& t) { return c10::hip::getCurrentHIPStrea
 
 at::Tensor workspace(size_t bytes, const at::Tensor& like) {
     return at::empty({(int64_t)(bytes ? bytes : 1)}, like.options().dtype(at::kByte));
+}
+
+// Checks of a paged call's queries [W,Hq,S,E], views, keys and tables against `like`'s
+// type and device, and the shape they make (Ev is left to the caller).
+dvattn_shape paged_query_shape(const at::Tensor& like, const at::Tensor& locations, const at::Tensor& queries,
+                               const at::Tensor& cosines, const at::Tensor& sines,
+                               const at::Tensor& fragment_lengths, const at::Tensor& k_cache,
+                               const at::Tensor& block_tables, const char* op) {
+    check_dim(locations, 3, "locations");
+    check_dim(queries, 4, "queries");
+    check_dim(cosines, 4, "cosines");
+    check_dim(sines, 4, "sines");
+    check_dim(fragment_lengths, 1, "fragment_lengths");
+    check_dim(k_cache, 4, "k_cache");
+    check_dim(block_tables, 2, "block_tables");
+    check_same(queries, like, "queries");
+    check_same(k_cache, like, "k_cache");
+    check_i32(locations, "locations");
+    check_i32(fragment_lengths, "fragment_lengths");
+    check_i32(block_tables, "block_tables");
+    check_f32(cosines, "cosines");
+    check_f32(sines, "sines");
+    const at::Tensor* all[] = {&locations, &queries, &cosines, &sines, &fragment_lengths, &k_cache, &block_tables};
+    const char* names[] = {"locations", "queries", "cosines", "sines", "fragment_lengths", "k_cache", "block_tables"};
+    for (int i = 0; i < 7; ++i) {
+        check_contig(*all[i], names[i]);
+        check_dev(*all[i], like, names[i]);
+    }
+    const int64_t W = queries.size(0), Hq = queries.size(1), S = queries.size(2), E = queries.size(3);
+    const int64_t F = locations.size(0);
+    TORCH_CHECK(locations.size(1) == W && locations.size(2) == S, op, ": locations must be [F,W,S], got ",
+                locations.sizes());
+    TORCH_CHECK(cosines.size(0) == F && cosines.size(1) == W && cosines.size(2) == S, op,
+                ": cosines must be [F,W,S,R], got ", cosines.sizes());
+    TORCH_CHECK(sines.sizes() == cosines.sizes(), op, ": sines must match cosines");
+    TORCH_CHECK(fragment_lengths.size(0) == F, op, ": fragment_lengths must be [F], got ", fragment_lengths.sizes());
+    TORCH_CHECK(k_cache.size(3) == E, op, ": k_cache head dim ", k_cache.size(3), " != query dim ", E);
+    TORCH_CHECK(block_tables.size(0) >= W, op, ": block_tables needs a row per sequence (", W, "), got ",
+                block_tables.sizes());
+    dvattn_shape s{};
+    s.F = as_int(F, "F");
+    s.W = as_int(W, "W");
+    s.Hq = as_int(Hq, "Hq");
+    s.Hkv = as_int(k_cache.size(2), "Hkv");
+    s.E = as_int(E, "E");
+    s.S = as_int(S, "S");
+    s.block_size = as_int(k_cache.size(1), "block_size");
+    s.max_blocks_per_seq = as_int(block_tables.size(1), "max_blocks_per_seq");
+    s.num_blocks = as_int(k_cache.size(0), "num_blocks");
+    s.rotary_dim = as_int(cosines.size(3), "rotary_dim");
+    return s;
 }
 
 // ---------------------------------------------------------------------------
@@ -572,6 +624,258 @@ void dvattn_view_metadata_op(at::Tensor& locations, at::Tensor& cosines, at::Ten
                  "dvattn_view_metadata");
 }
 
+// ---------------------------------------------------------------------------
+// Drafted token trees and bounded caches (no counterpart in the reference).
+
+// dvattn_tree_metadata(Tensor(a!) locations, Tensor(b!) cosines, Tensor(c!) sines, Tensor(d!) tree_views,
+//   Tensor(e!) tree_rows, Tensor fragment_lengths, Tensor order, Tensor parents, Tensor inv_freq,
+//   float attention_scaling, ScalarType? round_to=None)
+void dvattn_tree_metadata_op(at::Tensor& locations, at::Tensor& cosines, at::Tensor& sines, at::Tensor& tree_views,
+                             at::Tensor& tree_rows, const at::Tensor& fragment_lengths, const at::Tensor& order,
+                             const at::Tensor& parents, const at::Tensor& inv_freq, double attention_scaling,
+                             std::optional<at::ScalarType> round_to) {
+    check_dim(locations, 3, "locations");
+    check_dim(cosines, 4, "cosines");
+    check_dim(sines, 4, "sines");
+    check_dim(tree_views, 1, "tree_views");
+    check_dim(tree_rows, 1, "tree_rows");
+    check_dim(fragment_lengths, 1, "fragment_lengths");
+    check_dim(order, 2, "order");
+    check_dim(parents, 2, "parents");
+    check_dim(inv_freq, 1, "inv_freq");
+    const at::Tensor* all[] = {&locations, &tree_views, &tree_rows, &fragment_lengths, &order,
+                               &parents,   &cosines,    &sines,     &inv_freq};
+    const char* names[] = {"locations", "tree_views", "tree_rows", "fragment_lengths", "order",
+                           "parents",   "cosines",    "sines",     "inv_freq"};
+    for (int i = 0; i < 9; ++i) {
+        if (i < 6) check_i32(*all[i], names[i]);
+        else check_f32(*all[i], names[i]);
+        check_contig(*all[i], names[i]);
+        check_dev(*all[i], locations, names[i]);
+    }
+    const int64_t F = locations.size(0), W = locations.size(1), S = locations.size(2), R = cosines.size(3);
+    TORCH_CHECK(cosines.size(0) == F && cosines.size(1) == W && cosines.size(2) == S,
+                "dvattn_tree_metadata: cosines must be [F,W,S,R], got ", cosines.sizes());
+    TORCH_CHECK(sines.sizes() == cosines.sizes(), "dvattn_tree_metadata: sines must match cosines");
+    TORCH_CHECK(tree_views.size(0) == W && tree_rows.size(0) == W,
+                "dvattn_tree_metadata: tree_views and tree_rows must be [W], got ", tree_views.sizes(), " and ",
+                tree_rows.sizes());
+    TORCH_CHECK(fragment_lengths.size(0) == F, "dvattn_tree_metadata: fragment_lengths must be [F], got ",
+                fragment_lengths.sizes());
+    TORCH_CHECK(order.size(0) == W && order.size(1) == F, "dvattn_tree_metadata: order must be [W,F], got ",
+                order.sizes());
+    TORCH_CHECK(parents.size(0) == W && parents.size(1) == S, "dvattn_tree_metadata: parents must be [W,S], got ",
+                parents.sizes());
+    TORCH_CHECK(R % 2 == 0 && inv_freq.size(0) >= R / 2, "dvattn_tree_metadata: need an even rotary dim and R/2 ",
+                "inverse frequencies (R=", R, ", got ", inv_freq.size(0), ")");
+    int rd = -1;
+    if (round_to.has_value()) {
+        switch (*round_to) {
+            case at::kFloat: rd = -1; break;
+            case at::kHalf: rd = DVATTN_F16; break;
+            case at::kBFloat16: rd = DVATTN_BF16; break;
+            default: TORCH_CHECK(false, "dvattn_tree_metadata: round_to must be float32, float16 or bfloat16");
+        }
+    }
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(locations.device());
+    check_status(dvattn_tree_metadata(locations.data_ptr<int>(), cosines.data_ptr<float>(), sines.data_ptr<float>(),
+                                      tree_views.data_ptr<int>(), tree_rows.data_ptr<int>(),
+                                      fragment_lengths.data_ptr<int>(), order.data_ptr<int>(),
+                                      parents.data_ptr<int>(), inv_freq.data_ptr<float>(), (float)attention_scaling,
+                                      rd, as_int(F, "F"), as_int(W, "W"), as_int(S, "S"), as_int(R, "rotary_dim"),
+                                      stream_of(locations)),
+                 "dvattn_tree_metadata");
+}
+
+// dvattn_tree_paged_sdpa(Tensor(a!) output, float scale, <dvattn_paged_sdpa's tensors>, Tensor parents,
+//   Tensor tree_views, Tensor tree_rows)
+void dvattn_tree_paged_sdpa_op(at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
+                               const at::Tensor& cosines, const at::Tensor& sines,
+                               const at::Tensor& fragment_lengths, const at::Tensor& k_cache,
+                               const at::Tensor& v_cache, const at::Tensor& block_tables, const at::Tensor& parents,
+                               const at::Tensor& tree_views, const at::Tensor& tree_rows) {
+    const int dt = dtype_code(out);
+    check_dim(out, 4, "output");
+    check_dim(v_cache, 4, "v_cache");
+    check_dim(parents, 2, "parents");
+    check_dim(tree_views, 1, "tree_views");
+    check_dim(tree_rows, 1, "tree_rows");
+    check_same(v_cache, out, "v_cache");
+    dvattn_shape s = paged_query_shape(out, locations, queries, cosines, sines, fragment_lengths, k_cache,
+                                       block_tables, "dvattn_tree_paged_sdpa");
+    const at::Tensor* ints[] = {&parents, &tree_views, &tree_rows};
+    const char* names[] = {"parents", "tree_views", "tree_rows"};
+    for (int i = 0; i < 3; ++i) {
+        check_i32(*ints[i], names[i]);
+        check_contig(*ints[i], names[i]);
+        check_dev(*ints[i], out, names[i]);
+    }
+    check_contig(out, "output");
+    check_contig(v_cache, "v_cache");
+    check_dev(v_cache, out, "v_cache");
+    const int64_t W = queries.size(0), Hq = queries.size(1), S = queries.size(2), Ev = out.size(3);
+    TORCH_CHECK(out.size(0) == W && out.size(1) == Hq && out.size(2) == S,
+                "dvattn_tree_paged_sdpa: output must be [W,Hq,S,Ev], got ", out.sizes());
+    TORCH_CHECK(v_cache.size(0) == k_cache.size(0) && v_cache.size(1) == k_cache.size(1) &&
+                    v_cache.size(2) == k_cache.size(2) && v_cache.size(3) == Ev,
+                "dvattn_tree_paged_sdpa: v_cache must be [num_blocks, block_size, Hkv, Ev], got ", v_cache.sizes());
+    TORCH_CHECK(parents.size(0) == W && parents.size(1) == S, "dvattn_tree_paged_sdpa: parents must be [W,S], got ",
+                parents.sizes());
+    TORCH_CHECK(tree_views.size(0) == W && tree_rows.size(0) == W,
+                "dvattn_tree_paged_sdpa: tree_views and tree_rows must be [W], got ", tree_views.sizes(), " and ",
+                tree_rows.sizes());
+    s.Ev = as_int(Ev, "Ev");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(out.device());
+    const size_t ws = dvattn_tree_paged_sdpa_workspace_size(dt, &s, out.device().index());
+    at::Tensor w = workspace(ws, out);
+    check_status(dvattn_tree_paged_sdpa(dt, out.data_ptr(), (float)scale, locations.data_ptr<int>(),
+                                        queries.data_ptr(), cosines.data_ptr<float>(), sines.data_ptr<float>(),
+                                        fragment_lengths.data_ptr<int>(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                        block_tables.data_ptr<int>(), parents.data_ptr<int>(),
+                                        tree_views.data_ptr<int>(), tree_rows.data_ptr<int>(), &s, w.data_ptr(), ws,
+                                        stream_of(out)),
+                 "dvattn_tree_paged_sdpa");
+}
+
+// dvattn_paged_key_mass(Tensor(a!) output, Tensor? mass, float decay, float scale, Tensor locations,
+//   Tensor queries, Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor block_tables)
+void dvattn_paged_key_mass_op(at::Tensor& out, const std::optional<at::Tensor>& mass, double decay, double scale,
+                              const at::Tensor& locations, const at::Tensor& queries, const at::Tensor& cosines,
+                              const at::Tensor& sines, const at::Tensor& fragment_lengths, const at::Tensor& k_cache,
+                              const at::Tensor& block_tables) {
+    const int dt = dtype_code(queries);
+    check_dim(out, 3, "output");
+    check_f32(out, "output");
+    check_contig(out, "output");
+    dvattn_shape s = paged_query_shape(queries, locations, queries, cosines, sines, fragment_lengths, k_cache,
+                                       block_tables, "dvattn_paged_key_mass");
+    check_dev(out, queries, "output");
+    TORCH_CHECK(out.size(0) == queries.size(0) && out.size(1) == k_cache.size(2),
+                "dvattn_paged_key_mass: output must be [W,Hkv,capacity], got ", out.sizes());
+    const bool has = mass.has_value() && mass->defined();
+    TORCH_CHECK(has || (float)decay == 0.0f, "dvattn_paged_key_mass: decay ", decay, " needs a mass");
+    if (has) {
+        check_f32(*mass, "mass");
+        check_contig(*mass, "mass");
+        check_dev(*mass, queries, "mass");
+        TORCH_CHECK(mass->sizes() == out.sizes(), "dvattn_paged_key_mass: mass must match output ", out.sizes(),
+                    ", got ", mass->sizes());
+        at::assert_no_partial_overlap(out, *mass);
+    }
+    s.Ev = s.E;
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(out.device());
+    const size_t ws = dvattn_paged_key_mass_workspace_size(dt, &s, out.device().index());
+    at::Tensor w = workspace(ws, out);
+    check_status(dvattn_paged_key_mass(dt, out.data_ptr<float>(), has ? mass->data_ptr<float>() : nullptr,
+                                       (float)decay, out.size(2), (float)scale, locations.data_ptr<int>(),
+                                       queries.data_ptr(), cosines.data_ptr<float>(), sines.data_ptr<float>(),
+                                       fragment_lengths.data_ptr<int>(), k_cache.data_ptr(),
+                                       block_tables.data_ptr<int>(), &s, w.data_ptr(), ws, stream_of(out)),
+                 "dvattn_paged_key_mass");
+}
+
+// dvattn_kv_select(Tensor(a!) rows, Tensor mass, Tensor first_rows, Tensor lengths, int keep_first, int keep_last)
+void dvattn_kv_select_op(at::Tensor& rows, const at::Tensor& mass, const at::Tensor& first_rows,
+                         const at::Tensor& lengths, int64_t keep_first, int64_t keep_last) {
+    check_dim(rows, 3, "rows");
+    check_dim(mass, 3, "mass");
+    check_dim(first_rows, 1, "first_rows");
+    check_dim(lengths, 1, "lengths");
+    check_f32(mass, "mass");
+    const at::Tensor* all[] = {&rows, &first_rows, &lengths, &mass};
+    const char* names[] = {"rows", "first_rows", "lengths", "mass"};
+    for (int i = 0; i < 4; ++i) {
+        if (i < 3) check_i32(*all[i], names[i]);
+        check_contig(*all[i], names[i]);
+        check_dev(*all[i], rows, names[i]);
+    }
+    const int64_t W = mass.size(0), Hkv = mass.size(1);
+    TORCH_CHECK(rows.size(0) == W && rows.size(1) == Hkv, "dvattn_kv_select: rows must be [W,Hkv,budget] = [", W, ",",
+                Hkv, ",budget], got ", rows.sizes());
+    TORCH_CHECK(first_rows.size(0) == W && lengths.size(0) == W,
+                "dvattn_kv_select: first_rows and lengths must be [W], got ", first_rows.sizes(), " and ",
+                lengths.sizes());
+    TORCH_CHECK(keep_first >= 0 && keep_last >= 0 && keep_first <= rows.size(2) &&
+                    keep_last <= rows.size(2) - keep_first,
+                "dvattn_kv_select: keep_first ", keep_first, " and keep_last ", keep_last,
+                " must be >= 0 and together at most the budget ", rows.size(2));
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(rows.device());
+    check_status(dvattn_kv_select(rows.data_ptr<int>(), mass.data_ptr<float>(), first_rows.data_ptr<int>(),
+                                  lengths.data_ptr<int>(), mass.size(2), as_int(W, "W"), as_int(Hkv, "Hkv"),
+                                  as_int(rows.size(2), "budget"), as_int(keep_first, "keep_first"),
+                                  as_int(keep_last, "keep_last"), stream_of(rows)),
+                 "dvattn_kv_select");
+}
+
+// dvattn_paged_kv_compact(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_tables, Tensor rows,
+//   Tensor first_rows, Tensor? lengths=None, Tensor(c!)? mass=None)
+void dvattn_paged_kv_compact_op(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& block_tables,
+                                const at::Tensor& rows, const at::Tensor& first_rows,
+                                const std::optional<at::Tensor>& lengths, const std::optional<at::Tensor>& mass) {
+    const int dt = dtype_code(k_cache);
+    check_dim(k_cache, 4, "k_cache");
+    check_dim(v_cache, 4, "v_cache");
+    check_dim(block_tables, 2, "block_tables");
+    check_dim(rows, 3, "rows");
+    check_dim(first_rows, 1, "first_rows");
+    check_same(v_cache, k_cache, "v_cache");
+    check_dev(k_cache, k_cache, "k_cache");
+    check_dev(v_cache, k_cache, "v_cache");
+    const bool has_len = lengths.has_value() && lengths->defined(), has_mass = mass.has_value() && mass->defined();
+    TORCH_CHECK(has_len || !has_mass, "dvattn_paged_kv_compact: mass needs lengths");
+    const at::Tensor* ints[] = {&block_tables, &rows, &first_rows, has_len ? &*lengths : &first_rows};
+    const char* names[] = {"block_tables", "rows", "first_rows", "lengths"};
+    for (int i = 0; i < 4; ++i) {
+        check_i32(*ints[i], names[i]);
+        check_contig(*ints[i], names[i]);
+        check_dev(*ints[i], k_cache, names[i]);
+    }
+    const int64_t P = k_cache.size(0), bs = k_cache.size(1), Hkv = k_cache.size(2);
+    const int64_t W = rows.size(0);
+    for (const at::Tensor* c : {&k_cache, &v_cache})
+        TORCH_CHECK(c->size(3) <= 1 || c->stride(3) == 1,
+                    "dvattn_paged_kv_compact: the last dim of the caches must be contiguous");
+    TORCH_CHECK(v_cache.size(0) == P && v_cache.size(1) == bs && v_cache.size(2) == Hkv,
+                "dvattn_paged_kv_compact: v_cache must be [num_blocks, block_size, Hkv, Ev], got ", v_cache.sizes());
+    TORCH_CHECK(rows.size(1) == Hkv || rows.size(1) == 1, "dvattn_paged_kv_compact: rows must be [W,Hkv|1,N] with Hkv=",
+                Hkv, ", got ", rows.sizes());
+    TORCH_CHECK(first_rows.size(0) == W, "dvattn_paged_kv_compact: first_rows must be [W], got ", first_rows.sizes());
+    TORCH_CHECK(block_tables.size(0) >= W, "dvattn_paged_kv_compact: block_tables needs a row per sequence (", W,
+                "), got ", block_tables.sizes());
+    if (has_len)
+        TORCH_CHECK(lengths->dim() == 1 && lengths->size(0) == W, "dvattn_paged_kv_compact: lengths must be [W], got ",
+                    lengths->sizes());
+    if (has_mass) {
+        check_dim(*mass, 3, "mass");
+        check_f32(*mass, "mass");
+        check_contig(*mass, "mass");
+        check_dev(*mass, k_cache, "mass");
+        TORCH_CHECK(mass->size(0) == W && mass->size(1) == Hkv,
+                    "dvattn_paged_kv_compact: mass must be [W,Hkv,capacity], got ", mass->sizes());
+    }
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    dvattn_shape s{};
+    s.W = as_int(W, "W");
+    s.Hkv = as_int(Hkv, "Hkv");
+    s.E = as_int(k_cache.size(3), "E");
+    s.Ev = as_int(v_cache.size(3), "Ev");
+    s.block_size = as_int(bs, "block_size");
+    s.max_blocks_per_seq = as_int(block_tables.size(1), "max_blocks_per_seq");
+    s.num_blocks = as_int(P, "num_blocks");
+    dvattn_kv_layout lay{};
+    for (int i = 0; i < 3; ++i) {
+        lay.k_cache_strides[i] = k_cache.stride(i);
+        lay.v_cache_strides[i] = v_cache.stride(i);
+    }
+    check_status(dvattn_paged_kv_compact(dt, k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr<int>(),
+                                         rows.data_ptr<int>(), as_int(rows.size(1), "row heads"),
+                                         as_int(rows.size(2), "N"), first_rows.data_ptr<int>(),
+                                         has_len ? lengths->data_ptr<int>() : nullptr,
+                                         has_mass ? mass->data_ptr<float>() : nullptr, has_mass ? mass->size(2) : 0,
+                                         &s, &lay, stream_of(k_cache)),
+                 "dvattn_paged_kv_compact");
+}
+
 }  // namespace
 
 TORCH_LIBRARY(libdvatt, m) {
@@ -602,6 +906,20 @@ TORCH_LIBRARY(libdvatt, m) {
     m.def("dvattn_view_metadata(Tensor(a!) locations, Tensor(b!) cosines, Tensor(c!) sines, "
           "Tensor fragment_lengths, Tensor order, Tensor inv_freq, float attention_scaling, "
           "ScalarType? round_to=None) -> ()");
+    // drafted token trees and bounded caches
+    m.def("dvattn_tree_metadata(Tensor(a!) locations, Tensor(b!) cosines, Tensor(c!) sines, "
+          "Tensor(d!) tree_views, Tensor(e!) tree_rows, Tensor fragment_lengths, Tensor order, Tensor parents, "
+          "Tensor inv_freq, float attention_scaling, ScalarType? round_to=None) -> ()");
+    m.def("dvattn_tree_paged_sdpa(Tensor(a!) output, float scale, Tensor locations, Tensor queries, "
+          "Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor v_cache, "
+          "Tensor block_tables, Tensor parents, Tensor tree_views, Tensor tree_rows) -> ()");
+    m.def("dvattn_paged_key_mass(Tensor(a!) output, Tensor? mass, float decay, float scale, Tensor locations, "
+          "Tensor queries, Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, "
+          "Tensor block_tables) -> ()");
+    m.def("dvattn_kv_select(Tensor(a!) rows, Tensor mass, Tensor first_rows, Tensor lengths, int keep_first, "
+          "int keep_last) -> ()");
+    m.def("dvattn_paged_kv_compact(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_tables, Tensor rows, "
+          "Tensor first_rows, Tensor? lengths=None, Tensor(c!)? mass=None) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(libdvatt, CUDA, m) {
@@ -613,4 +931,9 @@ TORCH_LIBRARY_IMPL(libdvatt, CUDA, m) {
     m.impl("dvattn_varlen_paged_sdpa", dvattn_varlen_paged_sdpa_op);
     m.impl("dvattn_paged_kv_append", dvattn_paged_kv_append_op);
     m.impl("dvattn_view_metadata", dvattn_view_metadata_op);
+    m.impl("dvattn_tree_metadata", dvattn_tree_metadata_op);
+    m.impl("dvattn_tree_paged_sdpa", dvattn_tree_paged_sdpa_op);
+    m.impl("dvattn_paged_key_mass", dvattn_paged_key_mass_op);
+    m.impl("dvattn_kv_select", dvattn_kv_select_op);
+    m.impl("dvattn_paged_kv_compact", dvattn_paged_kv_compact_op);
 }

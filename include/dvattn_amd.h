@@ -26,6 +26,9 @@
  *                               cache append of a decode step), 245-251 (merge_caches)
  *   dvattn_view_metadata     <- python/dvattn/attention.py:158-186 (per-view locations,
  *                               cos/sin)
+ * and, with no counterpart there, for drafted token trees and bounded caches:
+ *   dvattn_tree_metadata, dvattn_tree_paged_sdpa, dvattn_paged_key_mass,
+ *   dvattn_kv_select, dvattn_paged_kv_compact.
  *
  * Semantics (identical to the reference operators):
  *   - GQA factor 16 (Hq == 16*Hkv) and head dims E == Ev == 128 only; other
@@ -49,10 +52,11 @@
  * Alignment (checked; the reference's kernels assumed 16-byte vectors,
  * paged_kernel_v21.cuh:58-62, without checking): the attention entry points
  * (dvattn_paged_sdpa[_noalloc], dvattn_varlen_paged_sdpa, dvattn_sdpa,
- * dvattn_fused) need out, queries, rotated_queries, k_cache, v_cache, every
+ * dvattn_fused, dvattn_tree_paged_sdpa, dvattn_paged_key_mass) need out, queries, rotated_queries, k_cache, v_cache, every
  * key/value fragment and the workspace 16-byte aligned and the int32 / fp32
- * arrays 4-byte aligned; dvattn_rope, dvattn_varlen_rope and
- * dvattn_paged_kv_append need each array aligned to its element size.  A
+ * arrays 4-byte aligned; dvattn_rope, dvattn_varlen_rope,
+ * dvattn_paged_kv_append, the metadata entries, dvattn_kv_select and
+ * dvattn_paged_kv_compact need each array aligned to its element size.  A
  * pointer off its alignment returns DVATTN_ERR_INVALID, naming the argument.
  * Tensors from a device allocator, and views of them that start on a row of
  * the last dimension, always qualify.
@@ -264,6 +268,102 @@ DVATTN_API dvattn_status dvattn_view_metadata(int* locations, float* cosines, fl
                                    const int* fragment_lengths, const int* order, const float* inv_freq,
                                    float attention_scaling, int round_dtype, int F, int W, int S,
                                    int rotary_dim, void* stream);
+
+/* ---- a step that drafts a token tree per sequence: metadata --------------------
+ * Each of W sequences drafts a tree of up to S nodes.  parents [W,S] i32:
+ * parents[w,s] = -1 for a child of the committed tokens, or the index of an
+ * earlier node (0 .. s-1); any other entry makes the node absent (padding of a
+ * smaller tree), and with it every node below it.  The S drafted rows are the
+ * last S of each sequence's own view (its last in order): fragment_lengths
+ * count them, and c(g), the committed tokens of view g, is fragment_lengths[g] -
+ * S where g is the own view of some sequence, else fragment_lengths[g] (at least
+ * 0).  With d(s) the depth of node s (0 for a child of the committed tokens):
+ *   position(f,w,s)    = (sum of c over w's segments from f's place in its order
+ *                        to the end) + d(s)
+ *   locations[f,w,s]   = c(f) - 1          (the committed keys of the view)
+ *   cos/sin[f,w,s,i]   = cos/sin(float(position) * inv_freq[i % (R/2)])
+ *                        * attention_scaling, rounded as round_dtype says
+ *   tree_views[w]      = w's own view (-1: none)
+ *   tree_rows[w]       = the stream row of node 0: c(own) after the sum of the
+ *                        fragment_lengths before the view; node s is written to
+ *                        tree_rows[w] + s (dvattn_paged_kv_append's positions)
+ * Absent nodes and views missing from a sequence's order get location -1, cos 1,
+ * sin 0.  The other sequences' drafted nodes are neither seen nor counted.  For
+ * one sequence and a chain (parents -1, 0, 1, ...) cos/sin are
+ * dvattn_view_metadata's.  S <= 4096, F <= 4096. */
+#define DVATTN_MAX_TREE_NODES 4096
+DVATTN_API dvattn_status dvattn_tree_metadata(int* locations, float* cosines, float* sines, int* tree_views,
+                                   int* tree_rows, const int* fragment_lengths, const int* order,
+                                   const int* parents, const float* inv_freq, float attention_scaling,
+                                   int round_dtype, int F, int W, int S, int rotary_dim, void* stream);
+
+/* ---- attention of drafted token trees over a paged cache -------------------------
+ * dvattn_paged_sdpa's arguments, with S drafted nodes per sequence, and parents
+ * [W,S], tree_views [W], tree_rows [W] as above.  Node s of sequence w sees
+ *   - key l of view f iff l <= locations[f,w,s] and l < fragment_lengths[f], as in
+ *     dvattn_paged_sdpa, and
+ *   - of view tree_views[w], the keys in stream rows tree_rows[w] + j for j = s and
+ *     every ancestor j of s, if the row lies inside the view,
+ * each key once.  An absent node's output is zeros.  A drafted row that a node
+ * does not see is not read for it, whatever it holds; a committed key past a
+ * node's location but within that of another node of its sequence takes part with
+ * weight 0 and must be finite, as in dvattn_paged_sdpa.  S <= 4096. */
+DVATTN_API size_t dvattn_tree_paged_sdpa_workspace_size(int dtype, const dvattn_shape* shape, int device);
+DVATTN_API dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scale, const int* locations,
+                                     const void* queries, const float* cosines, const float* sines,
+                                     const int* fragment_lengths, const void* k_cache, const void* v_cache,
+                                     const int* block_tables, const int* parents, const int* tree_views,
+                                     const int* tree_rows, const dvattn_shape* shape, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
+/* ---- attention weight that every cached key receives ------------------------------
+ * out, mass [W,Hkv,capacity] f32 by stream row (view f's key l is row l + the sum of
+ * the fragment_lengths before f; negative lengths count as 0):
+ *   out[w,h,c] = decay * mass[w,h,c] + the softmax weights that the S queries and 16
+ *                query heads of KV head h give to the key in row c
+ * with the weights of dvattn_paged_sdpa (same queries, locations, cos/sin, scale), in
+ * fp32.  Rows no query sees only decay; rows from capacity on take part in the
+ * softmax and are not stored.  out may be mass (accumulation in place), else they
+ * must not overlap; with decay 0 mass is not read and may be null.  Every key is
+ * summed in a fixed order: the same call gives the same bits.  Workspace of a single
+ * token: about a quarter of a 16-bit K cache of W * max_blocks_per_seq pages, at most
+ * 1 GiB of scores. */
+DVATTN_API size_t dvattn_paged_key_mass_workspace_size(int dtype, const dvattn_shape* shape, int device);
+DVATTN_API dvattn_status dvattn_paged_key_mass(int dtype, float* out, const float* mass, float decay,
+                                    long long capacity, float scale, const int* locations, const void* queries,
+                                    const float* cosines, const float* sines, const int* fragment_lengths,
+                                    const void* k_cache, const int* block_tables, const dvattn_shape* shape,
+                                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- which rows of a cache to keep --------------------------------------------------
+ * rows [W,Hkv,budget] i32 from mass [W,Hkv,capacity] f32: of the n = lengths[w] rows
+ * from stream row first_rows[w] on (n at least 0 and at most capacity -
+ * first_rows[w]; none for a negative first row), relative to it and ascending: all
+ * of them if n <= budget, followed by -1; else the first keep_first, the last
+ * keep_last and the budget - keep_first - keep_last of greatest mass among the
+ * others (ties to the lowest row; NaN weighs least).  keep_first + keep_last <=
+ * budget; capacity <= 2^30. */
+DVATTN_API dvattn_status dvattn_kv_select(int* rows, const float* mass, const int* first_rows, const int* lengths,
+                               long long capacity, int W, int Hkv, int budget, int keep_first, int keep_last,
+                               void* stream);
+
+/* ---- moving kept rows together --------------------------------------------------------
+ * In place, for every sequence, KV head and i < N with rows[w,h,i] >= i (and <
+ * lengths[w] where lengths is given):
+ *   cache row (stream row first_rows[w] + i) = what row first_rows[w] + rows[w,h,i] held
+ * in K and V; other rows are left as they are.  rows [W,row_heads,N] i32, row_heads
+ * Hkv or 1 (the same rows for every KV head: a tree's accepted path, with first_rows =
+ * tree_rows).  Entries may come in any order and more than once; one below its place,
+ * past the range, or whose source or destination lies on no valid page moves nothing.
+ * With mass [W,Hkv,capacity] f32 (needs lengths) its entries move alike, and those of
+ * the rows first_rows[w] + i, i < lengths[w], that nothing moves into become 0.  Uses
+ * shape fields W, Hkv, E, Ev, block_size, max_blocks_per_seq, num_blocks and the
+ * layout's cache strides.  The pages of the rows moved must each be named once in
+ * block_tables (pages shared by sequences or segments lie before first_rows). */
+DVATTN_API dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, const int* block_tables,
+                                      const int* rows, int row_heads, int N, const int* first_rows,
+                                      const int* lengths, float* mass, long long capacity,
+                                      const dvattn_shape* shape, const dvattn_kv_layout* layout, void* stream);
 
 #ifdef __cplusplus
 }
