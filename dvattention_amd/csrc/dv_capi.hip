@@ -823,8 +823,10 @@ dvattn_status dvattn_tree_metadata(int* locations, float* cosines, float* sines,
         return fail(DVATTN_ERR_UNSUPPORTED, "at most %d drafted nodes and %d views (S=%d, F=%d)", dv::kMaxTreeNodes,
                     dv::kMaxTreeViews, S, F);
     if ((long long)F * W * S == 0) return ok();
-    if ((long long)F * W * S >= (1ll << 31))
-        return fail(DVATTN_ERR_UNSUPPORTED, "%lld (view, node) pairs in one call exceed 2^31", (long long)F * W * S);
+    // a launch holds 2^24 blocks of 256 threads: one per (view, sequence) and 64 nodes
+    if ((long long)F * W * ((S + 63) / 64) >= (1ll << 24))
+        return fail(DVATTN_ERR_UNSUPPORTED, "%lld (view, sequence) pairs of %d nodes exceed one launch",
+                    (long long)F * W, S);
     if (!locations || !tree_views || !tree_rows || !fragment_lengths || !order || !parents ||
         (rotary_dim > 0 && (!cosines || !sines || !inv_freq)))
         return fail(DVATTN_ERR_INVALID, "null pointer");
@@ -949,9 +951,12 @@ dvattn_status dvattn_paged_key_mass(int dtype, float* out, const float* mass, fl
     if ((st = check_pages(s)) != DVATTN_OK) return st;
     const long long max_rows = (long long)s->max_blocks_per_seq * s->block_size;
     const long long rows = max_rows > capacity ? max_rows : capacity;
-    // one block per 128 rows at least
-    if ((long long)s->W * s->Hkv * (rows / 128 + 1) >= (1ll << 31) ||
-        (long long)s->W * s->Hkv * s->S >= (1ll << 31))
+    if (max_rows >= (1ll << 32))
+        return fail(DVATTN_ERR_UNSUPPORTED, "block tables of %lld rows exceed 2^32", max_rows);
+    // a launch holds 2^24 blocks of 256 threads: one per 128 rows at least, two per token's query operand
+    const long long wh = (long long)s->W * s->Hkv;
+    if (wh >= (1ll << 24) || wh * (rows / 128 + 1) >= (1ll << 24) ||
+        wh * s->S * (s->F > 0 ? s->F : 1) >= (1ll << 23))
         return fail(DVATTN_ERR_UNSUPPORTED, "W=%d, Hkv=%d, S=%d, %lld rows: too many blocks for one launch", s->W,
                     s->Hkv, s->S, rows);
     if (!out || (s->S > 0 && !queries) || (decay != 0.0f && !mass))
@@ -1009,8 +1014,8 @@ dvattn_status dvattn_kv_select(int* rows, const float* mass, const int* first_ro
                     budget);
     if (capacity > (1ll << 30)) return fail(DVATTN_ERR_UNSUPPORTED, "capacity %lld exceeds 2^30 rows", capacity);
     if (budget > (1 << 30)) return fail(DVATTN_ERR_UNSUPPORTED, "budget %d exceeds 2^30 rows", budget);
-    if ((long long)W * Hkv >= (1ll << 31))
-        return fail(DVATTN_ERR_UNSUPPORTED, "%lld (sequence, KV head) pairs exceed 2^31", (long long)W * Hkv);
+    if ((long long)W * Hkv >= (1ll << 22))  // blocks of 1024 threads of one launch
+        return fail(DVATTN_ERR_UNSUPPORTED, "%lld (sequence, KV head) pairs exceed 2^22", (long long)W * Hkv);
     if ((long long)W * Hkv == 0 || budget == 0) return ok();
     if (!rows || !first_rows || !lengths || (capacity > 0 && !mass)) return fail(DVATTN_ERR_INVALID, "null pointer");
     const dvattn_status st = check_aligned({{rows, "rows", 4}, {mass, "mass", 4}, {first_rows, "first_rows", 4},
@@ -1049,8 +1054,9 @@ dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, c
         return fail(DVATTN_ERR_INVALID, "max_blocks_per_seq / num_blocks must be >= 0");
     if (s->E > 8192 || s->Ev > 8192)
         return fail(DVATTN_ERR_UNSUPPORTED, "head dims up to 8192 (E=%d, Ev=%d)", s->E, s->Ev);
-    if ((long long)s->W * s->Hkv >= (1ll << 24) || N > (1 << 30))
-        return fail(DVATTN_ERR_UNSUPPORTED, "W * Hkv = %lld and N = %d: at most 2^24 and 2^30",
+    // blocks of 1024 threads of one launch: up to 65 per (sequence, KV head)
+    if ((long long)s->W * s->Hkv >= (1ll << 15) || N > (1 << 30))
+        return fail(DVATTN_ERR_UNSUPPORTED, "W * Hkv = %lld and N = %d: below 2^15 and at most 2^30",
                     (long long)s->W * s->Hkv, N);
     if (mass && !lengths) return fail(DVATTN_ERR_INVALID, "mass needs lengths");
     if (N == 0 && !mass) return ok();
@@ -1083,6 +1089,7 @@ dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, c
     p.E = s->E;
     p.Ev = s->Ev;
     p.bs = s->block_size;
+    p.bs_shift = log2_exact(s->block_size);
     p.maxB = s->max_blocks_per_seq;
     p.nblocks = s->num_blocks;
     const hipError_t e = dv::launch_kv_compact(dtype, p, (hipStream_t)stream);

@@ -176,6 +176,7 @@ struct MassParams {
     float* lse;               // minus the base-2 log-sum-exp of each (sequence, KV head, token, head) (S > 1)
     float* scores;            // base-2 scores, tile by tile (S = 1)
     int nchunks;              // workgroups along the keys of one (sequence, KV head)
+    int units;                // units of keys per wave (S = 1)
     int s0, ns;               // tokens of this launch
 };
 
@@ -200,7 +201,7 @@ struct CompactParams {
     float* mass;              // [W, Hkv, C] or null
     long long C;
     int W, Hkv, heads, N, E, Ev;
-    int bs, maxB, nblocks;
+    int bs, bs_shift, maxB, nblocks;
     int slices;               // column slices of a row, a workgroup each
 };
 

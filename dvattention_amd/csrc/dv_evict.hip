@@ -11,8 +11,13 @@ typedef __attribute__((address_space(1))) u32x4 gw_u32x4;
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
-constexpr int kDigit = 11;  // bits of a weight resolved per pass: 11 + 11 + 10
-constexpr int kBins = 1 << kDigit;
+// Bits of a weight resolved per pass.  The first digit is the widest: sign, exponent
+// and four bits of the fraction spread weights of a few octaves over a hundred bins and
+// more, where lanes of a wave rarely meet in one (an LDS atomic serialises those).
+constexpr int kDigit0 = 13, kDigit1 = 10, kDigit2 = 9;
+static_assert(kDigit0 + kDigit1 + kDigit2 == 32, "all bits of a weight");
+constexpr int kBins = 1 << kDigit0;
+constexpr int kSelHeld = 32;  // rows per thread held in registers
 
 // Weights as integers in their order; a NaN is lighter than any number.
 __device__ inline uint32_t order_of(float f) {
@@ -22,8 +27,8 @@ __device__ inline uint32_t order_of(float f) {
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sum of v over the block's threads, and the total.
-__device__ inline int block_excl(int v, int* s_wave, int& total) {
+// Exclusive sum of v over the block's threads.
+__device__ inline int block_excl(int v, int* s_wave) {
     const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
     int incl = v;
 #pragma unroll
@@ -33,15 +38,9 @@ __device__ inline int block_excl(int v, int* s_wave, int& total) {
     }
     if (lane == 63) s_wave[wv] = incl;
     __syncthreads();
-    int before = 0, all = 0;
+    int before = 0;
 #pragma unroll
-    for (int i = 0; i < kSelWaves; ++i) {
-        const int x = s_wave[i];
-        before += i < wv ? x : 0;
-        all += x;
-    }
-    __syncthreads();
-    total = all;
+    for (int i = 0; i < kSelWaves; ++i) before += i < wv ? s_wave[i] : 0;
     return before + incl - v;
 }
 
@@ -51,14 +50,17 @@ __device__ inline int block_excl(int v, int* s_wave, int& total) {
 // keep_last stay, and of those between the `need` heaviest: the weight T of the
 // need-th is found digit by digit (a histogram of the digit over the rows that
 // agree with T so far, most significant first), then the rows above T and the first
-// of those equal to it (ties go to the lowest row) are written in ascending order,
-// their places from a running count.  Bound by latency: the weights are read from
-// memory once and then from L2 three more times, each pass a few barriers.
+// of those equal to it (ties go to the lowest row) are written in ascending order.
+// A wave owns a contiguous stretch of rows, so its places follow from one count per
+// wave and a running one inside it, and no pass has a barrier in its loop.  Up to
+// kSelHeld * 1024 rows are read once and held in registers; more are read again
+// (from L2) in each of the five passes.
 __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p) {
     __shared__ int s_hist[kBins];
-    __shared__ int s_wave[kSelWaves];
+    __shared__ int s_wave[kSelWaves], s_gt[kSelWaves], s_eq[kSelWaves];
     __shared__ int s_digit, s_above;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wv = uniform(tid >> 6);
     const int w = blockIdx.x / p.Hkv;
     int* rows = p.rows + (long long)blockIdx.x * p.budget;
     const long long first = p.first[w];
@@ -71,72 +73,121 @@ __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p
         for (int i = tid; i < p.budget; i += kSelThreads) rows[i] = i < n ? i : -1;
         return;
     }
-    const int a = p.keep_first, b = n - p.keep_last;  // rows [a, b) compete
+    const int a = p.keep_first, m = n - p.keep_last - a;  // rows [a, a + m) compete
     const int need = p.budget - p.keep_first - p.keep_last;
-    const float* mass = p.mass + (long long)blockIdx.x * p.C + first;
+    const float* mass = p.mass + (long long)blockIdx.x * p.C + first + a;
     for (int i = tid; i < a; i += kSelThreads) rows[i] = i;
-    for (int i = tid; i < p.keep_last; i += kSelThreads) rows[a + need + i] = b + i;
+    for (int i = tid; i < p.keep_last; i += kSelThreads) rows[a + need + i] = a + m + i;
     if (need == 0) return;
+
+    const int steps = (m + kSelThreads - 1) / kSelThreads;  // of 64 rows per wave
+    const int base = wv * steps * kWave + lane;
+    const bool held = steps <= kSelHeld;
+    uint32_t key[kSelHeld];
+    if (held) {
+#pragma unroll
+        for (int j = 0; j < kSelHeld; ++j) {
+            key[j] = 0u;
+            if (j < steps && base + j * kWave < m) key[j] = __float_as_uint(mass[base + j * kWave]);
+        }
+#pragma unroll
+        for (int j = 0; j < kSelHeld; ++j) {
+            if (j >= steps) break;
+            key[j] = order_of(__uint_as_float(key[j]));
+        }
+    }
+    // fn(weight, whether the lane has a row, the row) for the wave's rows in order
+    auto visit = [&](auto&& fn) {
+        if (held) {
+#pragma unroll
+            for (int j = 0; j < kSelHeld; ++j) {
+                if (j >= steps) break;
+                fn(key[j], base + j * kWave < m, base + j * kWave);
+            }
+        } else {
+            for (int j0 = 0; j0 < steps; j0 += 8) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = base + (j0 + j) * kWave;
+                    x[j] = 0.0f;
+                    if (j0 + j < steps && i < m) x[j] = mass[i];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = base + (j0 + j) * kWave;
+                    if (j0 + j < steps) fn(order_of(x[j]), i < m, i);
+                }
+            }
+        }
+    };
 
     uint32_t top = 0;   // T's digits so far
     int want = need;    // of the rows that agree with them, how many stay
     for (int pass = 0; pass < 3; ++pass) {
-        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-        const uint32_t known = pass == 0 ? 0u : pass == 1 ? 0xffe00000u : 0xfffffc00u;
-        const uint32_t mask = pass == 2 ? 0x3ffu : 0x7ffu;
-        for (int i = tid; i < kBins; i += kSelThreads) s_hist[i] = 0;
+        const int bits = pass == 0 ? kDigit0 : pass == 1 ? kDigit1 : kDigit2;
+        const int shift = pass == 0 ? kDigit1 + kDigit2 : pass == 1 ? kDigit2 : 0;
+        const uint32_t known = pass == 0 ? 0u : ~0u << (shift + bits);
+        const int bins = 1 << bits;
+        for (int i = tid; i < bins; i += kSelThreads) s_hist[i] = 0;
         __syncthreads();
-        for (int i0 = a; i0 < b; i0 += kSelThreads) {
-            const int i = i0 + tid;
-            const bool in = i < b;
-            const uint32_t u = order_of(in ? mass[i] : 0.0f);
+        visit([&](uint32_t u, bool in, int) {
             const bool match = in && (u & known) == top;
-            const int dg = (int)((u >> shift) & mask);
-            // lanes of one digit count together (weights of one power of two, or all zero)
+            const int dg = (int)((u >> shift) & (uint32_t)(bins - 1));
+            // lanes of the first lane's digit count together (all weights zero, say)
             const uint64_t live = ballot(match);
             if (live) {
                 const int lead = __builtin_amdgcn_readlane(dg, __builtin_ctzll(live));
                 const uint64_t same = ballot(match && dg == lead);
-                if ((tid & 63) == __builtin_ctzll(live)) atomicAdd(&s_hist[lead], __builtin_popcountll(same));
+                if (lane == __builtin_ctzll(live)) atomicAdd(&s_hist[lead], __builtin_popcountll(same));
                 if (match && dg != lead) atomicAdd(&s_hist[dg], 1);
             }
-        }
+        });
         __syncthreads();
-        // the digit whose rows hold the want-th heaviest: thread t owns bins 2t, 2t + 1
+        // the digit whose rows hold the want-th heaviest: a thread owns `per` bins,
         // counted from the heaviest
-        const int h0 = s_hist[kBins - 1 - 2 * tid], h1 = s_hist[kBins - 2 - 2 * tid];
-        int total;
-        const int before = block_excl(h0 + h1, s_wave, total);
-        if (before < want && want <= before + h0) {
-            s_digit = kBins - 1 - 2 * tid;
+        const int per = bins > kSelThreads ? bins / kSelThreads : 1;
+        const int b0 = bins - 1 - per * tid;  // negative: none
+        int sum = 0;
+        for (int i = 0; i < per; ++i) sum += b0 - i >= 0 ? s_hist[b0 - i] : 0;
+        int before = block_excl(sum, s_wave);
+        if (before < want && want <= before + sum) {
+            int i = 0;
+            while (before + s_hist[b0 - i] < want) before += s_hist[b0 - i++];
+            s_digit = b0 - i;
             s_above = before;
-        } else if (before + h0 < want && want <= before + h0 + h1) {
-            s_digit = kBins - 2 - 2 * tid;
-            s_above = before + h0;
         }
         __syncthreads();
         top |= (uint32_t)s_digit << shift;
         want -= s_above;
     }
 
-    // rows above T, and the first `want` of those equal to it
-    int out = a, ties = 0;
-    for (int i0 = a; i0 < b; i0 += kSelThreads) {
-        const int i = i0 + tid;
-        const uint32_t u = i < b ? order_of(mass[i]) : 0u;
-        const bool gt = i < b && u > top, eq = i < b && u == top;
-        // both counts in one scan: at most 1024 of each
-        int total;
-        const int e = block_excl((gt ? 1 : 0) | (eq ? 1 << 16 : 0), s_wave, total);
-        const int eqs = ties + (e >> 16);              // equal rows before this one
-        const int eq_kept = eqs < want ? eqs : want;   // of them, kept
-        const int gts = e & 0xffff;
-        const int ties_kept0 = ties < want ? ties : want;
-        if (gt || (eq && eqs < want)) rows[out + gts + (eq_kept - ties_kept0)] = i;
-        const int ties1 = ties + (total >> 16);
-        out += (total & 0xffff) + ((ties1 < want ? ties1 : want) - ties_kept0);
-        ties = ties1;
+    // rows above T and equal to it, per wave and then before each wave
+    int gts = 0, eqs = 0;
+    visit([&](uint32_t u, bool in, int) {
+        gts += __builtin_popcountll(ballot(in && u > top));
+        eqs += __builtin_popcountll(ballot(in && u == top));
+    });
+    if (lane == 0) {
+        s_gt[wv] = gts;
+        s_eq[wv] = eqs;
     }
+    __syncthreads();
+    gts = eqs = 0;
+    for (int i = 0; i < wv; ++i) {
+        gts += s_gt[i];
+        eqs += s_eq[i];
+    }
+    int* out = rows + a;
+    const uint64_t below = (1ull << lane) - 1ull;
+    visit([&](uint32_t u, bool in, int i) {
+        const uint64_t gt = ballot(in && u > top), eq = ballot(in && u == top);
+        const int e = eqs + __builtin_popcountll(eq & below);  // equal rows before this one, the first `want` kept
+        const int at = gts + __builtin_popcountll(gt & below) + (e < want ? e : want);
+        if (in && (u > top || (u == top && e < want))) out[at] = a + i;
+        gts += __builtin_popcountll(gt);
+        eqs += __builtin_popcountll(eq);
+    });
 }
 
 hipError_t launch_kv_select(const SelectParams& p, hipStream_t stream) {
@@ -159,18 +210,27 @@ hipError_t launch_kv_select(const SelectParams& p, hipStream_t stream) {
 // of those also cuts the rows into column slices, which move independently.
 namespace {
 constexpr int kMoveThreads = 1024;
-constexpr int kMoveRows = 8;  // rows per thread and batch
+constexpr int kMoveRows = 8;                                    // rows per thread and batch
+constexpr int kMoveBatch = kMoveThreads;                        // rows per batch, at most
+constexpr int kMoveSide = kMoveBatch / kMoveRows;               // rows side by side, at most
+struct Move {
+    long long src, dst;  // byte offsets of a row's head; src < 0: nothing to move
+};
 }  // namespace
 
+// Where the rows of a batch lie is worked out by one thread per row (into LDS), for
+// the next batch while this one's rows are on their way; the rows of the next batch
+// are asked for before this one's are written.
 template <typename VT>
 __global__ __launch_bounds__(kMoveThreads) void dv_kv_compact(const CompactParams p, int k_vecs, int v_vecs,
-                                                              int vec_elems, int es) {
+                                                              int vec_bytes, int es) {
+    __shared__ Move s_move[3][kMoveBatch];  // three: a batch's is read until its rows are written
     const int tid = threadIdx.x;
     const int parts = 2 * p.slices + (p.mass ? 1 : 0);
     const int part = blockIdx.x % parts;
     const int wh = blockIdx.x / parts;
     const int w = wh / p.Hkv, h = wh - w * p.Hkv;
-    const long long first = p.first[w];
+    const int first = p.first[w];
     if (first < 0) return;
     const int limit = p.lengths ? p.lengths[w] : 0x7fffffff;  // rows of the range
     const int* rows = p.rows + ((long long)w * p.heads + (p.heads > 1 ? h : 0)) * p.N;
@@ -204,49 +264,79 @@ __global__ __launch_bounds__(kMoveThreads) void dv_kv_compact(const CompactParam
     const bool is_v = part >= p.slices;
     const int slice = is_v ? part - p.slices : part;
     const int vecs = is_v ? v_vecs : k_vecs;  // vectors of a row
-    if (vecs == 0) return;
-    const long long* st = is_v ? p.vcs : p.kcs;
-    unsigned char* cache = reinterpret_cast<unsigned char*>(is_v ? p.vc : p.kc) + (long long)h * st[2] * es;
     const int c0 = vecs * slice / p.slices, c1 = vecs * (slice + 1) / p.slices;
     const int lanes = c1 - c0;  // vectors of this slice; the launcher keeps it at most kMoveThreads
     if (lanes == 0) return;
-    const int per = kMoveThreads / lanes;  // rows moved side by side
+    const long long s0 = is_v ? p.vcs[0] : p.kcs[0], s1 = is_v ? p.vcs[1] : p.kcs[1];
+    unsigned char* cache = reinterpret_cast<unsigned char*>(is_v ? p.vc : p.kc) +
+                           (long long)h * (is_v ? p.vcs[2] : p.kcs[2]) * es;
+    const int fit = kMoveThreads / lanes;
+    const int per = fit < kMoveSide ? fit : kMoveSide;  // rows moved side by side
     const int lane = tid % lanes, sub = tid / lanes;
     const bool active = sub < per;
-    const long long col = (long long)(c0 + lane) * vec_elems;
+    unsigned char* col = cache + (long long)(c0 + lane) * vec_bytes;
     const int* bt = p.bt + (long long)w * p.maxB;
-    // address of a row's vector, null where it lies on no valid page
-    auto at = [&](long long row) -> VT* {
-        const long long lp = row / p.bs;
-        if (lp >= p.maxB) return nullptr;
-        const int page = bt[lp];
-        if (page < 0 || page >= p.nblocks) return nullptr;
-        return reinterpret_cast<VT*>(cache + (page * st[0] + (row - lp * p.bs) * st[1] + col) * es);
-    };
     const int batch = per * kMoveRows;
-    for (int i0 = 0; i0 < p.N; i0 += batch) {
-        VT x[kMoveRows];
-        VT* dst[kMoveRows];
-#pragma unroll
-        for (int u = 0; u < kMoveRows; ++u) {
-            const int i = i0 + u * per + sub;
-            dst[u] = nullptr;
-            if (active && i < p.N) {
-                const int r = rows[i];
-                if (r > i && r < limit) {  // r == i: the row is there already
-                    const VT* src = at(first + r);
-                    if (src) {
-                        dst[u] = at(first + i);
-                        if (dst[u]) x[u] = *src;
-                    }
-                }
+
+    // byte offset of a stream row (below 2^32: two ints), negative on no valid page
+    auto at = [&](uint32_t row) -> long long {
+        uint32_t lp, in;
+        if (p.bs_shift >= 0) {
+            lp = row >> p.bs_shift;
+            in = row & ((1u << p.bs_shift) - 1u);
+        } else {
+            lp = row / (uint32_t)p.bs;
+            in = row - lp * (uint32_t)p.bs;
+        }
+        if (lp >= (uint32_t)p.maxB) return -1;
+        const int page = bt[lp];
+        if (page < 0 || page >= p.nblocks) return -1;
+        return (page * s0 + (long long)in * s1) * es;
+    };
+    auto plan = [&](int i0, Move* to) {
+        if (tid >= batch) return;
+        const int i = i0 + tid;
+        Move m{-1, -1};
+        if (i < p.N) {
+            const int r = rows[i];
+            if (r > i && r < limit) {  // r == i: the row is there already
+                m.dst = at((uint32_t)first + (uint32_t)i);
+                if (m.dst >= 0) m.src = at((uint32_t)first + (uint32_t)r);
             }
         }
+        to[tid] = m;
+    };
+    auto fetch = [&](const Move* from, VT (&x)[kMoveRows]) {
+        if (!active) return;
+#pragma unroll
+        for (int u = 0; u < kMoveRows; ++u) {
+            const long long src = from[u * per + sub].src;
+            if (src >= 0) x[u] = *reinterpret_cast<const VT*>(col + src);
+        }
+    };
+    VT x[2][kMoveRows];
+    plan(0, s_move[0]);
+    __syncthreads();
+    fetch(s_move[0], x[0]);
+    int t = 0;  // the batch's table
+    auto step = [&](int i0, const int cur) {
+        const bool more = i0 + batch < p.N;
+        const Move* now = s_move[t];
+        t = t == 2 ? 0 : t + 1;
+        if (more) plan(i0 + batch, s_move[t]);
         wait_vmcnt<0>();  // this thread's rows are here before any thread writes one
         __syncthreads();
+        if (more) fetch(s_move[t], x[cur ^ 1]);
+        if (!active) return;
 #pragma unroll
-        for (int u = 0; u < kMoveRows; ++u)
-            if (dst[u]) *dst[u] = x[u];
+        for (int u = 0; u < kMoveRows; ++u) {
+            const Move m = now[u * per + sub];
+            if (m.src >= 0) *reinterpret_cast<VT*>(col + m.dst) = x[cur][u];
+        }
+    };
+    for (int i0 = 0; i0 < p.N; i0 += 2 * batch) {
+        step(i0, 0);
+        if (i0 + batch < p.N) step(i0 + batch, 1);
     }
 }
 
@@ -267,9 +357,9 @@ hipError_t launch_kv_compact(int dtype, const CompactParams& base, hipStream_t s
     while ((widest + slices - 1) / slices > kMoveThreads) slices *= 2;
     p.slices = slices;
     const dim3 grid((unsigned)(p.W * p.Hkv * (2 * slices + (p.mass ? 1 : 0)))), block(kMoveThreads);
-    if (vec) hipLaunchKernelGGL(dv_kv_compact<u32x4>, grid, block, 0, stream, p, kv, vv, elems, es);
-    else if (es == 4) hipLaunchKernelGGL(dv_kv_compact<uint32_t>, grid, block, 0, stream, p, kv, vv, 1, es);
-    else hipLaunchKernelGGL(dv_kv_compact<uint16_t>, grid, block, 0, stream, p, kv, vv, 1, es);
+    if (vec) hipLaunchKernelGGL(dv_kv_compact<u32x4>, grid, block, 0, stream, p, kv, vv, 16, es);
+    else if (es == 4) hipLaunchKernelGGL(dv_kv_compact<uint32_t>, grid, block, 0, stream, p, kv, vv, es, es);
+    else hipLaunchKernelGGL(dv_kv_compact<uint16_t>, grid, block, 0, stream, p, kv, vv, es, es);
     return hipGetLastError();
 }
 

@@ -43,12 +43,15 @@ struct Run8 {
     }
 };
 
-constexpr int kTreeBatch = 8;  // ancestors whose rows are loaded together
+// Ancestors, and committed pieces, whose rows are loaded together.  Four: a node of
+// depth 6 takes two rounds, and eight would hold twice the registers, half as many
+// blocks per CU for a kernel that waits for memory.
+constexpr int kTreeBatch = 4;
 
 // Block (segment, node of the group): thread t -> head t / 16, dims [(t % 16) * 8, +8).
-// LDS: the sequence's parents, then the node's ancestors as cache rows.  An absent
-// node (its path leaves the tree at an entry that is no earlier node and not -1)
-// writes zeros.
+// LDS: the sequence's parents, then the node's ancestors as cache rows, which the first
+// wave looks up while the others join the committed pieces.  An absent node (its
+// path leaves the tree at an entry that is no earlier node and not -1) writes zeros.
 template <int DT>
 __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int ntb) {
     using raw = typename Tr<DT>::raw;
@@ -66,77 +69,65 @@ __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int n
     int* s_par = s_tree;
     int* s_row = s_tree + p.S;
 
+    for (int i = tid; i < p.S; i += 256) s_par[i] = p.parents[(long long)w * p.S + i];
     const int base = p.dir[2 * sg], cnt = p.dir[2 * sg + 1];
     const int tv = p.tree_views[w], first = p.tree_rows[w];
-    for (int i = tid; i < p.S; i += 256) s_par[i] = p.parents[(long long)w * p.S + i];
-
-    // the view of the drafted rows: its first stream row, length and this node's location
     const bool has_view = tv >= 0 && tv < p.F;
-    long long off = 0, len = 0;
-    int loc = -1;
-    float q[8];
-    if (has_view) {
-        for (int f = 0; f < tv; ++f) off += p.fl[f];
-        len = p.fl[tv];
-        const long long row = ((long long)tv * p.W + w) * p.S + s;
-        loc = p.loc[row];
-        raw qr[8];
-        const raw* qrow = reinterpret_cast<const raw*>(p.q) + (((long long)w * p.Hq + h) * p.S + s) * kHeadDim;
-        rotate_run<DT, 8>(qrow, p.cosv + row * p.R, p.sinv + row * p.R, p.R, d, qr);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) q[e] = Tr<DT>::tof(qr[e]);
-    }
+    const long long row = ((long long)(has_view ? tv : 0) * p.W + w) * p.S + s;
     __syncthreads();
-    if (tid == 0) {
-        // every step goes to an earlier node, so the walk ends
-        int j = s, c = 0;
-        bool there = true;
-        for (;;) {
-            const int up = s_par[j];
-            s_row[c++] = j;
-            if (up == -1) break;
-            if (up < -1 || up >= j) {
-                there = false;
-                break;
+    if (tid < kWave) {
+        int count = 0;
+        if (tid == 0) {
+            // every step goes to an earlier node, so the walk ends
+            int j = s;
+            for (;;) {
+                const int up = s_par[j];
+                s_row[count++] = j;
+                if (up == -1) break;
+                if (up < -1 || up >= j) {
+                    count = -1;
+                    break;
+                }
+                j = up;
             }
-            j = up;
+            s_count = count;
         }
-        s_count = there ? c : -1;
-    }
-    __syncthreads();
-    const int count = s_count;
-    raw* o = reinterpret_cast<raw*>(p.out) + out_row<kRowWS>(p, gr, tb, h) + d;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (count < 0) {
-        store_run8<DT>(o, v);
-        return;
-    }
-    // ancestors -> cache rows (-1: not in the view, on no valid page, or at most the
-    // node's location and so among the committed keys already)
-    for (int i = tid; i < count; i += 256) {
-        const long long pos = (long long)first + s_row[i];
-        const long long l = pos - off;
-        int row = -1;
-        if (has_view && l >= 0 && l < len && l > loc && pos >= 0) {
-            const long long lp = p.bs_shift >= 0 ? pos >> p.bs_shift : pos / p.bs;
-            if (lp < p.maxB) {
-                const int page = p.bt[(long long)w * p.maxB + lp];
-                if (page >= 0 && page < p.nblocks) row = (int)(uint32_t)((long long)page * p.bs + (pos - lp * p.bs));
+        count = uniform(count);
+        // ancestors -> cache rows (-1: not in the view, on no valid page, or at most the
+        // node's location and so among the committed keys already)
+        long long off = 0, len = 0;
+        int loc = -1;
+        if (has_view && count > 0) {
+            for (int f = 0; f < tv; ++f) off += p.fl[f];
+            len = p.fl[tv];
+            loc = p.loc[row];
+        }
+        for (int i = tid; i < count; i += kWave) {
+            const long long pos = (long long)first + s_row[i];
+            const long long l = pos - off;
+            int at = -1;
+            if (l >= 0 && l < len && l > loc && pos >= 0) {
+                const long long lp = p.bs_shift >= 0 ? pos >> p.bs_shift : (long long)((uint32_t)pos / (uint32_t)p.bs);
+                if (lp < p.maxB) {
+                    const int page = p.bt[(long long)w * p.maxB + lp];
+                    if (page >= 0 && page < p.nblocks) at = (int)(uint32_t)((long long)page * p.bs + (pos - lp * p.bs));
+                }
             }
+            s_row[i] = at;
         }
-        s_row[i] = row;
     }
 
     // the committed keys' pieces: running base-2 maximum m, weight sum, weighted sum.
     // A piece that saw no key (-inf) holds nothing, whatever its values are.
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     float m = -DV_INF, wsum = 0.0f;
-    for (int k0 = 0; k0 < cnt; k0 += kMergeBatch) {
-        float lse[kMergeBatch];
-        int kx[kMergeBatch];
-        Run8<kHalfPartials<DT> ? kF16 : kF32> x[kMergeBatch];
+    for (int k0 = 0; k0 < cnt; k0 += kTreeBatch) {
+        float lse[kTreeBatch];
+        int kx[kTreeBatch];
+        Run8<kHalfPartials<DT> ? kF16 : kF32> x[kTreeBatch];
         const int jrow = tb * kGqa + n;
 #pragma unroll
-        for (int i = 0; i < kMergeBatch; ++i) {
+        for (int i = 0; i < kTreeBatch; ++i) {
             const bool in = k0 + i < cnt;
             const float* sp = p.part + (long long)(base + (in ? k0 + i : k0)) * p.slot_floats;
             lse[i] = in ? sp[kTokBlk * kGqa * kHeadDim + jrow] : -DV_INF;
@@ -150,14 +141,14 @@ __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int n
         }
         float bm = m;
 #pragma unroll
-        for (int i = 0; i < kMergeBatch; ++i) bm = fmaxf(bm, lse[i]);
+        for (int i = 0; i < kTreeBatch; ++i) bm = fmaxf(bm, lse[i]);
         const float bz = bm == -DV_INF ? 0.0f : bm;
         const float sc = __builtin_amdgcn_exp2f(m - bz);
         wsum *= sc;
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] *= sc;
 #pragma unroll
-        for (int i = 0; i < kMergeBatch; ++i) {
+        for (int i = 0; i < kTreeBatch; ++i) {
             if (lse[i] == -DV_INF) continue;
             const float wgt = __builtin_amdgcn_exp2f(lse[i] - bz);
             wsum += wgt;
@@ -167,7 +158,22 @@ __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int n
         }
         m = bm;
     }
-    __syncthreads();  // s_row holds cache rows
+    float q[8];
+    if (has_view) {
+        raw qr[8];
+        const raw* qrow = reinterpret_cast<const raw*>(p.q) + (((long long)w * p.Hq + h) * p.S + s) * kHeadDim;
+        rotate_run<DT, 8>(qrow, p.cosv + row * p.R, p.sinv + row * p.R, p.R, d, qr);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = Tr<DT>::tof(qr[e]);
+    }
+    __syncthreads();
+    const int count = s_count;
+    raw* o = reinterpret_cast<raw*>(p.out) + out_row<kRowWS>(p, gr, tb, h) + d;
+    if (count < 0) {
+        const float zero[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        store_run8<DT>(o, zero);
+        return;
+    }
 
     // the ancestors: a row's 16 lanes hold one head's 128 dims
     const raw* kc = reinterpret_cast<const raw*>(p.kc);
@@ -177,12 +183,12 @@ __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int n
         bool in[kTreeBatch];
 #pragma unroll
         for (int i = 0; i < kTreeBatch; ++i) {
-            const int row = uniform(i0 + i < count ? s_row[i0 + i] : -1);
-            in[i] = row != -1;
+            const int at = uniform(i0 + i < count ? s_row[i0 + i] : -1);
+            in[i] = at != -1;
             if (in[i]) {
-                const long long at = ((long long)(uint32_t)row * p.Hkv + hkv) * kHeadDim;
-                kr[i].load(kc + at, d);
-                vr[i].load(vc + at, d);
+                const long long e = ((long long)(uint32_t)at * p.Hkv + hkv) * kHeadDim;
+                kr[i].load(kc + e, d);
+                vr[i].load(vc + e, d);
             }
         }
         float x[kTreeBatch];

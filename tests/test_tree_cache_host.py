@@ -89,6 +89,7 @@ def test_limits_refused(lib):
     assert mass(lib, shape(), capacity=-1) == INVALID
     assert mass(lib, shape(W=1 << 20, S=1), capacity=1 << 20) == UNSUPPORTED and "blocks" in error(lib)
     assert mass(lib, shape(W=1 << 20, S=1 << 12)) == UNSUPPORTED
+    assert mass(lib, shape(max_blocks_per_seq=1 << 30)) == UNSUPPORTED and "2^32" in error(lib)
 
 
 def test_workspace_is_bounded(lib):
@@ -120,7 +121,7 @@ def select(lib, capacity=100, W=2, Hkv=1, budget=8, kf=1, kl=2, rows=P, m=P, fir
     (dict(kf=-1), INVALID, "negative"),
     (dict(budget=-1, kf=0, kl=0), INVALID, "negative"),
     (dict(capacity=(1 << 30) + 1), UNSUPPORTED, "2^30"),
-    (dict(W=1 << 20, Hkv=1 << 12), UNSUPPORTED, "2^31"),
+    (dict(W=1 << 20, Hkv=1 << 12), UNSUPPORTED, "2^22"),
     (dict(rows=None), INVALID, "null"),
     (dict(m=None), INVALID, "null"),
     (dict(first=None), INVALID, "null"),
@@ -166,7 +167,7 @@ def test_compact_refused(lib, kw, status, needle):
 
 @pytest.mark.parametrize("kw,needle", [
     (dict(block_size=0), "block_size"), (dict(num_blocks=-1), "num_blocks"), (dict(E=9000), "8192"),
-    (dict(W=1 << 24), "2^24"), (dict(Ev=-1), "negative"),
+    (dict(W=1 << 15), "2^15"), (dict(Ev=-1), "negative"),
 ])
 def test_compact_shapes_refused(lib, kw, needle):
     assert compact(lib, shape(**kw)) in (INVALID, UNSUPPORTED)
@@ -186,7 +187,7 @@ def meta(lib, F=1, W=2, S=4, R=64, round_dtype=-1, **ptr):
     (dict(round_dtype=5), UNSUPPORTED, "round_dtype"),
     (dict(S=4097), UNSUPPORTED, "drafted nodes"),
     (dict(F=4097), UNSUPPORTED, "views"),
-    (dict(F=4096, W=1 << 10, S=4096), UNSUPPORTED, "2^31"),
+    (dict(F=4096, W=1 << 10, S=4096), UNSUPPORTED, "one launch"),
     (dict(loc=None), INVALID, "null"),
     (dict(parents=None), INVALID, "null"),
     (dict(views=None), INVALID, "null"),
