@@ -77,8 +77,7 @@ def lib() -> ctypes.CDLL:
         L.dvattn_abi_version.restype = _I
         L.dvattn_abi_version.argtypes = []
         for n in ("dvattn_paged_sdpa_workspace_size", "dvattn_varlen_paged_sdpa_workspace_size",
-                  "dvattn_sdpa_workspace_size", "dvattn_tree_paged_sdpa_workspace_size",
-                  "dvattn_paged_key_mass_workspace_size"):
+                  "dvattn_sdpa_workspace_size", "dvattn_tree_paged_sdpa_workspace_size"):
             getattr(L, n).restype = _SZ
             getattr(L, n).argtypes = [_I, _SP, _I]
         L.dvattn_paged_sdpa.restype = _I
@@ -106,6 +105,8 @@ def lib() -> ctypes.CDLL:
         L.dvattn_tree_metadata.argtypes = [_VP] * 9 + [_F, _I, _I, _I, _I, _I, _VP]
         L.dvattn_tree_paged_sdpa.restype = _I
         L.dvattn_tree_paged_sdpa.argtypes = [_I, _VP, _F] + [_VP] * 11 + [_SP, _VP, _SZ, _VP]
+        L.dvattn_paged_key_mass_workspace_size.restype = _SZ
+        L.dvattn_paged_key_mass_workspace_size.argtypes = [_I, _SP, _LL]
         L.dvattn_paged_key_mass.restype = _I
         L.dvattn_paged_key_mass.argtypes = [_I, _VP, _VP, _F, _LL, _F] + [_VP] * 7 + [_SP, _VP, _SZ, _VP]
         L.dvattn_kv_select.restype = _I
@@ -331,7 +332,7 @@ def paged_key_mass(out, mass, decay, scale, locations, queries, cosines, sines, 
     L = lib()
     s = paged_shape(queries, locations, cosines, k_cache, k_cache, block_tables)
     dt = dtype_code(queries.dtype)
-    need = L.dvattn_paged_key_mass_workspace_size(dt, ctypes.byref(s), out.device.index or 0)
+    need = L.dvattn_paged_key_mass_workspace_size(dt, ctypes.byref(s), out.shape[2])
     ws = workspace if workspace is not None and workspace.numel() >= need else _workspace(need, out)
     _check(L.dvattn_paged_key_mass(dt, _ptr(out), _ptr(mass), decay, out.shape[2], scale, _ptr(locations),
                                    _ptr(queries), _ptr(cosines), _ptr(sines), _ptr(fragment_lengths), _ptr(k_cache),

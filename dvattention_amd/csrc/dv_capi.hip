@@ -929,10 +929,10 @@ dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scale, const in
 }
 
 // ---------------------------------------------------------------------------
-size_t dvattn_paged_key_mass_workspace_size(int dtype, const dvattn_shape* s, int device) {
+size_t dvattn_paged_key_mass_workspace_size(int dtype, const dvattn_shape* s, long long capacity) {
     if (!s || !valid_dtype(dtype)) return 0;
     return dv::mass_workspace_bytes(dtype, s->F, s->W, s->S, s->Hkv,
-                                    (long long)s->max_blocks_per_seq * s->block_size, current_device(device));
+                                    (long long)s->max_blocks_per_seq * s->block_size, capacity);
 }
 
 dvattn_status dvattn_paged_key_mass(int dtype, float* out, const float* mass, float decay, long long capacity,
@@ -953,9 +953,9 @@ dvattn_status dvattn_paged_key_mass(int dtype, float* out, const float* mass, fl
     const long long rows = max_rows > capacity ? max_rows : capacity;
     if (max_rows >= (1ll << 32))
         return fail(DVATTN_ERR_UNSUPPORTED, "block tables of %lld rows exceed 2^32", max_rows);
-    // a launch holds 2^24 blocks of 256 threads: one per 128 rows at least, two per token's query operand
+    // a launch holds 2^24 blocks of 256 threads: one per 128 rows and view at least, two per token's query operand
     const long long wh = (long long)s->W * s->Hkv;
-    if (wh >= (1ll << 24) || wh * (rows / 128 + 1) >= (1ll << 24) ||
+    if (wh >= (1ll << 24) || wh * (rows / 128 + s->F + 2) >= (1ll << 24) ||
         wh * s->S * (s->F > 0 ? s->F : 1) >= (1ll << 23))
         return fail(DVATTN_ERR_UNSUPPORTED, "W=%d, Hkv=%d, S=%d, %lld rows: too many blocks for one launch", s->W,
                     s->Hkv, s->S, rows);
@@ -970,7 +970,7 @@ dvattn_status dvattn_paged_key_mass(int dtype, float* out, const float* mass, fl
                              {fragment_lengths, "fragment_lengths", 4}, {cosines, "cosines", 4},
                              {sines, "sines", 4}, {block_tables, "block_tables", 4}})) != DVATTN_OK)
         return st;
-    const size_t need = dvattn_paged_key_mass_workspace_size(dtype, s, -1);
+    const size_t need = dvattn_paged_key_mass_workspace_size(dtype, s, capacity);
     if (workspace_bytes < need || (need && !workspace))
         return fail(DVATTN_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
 

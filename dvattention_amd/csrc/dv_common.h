@@ -177,6 +177,10 @@ struct MassParams {
     float* scores;            // base-2 scores, tile by tile (S = 1)
     int nchunks;              // workgroups along the keys of one (sequence, KV head)
     int units;                // units of keys per wave (S = 1)
+    int* plan_seen;           // S > 1: most keys of view f that a token of sequence w sees, [W, F]
+    int* plan_count;          // parts of sequence w that some token sees, then all its parts, [2, W]
+    int4* plan_list;          // [W, nparts]: view, first row, and the view's first row and length
+    int nparts;               // entries of plan_list per sequence
     int s0, ns;               // tokens of this launch
 };
 
@@ -266,9 +270,9 @@ hipError_t launch_tree_meta(const TreeMetaParams& p, hipStream_t stream);
 // of launch_chunk whose parameters carry parents.
 hipError_t launch_merge_tree(int dtype, const DecodeParams& p, int ntb, hipStream_t stream);
 
-// Key mass: workspace of a call with at most max_rows stream rows per sequence, and
-// its launches.
-size_t mass_workspace_bytes(int dtype, int F, int W, int S, int Hkv, long long max_rows, int device);
+// Key mass: workspace of a call with at most max_rows stream rows and `capacity` outputs
+// per sequence and KV head, and its launches.
+size_t mass_workspace_bytes(int dtype, int F, int W, int S, int Hkv, long long max_rows, long long capacity);
 hipError_t launch_key_mass(int dtype, const MassParams& p, void* workspace, hipStream_t stream);
 
 hipError_t launch_kv_select(const SelectParams& p, hipStream_t stream);

@@ -11,12 +11,7 @@ typedef __attribute__((address_space(1))) u32x4 gw_u32x4;
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
-// Bits of a weight resolved per pass.  The first digit is the widest: sign, exponent
-// and four bits of the fraction spread weights of a few octaves over a hundred bins and
-// more, where lanes of a wave rarely meet in one (an LDS atomic serialises those).
-constexpr int kDigit0 = 13, kDigit1 = 10, kDigit2 = 9;
-static_assert(kDigit0 + kDigit1 + kDigit2 == 32, "all bits of a weight");
-constexpr int kBins = 1 << kDigit0;
+constexpr int kBins = 1 << 13;
 constexpr int kSelHeld = 32;  // rows per thread held in registers
 
 // Weights as integers in their order; a NaN is lighter than any number.
@@ -25,6 +20,11 @@ __device__ inline uint32_t order_of(float f) {
     if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
     if ((u & 0x7fffffffu) == 0u) return 0x80000000u;  // -0 and +0 weigh the same
     return (u >> 31) ? ~u : u | 0x80000000u;
+}
+
+// Set bits of a wave's mask below this lane.
+__device__ inline int lanes_below(uint64_t mask) {
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
 }
 
 // Exclusive sum of v over the block's threads.
@@ -122,26 +122,23 @@ __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p
         }
     };
 
+    // Bits of a weight resolved per pass.  A wide first digit (sign, exponent, four bits of
+    // the fraction) spreads weights of a few octaves over a hundred bins and more,
+    // where lanes of a wave rarely meet in one (an LDS atomic serialises those); clearing
+    // and summing its bins costs a short call more than that saves.
+    const int bits0 = m <= 4096 ? 11 : 13, bits1 = m <= 4096 ? 11 : 10;
     uint32_t top = 0;   // T's digits so far
     int want = need;    // of the rows that agree with them, how many stay
+    int shift = 32;
     for (int pass = 0; pass < 3; ++pass) {
-        const int bits = pass == 0 ? kDigit0 : pass == 1 ? kDigit1 : kDigit2;
-        const int shift = pass == 0 ? kDigit1 + kDigit2 : pass == 1 ? kDigit2 : 0;
-        const uint32_t known = pass == 0 ? 0u : ~0u << (shift + bits);
+        const uint32_t known = pass == 0 ? 0u : ~0u << shift;
+        const int bits = pass == 0 ? bits0 : pass == 1 ? bits1 : shift;
+        shift -= bits;
         const int bins = 1 << bits;
         for (int i = tid; i < bins; i += kSelThreads) s_hist[i] = 0;
         __syncthreads();
         visit([&](uint32_t u, bool in, int) {
-            const bool match = in && (u & known) == top;
-            const int dg = (int)((u >> shift) & (uint32_t)(bins - 1));
-            // lanes of the first lane's digit count together (all weights zero, say)
-            const uint64_t live = ballot(match);
-            if (live) {
-                const int lead = __builtin_amdgcn_readlane(dg, __builtin_ctzll(live));
-                const uint64_t same = ballot(match && dg == lead);
-                if (lane == __builtin_ctzll(live)) atomicAdd(&s_hist[lead], __builtin_popcountll(same));
-                if (match && dg != lead) atomicAdd(&s_hist[dg], 1);
-            }
+            if (in && (u & known) == top) atomicAdd(&s_hist[(u >> shift) & (uint32_t)(bins - 1)], 1);
         });
         __syncthreads();
         // the digit whose rows hold the want-th heaviest: a thread owns `per` bins,
@@ -179,11 +176,10 @@ __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p
         eqs += s_eq[i];
     }
     int* out = rows + a;
-    const uint64_t below = (1ull << lane) - 1ull;
     visit([&](uint32_t u, bool in, int i) {
         const uint64_t gt = ballot(in && u > top), eq = ballot(in && u == top);
-        const int e = eqs + __builtin_popcountll(eq & below);  // equal rows before this one, the first `want` kept
-        const int at = gts + __builtin_popcountll(gt & below) + (e < want ? e : want);
+        const int e = eqs + lanes_below(eq);  // equal rows before this one, the first `want` kept
+        const int at = gts + lanes_below(gt) + (e < want ? e : want);
         if (in && (u > top || (u == top && e < want))) out[at] = a + i;
         gts += __builtin_popcountll(gt);
         eqs += __builtin_popcountll(eq);

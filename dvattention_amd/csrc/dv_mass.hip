@@ -22,6 +22,8 @@
 //    the MFMA's operand order; the second pass computes the scores again (storing
 //    them would cost more bytes than K from two tokens on).  At most kMassTokens
 //    tokens per launch bound the workspace.
+#include <type_traits>
+
 #include "dv_common.h"
 #include "dv_device.h"
 
@@ -31,6 +33,7 @@ namespace {
 
 constexpr int kMassWaves = 4;
 constexpr int kMassThreads = kMassWaves * kWave;
+constexpr int kMaxUnits = 4;        // S = 1: units of keys per wave
 constexpr int kMassTokens = kWave;  // one lane per token holds what it sees
 
 // 16-byte pieces of a K row per lane: lane (g, n) of a 16-key tile holds bytes
@@ -41,20 +44,26 @@ template <int DT> constexpr int kOperandBytes = kPieces<DT> * kWave * 16;  // on
 // 16-key tiles per wave: 64 registers of K
 template <int DT> constexpr int kTilesOf = DT == kF32 ? 2 : 4;
 
-template <int DT>
-__device__ inline f32x4 dot_tile(const u32x4 (&k)[kPieces<DT>], const u32x4 (&q)[kPieces<DT>]) {
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+// Scores of NT tiles: piece by piece over all tiles, so that consecutive MFMAs do not
+// wait for each other's result.
+template <int DT, int NT>
+__device__ inline void dot_tiles(const u32x4 (&k)[NT][kPieces<DT>], const u32x4 (&q)[kPieces<DT>], f32x4 (&x)[NT]) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) x[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int cc = 0; cc < kPieces<DT>; ++cc) {
         if constexpr (DT == kF32) {
-            const f32x4 kf = __builtin_bit_cast(f32x4, k[cc]), qf = __builtin_bit_cast(f32x4, q[cc]);
+            const f32x4 qf = __builtin_bit_cast(f32x4, q[cc]);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s = Tr<kF32>::mma1(kf[j], qf[j], s);
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    x[t] = Tr<kF32>::mma1(__builtin_bit_cast(f32x4, k[t][cc])[j], qf[j], x[t]);
         } else {
-            s = Tr<DT>::mma(k[cc], q[cc], s);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) x[t] = Tr<DT>::mma(k[t][cc], q[cc], x[t]);
         }
     }
-    return s;
 }
 
 __device__ inline int view_len(const MassParams& p, int f) { return p.fl[f] > 0 ? p.fl[f] : 0; }
@@ -135,15 +144,23 @@ __device__ inline void load_keys(const MassParams& p, uint32_t row, u32x4 (&k)[N
     }
 }
 
-// Keys [lo, hi) of NT * 16 as bits.
+// The first n of NT * 16 keys as bits.
 template <int NT>
-__device__ inline uint64_t range_bits(long long lo, long long hi) {
-    lo = lo < 0 ? 0 : lo;
-    hi = hi > NT * 16 ? NT * 16 : hi;
-    if (lo >= hi) return 0;
-    return (~0ull >> (64 - (hi - lo))) << lo;
+__device__ inline uint64_t first_keys(int n) {
+    return n <= 0 ? 0ull : ~0ull >> (64 - n);
 }
 template <int NT> constexpr uint64_t kAllKeys = ~0ull >> (64 - NT * 16);
+
+// Scheduling of a region of `mfmas` matrix instructions and the VALU work of one token:
+// one of the former, six of the latter.
+template <int mfmas>
+__device__ inline void interleave() {
+#pragma unroll
+    for (int i = 0; i < (mfmas < 16 ? mfmas : 16); ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, mfmas < 16 ? 1 : mfmas / 16, 0);  // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);                            // VALU
+    }
+}
 
 // Bits 0-3: keys t * 16 + g * 4 + i of a mask, for this lane's g.
 __device__ inline uint32_t lane_bits(uint64_t mask, int t) {
@@ -233,9 +250,11 @@ __device__ inline float row16_sum(float v) {
 // A weight: invisible keys (-inf) get none, whatever the row's sum is.
 __device__ inline float weight(float x, float nl) { return x == -DV_INF ? 0.0f : __builtin_amdgcn_exp2f(x + nl); }
 
-// out = decay * mass + acc summed over the 16 heads, for a unit's rows below C.
+// out = decay * mass + acc summed over the 16 heads, for a unit's rows below `end` and C.
 template <int NT>
-__device__ inline void store_mass(const MassParams& p, long long wh, long long c0, const f32x4 (&acc)[NT]) {
+__device__ inline void store_mass(const MassParams& p, long long wh, long long c0, long long end,
+                                  const f32x4 (&acc)[NT]) {
+    end = end < p.C ? end : p.C;
     const int lane = threadIdx.x & 63;
     const int g = lane >> 4, n = lane & 15;
     float old[NT];
@@ -243,7 +262,7 @@ __device__ inline void store_mass(const MassParams& p, long long wh, long long c
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         old[t] = 0.0f;
-        if (n < 4 && c + t * 16 < p.C && p.decay != 0.0f) old[t] = p.mass[wh * p.C + c + t * 16] * p.decay;
+        if (n < 4 && c + t * 16 < end && p.decay != 0.0f) old[t] = p.mass[wh * p.C + c + t * 16] * p.decay;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -253,7 +272,7 @@ __device__ inline void store_mass(const MassParams& p, long long wh, long long c
             const float a = row16_sum(acc[t][i]);
             mine = n == i ? a : mine;
         }
-        if (n < 4 && c + t * 16 < p.C) p.out[wh * p.C + c + t * 16] = old[t] + mine;
+        if (n < 4 && c + t * 16 < end) p.out[wh * p.C + c + t * 16] = old[t] + mine;
     }
 }
 
@@ -297,6 +316,12 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_scores(const MassParams 
         off += len;
         if (off <= b0) continue;
         const long long hi = lo + uniform(seen_of(p, f, it.w, p.s0, len));
+        auto row_of = [&](long long c0) {
+            const long long c = c0 + lane;
+            return cache_row(p, it.w, it.hkv, c, lane < kRows && c >= lo && c < hi);
+        };
+        long long c0 = b0 + wv * kRows;
+        uint32_t row = row_of(c0);  // on its way while the query is rotated
         if (!first) __syncthreads();  // the previous view's query is read
         for (int i = threadIdx.x; i < kPieces<DT> * kWave; i += kMassThreads)
             s_q[i] = rotated_piece<DT>(p, f, it.w, it.hkv, p.s0, i);
@@ -304,21 +329,13 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_scores(const MassParams 
         u32x4 q[kPieces<DT>];
 #pragma unroll
         for (int cc = 0; cc < kPieces<DT>; ++cc) q[cc] = s_q[cc * kWave + lane];
-
-        auto row_of = [&](long long c0) {
-            const long long c = c0 + lane;
-            return cache_row(p, it.w, it.hkv, c, lane < kRows && c >= lo && c < hi);
-        };
-        long long c0 = b0 + wv * kRows;
-        uint32_t row = row_of(c0);
         for (int u = 0; u < p.units && c0 < b1; ++u, c0 += kMassWaves * kRows) {
             u32x4 k[NT][kPieces<DT>];
             load_keys<DT, NT>(p, row, k);
             const uint64_t mask = ballot(row != 0xffffffffu);
             row = row_of(c0 + kMassWaves * kRows);
             f32x4 x[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t) x[t] = dot_tile<DT>(k[t], q);
+            dot_tiles<DT, NT>(k, q, x);
             scale_masked<NT>(x, mask, p.l2scale);
             float* dst = p.scores + ((it.wh * p.nchunks * rows + c0) / 16 * kWave + lane) * 4;
             if (first) {
@@ -362,167 +379,305 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_scores(const MassParams 
     }
 }
 
-// Block: the same rows as above.
+// Block: the same rows as above.  All of a wave's scores are on their way before the
+// block's heads' sums are joined.
 template <int NT>
 __global__ __launch_bounds__(kMassThreads) void dv_mass_apply_scores(const MassParams p) {
     __shared__ float2 s_pair[kMassThreads];
     constexpr int kRows = NT * 16;
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
     const Item it = item_of(p);
     const long long end = visible_end(p, it.w);
     const long long rows = (long long)kMassWaves * kRows * p.units;
-    long long c0 = it.chunk * rows + wv * kRows;
-    float nl = 0.0f;
-    if (it.chunk * rows < end)
-        nl = joined_lse(reinterpret_cast<const float2*>(p.part) + it.wh * p.nchunks * kGqa, (end + rows - 1) / rows,
-                        s_pair);
-    for (int u = 0; u < p.units; ++u, c0 += kMassWaves * kRows) {
-        if (c0 >= end) {
-            store_decayed(p, it.wh, c0, kRows);
+    const long long c0 = it.chunk * rows + wv * kRows;
+    if (it.chunk * rows >= end) {
+        for (int u = 0; u < p.units; ++u) store_decayed(p, it.wh, c0 + u * kMassWaves * kRows, kRows);
+        return;
+    }
+    const float* src = p.scores + ((it.wh * p.nchunks * rows + c0) / 16 * kWave + lane) * 4;
+    f32x4 x[kMaxUnits][NT];
+#pragma unroll
+    for (int u = 0; u < kMaxUnits; ++u)
+        if (u < p.units && c0 + u * kMassWaves * kRows < end)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) x[u][t] = ld16f_nt(src + ((long long)u * kMassWaves * NT + t) * kWave * 4);
+    const float nl = joined_lse(reinterpret_cast<const float2*>(p.part) + it.wh * p.nchunks * kGqa,
+                                (end + rows - 1) / rows, s_pair);
+#pragma unroll
+    for (int u = 0; u < kMaxUnits; ++u) {
+        if (u >= p.units) break;
+        const long long c = c0 + u * kMassWaves * kRows;
+        if (c >= end) {
+            store_decayed(p, it.wh, c, kRows);
             continue;
         }
-        const float* src = p.scores + ((it.wh * p.nchunks * rows + c0) / 16 * kWave + lane) * 4;
-        f32x4 x[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) x[t] = ld16f(src + t * kWave * 4);
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[t][i] = weight(x[t][i], nl);
-        store_mass<NT>(p, it.wh, c0, x);
+            for (int i = 0; i < 4; ++i) x[u][t][i] = weight(x[u][t][i], nl);
+        store_mass<NT>(p, it.wh, c, p.C, x[u]);
     }
 }
 
-// S > 1: the query operands, [F, W, Hkv, S] of kOperandBytes each; a thread per 16 bytes.
+// S > 1: the query operands, [F, W, Hkv, S] of kOperandBytes each, a thread per 16
+// bytes; and, in the first W blocks, the plan.  A part is what one block of the
+// kernels below takes: up to part_rows rows of one view (the rows behind the last view
+// and below the capacity count as one more view, F).  The list of a sequence's parts
+// has those that some token sees in front, and they get the first blocks of the
+// launches that follow.  Both matter where a launch is about one block per CU: parts
+// cut across the views' border took twice as long as the others (four sequences of
+// two views, 4000 keys, 32 tokens, 4 KV heads: 52 us, one view 26), and blocks with
+// nothing to do, strewn among the others, drew the blocks after them to the CUs that
+// had them.
 template <int DT>
-__global__ __launch_bounds__(kMassThreads) void dv_mass_rotate(const MassParams p, long long n) {
-    const long long i = (long long)blockIdx.x * kMassThreads + threadIdx.x;
-    if (i >= n) return;
-    constexpr int kPer = kPieces<DT> * kWave;
-    const long long op = i / kPer;
-    const int piece = (int)(i - op * kPer);
-    const int s = (int)(op % p.S);
-    const long long r = op / p.S;
-    const int hkv = (int)(r % p.Hkv);
-    const long long fw = r / p.Hkv;
-    reinterpret_cast<u32x4*>(p.rq)[i] =
-        rotated_piece<DT>(p, (int)(fw / p.W), (int)(fw % p.W), hkv, s, piece);
+__global__ __launch_bounds__(kMassThreads) void dv_mass_prepare(const MassParams p, long long n, int part_rows) {
+    if (blockIdx.x >= (unsigned)p.W) {
+        const long long i = (long long)(blockIdx.x - p.W) * kMassThreads + threadIdx.x;
+        if (i >= n) return;
+        constexpr int kPer = kPieces<DT> * kWave;
+        const long long op = i / kPer;
+        const int piece = (int)(i - op * kPer);
+        const int s = (int)(op % p.S);
+        const long long r = op / p.S;
+        const int hkv = (int)(r % p.Hkv);
+        const long long fw = r / p.Hkv;
+        reinterpret_cast<u32x4*>(p.rq)[i] = rotated_piece<DT>(p, (int)(fw / p.W), (int)(fw % p.W), hkv, s, piece);
+        return;
+    }
+    const int w = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
+    int* seen = p.plan_seen + (long long)w * p.F;
+    for (int f = wv; f < p.F; f += kMassWaves) {
+        const int len = view_len(p, f);
+        int best = 0;
+        for (int s = lane; s < p.S; s += kWave) {
+            const int v = seen_of(p, f, w, s, len);
+            best = v > best ? v : best;
+        }
+        best = lanes_max(best);
+        if (lane == 0) seen[f] = best;
+    }
+    __syncthreads();
+    const long long rows = (long long)p.maxB * p.bs;       // keys lie below
+    const long long limit = rows > p.C ? rows : p.C;       // and outputs
+    int4* list = p.plan_list + (long long)w * p.nparts;
+    // seen parts of the views before f, and other parts; the others go behind all seen ones
+    auto seen_parts = [&](int f, long long off) {
+        const long long left = rows - off;
+        const long long keys = seen[f] < left ? seen[f] : left;
+        return keys > 0 ? (int)((keys + part_rows - 1) / part_rows) : 0;
+    };
+    int count = 0;
+    long long off = 0;
+    for (int f = 0; f < p.F; ++f) {
+        count += seen_parts(f, off);
+        off += view_len(p, f);
+    }
+    int on = 0, idle = count;
+    off = 0;
+    for (int f = 0; f <= p.F && off < limit; ++f) {
+        const long long len = f < p.F ? view_len(p, f) : limit - off;
+        const long long here = len < limit - off ? len : limit - off;
+        const int all = (int)((here + part_rows - 1) / part_rows);
+        const int a = f < p.F ? seen_parts(f, off) : 0;
+        for (int k = tid; k < all; k += kMassThreads)
+            list[k < a ? on + k : idle + k - a] =
+                make_int4(f, (int)(uint32_t)(off + (long long)k * part_rows), (int)(uint32_t)off, (int)len);
+        on += a;
+        idle += all - a;
+        off += len;
+    }
+    if (tid == 0) {
+        p.plan_count[w] = count;
+        p.plan_count[p.W + w] = idle;
+    }
 }
 
 namespace {
+
+// The part of block blockIdx.x: parts that some token sees first (seen), in sequence
+// order, KV heads fastest; index: its place in its sequence's list.
+struct Part {
+    int w, hkv, index;
+    int f, len;          // view and its keys
+    long long c0, off;   // first stream row of the part, and of the view
+    long long wh;
+    bool seen, any;
+};
+
+__device__ inline Part part_of(const MassParams& p) {
+    const int lane = threadIdx.x & 63;
+    Part it;
+    it.hkv = (int)(blockIdx.x % (uint32_t)p.Hkv);
+    long long r = blockIdx.x / (uint32_t)p.Hkv;
+    it.any = false;
+    for (int pass = 0; pass < 2 && !it.any; ++pass)
+        for (int w0 = 0; w0 < p.W && !it.any; w0 += kWave) {
+            const int w = w0 + lane;
+            int base = 0, n = 0;
+            if (w < p.W) {
+                const int c = p.plan_count[w], all = p.plan_count[p.W + w];
+                base = pass == 0 ? 0 : c;
+                n = pass == 0 ? c : all - c;
+            }
+            int incl = n;
+#pragma unroll
+            for (int d = 1; d < kWave; d <<= 1) {
+                const int o = __shfl_up(incl, d, kWave);
+                if (lane >= d) incl += o;
+            }
+            const int total = __builtin_amdgcn_readlane(incl, 63);
+            if (r < total) {
+                const int l = __builtin_ctzll(ballot(incl > (int)r));
+                it.w = w0 + l;
+                it.seen = pass == 0;
+                it.index = (int)r - __builtin_amdgcn_readlane(incl - n - base, l);
+                it.any = true;
+            }
+            r -= total;
+        }
+    if (!it.any) return it;
+    const int4 e = p.plan_list[(long long)it.w * p.nparts + it.index];
+    it.f = uniform(e.x);
+    it.c0 = (uint32_t)uniform(e.y);
+    it.off = (uint32_t)uniform(e.z);
+    it.len = uniform(e.w);
+    it.wh = (long long)it.w * p.Hkv + it.hkv;
+    return it;
+}
 
 // Tokens whose operands one ring half holds, staged together.
 template <int DT> constexpr int kGroup = DT == kF32 ? 4 : 8;
 template <int DT> constexpr int kRingBytes = 2 * kGroup<DT> * kOperandBytes<DT>;
 
-// A block's keys (4 waves, one unit each) against every token of the launch, view by
-// view and kGroup tokens at a time: the operands of a group are copied to LDS, a
-// quarter by each wave (they lie in the order the waves read them), while the group
-// before it is computed.  prepare(s0) runs in every wave before the group of tokens s0 is
-// waited for; body(s, x, mask, all) gets token s's raw scores x and the keys of this
-// view it sees (all: every key of the unit; not called where it sees none);
-// done(s0, n, first) runs in every wave after a group (first: of the first view the
-// block meets) and may use block barriers of its own.
+// A seen part's keys (a unit per wave) against every token of the launch, kGroup tokens
+// at a time: the operands of a group are copied to LDS, in turns by the waves (they
+// lie in the order the waves read them), while the group before it is computed.
+// prepare(s0) runs in every wave before the group of tokens s0 is waited for; body(s, x,
+// all) gets token s's scores x: raw ones if it sees all of the unit (all, as a type),
+// else base-2 ones with -inf for keys that it does not see (not called where it sees
+// none); done(s0, n) runs in every wave after a group and may use block barriers.
+//
+// A group of tokens that see all of the unit (most of them) runs without masks, the
+// MFMAs of the next token beside the exponentials of this one.
 template <int DT, int NT, class Prepare, class Body, class Done>
-__device__ inline void walk_tokens(const MassParams& p, const Item& it, long long c0, unsigned char* ring,
-                                   Prepare&& prepare, Body&& body, Done&& done) {
+__device__ inline void walk_tokens(const MassParams& p, const Part& it, unsigned char* ring, Prepare&& prepare,
+                                   Body&& body, Done&& done) {
     constexpr int kRows = NT * 16;
+    constexpr int kG = kGroup<DT>;
     const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
-    const long long b0 = it.chunk * (kMassWaves * kRows), b1 = b0 + kMassWaves * kRows;
     const uint32_t ring_at = lds_addr(ring);
-    const int groups = (p.ns + kGroup<DT> - 1) / kGroup<DT>;
-    long long off = 0;
-    bool first = true;  // view of the block: a block below visible_end meets one
-    for (int f = 0; f < p.F && off < b1; ++f) {
-        const int len = view_len(p, f);
-        const long long lo = off;
-        off += len;
-        if (off <= b0 || len == 0) continue;  // the same for all waves
-        const int seen = seen_lane(p, f, it.w, len);
-        const long long c = c0 + lane, hi = lo + lanes_max(seen);
-        const uint32_t row = cache_row(p, it.w, it.hkv, c, lane < kRows && c >= lo && c < hi);
-        const unsigned char* ops = reinterpret_cast<const unsigned char*>(p.rq) +
-                                   ((((long long)f * p.W + it.w) * p.Hkv + it.hkv) * p.S + p.s0) * kOperandBytes<DT>;
-        auto stage = [&](int gi) {
-            const int n = p.ns - gi * kGroup<DT> < kGroup<DT> ? p.ns - gi * kGroup<DT> : kGroup<DT>;
-            for (int i = wv; i < n * kPieces<DT>; i += kMassWaves)
-                dma16(ops + ((long long)gi * kGroup<DT> * kPieces<DT> + i) * 1024 + lane * 16,
-                      __builtin_amdgcn_readfirstlane(ring_at + (uint32_t)((gi & 1) * kGroup<DT> * kOperandBytes<DT> + i * 1024)));
+    const int groups = (p.ns + kG - 1) / kG;
+    const unsigned char* ops = reinterpret_cast<const unsigned char*>(p.rq) +
+                               ((((long long)it.f * p.W + it.w) * p.Hkv + it.hkv) * p.S + p.s0) * kOperandBytes<DT>;
+    auto stage = [&](int gi) {
+        const int n = p.ns - gi * kG < kG ? p.ns - gi * kG : kG;
+        const uint32_t half = ring_at + (uint32_t)((gi & 1) * kG * kOperandBytes<DT>);
+        for (int i = wv; i < n * kPieces<DT>; i += kMassWaves)
+            dma16(ops + ((long long)gi * kG * kPieces<DT> + i) * 1024 + lane * 16,
+                  __builtin_amdgcn_readfirstlane(half + (uint32_t)(i * 1024)));
+    };
+    stage(0);
+    // keys of the unit before the end of what token s sees, in lane s
+    const long long c0 = it.c0 + wv * kRows;
+    const int before = (int)(c0 - it.off);  // the view's keys before the unit
+    const int left = seen_lane(p, it.f, it.w, it.len) - before;
+    const int ends = left < 0 ? 0 : left < kRows ? left : kRows;
+    const int most = lanes_max(ends);
+    const uint32_t row = cache_row(p, it.w, it.hkv, c0 + lane, lane < most);
+    const uint64_t valid = ballot(row != 0xffffffffu);
+    u32x4 k[NT][kPieces<DT>];
+    load_keys<DT, NT>(p, row, k);
+    // the keys are here before the token loop: a wait for them inside it would wait for the
+    // next group's operands too (one counter for all loads)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int cc = 0; cc < kPieces<DT>; ++cc) asm volatile("" : "+v"(k[t][cc]));
+    // tokens that see the whole unit
+    const uint64_t whole = valid == kAllKeys<NT> ? ballot(ends == kRows) : 0ull;
+    for (int gi = 0; gi < groups; ++gi) {
+        const int t0 = gi * kG;
+        const int n = p.ns - t0 < kG ? p.ns - t0 : kG;
+        prepare(t0);
+        wait_vmcnt<0>();
+        __syncthreads();  // the group is here; every wave is done with the other half
+        if (gi + 1 < groups) stage(gi + 1);
+        const u32x4* half = reinterpret_cast<const u32x4*>(ring + (gi & 1) * kG * kOperandBytes<DT>) + lane;
+        auto query = [&](int s, u32x4(&q)[kPieces<DT>]) {
+#pragma unroll
+            for (int cc = 0; cc < kPieces<DT>; ++cc) q[cc] = half[(s * kPieces<DT> + cc) * kWave];
         };
-        stage(0);
-        const uint64_t valid = ballot(row != 0xffffffffu);
-        u32x4 k[NT][kPieces<DT>];
-        load_keys<DT, NT>(p, row, k);
-        // keys of the unit before the end of what token s sees, in lane s
-        const long long upto = lo - c0 + seen;
-        const int ends = (int)(upto < 0 ? 0 : upto < kRows ? upto : kRows);
-        const uint64_t from = range_bits<NT>(lo - c0, kRows);
-        for (int gi = 0; gi < groups; ++gi) {
-            const int t0 = gi * kGroup<DT>;
-            const int n = p.ns - t0 < kGroup<DT> ? p.ns - t0 : kGroup<DT>;
-            prepare(t0);
-            wait_vmcnt<0>();
-            __syncthreads();  // the group is here; every wave is done with the other half
-            if (gi + 1 < groups) stage(gi + 1);
-            const u32x4* half = reinterpret_cast<const u32x4*>(ring + (gi & 1) * kGroup<DT> * kOperandBytes<DT>) + lane;
-            if (valid) {
+        if (n == kG && (uint32_t)((whole >> t0) & ((1u << kG) - 1u)) == (1u << kG) - 1u) {
+            u32x4 q[kPieces<DT>];
+            f32x4 x[NT], y[NT];
+            query(0, q);
+            dot_tiles<DT, NT>(k, q, x);
+            query(1, q);
 #pragma unroll 1
-                for (int s = 0; s < n; ++s) {
-                    const uint64_t mask = valid & from & range_bits<NT>(0, __builtin_amdgcn_readlane(ends, t0 + s));
-                    if (!mask) continue;
-                    u32x4 q[kPieces<DT>];
-#pragma unroll
-                    for (int cc = 0; cc < kPieces<DT>; ++cc) q[cc] = half[(s * kPieces<DT> + cc) * kWave];
-                    f32x4 x[NT];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) x[t] = dot_tile<DT>(k[t], q);
-                    body(t0 + s, x, mask, mask == kAllKeys<NT>);
-                }
+            for (int s = 0; s < kG; s += 2) {
+                dot_tiles<DT, NT>(k, q, y);
+                query(s + 2 < kG ? s + 2 : s, q);
+                body(t0 + s, x, std::true_type{});
+                interleave<NT * kPieces<DT>>();
+                dot_tiles<DT, NT>(k, q, x);  // of the next pair; after the last one, not used
+                query(s + 3 < kG ? s + 3 : s, q);
+                body(t0 + s + 1, y, std::true_type{});
+                interleave<NT * kPieces<DT>>();
             }
-            done(t0, n, first);
+        } else if (valid) {
+#pragma unroll 1
+            for (int s = 0; s < n; ++s) {
+                const uint64_t mask = valid & first_keys<NT>(__builtin_amdgcn_readlane(ends, t0 + s));
+                if (!mask) continue;
+                u32x4 q[kPieces<DT>];
+                query(s, q);
+                f32x4 x[NT];
+                dot_tiles<DT, NT>(k, q, x);
+                scale_masked<NT>(x, mask, p.l2scale);
+                body(t0 + s, x, std::false_type{});
+            }
         }
-        first = false;
-        __syncthreads();  // the ring is read before the next view fills it
+        done(t0, n);
     }
 }
 
 }  // namespace
 
-// Per block of keys, token of the launch and head, (max, sum).
+// Per seen part, token of the launch and head, (max, sum).
 template <int DT, int NT>
 __global__ __launch_bounds__(kMassThreads) void dv_mass_stats(const MassParams p) {
     extern __shared__ __align__(16) unsigned char ring[];
     __shared__ float2 s_pair[kMassWaves][kGroup<DT>][kGqa];
-    constexpr int kRows = NT * 16;
     const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
-    const Item it = item_of(p);
-    if (it.chunk * (kMassWaves * kRows) >= visible_end(p, it.w)) return;
-    float2* part = reinterpret_cast<float2*>(p.part) + (it.wh * p.ns * p.nchunks + it.chunk) * kGqa;
+    const Part it = part_of(p);
+    if (!it.any || !it.seen) return;
+    float2* part = reinterpret_cast<float2*>(p.part) + (it.wh * p.ns * p.nchunks + it.index) * kGqa;
     const float l2 = p.l2scale;
     const float2 none = make_float2(-DV_INF, 0.0f);
     walk_tokens<DT, NT>(
-        p, it, (it.chunk * kMassWaves + wv) * kRows, ring,
+        p, it, ring,
         [&](int) {
             // tokens that see none of the wave's keys (the wave's own entries, read before
             // the last group's end)
             for (int i = lane; i < kGroup<DT> * kGqa; i += kWave) s_pair[wv][i >> 4][i & 15] = none;
         },
-        [&](int s, f32x4(&x)[NT], uint64_t mask, bool all) {
-            if (!all) scale_masked<NT>(x, mask, l2);
+        [&](int s, f32x4(&x)[NT], auto all) {
+            constexpr bool kRaw = decltype(all)::value;
+            // the largest base-2 score: of the largest raw one, or the smallest for a negative scale
+            const bool flip = kRaw && l2 < 0.0f;
             float mx = -DV_INF;
-            if (all && l2 < 0.0f) {
-                float mn = DV_INF;
+            if (flip) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) mn = fminf(mn, fminf(fminf(x[t][0], x[t][1]), fminf(x[t][2], x[t][3])));
-                mx = mn * l2;
+                for (int t = 0; t < NT; ++t)
+                    mx = fmaxf(mx, fmaxf(fmaxf(-x[t][0], -x[t][1]), fmaxf(-x[t][2], -x[t][3])));
             } else {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) mx = fmaxf(mx, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
-                if (all) mx *= l2;
             }
-            const float m = rows4_max(mx);
+            const float f = kRaw ? l2 : 1.0f;
+            const float m = rows4_max(mx) * (flip ? -f : f);
             const float mz = m == -DV_INF ? 0.0f : m;
-            const float f = all ? l2 : 1.0f;
             float l = 0.0f;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -531,28 +686,26 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_stats(const MassParams p
             l = rows4_sum(l);
             if (lane < kGqa) s_pair[wv][s & (kGroup<DT> - 1)][lane] = make_float2(m, l);
         },
-        [&](int t0, int n, bool first) {
-            // the block's waves, and the keys of an earlier view
+        [&](int t0, int n) {
             __syncthreads();
-            const int s = tid >> 4, h = tid & 15;
-            if (s < n) {
-                float2* to = part + (long long)(t0 + s) * p.nchunks * kGqa + h;
-                float2 e = first ? none : *to;
+            for (int i = tid; i < n * kGqa; i += kMassThreads) {
+                const int s = i >> 4, h = i & 15;
+                float2 e = none;
 #pragma unroll
                 for (int v = 0; v < kMassWaves; ++v) join(e.x, e.y, s_pair[v][s][h].x, s_pair[v][s][h].y);
-                *to = e;
+                part[(long long)(t0 + s) * p.nchunks * kGqa + h] = e;
             }
             __syncthreads();
         });
 }
 
 // Block (sequence, KV head, token): minus the log-sum-exp of its heads.
-__global__ __launch_bounds__(kMassThreads) void dv_mass_lse(const MassParams p, int block_rows) {
+__global__ __launch_bounds__(kMassThreads) void dv_mass_lse(const MassParams p) {
     __shared__ float2 s_pair[kMassThreads];
     const long long row = blockIdx.x;  // (w * Hkv + hkv) * ns + s
     const int w = (int)(row / ((long long)p.ns * p.Hkv));
-    const long long live = (visible_end(p, w) + block_rows - 1) / block_rows;
-    const float nl = joined_lse(reinterpret_cast<const float2*>(p.part) + row * p.nchunks * kGqa, live, s_pair);
+    const float nl =
+        joined_lse(reinterpret_cast<const float2*>(p.part) + row * p.nchunks * kGqa, p.plan_count[w], s_pair);
     if (threadIdx.x < kGqa) p.lse[row * kGqa + threadIdx.x] = nl;
 }
 
@@ -562,10 +715,11 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_apply(const MassParams p
     __shared__ float s_nl[2][kGroup<DT> * kGqa];
     constexpr int kRows = NT * 16;
     const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
-    const Item it = item_of(p);
-    const long long c0 = (it.chunk * kMassWaves + wv) * kRows;
-    if (it.chunk * (kMassWaves * kRows) >= visible_end(p, it.w)) {
-        store_decayed(p, it.wh, c0, kRows);
+    const Part it = part_of(p);
+    if (!it.any) return;
+    const long long c0 = it.c0 + wv * kRows, end = it.off + it.len;
+    if (!it.seen) {
+        store_decayed(p, it.wh, c0, end - c0 < kRows ? (int)(end - c0) : kRows);
         return;
     }
     const float* lse = p.lse + it.wh * p.ns * kGqa;
@@ -574,30 +728,26 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_apply(const MassParams p
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
     walk_tokens<DT, NT>(
-        p, it, c0, ring,
+        p, it, ring,
         [&](int t0) {
             // the half that the group before this one does not read
-            const int at = t0 * kGqa + (int)threadIdx.x;
-            if (threadIdx.x < kGroup<DT> * kGqa)
-                s_nl[(t0 / kGroup<DT>)&1][threadIdx.x] = at < p.ns * kGqa ? lse[at] : 0.0f;
+            for (int i = threadIdx.x; i < kGroup<DT> * kGqa; i += kMassThreads)
+                s_nl[(t0 / kGroup<DT>)&1][i] = t0 * kGqa + i < p.ns * kGqa ? lse[t0 * kGqa + i] : 0.0f;
         },
-        [&](int s, f32x4(&x)[NT], uint64_t mask, bool all) {
+        [&](int s, f32x4(&x)[NT], auto all) {
             const float nl = s_nl[(s / kGroup<DT>)&1][(s & (kGroup<DT> - 1)) * kGqa + (lane & 15)];
-            if (all) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[t][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], l2, nl));
-            } else {
-                scale_masked<NT>(x, mask, l2);
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[t][i] += weight(x[t][i], nl);
-            }
+                for (int i = 0; i < 4; ++i) {
+                    if constexpr (decltype(all)::value)
+                        acc[t][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(x[t][i], l2, nl));
+                    else
+                        acc[t][i] += weight(x[t][i], nl);
+                }
         },
-        [](int, int, bool) {});
-    store_mass<NT>(p, it.wh, c0, acc);
+        [](int, int) {});
+    store_mass<NT>(p, it.wh, c0, end, acc);
 }
 
 // ---- launches --------------------------------------------------------------------
@@ -615,30 +765,35 @@ struct MassWs {
     bool stored;
     int units;   // per wave (stored)
     int tokens;  // per launch
-    long long chunks;
-    size_t rq, part, lse, scores, total;
+    long long rows, chunks, parts;  // stream rows of a block; blocks of a (sequence, KV head)'s keys; those of all its rows
+    size_t rq, part, lse, scores, plan, total;
 };
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
-MassWs mass_ws(int dtype, int F, int W, int S, int Hkv, long long max_rows) {
+MassWs mass_ws(int dtype, int F, int W, int S, int Hkv, long long max_rows, long long capacity) {
     MassWs l{};
     const long long wh = (long long)W * Hkv;
-    long long rows = (long long)kMassWaves * tiles_of(dtype) * 16;  // of a block
+    const int unit = tiles_of(dtype) * 16;
+    long long rows = (long long)kMassWaves * unit;  // of a block
     l.units = 1;
     if (S == 1) {
         // as many units per wave, up to four, as leave 2048 blocks
-        while (l.units < 4 && wh * (max_rows / (rows * 2 * l.units)) >= 2048) l.units *= 2;
+        while (l.units < kMaxUnits && wh * (max_rows / (rows * 2 * l.units)) >= 2048) l.units *= 2;
         rows *= l.units;
     }
     l.chunks = (max_rows + rows - 1) / rows;
     const long long score_bytes = wh * l.chunks * rows * kGqa * 4;
     l.stored = S == 1 && score_bytes <= kMaxScoreBytes;
-    if (!l.stored && l.units > 1) {
-        rows /= l.units;
+    if (!l.stored) {
+        rows = (long long)kMassWaves * unit;
         l.units = 1;
-        l.chunks = (max_rows + rows - 1) / rows;
+        // parts end with their view
+        l.chunks = (max_rows + rows - 1) / rows + F;
     }
+    l.rows = rows;
+    const long long all = capacity > max_rows ? capacity : max_rows;
+    l.parts = (all + rows - 1) / rows + F + 1;
     l.tokens = S < kMassTokens ? S : kMassTokens;
     if (l.stored) {
         l.part = up256((size_t)(wh * l.chunks * kGqa * 8));
@@ -647,52 +802,49 @@ MassWs mass_ws(int dtype, int F, int W, int S, int Hkv, long long max_rows) {
         l.rq = up256((size_t)F * wh * kGqa * S * kHeadDim * (dtype == kF32 ? 4 : 2));
         l.part = up256((size_t)(wh * l.tokens * l.chunks * kGqa * 8));
         l.lse = up256((size_t)(wh * l.tokens * kGqa * 4));
+        l.plan = up256((size_t)W * (F + 2) * 4) + (size_t)W * l.parts * 16;
     }
-    l.total = l.rq + l.part + l.lse + l.scores;
+    l.total = l.rq + l.part + l.lse + l.scores + l.plan;
     return l;
 }
 
 template <int DT>
 hipError_t mass_go(MassParams p, const MassWs& l, int device, hipStream_t stream) {
     constexpr int NT = kTilesOf<DT>;
-    const long long rows = (long long)kMassWaves * NT * 16 * l.units;  // stream rows of a block
+    const long long rows = l.rows;
     const unsigned wh = (unsigned)(p.W * p.Hkv);
     const dim3 block(kMassThreads);
     const dim3 keys((unsigned)(wh * l.chunks)), outs((unsigned)(wh * ((p.C + rows - 1) / rows)));
     hipError_t e;
     p.nchunks = (int)l.chunks;
     p.units = l.units;
-    if (!l.stored) {
-        static std::atomic<unsigned long long> attr_done{0};
-        e = once_per_device(attr_done, device, [] {
-            const hipError_t es = hipFuncSetAttribute(reinterpret_cast<const void*>(&dv_mass_stats<DT, NT>),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kRingBytes<DT>);
-            return es != hipSuccess ? es
-                                    : hipFuncSetAttribute(reinterpret_cast<const void*>(&dv_mass_apply<DT, NT>),
-                                                          hipFuncAttributeMaxDynamicSharedMemorySize, kRingBytes<DT>);
-        });
-        if (e != hipSuccess) return e;
-    }
-    if (p.S == 0) {  // no token votes: every row only decays
-        if (outs.x) hipLaunchKernelGGL((dv_mass_apply<DT, NT>), outs, block, kRingBytes<DT>, stream, p);
-        return hipGetLastError();
-    }
-    if (l.stored) {
+    if (p.S == 0 || l.stored) {
         p.s0 = 0;
-        p.ns = 1;
-        if (keys.x) {
+        p.ns = p.S;
+        if (keys.x && p.S) {
             hipLaunchKernelGGL((dv_mass_scores<DT, NT>), keys, block, 0, stream, p);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
+        // without a token every row only decays
         if (outs.x) hipLaunchKernelGGL(dv_mass_apply_scores<NT>, outs, block, 0, stream, p);
         return hipGetLastError();
     }
+    static std::atomic<unsigned long long> attr_done{0};
+    e = once_per_device(attr_done, device, [] {
+        const hipError_t es = hipFuncSetAttribute(reinterpret_cast<const void*>(&dv_mass_stats<DT, NT>),
+                                                  hipFuncAttributeMaxDynamicSharedMemorySize, kRingBytes<DT>);
+        return es != hipSuccess ? es
+                                : hipFuncSetAttribute(reinterpret_cast<const void*>(&dv_mass_apply<DT, NT>),
+                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kRingBytes<DT>);
+    });
+    if (e != hipSuccess) return e;
+    p.nparts = (int)l.parts;
+    const dim3 parts((unsigned)(wh * l.parts));
     const long long pieces = (long long)p.F * wh * p.S * (kPieces<DT> * kWave);
-    if (pieces) {
-        hipLaunchKernelGGL(dv_mass_rotate<DT>, dim3((unsigned)((pieces + kMassThreads - 1) / kMassThreads)), block, 0,
-                           stream, p, pieces);
-        if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
+    hipLaunchKernelGGL(dv_mass_prepare<DT>,
+                       dim3((unsigned)p.W + (unsigned)((pieces + kMassThreads - 1) / kMassThreads)), block, 0, stream,
+                       p, pieces, (int)rows);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
     for (int s0 = 0; s0 < p.S; s0 += l.tokens) {
         p.s0 = s0;
         p.ns = p.S - s0 < l.tokens ? p.S - s0 : l.tokens;
@@ -700,9 +852,9 @@ hipError_t mass_go(MassParams p, const MassWs& l, int device, hipStream_t stream
             hipLaunchKernelGGL((dv_mass_stats<DT, NT>), keys, block, kRingBytes<DT>, stream, p);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
-        hipLaunchKernelGGL(dv_mass_lse, dim3(wh * (unsigned)p.ns), block, 0, stream, p, (int)rows);
+        hipLaunchKernelGGL(dv_mass_lse, dim3(wh * (unsigned)p.ns), block, 0, stream, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
-        if (outs.x) hipLaunchKernelGGL((dv_mass_apply<DT, NT>), outs, block, kRingBytes<DT>, stream, p);
+        hipLaunchKernelGGL((dv_mass_apply<DT, NT>), parts, block, kRingBytes<DT>, stream, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         p.mass = p.out;  // the launches after the first add to the first's result
         p.decay = 1.0f;
@@ -712,19 +864,22 @@ hipError_t mass_go(MassParams p, const MassWs& l, int device, hipStream_t stream
 
 }  // namespace
 
-size_t mass_workspace_bytes(int dtype, int F, int W, int S, int Hkv, long long max_rows, int) {
-    if (F < 0 || W <= 0 || S <= 0 || Hkv <= 0 || max_rows < 0) return 0;
-    return mass_ws(dtype, F, W, S, Hkv, max_rows).total;
+size_t mass_workspace_bytes(int dtype, int F, int W, int S, int Hkv, long long max_rows, long long capacity) {
+    if (F < 0 || W <= 0 || S <= 0 || Hkv <= 0 || max_rows < 0 || capacity < 0) return 0;
+    return mass_ws(dtype, F, W, S, Hkv, max_rows, capacity).total;
 }
 
 hipError_t launch_key_mass(int dtype, const MassParams& base, void* workspace, hipStream_t stream) {
     MassParams p = base;
-    const MassWs l = mass_ws(dtype, p.F, p.W, p.S, p.Hkv, (long long)p.maxB * p.bs);
+    const MassWs l = mass_ws(dtype, p.F, p.W, p.S, p.Hkv, (long long)p.maxB * p.bs, p.C);
     unsigned char* ws = reinterpret_cast<unsigned char*>(workspace);
     p.rq = ws;
     p.part = reinterpret_cast<float*>(ws + l.rq);
     p.lse = reinterpret_cast<float*>(ws + l.rq + l.part);
     p.scores = reinterpret_cast<float*>(ws + l.rq + l.part + l.lse);
+    p.plan_seen = reinterpret_cast<int*>(ws + l.rq + l.part + l.lse + l.scores);
+    p.plan_count = p.plan_seen + (size_t)p.W * p.F;
+    p.plan_list = reinterpret_cast<int4*>(ws + l.rq + l.part + l.lse + l.scores + up256((size_t)p.W * (p.F + 2) * 4));
     int device = 0;
     const hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return e;

@@ -764,7 +764,7 @@ void dvattn_paged_key_mass_op(at::Tensor& out, const std::optional<at::Tensor>& 
     }
     s.Ev = s.E;
     c10::hip::HIPGuardMasqueradingAsCUDA guard(out.device());
-    const size_t ws = dvattn_paged_key_mass_workspace_size(dt, &s, out.device().index());
+    const size_t ws = dvattn_paged_key_mass_workspace_size(dt, &s, out.size(2));
     at::Tensor w = workspace(ws, out);
     check_status(dvattn_paged_key_mass(dt, out.data_ptr<float>(), has ? mass->data_ptr<float>() : nullptr,
                                        (float)decay, out.size(2), (float)scale, locations.data_ptr<int>(),

@@ -328,7 +328,7 @@ DVATTN_API dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scal
  * summed in a fixed order: the same call gives the same bits.  Workspace of a single
  * token: about a quarter of a 16-bit K cache of W * max_blocks_per_seq pages, at most
  * 1 GiB of scores. */
-DVATTN_API size_t dvattn_paged_key_mass_workspace_size(int dtype, const dvattn_shape* shape, int device);
+DVATTN_API size_t dvattn_paged_key_mass_workspace_size(int dtype, const dvattn_shape* shape, long long capacity);
 DVATTN_API dvattn_status dvattn_paged_key_mass(int dtype, float* out, const float* mass, float decay,
                                     long long capacity, float scale, const int* locations, const void* queries,
                                     const float* cosines, const float* sines, const int* fragment_lengths,

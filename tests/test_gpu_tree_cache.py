@@ -198,11 +198,11 @@ def mass_case(dtype, W, Hkv, S, fl, bs, R, seed, extra=3, bad=False):
     return d, mass
 
 
-def check_mass(dv, gpu, d, mass, decay, in_place=False):
-    want, spread = TO.key_mass(mass, decay, SCALE, **d)
+def check_mass(dv, gpu, d, mass, decay, in_place=False, scale=SCALE):
+    want, spread = TO.key_mass(mass, decay, scale, **d)
     g, m = to(gpu, d), mass.to(gpu)
     out = None if in_place else torch.full_like(m, math.nan)
-    got = dv.dvattn_paged_key_mass(m, scale=SCALE, decay=decay, out=out, **g).cpu()
+    got = dv.dvattn_paged_key_mass(m, scale=scale, decay=decay, out=out, **g).cpu()
     if not in_place:
         assert torch.equal(m.cpu(), mass)
     n = int(d["fragment_lengths"].clamp(min=0).sum())
@@ -232,6 +232,16 @@ def test_key_mass(dv, gpu, dtype, shape):
     W, Hkv, S, fl, bs, R = shape
     d, mass = mass_case(dtype, W, Hkv, S, fl, bs, R, seed=S + len(fl))
     check_mass(dv, gpu, d, mass, 0.75)
+
+
+def test_key_mass_whole_units(dv, gpu):
+    """Tokens that all see whole units of keys, in whole groups (the loop without masks),
+    for either sign of the scale."""
+    for dtype in DTYPES:
+        d, mass = mass_case(dtype, 2, 1, 17, [530], 16, 128, seed=12)
+        d["locations"][:] = 529
+        check_mass(dv, gpu, d, mass, 1.0)
+        check_mass(dv, gpu, d, mass, 1.0, scale=-SCALE)
 
 
 @pytest.mark.parametrize("S", [1, 3])
@@ -278,6 +288,34 @@ def test_key_mass_nan_stays_in_its_head(dv, gpu):
         got = dv.dvattn_paged_key_mass(mass.to(gpu), scale=SCALE, **to(gpu, d)).cpu()
         assert got[0, 0, :30].isnan().all() and torch.equal(got[0, 0, 30:], mass[0, 0, 30:])
         assert got[0, 1].isfinite().all()
+
+
+@pytest.mark.parametrize("S", [1, 2])
+def test_key_mass_many_ragged_sequences(dv, gpu, S):
+    """More sequences than a wave has lanes, most of them short, and block tables so wide
+    that the scores of one token are not kept (more than 1 GiB of them)."""
+    g = torch.Generator().manual_seed(S)
+    W, fl, bs = 70, [40, 700], 16
+    d, mass = mass_case(torch.float16, W, 1, S, fl, bs, 64, seed=S)
+    d["locations"][1] = torch.randint(-1, 30, (W, S), generator=g)
+    d["locations"][1, ::13] = torch.randint(300, 700, (6, S), generator=g)
+    d["locations"][0, 5:9] = -1
+    narrow = check_mass(dv, gpu, d, mass, 0.5)
+    wide = torch.full((W, 15500), -1, dtype=torch.int32)
+    wide[:, :d["block_tables"].shape[1]] = d["block_tables"]
+    d["block_tables"] = wide
+    assert W * wide.shape[1] * bs * 64 > 1 << 30
+    again = check_mass(dv, gpu, d, mass, 0.5)
+    assert (narrow - again).abs().max() <= 1e-4
+
+
+def test_key_mass_windows_of_a_prompt(dv, gpu):
+    """Every token of a prompt votes: more tokens than a launch takes, each seeing the
+    keys before it, whole parts of the keys seen by later launches only."""
+    d, mass = mass_case(torch.bfloat16, 1, 1, 150, [600], 16, 64, seed=6)
+    d["locations"][0, 0] = 4 * torch.arange(150, dtype=torch.int32)
+    got = check_mass(dv, gpu, d, mass, 0.0)
+    assert got[0, 0, 597:].eq(0).all()
 
 
 def test_key_mass_no_tokens_decays(dv, gpu):
