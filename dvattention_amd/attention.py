@@ -173,18 +173,8 @@ def dvattn_tree_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, pa
     The last four and the first are ``dvattn_tree_paged_sdpa``'s arguments.  Another
     sequence's drafted nodes are neither seen nor counted.  S and F are at most 4096.
     """
-    F = fragment_lengths.numel()
-    W, S = parents.shape
-    R = 2 * inv_freq.numel()
-    dev = fragment_lengths.device
-    loc = torch.empty((F, W, S), dtype=torch.int32, device=dev)
-    cos = torch.empty((F, W, S, R), dtype=torch.float32, device=dev)
-    sin = torch.empty_like(cos)
-    views = torch.empty((W,), dtype=torch.int32, device=dev)
-    rows = torch.empty_like(views)
-    torch.ops.libdvatt.dvattn_tree_metadata(loc, cos, sin, views, rows, fragment_lengths, order, parents, inv_freq,
-                                            float(attention_scaling), round_to)
-    return loc, cos, sin, views, rows
+    return torch.ops.libdvatt.dvattn_tree_metadata(fragment_lengths, order, parents, inv_freq,
+                                                   float(attention_scaling), round_to)
 
 
 def dvattn_tree_paged_sdpa(queries: torch.Tensor, locations: torch.Tensor, cosines: torch.Tensor,

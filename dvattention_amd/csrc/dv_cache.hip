@@ -358,8 +358,9 @@ __global__ __launch_bounds__(256) void dv_tree_meta(const TreeMetaParams tp, int
             sn[e] = 0.0f;
             if (found && dep >= 0) {
                 const float ang = (float)(int)(base + dep) * p.inv_freq[i + e];
-                c[e] = cosf(ang) * p.scaling;
-                sn[e] = sinf(ang) * p.scaling;
+                sincosf(ang, &sn[e], &c[e]);
+                c[e] *= p.scaling;
+                sn[e] *= p.scaling;
             }
             if (p.round_dt == kBF16) {
                 c[e] = round_to<kBF16>(c[e]);

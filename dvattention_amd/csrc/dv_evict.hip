@@ -12,12 +12,16 @@ typedef __attribute__((address_space(1))) u32x4 gw_u32x4;
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kBins = 1 << 13;
-constexpr int kSelHeld = 32;  // rows per thread held in registers
+// Rows per thread held in registers: an instance for capacities of up to 4096 rows,
+// whose code is short, and one for the others.
+constexpr int kSelHeldFew = 4, kSelHeldMany = 32;
+constexpr int kSelList = 4096;  // rows that share T's first digit, held in LDS
 
-// Weights as integers in their order; a NaN is lighter than any number.
+// Weights as integers in their order; a NaN is lighter than any number, and 0 is left
+// for lanes without a row.
 __device__ inline uint32_t order_of(float f) {
     const uint32_t u = __float_as_uint(f);
-    if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
+    if ((u & 0x7fffffffu) > 0x7f800000u) return 1u;
     if ((u & 0x7fffffffu) == 0u) return 0x80000000u;  // -0 and +0 weigh the same
     return (u >> 31) ? ~u : u | 0x80000000u;
 }
@@ -55,10 +59,12 @@ __device__ inline int block_excl(int v, int* s_wave) {
 // wave and a running one inside it, and no pass has a barrier in its loop.  Up to
 // kSelHeld * 1024 rows are read once and held in registers; more are read again
 // (from L2) in each of the five passes.
+template <int kSelHeld>
 __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p) {
     __shared__ int s_hist[kBins];
+    __shared__ uint32_t s_list[kSelList];
     __shared__ int s_wave[kSelWaves], s_gt[kSelWaves], s_eq[kSelWaves];
-    __shared__ int s_digit, s_above;
+    __shared__ int s_digit, s_above, s_listed;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wv = uniform(tid >> 6);
     const int w = blockIdx.x / p.Hkv;
@@ -85,24 +91,25 @@ __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p
     const bool held = steps <= kSelHeld;
     uint32_t key[kSelHeld];
     if (held) {
+        float x[kSelHeld];
+#pragma unroll
+        for (int j = 0; j < kSelHeld; ++j) {
+            x[j] = 0.0f;
+            if (j < steps && base + j * kWave < m) x[j] = mass[base + j * kWave];
+        }
 #pragma unroll
         for (int j = 0; j < kSelHeld; ++j) {
             key[j] = 0u;
-            if (j < steps && base + j * kWave < m) key[j] = __float_as_uint(mass[base + j * kWave]);
-        }
-#pragma unroll
-        for (int j = 0; j < kSelHeld; ++j) {
-            if (j >= steps) break;
-            key[j] = order_of(__uint_as_float(key[j]));
+            if (j < steps) key[j] = base + j * kWave < m ? order_of(x[j]) : 0u;
         }
     }
-    // fn(weight, whether the lane has a row, the row) for the wave's rows in order
+    // fn(weight, the row) for the wave's rows in order (weight 0: no row)
     auto visit = [&](auto&& fn) {
         if (held) {
 #pragma unroll
             for (int j = 0; j < kSelHeld; ++j) {
                 if (j >= steps) break;
-                fn(key[j], base + j * kWave < m, base + j * kWave);
+                fn(key[j], base + j * kWave);
             }
         } else {
             for (int j0 = 0; j0 < steps; j0 += 8) {
@@ -116,7 +123,7 @@ __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int i = base + (j0 + j) * kWave;
-                    if (j0 + j < steps) fn(order_of(x[j]), i < m, i);
+                    if (j0 + j < steps) fn(i < m ? order_of(x[j]) : 0u, i);
                 }
             }
         }
@@ -125,21 +132,42 @@ __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p
     // Bits of a weight resolved per pass.  A wide first digit (sign, exponent, four bits of
     // the fraction) spreads weights of a few octaves over a hundred bins and more,
     // where lanes of a wave rarely meet in one (an LDS atomic serialises those); clearing
-    // and summing its bins costs a short call more than that saves.
+    // and summing its bins costs a short call more than that saves.  Lanes without a
+    // row count in the lowest bin, which no heavier weight's place depends on.
     const int bits0 = m <= 4096 ? 11 : 13, bits1 = m <= 4096 ? 11 : 10;
     uint32_t top = 0;   // T's digits so far
     int want = need;    // of the rows that agree with them, how many stay
     int shift = 32;
+    bool listed = false;  // the rows that agree with them are in the list
+    if (tid == 0) s_listed = 0;
     for (int pass = 0; pass < 3; ++pass) {
         const uint32_t known = pass == 0 ? 0u : ~0u << shift;
         const int bits = pass == 0 ? bits0 : pass == 1 ? bits1 : shift;
         shift -= bits;
         const int bins = 1 << bits;
         for (int i = tid; i < bins; i += kSelThreads) s_hist[i] = 0;
+        if (pass == 1 && steps > 8) {
+            // the few rows that share T's first digit go to the list, as far as it holds
+            // them: less to go through than all rows, if those are many
+            visit([&](uint32_t u, int) {
+                const uint64_t same = ballot((u & known) == top);
+                if (same) {
+                    int at = 0;
+                    if (lane == 0) at = atomicAdd(&s_listed, __builtin_popcountll(same));
+                    at = uniform(at) + lanes_below(same);
+                    if ((u & known) == top && at < kSelList) s_list[at] = u;
+                }
+            });
+        }
         __syncthreads();
-        visit([&](uint32_t u, bool in, int) {
-            if (in && (u & known) == top) atomicAdd(&s_hist[(u >> shift) & (uint32_t)(bins - 1)], 1);
-        });
+        if (pass == 1 && steps > 8) listed = s_listed <= kSelList;
+        auto count = [&](uint32_t u) {
+            if ((u & known) == top) atomicAdd(&s_hist[(u >> shift) & (uint32_t)(bins - 1)], 1);
+        };
+        if (listed)
+            for (int i = tid; i < s_listed; i += kSelThreads) count(s_list[i]);
+        else
+            visit([&](uint32_t u, int) { count(u); });
         __syncthreads();
         // the digit whose rows hold the want-th heaviest: a thread owns `per` bins,
         // counted from the heaviest
@@ -161,9 +189,9 @@ __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p
 
     // rows above T and equal to it, per wave and then before each wave
     int gts = 0, eqs = 0;
-    visit([&](uint32_t u, bool in, int) {
-        gts += __builtin_popcountll(ballot(in && u > top));
-        eqs += __builtin_popcountll(ballot(in && u == top));
+    visit([&](uint32_t u, int) {
+        gts += __builtin_popcountll(ballot(u > top));
+        eqs += __builtin_popcountll(ballot(u == top));
     });
     if (lane == 0) {
         s_gt[wv] = gts;
@@ -175,19 +203,26 @@ __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p
         gts += s_gt[i];
         eqs += s_eq[i];
     }
+    // rows kept before the wave's next one; of the equal rows, the first `want` are
+    int kept = gts + (eqs < want ? eqs : want);
     int* out = rows + a;
-    visit([&](uint32_t u, bool in, int i) {
-        const uint64_t gt = ballot(in && u > top), eq = ballot(in && u == top);
-        const int e = eqs + lanes_below(eq);  // equal rows before this one, the first `want` kept
-        const int at = gts + lanes_below(gt) + (e < want ? e : want);
-        if (in && (u > top || (u == top && e < want))) out[at] = a + i;
-        gts += __builtin_popcountll(gt);
-        eqs += __builtin_popcountll(eq);
+    visit([&](uint32_t u, int i) {
+        uint64_t keep = ballot(u > top);
+        const uint64_t eq = ballot(u == top);
+        if (eq) {
+            const int left = want - eqs;
+            keep |= left > 0 ? ballot(u == top && lanes_below(eq) < left) : 0ull;
+            eqs += __builtin_popcountll(eq);
+        }
+        if ((keep >> lane) & 1ull) out[kept + lanes_below(keep)] = a + i;
+        kept += __builtin_popcountll(keep);
     });
 }
 
 hipError_t launch_kv_select(const SelectParams& p, hipStream_t stream) {
-    hipLaunchKernelGGL(dv_kv_select, dim3((unsigned)(p.W * p.Hkv)), dim3(kSelThreads), 0, stream, p);
+    const dim3 grid((unsigned)(p.W * p.Hkv)), block(kSelThreads);
+    if (p.C <= kSelHeldFew * kSelThreads) hipLaunchKernelGGL(dv_kv_select<kSelHeldFew>, grid, block, 0, stream, p);
+    else hipLaunchKernelGGL(dv_kv_select<kSelHeldMany>, grid, block, 0, stream, p);
     return hipGetLastError();
 }
 

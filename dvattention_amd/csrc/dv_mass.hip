@@ -291,74 +291,138 @@ __device__ inline void store_decayed(const MassParams& p, long long wh, long lon
 
 }  // namespace
 
-// S = 1.  Block: 4 waves times p.units units of NT tiles of one (sequence, KV head),
-// unit u of wave v at rows (u * 4 + v) * NT * 16 of the block's.  Leaves the scores (tile
-// by tile, as the lanes hold them) and, per block and head, (max, sum).  A unit's
-// page ids are loaded while the unit before it is computed.
+// S = 1.  Block: p.units * 4 * NT * 16 rows of one (sequence, KV head), a contiguous
+// quarter for each wave.  Leaves the scores (tile by tile, as the lanes hold them) and,
+// per block and head, (max, sum).
+//
+// K rows come through LDS: a wave copies 8 KiB at a time into one half of a ring of its
+// own (whole rows per instruction) while it computes the other half; rows are
+// XOR-swizzled by 16-byte pieces so that an operand read of sixteen rows meets
+// different banks.  Loads straight into the operands' registers touch a row in four
+// instructions of 64 bytes and ran 84 us on 32 sequences of 1k - 8k keys, 8 KV heads.
+constexpr int kScoreBytes = 8192;
+constexpr int kScoreRing = kMassWaves * 2 * kScoreBytes;
+
+static __device__ __align__(16) unsigned char zero_row[kHeadDim * 4];
+
 template <int DT, int NT>
 __global__ __launch_bounds__(kMassThreads) void dv_mass_scores(const MassParams p) {
+    constexpr int kRowBytes = kHeadDim * Tr<DT>::kBytes;
+    constexpr int kKeys = kScoreBytes / kRowBytes;          // keys per ring half
+    constexpr int kTiles = kKeys / 16;
+    constexpr int kLanes = kRowBytes / 16;                  // lanes that copy one row
+    constexpr int kIds = kMaxUnits * NT * 16 / kWave;       // registers of cache rows
+    static_assert(kIds * kWave == kMaxUnits * NT * 16, "whole registers of cache rows");
+    extern __shared__ __align__(256) unsigned char ring[];
     __shared__ u32x4 s_q[kPieces<DT> * kWave];
     __shared__ float2 s_pair[kMassWaves][kGqa];
-    constexpr int kRows = NT * 16;
     const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
+    const int g = lane >> 4, n = lane & 15;
     const Item it = item_of(p);
     const long long end = visible_end(p, it.w);
-    const long long rows = (long long)kMassWaves * kRows * p.units;
+    const int mine_rows = NT * 16 * p.units;  // of a wave
+    const long long rows = (long long)kMassWaves * mine_rows;
     const long long b0 = it.chunk * rows;
     if (b0 >= end) return;
-    const long long b1 = b0 + rows < end ? b0 + rows : end;  // the block's visible part
+    const long long w0 = b0 + wv * mine_rows;
+    // the wave's visible part
+    const int keys = uniform((int)(end - w0 < mine_rows ? (end - w0 > 0 ? end - w0 : 0) : mine_rows));
+    // whole units of NT tiles, as dv_mass_apply_scores reads them
+    const int steps = (keys + NT * 16 - 1) / (NT * 16) * (NT * 16 / kKeys);
+    unsigned char* mine = ring + wv * 2 * kScoreBytes;
+    const uint32_t mine_at = lds_addr(mine);
     float m = -DV_INF, l = 0.0f;  // this lane's keys
     long long off = 0;
     bool first = true;            // no view's scores are stored yet
-    for (int f = 0; f < p.F && off < b1; ++f) {
+    for (int f = 0; f < p.F && off < b0 + rows && off < end; ++f) {
         const int len = view_len(p, f);
         const long long lo = off;
         off += len;
         if (off <= b0) continue;
         const long long hi = lo + uniform(seen_of(p, f, it.w, p.s0, len));
-        auto row_of = [&](long long c0) {
-            const long long c = c0 + lane;
-            return cache_row(p, it.w, it.hkv, c, lane < kRows && c >= lo && c < hi);
-        };
-        long long c0 = b0 + wv * kRows;
-        uint32_t row = row_of(c0);  // on its way while the query is rotated
+        uint32_t ids[kIds];
+#pragma unroll
+        for (int r = 0; r < kIds; ++r) {
+            const long long c = w0 + r * kWave + lane;
+            ids[r] = 0xffffffffu;
+            if (r * kWave < keys) ids[r] = cache_row(p, it.w, it.hkv, c, r * kWave + lane < keys && c >= lo && c < hi);
+        }
         if (!first) __syncthreads();  // the previous view's query is read
         for (int i = threadIdx.x; i < kPieces<DT> * kWave; i += kMassThreads)
             s_q[i] = rotated_piece<DT>(p, f, it.w, it.hkv, p.s0, i);
+        // the page ids are here: no wait for them (for all loads, that is) among the copies
+#pragma unroll
+        for (int r = 0; r < kIds; ++r) asm volatile("" : "+v"(ids[r]));
+        // ids of a step, from lane `at` on
+        auto ids_of = [&](int step, int& at) {
+            uint32_t v = ids[0];
+#pragma unroll
+            for (int r = 1; r < kIds; ++r) v = step * kKeys >= r * kWave ? ids[r] : v;
+            at = step * kKeys & (kWave - 1);
+            return v;
+        };
+        auto copy = [&](int step) {
+            int at;
+            const uint32_t v = ids_of(step, at);
+#pragma unroll
+            for (int i = 0; i < kScoreBytes / 1024; ++i) {
+                const int row = i * (kWave / kLanes) + lane / kLanes;
+                const uint32_t id = (uint32_t)__shfl((int)v, at + row, kWave);
+                const unsigned char* src = id != 0xffffffffu ? reinterpret_cast<const unsigned char*>(p.kc) +
+                                                                   (unsigned long long)id * kRowBytes
+                                                             : zero_row;
+                dma16(src + ((lane % kLanes) ^ (row & 15)) * 16,
+                      __builtin_amdgcn_readfirstlane(mine_at + (uint32_t)((step & 1) * kScoreBytes + i * 1024)));
+            }
+        };
+        if (steps > 0) copy(0);
+        if (steps > 1) copy(1);
         __syncthreads();
         u32x4 q[kPieces<DT>];
 #pragma unroll
         for (int cc = 0; cc < kPieces<DT>; ++cc) q[cc] = s_q[cc * kWave + lane];
-        for (int u = 0; u < p.units && c0 < b1; ++u, c0 += kMassWaves * kRows) {
-            u32x4 k[NT][kPieces<DT>];
-            load_keys<DT, NT>(p, row, k);
-            const uint64_t mask = ballot(row != 0xffffffffu);
-            row = row_of(c0 + kMassWaves * kRows);
-            f32x4 x[NT];
-            dot_tiles<DT, NT>(k, q, x);
-            scale_masked<NT>(x, mask, p.l2scale);
-            float* dst = p.scores + ((it.wh * p.nchunks * rows + c0) / 16 * kWave + lane) * 4;
+        float* out = p.scores + (it.wh * p.nchunks * rows + w0) / 16 * (kWave * 4) + lane * 4;
+        for (int step = 0; step < steps; ++step) {
+            if (step + 1 < steps) wait_vmcnt<kScoreBytes / 1024>();  // all but the next step's copies
+            else wait_vmcnt<0>();
+            compiler_fence();
+            u32x4 k[kTiles][kPieces<DT>];
+            const unsigned char* half = mine + (step & 1) * kScoreBytes + n * kRowBytes;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+                for (int cc = 0; cc < kPieces<DT>; ++cc)
+                    k[t][cc] = *reinterpret_cast<const u32x4*>(half + t * 16 * kRowBytes + ((cc * 4 + g) ^ n) * 16);
+            f32x4 x[kTiles];
+            dot_tiles<DT, kTiles>(k, q, x);
+            int at;
+            const uint32_t v = ids_of(step, at);
+            const uint64_t mask = (ballot(v != 0xffffffffu) >> at) & kAllKeys<kTiles>;
+            scale_masked<kTiles>(x, mask, p.l2scale);
             if (first) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) *reinterpret_cast<f32x4*>(dst + t * kWave * 4) = x[t];
+                for (int t = 0; t < kTiles; ++t) *reinterpret_cast<f32x4*>(out + t * kWave * 4) = x[t];
             } else {
                 // rows of earlier views keep theirs
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
+                for (int t = 0; t < kTiles; ++t) {
                     const uint32_t b = lane_bits(mask, t);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if ((b >> i) & 1u) dst[t * kWave * 4 + i] = x[t][i];
+                        if ((b >> i) & 1u) out[t * kWave * 4 + i] = x[t][i];
                 }
             }
+            out += kTiles * kWave * 4;
+            lds_wait();  // the half is read
+            if (step + 2 < steps) copy(step + 2);
             float mx = -DV_INF;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mx = fmaxf(mx, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
+            for (int t = 0; t < kTiles; ++t) mx = fmaxf(mx, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
             const float mn = fmaxf(m, mx);
             const float mz = mn == -DV_INF ? 0.0f : mn;
             l *= __builtin_amdgcn_exp2f(m - mz);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < kTiles; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(x[t][i] - mz);
             m = mn;
@@ -379,8 +443,7 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_scores(const MassParams 
     }
 }
 
-// Block: the same rows as above.  All of a wave's scores are on their way before the
-// block's heads' sums are joined.
+// Block: the same rows as above.
 template <int NT>
 __global__ __launch_bounds__(kMassThreads) void dv_mass_apply_scores(const MassParams p) {
     __shared__ float2 s_pair[kMassThreads];
@@ -389,33 +452,34 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_apply_scores(const MassP
     const Item it = item_of(p);
     const long long end = visible_end(p, it.w);
     const long long rows = (long long)kMassWaves * kRows * p.units;
-    const long long c0 = it.chunk * rows + wv * kRows;
-    if (it.chunk * rows >= end) {
-        for (int u = 0; u < p.units; ++u) store_decayed(p, it.wh, c0 + u * kMassWaves * kRows, kRows);
-        return;
-    }
+    long long c0 = it.chunk * rows + wv * kRows;
     const float* src = p.scores + ((it.wh * p.nchunks * rows + c0) / 16 * kWave + lane) * 4;
-    f32x4 x[kMaxUnits][NT];
+    f32x4 x[NT];
+    auto fetch = [&](long long c, const float* from) {
+        if (c < end)
 #pragma unroll
-    for (int u = 0; u < kMaxUnits; ++u)
-        if (u < p.units && c0 + u * kMassWaves * kRows < end)
-#pragma unroll
-            for (int t = 0; t < NT; ++t) x[u][t] = ld16f_nt(src + ((long long)u * kMassWaves * NT + t) * kWave * 4);
-    const float nl = joined_lse(reinterpret_cast<const float2*>(p.part) + it.wh * p.nchunks * kGqa,
-                                (end + rows - 1) / rows, s_pair);
-#pragma unroll
-    for (int u = 0; u < kMaxUnits; ++u) {
-        if (u >= p.units) break;
-        const long long c = c0 + u * kMassWaves * kRows;
+            for (int t = 0; t < NT; ++t) x[t] = ld16f_nt(from + t * kWave * 4);
+    };
+    fetch(c0, src);  // on its way while the block's heads' sums are joined
+    float nl = 0.0f;
+    if (it.chunk * rows < end)
+        nl = joined_lse(reinterpret_cast<const float2*>(p.part) + it.wh * p.nchunks * kGqa, (end + rows - 1) / rows,
+                        s_pair);
+    for (int u = 0; u < p.units; ++u) {
+        const long long c = c0;
+        c0 += kMassWaves * kRows;
+        src += kMassWaves * NT * kWave * 4;
         if (c >= end) {
             store_decayed(p, it.wh, c, kRows);
             continue;
         }
+        f32x4 acc[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[u][t][i] = weight(x[u][t][i], nl);
-        store_mass<NT>(p, it.wh, c, p.C, x[u]);
+            for (int i = 0; i < 4; ++i) acc[t][i] = weight(x[t][i], nl);
+        if (u + 1 < p.units) fetch(c0, src);
+        store_mass<NT>(p, it.wh, c, p.C, acc);
     }
 }
 
@@ -822,7 +886,13 @@ hipError_t mass_go(MassParams p, const MassWs& l, int device, hipStream_t stream
         p.s0 = 0;
         p.ns = p.S;
         if (keys.x && p.S) {
-            hipLaunchKernelGGL((dv_mass_scores<DT, NT>), keys, block, 0, stream, p);
+            static std::atomic<unsigned long long> ring_done{0};
+            e = once_per_device(ring_done, device, [] {
+                return hipFuncSetAttribute(reinterpret_cast<const void*>(&dv_mass_scores<DT, NT>),
+                                           hipFuncAttributeMaxDynamicSharedMemorySize, kScoreRing);
+            });
+            if (e != hipSuccess) return e;
+            hipLaunchKernelGGL((dv_mass_scores<DT, NT>), keys, block, kScoreRing, stream, p);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
         // without a token every row only decays

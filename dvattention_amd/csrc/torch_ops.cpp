@@ -12,6 +12,7 @@
 #include <torch/library.h>
 
 #include <string>
+#include <tuple>
 #include <vector>
 
 #include "dvattn_amd.h"
@@ -627,47 +628,28 @@ void dvattn_view_metadata_op(at::Tensor& locations, at::Tensor& cosines, at::Ten
 // ---------------------------------------------------------------------------
 // Drafted token trees and bounded caches (no counterpart in the reference).
 
-// dvattn_tree_metadata(Tensor(a!) locations, Tensor(b!) cosines, Tensor(c!) sines, Tensor(d!) tree_views,
-//   Tensor(e!) tree_rows, Tensor fragment_lengths, Tensor order, Tensor parents, Tensor inv_freq,
+// dvattn_tree_metadata(Tensor fragment_lengths, Tensor order, Tensor parents, Tensor inv_freq,
 //   float attention_scaling, ScalarType? round_to=None)
-void dvattn_tree_metadata_op(at::Tensor& locations, at::Tensor& cosines, at::Tensor& sines, at::Tensor& tree_views,
-                             at::Tensor& tree_rows, const at::Tensor& fragment_lengths, const at::Tensor& order,
-                             const at::Tensor& parents, const at::Tensor& inv_freq, double attention_scaling,
-                             std::optional<at::ScalarType> round_to) {
-    check_dim(locations, 3, "locations");
-    check_dim(cosines, 4, "cosines");
-    check_dim(sines, 4, "sines");
-    check_dim(tree_views, 1, "tree_views");
-    check_dim(tree_rows, 1, "tree_rows");
+//   -> (Tensor locations, Tensor cosines, Tensor sines, Tensor tree_views, Tensor tree_rows)
+// The outputs are allocated here: five allocations from Python took longer than the call.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dvattn_tree_metadata_op(
+    const at::Tensor& fragment_lengths, const at::Tensor& order, const at::Tensor& parents,
+    const at::Tensor& inv_freq, double attention_scaling, std::optional<at::ScalarType> round_to) {
     check_dim(fragment_lengths, 1, "fragment_lengths");
     check_dim(order, 2, "order");
     check_dim(parents, 2, "parents");
     check_dim(inv_freq, 1, "inv_freq");
-    const at::Tensor* all[] = {&locations, &tree_views, &tree_rows, &fragment_lengths, &order,
-                               &parents,   &cosines,    &sines,     &inv_freq};
-    const char* names[] = {"locations", "tree_views", "tree_rows", "fragment_lengths", "order",
-                           "parents",   "cosines",    "sines",     "inv_freq"};
-    for (int i = 0; i < 9; ++i) {
-        if (i < 6) check_i32(*all[i], names[i]);
+    const at::Tensor* all[] = {&fragment_lengths, &order, &parents, &inv_freq};
+    const char* names[] = {"fragment_lengths", "order", "parents", "inv_freq"};
+    for (int i = 0; i < 4; ++i) {
+        if (i < 3) check_i32(*all[i], names[i]);
         else check_f32(*all[i], names[i]);
         check_contig(*all[i], names[i]);
-        check_dev(*all[i], locations, names[i]);
+        check_dev(*all[i], fragment_lengths, names[i]);
     }
-    const int64_t F = locations.size(0), W = locations.size(1), S = locations.size(2), R = cosines.size(3);
-    TORCH_CHECK(cosines.size(0) == F && cosines.size(1) == W && cosines.size(2) == S,
-                "dvattn_tree_metadata: cosines must be [F,W,S,R], got ", cosines.sizes());
-    TORCH_CHECK(sines.sizes() == cosines.sizes(), "dvattn_tree_metadata: sines must match cosines");
-    TORCH_CHECK(tree_views.size(0) == W && tree_rows.size(0) == W,
-                "dvattn_tree_metadata: tree_views and tree_rows must be [W], got ", tree_views.sizes(), " and ",
-                tree_rows.sizes());
-    TORCH_CHECK(fragment_lengths.size(0) == F, "dvattn_tree_metadata: fragment_lengths must be [F], got ",
-                fragment_lengths.sizes());
-    TORCH_CHECK(order.size(0) == W && order.size(1) == F, "dvattn_tree_metadata: order must be [W,F], got ",
-                order.sizes());
-    TORCH_CHECK(parents.size(0) == W && parents.size(1) == S, "dvattn_tree_metadata: parents must be [W,S], got ",
-                parents.sizes());
-    TORCH_CHECK(R % 2 == 0 && inv_freq.size(0) >= R / 2, "dvattn_tree_metadata: need an even rotary dim and R/2 ",
-                "inverse frequencies (R=", R, ", got ", inv_freq.size(0), ")");
+    const int64_t F = fragment_lengths.size(0), W = parents.size(0), S = parents.size(1), R = 2 * inv_freq.size(0);
+    TORCH_CHECK(order.size(0) == W && order.size(1) == F, "dvattn_tree_metadata: order must be [W,F] = [", W, ",", F,
+                "], got ", order.sizes());
     int rd = -1;
     if (round_to.has_value()) {
         switch (*round_to) {
@@ -677,14 +659,18 @@ void dvattn_tree_metadata_op(at::Tensor& locations, at::Tensor& cosines, at::Ten
             default: TORCH_CHECK(false, "dvattn_tree_metadata: round_to must be float32, float16 or bfloat16");
         }
     }
-    c10::hip::HIPGuardMasqueradingAsCUDA guard(locations.device());
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(parents.device());
+    at::Tensor locations = at::empty({F, W, S}, parents.options());
+    at::Tensor cosines = at::empty({F, W, S, R}, inv_freq.options());
+    at::Tensor sines = at::empty({F, W, S, R}, inv_freq.options());
+    at::Tensor views = at::empty({W}, parents.options()), rows = at::empty({W}, parents.options());
     check_status(dvattn_tree_metadata(locations.data_ptr<int>(), cosines.data_ptr<float>(), sines.data_ptr<float>(),
-                                      tree_views.data_ptr<int>(), tree_rows.data_ptr<int>(),
-                                      fragment_lengths.data_ptr<int>(), order.data_ptr<int>(),
-                                      parents.data_ptr<int>(), inv_freq.data_ptr<float>(), (float)attention_scaling,
-                                      rd, as_int(F, "F"), as_int(W, "W"), as_int(S, "S"), as_int(R, "rotary_dim"),
-                                      stream_of(locations)),
+                                      views.data_ptr<int>(), rows.data_ptr<int>(), fragment_lengths.data_ptr<int>(),
+                                      order.data_ptr<int>(), parents.data_ptr<int>(), inv_freq.data_ptr<float>(),
+                                      (float)attention_scaling, rd, as_int(F, "F"), as_int(W, "W"), as_int(S, "S"),
+                                      as_int(R, "rotary_dim"), stream_of(parents)),
                  "dvattn_tree_metadata");
+    return {locations, cosines, sines, views, rows};
 }
 
 // dvattn_tree_paged_sdpa(Tensor(a!) output, float scale, <dvattn_paged_sdpa's tensors>, Tensor parents,
@@ -907,9 +893,9 @@ TORCH_LIBRARY(libdvatt, m) {
           "Tensor fragment_lengths, Tensor order, Tensor inv_freq, float attention_scaling, "
           "ScalarType? round_to=None) -> ()");
     // drafted token trees and bounded caches
-    m.def("dvattn_tree_metadata(Tensor(a!) locations, Tensor(b!) cosines, Tensor(c!) sines, "
-          "Tensor(d!) tree_views, Tensor(e!) tree_rows, Tensor fragment_lengths, Tensor order, Tensor parents, "
-          "Tensor inv_freq, float attention_scaling, ScalarType? round_to=None) -> ()");
+    m.def("dvattn_tree_metadata(Tensor fragment_lengths, Tensor order, Tensor parents, Tensor inv_freq, "
+          "float attention_scaling, ScalarType? round_to=None) -> (Tensor locations, Tensor cosines, Tensor sines, "
+          "Tensor tree_views, Tensor tree_rows)");
     m.def("dvattn_tree_paged_sdpa(Tensor(a!) output, float scale, Tensor locations, Tensor queries, "
           "Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor v_cache, "
           "Tensor block_tables, Tensor parents, Tensor tree_views, Tensor tree_rows) -> ()");
