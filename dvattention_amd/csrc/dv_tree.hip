@@ -43,9 +43,10 @@ struct Run8 {
     }
 };
 
-// Ancestors, and committed pieces, whose rows are loaded together.  Four: a node of
-// depth 6 takes two rounds, and eight would hold twice the registers, half as many
-// blocks per CU for a kernel that waits for memory.
+// Ancestors, and committed pieces, whose rows are loaded together.  Four: eight would
+// hold 76-100 registers instead of 64, fewer blocks per CU for a kernel that waits for
+// memory (16 trees of 64 nodes: 51 us with eight, 35 with four; few long sequences with
+// 30 pieces per segment: 9.1 and 10.0).
 constexpr int kTreeBatch = 4;
 
 // Block (segment, node of the group): thread t -> head t / 16, dims [(t % 16) * 8, +8).
