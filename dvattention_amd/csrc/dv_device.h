@@ -203,6 +203,14 @@ __device__ inline float rows4_sum(float v) {
     const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(s), __float_as_uint(s), false, false);
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
+// Sum over the 16 lanes of a row, in every lane (rotations within the row).
+__device__ inline float row16_sum(float v) {
+    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x128, 0xf, 0xf, false));  // ror 8
+    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x124, 0xf, 0xf, false));  // ror 4
+    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x122, 0xf, 0xf, false));  // ror 2
+    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x121, 0xf, 0xf, false));  // ror 1
+    return v;
+}
 __device__ inline int shfl_i(int v, int src) { return __shfl(v, src, kWave); }
 __device__ inline uint64_t ballot(bool b) { return __ballot(b); }
 

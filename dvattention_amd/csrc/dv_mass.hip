@@ -18,7 +18,8 @@
 //    and the scores stored (64 bytes per key and KV head, a quarter of a 16-bit K row, an
 //    eighth of an fp32 one), so the second pass reads those and not K.
 //  * S > 1 (a window of tokens; bound by the exponentials): a wave holds 64 keys (32
-//    for fp32) and walks the tokens, whose queries one launch beforehand rotated into
+//    for fp32) and walks the tokens (over few keys, where that walk is all a call's time,
+//    the waves of a block share the tokens instead: dv_mass_small), whose queries one launch beforehand rotated into
 //    the MFMA's operand order; the second pass computes the scores again (storing
 //    them would cost more bytes than K from two tokens on).  At most kMassTokens
 //    tokens per launch bound the workspace.
@@ -33,6 +34,8 @@ namespace {
 
 constexpr int kMassWaves = 4;
 constexpr int kMassThreads = kMassWaves * kWave;
+constexpr int kSmallWaves = 8;      // of a block that shares its tokens among them
+constexpr int kSmallThreads = kSmallWaves * kWave;
 constexpr int kMaxUnits = 4;        // S = 1: units of keys per wave
 constexpr int kMassTokens = kWave;  // one lane per token holds what it sees
 
@@ -219,9 +222,11 @@ __device__ inline void join(float& m, float& l, float m2, float l2) {
     m = mn;
 }
 
-// Minus the log-sum-exp of head tid % 16 over `count` pairs (pair u of head n at
-// pairs[u * 16 + n]), in every thread of the block; -inf where no key is seen, so that
-// 2^(x + it) is 0.
+// Minus the log-sum-exp; -inf where no key is seen, so that 2^(x + it) is 0.
+__device__ inline float minus_lse(float m, float l) { return l == 0.0f ? -DV_INF : -(m + log2f(l)); }
+
+// That of head tid % 16 over `count` pairs (pair u of head n at pairs[u * 16 + n]), in
+// every thread of the block.
 __device__ inline float joined_lse(const float2* pairs, long long count, float2 (&s_pair)[kMassThreads]) {
     const int tid = threadIdx.x;
     const int n = tid & 15;
@@ -236,15 +241,7 @@ __device__ inline float joined_lse(const float2* pairs, long long count, float2 
     l = 0.0f;
 #pragma unroll
     for (int u = 0; u < kMassThreads / 16; ++u) join(m, l, s_pair[u * 16 + n].x, s_pair[u * 16 + n].y);
-    return l == 0.0f ? -DV_INF : -(m + log2f(l));
-}
-
-__device__ inline float row16_sum(float v) {
-    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x128, 0xf, 0xf, false));  // ror 8
-    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x124, 0xf, 0xf, false));  // ror 4
-    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x122, 0xf, 0xf, false));  // ror 2
-    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x121, 0xf, 0xf, false));  // ror 1
-    return v;
+    return minus_lse(m, l);
 }
 
 // A weight: invisible keys (-inf) get none, whatever the row's sum is.
@@ -483,8 +480,161 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_apply_scores(const MassP
     }
 }
 
+// S > 1 and few keys in all (a short cache, a single sequence): no launch fills the card,
+// so a call costs the longest chain of one of its waves and not its work.  Here the chain
+// is short: a block of eight waves takes NT * 16 stream rows, every wave holds all of
+// their K rows and takes every eighth token.  The first launch leaves (max, sum) per
+// block, token and head; the second joins them (each wave for its own tokens, eight
+// blocks' pairs loaded together: one after the other took up to 20 us of a call's 49),
+// adds the weights over its tokens, and the waves' shares in order.  The K rows come
+// through LDS: eight waves that each load them into registers cost 0.5 us per wave.
+template <int DT, int NT, bool APPLY>
+__global__ __launch_bounds__(kSmallThreads) void dv_mass_small(const MassParams p) {
+    constexpr int kRows = NT * 16;
+    constexpr int kRowBytes = kHeadDim * Tr<DT>::kBytes;
+    constexpr int kLanes = kRowBytes / 16;                       // lanes that copy one row
+    __shared__ __align__(256) unsigned char s_keys[kRows * kRowBytes];
+    __shared__ float2 s_pair[APPLY ? 1 : kMassTokens][kGqa];     // (max, sum) of a token: its wave's own
+    __shared__ float s_nl[APPLY ? kMassTokens : 1][kGqa];        // minus its log-sum-exp
+    __shared__ float s_part[APPLY ? kSmallWaves : 1][kRows];
+    const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
+    const int n = lane & 15, S = p.ns;
+    const Item it = item_of(p);
+    const long long end = visible_end(p, it.w);
+    const long long b0 = it.chunk * kRows;
+    if (b0 >= end) {
+        if (APPLY && wv == 0) store_decayed(p, it.wh, b0, kRows);
+        return;
+    }
+    float2* part = reinterpret_cast<float2*>(p.part) + it.wh * p.nchunks * S * kGqa;
+    if constexpr (APPLY) {
+        constexpr int kBatch = 8;
+        const int count = (int)((end + kRows - 1) / kRows);
+        for (int s = wv; s < S; s += kSmallWaves) {
+            float m = -DV_INF, l = 0.0f;
+            for (int u0 = lane >> 4; u0 < count; u0 += 4 * kBatch) {
+                float2 e[kBatch];
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int u = u0 + 4 * j;
+                    e[j] = u < count ? part[((long long)u * S + s) * kGqa + n] : make_float2(-DV_INF, 0.0f);
+                }
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) join(m, l, e[j].x, e[j].y);
+            }
+            const float mw = rows4_max(m);
+            const float lw = rows4_sum(l * __builtin_amdgcn_exp2f(m - (mw == -DV_INF ? 0.0f : mw)));
+            if (lane < kGqa) s_nl[s][n] = minus_lse(mw, lw);
+        }
+    } else {
+        for (int s = wv; s < S; s += kSmallWaves)
+            if (lane < kGqa) s_pair[s][n] = make_float2(-DV_INF, 0.0f);
+    }
+    f32x4 acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    long long off = 0;
+    bool staged = false;
+    for (int f = 0; f < p.F && off < b0 + kRows && off < end; ++f) {
+        const int len = view_len(p, f);
+        const long long lo = off - b0;  // the view's first row in the block
+        off += len;
+        if (off <= b0) continue;
+        // keys of the block below what each token sees, token i in lane i
+        const long long below = seen_lane(p, f, it.w, len) + lo;
+        const int ends = below < 0 ? 0 : below < kRows ? (int)below : kRows;
+        const int most = lanes_max(ends);
+        const uint32_t row = cache_row(p, it.w, it.hkv, b0 + lane, lane >= lo && lane < most);
+        const uint64_t valid = ballot(row != 0xffffffffu);
+        if (!valid) continue;
+        if (staged) __syncthreads();  // the previous view's keys are read
+        staged = true;
+#pragma unroll
+        for (int i = wv; i < kRows * kLanes / kWave; i += kSmallWaves) {
+            const int r = i * (kWave / kLanes) + lane / kLanes;
+            const uint32_t id = (uint32_t)__shfl((int)row, r, kWave);
+            const unsigned char* src = id != 0xffffffffu ? reinterpret_cast<const unsigned char*>(p.kc) +
+                                                               (unsigned long long)id * kRowBytes
+                                                         : zero_row;
+            dma16(src + ((lane % kLanes) ^ (r & 15)) * 16,
+                  __builtin_amdgcn_readfirstlane(lds_addr(s_keys) + (uint32_t)(i * 1024)));
+        }
+        u32x4 q[kPieces<DT>];
+        const u32x4* ops = reinterpret_cast<const u32x4*>(p.rq) +
+                           (((long long)f * p.W + it.w) * p.Hkv + it.hkv) * S * (kPieces<DT> * kWave) + lane;
+        auto query = [&](int s) {
+#pragma unroll
+            for (int cc = 0; cc < kPieces<DT>; ++cc) q[cc] = ld16(ops + (s * kPieces<DT> + cc) * kWave);
+        };
+        if (wv < S) query(wv);
+        wait_vmcnt<0>();
+        __syncthreads();
+        u32x4 k[NT][kPieces<DT>];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int cc = 0; cc < kPieces<DT>; ++cc)
+                k[t][cc] = *reinterpret_cast<const u32x4*>(s_keys + (t * 16 + n) * kRowBytes +
+                                                           ((cc * 4 + (lane >> 4)) ^ n) * 16);
+#pragma unroll 1
+        for (int s = wv; s < S; s += kSmallWaves) {
+            const uint64_t mask = valid & first_keys<NT>(__builtin_amdgcn_readlane(ends, s));
+            f32x4 x[NT];
+            dot_tiles<DT, NT>(k, q, x);
+            if (s + kSmallWaves < S) query(s + kSmallWaves);
+            scale_masked<NT>(x, mask, p.l2scale);
+            if constexpr (APPLY) {
+                const float nl = s_nl[s][n];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[t][i] += weight(x[t][i], nl);
+            } else {
+                float mx = -DV_INF;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    mx = fmaxf(mx, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
+                const float m = rows4_max(mx);
+                const float mz = m == -DV_INF ? 0.0f : m;
+                float l = 0.0f;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(x[t][i] - mz);
+                l = rows4_sum(l);
+                if (lane < kGqa) {
+                    float2 e = s_pair[s][n];
+                    join(e.x, e.y, m, l);
+                    s_pair[s][n] = e;
+                }
+            }
+        }
+    }
+    if constexpr (!APPLY) {
+        for (int s = wv; s < S; s += kSmallWaves)
+            if (lane < kGqa) part[(it.chunk * S + s) * kGqa + n] = s_pair[s][n];
+    } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = row16_sum(acc[t][i]);
+                if (n == i) s_part[wv][t * 16 + (lane >> 4) * 4 + i] = a;
+            }
+        __syncthreads();
+        const long long c = b0 + threadIdx.x;
+        if (threadIdx.x < kRows && c < p.C) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kSmallWaves; ++v) sum += s_part[v][threadIdx.x];
+            const long long at = it.wh * p.C + c;
+            p.out[at] = (p.decay == 0.0f ? 0.0f : p.mass[at] * p.decay) + sum;
+        }
+    }
+}
+
 // S > 1: the query operands, [F, W, Hkv, S] of kOperandBytes each, a thread per 16
-// bytes; and, in the first W blocks, the plan.  A part is what one block of the
+// bytes; and, in the first `plans` blocks (W, or none), the plan.  A part is what one block of the
 // kernels below takes: up to part_rows rows of one view (the rows behind the last view
 // and below the capacity count as one more view, F).  The list of a sequence's parts
 // has those that some token sees in front, and they get the first blocks of the
@@ -494,9 +644,10 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_apply_scores(const MassP
 // nothing to do, strewn among the others, drew the blocks after them to the CUs that
 // had them.
 template <int DT>
-__global__ __launch_bounds__(kMassThreads) void dv_mass_prepare(const MassParams p, long long n, int part_rows) {
-    if (blockIdx.x >= (unsigned)p.W) {
-        const long long i = (long long)(blockIdx.x - p.W) * kMassThreads + threadIdx.x;
+__global__ __launch_bounds__(kMassThreads) void dv_mass_prepare(const MassParams p, long long n, int plans,
+                                                                int part_rows) {
+    if (blockIdx.x >= (unsigned)plans) {
+        const long long i = (long long)(blockIdx.x - plans) * kMassThreads + threadIdx.x;
         if (i >= n) return;
         constexpr int kPer = kPieces<DT> * kWave;
         const long long op = i / kPer;
@@ -825,8 +976,16 @@ int tiles_of(int dtype) { return dtype == kF32 ? kTilesOf<kF32> : kTilesOf<kBF16
 // from here on the second pass computes the scores again.
 constexpr long long kMaxScoreBytes = 1ll << 30;
 
+// dv_mass_small up to so many blocks of it: one per CU, two where a wave has more than one
+// token.  Beside the kernels of the plan (16-bit, 4 KV heads, 64-row blocks; fp32 takes
+// 32 rows): 20 blocks, 2 / 33 tokens 13 / 23 us instead of 20 / 55; 252 blocks 15 / 29
+// instead of 21 / 55; 504 blocks 22 / 49 instead of 21 / 55 (fp32 28 / 91 instead of 23 /
+// 111); 1008 blocks 38 / 91 instead of 22 / 58.
+constexpr long long kSmallBlocks = 256;
+
 struct MassWs {
     bool stored;
+    bool small;  // dv_mass_small
     int units;   // per wave (stored)
     int tokens;  // per launch
     long long rows, chunks, parts;  // stream rows of a block; blocks of a (sequence, KV head)'s keys; those of all its rows
@@ -849,6 +1008,18 @@ MassWs mass_ws(int dtype, int F, int W, int S, int Hkv, long long max_rows, long
     l.chunks = (max_rows + rows - 1) / rows;
     const long long score_bytes = wh * l.chunks * rows * kGqa * 4;
     l.stored = S == 1 && score_bytes <= kMaxScoreBytes;
+    const long long all = capacity > max_rows ? capacity : max_rows;
+    l.small = S > 1 && S <= kMassTokens && wh * ((all + unit - 1) / unit) <= (S > kSmallWaves ? 2 * kSmallBlocks : kSmallBlocks);
+    if (l.small) {
+        l.units = 1;
+        l.rows = unit;
+        l.tokens = S;
+        l.chunks = (max_rows + unit - 1) / unit;
+        l.rq = up256((size_t)F * wh * kGqa * S * kHeadDim * (dtype == kF32 ? 4 : 2));
+        l.part = up256((size_t)(wh * l.chunks * S * kGqa * 8));
+        l.total = l.rq + l.part;
+        return l;
+    }
     if (!l.stored) {
         rows = (long long)kMassWaves * unit;
         l.units = 1;
@@ -856,7 +1027,6 @@ MassWs mass_ws(int dtype, int F, int W, int S, int Hkv, long long max_rows, long
         l.chunks = (max_rows + rows - 1) / rows + F;
     }
     l.rows = rows;
-    const long long all = capacity > max_rows ? capacity : max_rows;
     l.parts = (all + rows - 1) / rows + F + 1;
     l.tokens = S < kMassTokens ? S : kMassTokens;
     if (l.stored) {
@@ -899,6 +1069,20 @@ hipError_t mass_go(MassParams p, const MassWs& l, int device, hipStream_t stream
         if (outs.x) hipLaunchKernelGGL(dv_mass_apply_scores<NT>, outs, block, 0, stream, p);
         return hipGetLastError();
     }
+    const long long pieces = (long long)p.F * wh * p.S * (kPieces<DT> * kWave);
+    const int plans = l.small ? 0 : p.W;
+    const dim3 prep((unsigned)plans + (unsigned)((pieces + kMassThreads - 1) / kMassThreads));
+    p.nparts = (int)l.parts;
+    if (prep.x) hipLaunchKernelGGL(dv_mass_prepare<DT>, prep, block, 0, stream, p, pieces, plans, (int)rows);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    if (l.small) {
+        p.s0 = 0;
+        p.ns = p.S;
+        if (keys.x) hipLaunchKernelGGL((dv_mass_small<DT, NT, false>), keys, dim3(kSmallThreads), 0, stream, p);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        if (outs.x) hipLaunchKernelGGL((dv_mass_small<DT, NT, true>), outs, dim3(kSmallThreads), 0, stream, p);
+        return hipGetLastError();
+    }
     static std::atomic<unsigned long long> attr_done{0};
     e = once_per_device(attr_done, device, [] {
         const hipError_t es = hipFuncSetAttribute(reinterpret_cast<const void*>(&dv_mass_stats<DT, NT>),
@@ -908,13 +1092,7 @@ hipError_t mass_go(MassParams p, const MassWs& l, int device, hipStream_t stream
                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kRingBytes<DT>);
     });
     if (e != hipSuccess) return e;
-    p.nparts = (int)l.parts;
     const dim3 parts((unsigned)(wh * l.parts));
-    const long long pieces = (long long)p.F * wh * p.S * (kPieces<DT> * kWave);
-    hipLaunchKernelGGL(dv_mass_prepare<DT>,
-                       dim3((unsigned)p.W + (unsigned)((pieces + kMassThreads - 1) / kMassThreads)), block, 0, stream,
-                       p, pieces, (int)rows);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
     for (int s0 = 0; s0 < p.S; s0 += l.tokens) {
         p.s0 = s0;
         p.ns = p.S - s0 < l.tokens ? p.S - s0 : l.tokens;

@@ -19,15 +19,6 @@
 namespace dv {
 namespace chunk {
 
-// Sum over the 16 lanes of a row, in every lane (rotations within the row).
-__device__ inline float row16_sum(float v) {
-    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x128, 0xf, 0xf, false));  // ror 8
-    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x124, 0xf, 0xf, false));  // ror 4
-    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x122, 0xf, 0xf, false));  // ror 2
-    v += __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(v), 0x121, 0xf, 0xf, false));  // ror 1
-    return v;
-}
-
 // Eight elements of a row as fp32.
 template <int DT>
 struct Run8 {

@@ -244,6 +244,30 @@ def test_key_mass_whole_units(dv, gpu):
         check_mass(dv, gpu, d, mass, 1.0, scale=-SCALE)
 
 
+WINDOWS = [s for s in MASSES if s[2] > 1] + [(3, 2, 8, [50, 0, 300, 9], 16, 64), (1, 2, 9, [517], 24, 128),
+                                             (2, 1, 64, [100, 31], 16, 32)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", WINDOWS)
+@pytest.mark.parametrize("bad", [False, True])
+def test_key_mass_narrow_and_wide_tables(dv, gpu, dtype, shape, bad):
+    """The same keys under a block table of their size, where few blocks cover them and the
+    waves of a block share the tokens, and under one so wide that a plan cuts them."""
+    W, Hkv, S, fl, bs, R = shape
+    d, mass = mass_case(dtype, W, Hkv, S, fl, bs, R, seed=S + W, bad=bad)
+    d["locations"][-1, 0, 0] = -1
+    narrow = check_mass(dv, gpu, d, mass, 0.75)
+    wide = torch.full((W, 40000 // bs), -1, dtype=torch.int32)
+    wide[:, :d["block_tables"].shape[1]] = d["block_tables"]
+    d["block_tables"] = wide
+    again = check_mass(dv, gpu, d, mass, 0.75)
+    assert (narrow - again).abs().max() <= 1e-4 * S
+    assert torch.equal(again, check_mass(dv, gpu, d, mass, 0.75, in_place=True))
+    d["locations"][:] = 10 ** 6  # every token sees whole views
+    check_mass(dv, gpu, d, mass, 1.0, scale=-SCALE)
+
+
 @pytest.mark.parametrize("S", [1, 3])
 @pytest.mark.parametrize("extra", [-40, 0, 700])
 @pytest.mark.parametrize("decay", [0.0, 1.0])
