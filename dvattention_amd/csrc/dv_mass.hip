@@ -761,8 +761,11 @@ __device__ inline Part part_of(const MassParams& p) {
     return it;
 }
 
-// Tokens whose operands one ring half holds, staged together.
-template <int DT> constexpr int kGroup = DT == kF32 ? 4 : 8;
+// Tokens whose operands one ring half holds, staged together: a ring of 32 KiB lets as many
+// blocks share a CU as their registers do (three).  One of 64 KiB, for two of them, took
+// 20 % longer for fp32 at every size and up to 20 % for 16 bits where the parts did not
+// fill the card evenly (but 5 % less where they did).
+template <int DT> constexpr int kGroup = DT == kF32 ? 2 : 4;
 template <int DT> constexpr int kRingBytes = 2 * kGroup<DT> * kOperandBytes<DT>;
 
 // A seen part's keys (a unit per wave) against every token of the launch, kGroup tokens
@@ -862,7 +865,7 @@ __device__ inline void walk_tokens(const MassParams& p, const Part& it, unsigned
 // Per seen part, token of the launch and head, (max, sum).
 template <int DT, int NT>
 __global__ __launch_bounds__(kMassThreads) void dv_mass_stats(const MassParams p) {
-    extern __shared__ __align__(16) unsigned char ring[];
+    __shared__ __align__(16) unsigned char ring[kRingBytes<DT>];
     __shared__ float2 s_pair[kMassWaves][kGroup<DT>][kGqa];
     const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
     const Part it = part_of(p);
@@ -926,7 +929,7 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_lse(const MassParams p) 
 
 template <int DT, int NT>
 __global__ __launch_bounds__(kMassThreads) void dv_mass_apply(const MassParams p) {
-    extern __shared__ __align__(16) unsigned char ring[];
+    __shared__ __align__(16) unsigned char ring[kRingBytes<DT>];
     __shared__ float s_nl[2][kGroup<DT> * kGqa];
     constexpr int kRows = NT * 16;
     const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
@@ -1083,26 +1086,17 @@ hipError_t mass_go(MassParams p, const MassWs& l, int device, hipStream_t stream
         if (outs.x) hipLaunchKernelGGL((dv_mass_small<DT, NT, true>), outs, dim3(kSmallThreads), 0, stream, p);
         return hipGetLastError();
     }
-    static std::atomic<unsigned long long> attr_done{0};
-    e = once_per_device(attr_done, device, [] {
-        const hipError_t es = hipFuncSetAttribute(reinterpret_cast<const void*>(&dv_mass_stats<DT, NT>),
-                                                  hipFuncAttributeMaxDynamicSharedMemorySize, kRingBytes<DT>);
-        return es != hipSuccess ? es
-                                : hipFuncSetAttribute(reinterpret_cast<const void*>(&dv_mass_apply<DT, NT>),
-                                                      hipFuncAttributeMaxDynamicSharedMemorySize, kRingBytes<DT>);
-    });
-    if (e != hipSuccess) return e;
     const dim3 parts((unsigned)(wh * l.parts));
     for (int s0 = 0; s0 < p.S; s0 += l.tokens) {
         p.s0 = s0;
         p.ns = p.S - s0 < l.tokens ? p.S - s0 : l.tokens;
         if (keys.x) {
-            hipLaunchKernelGGL((dv_mass_stats<DT, NT>), keys, block, kRingBytes<DT>, stream, p);
+            hipLaunchKernelGGL((dv_mass_stats<DT, NT>), keys, block, 0, stream, p);
             if ((e = hipGetLastError()) != hipSuccess) return e;
         }
         hipLaunchKernelGGL(dv_mass_lse, dim3(wh * (unsigned)p.ns), block, 0, stream, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
-        hipLaunchKernelGGL((dv_mass_apply<DT, NT>), parts, block, kRingBytes<DT>, stream, p);
+        hipLaunchKernelGGL((dv_mass_apply<DT, NT>), parts, block, 0, stream, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
         p.mass = p.out;  // the launches after the first add to the first's result
         p.decay = 1.0f;

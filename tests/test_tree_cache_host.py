@@ -97,7 +97,7 @@ def test_workspace_is_bounded(lib):
     size = lib.dvattn_paged_key_mass_workspace_size
     wide = shape(S=1, W=64, Hkv=8, Hq=128, max_blocks_per_seq=8192, num_blocks=1 << 16)
     assert size(2, ctypes.byref(wide), 0) < 2 << 30
-    a, b = shape(S=64, W=1), shape(S=64 * 32, W=1)
+    a, b = (shape(S=s, W=1, max_blocks_per_seq=4096) for s in (64, 64 * 32))
     queries = 16 * 128 * 2
     assert size(2, ctypes.byref(b), 0) - size(2, ctypes.byref(a), 0) == (b.S - a.S) * queries
 
