@@ -920,10 +920,15 @@ dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scale, const in
     p.bs_shift = log2_exact(s->block_size);
     p.maxB = s->max_blocks_per_seq;
     p.nblocks = s->num_blocks;
+    if (dv::tree_entries(dtype, p) > 0) {
+        const hipError_t e = dv::launch_tree_small(dtype, p, (hipStream_t)stream);
+        if (e != hipSuccess) return hip_fail(e, "dvattn_tree_paged_sdpa launch");
+        return ok();
+    }
     const long long max_keys = (long long)s->max_blocks_per_seq * s->block_size;
     // Smallest key range of a workgroup.  A call too small for the GPU is cut finer: every
-    // piece is merged anyway.  One sequence, 8 KV heads, with 256 / 96 keys: 8 nodes on
-    // 1000 keys 29.9 / 25.1 us, 32 on 1000 38.5 / 33.9; 8 on 4000 (more workgroups than
+    // piece is merged anyway.  bf16, one sequence, 8 KV heads, with 256 / 96 keys: 8 nodes
+    // on 1000 keys 29.9 / 25.1 us, 32 on 1000 38.5 / 33.9; 8 on 4000 (more workgroups than
     // that, and more pieces to merge) 30.5 / 33.4.
     const long long segments = (long long)s->W * ((s->S + 15) / 16) * s->Hkv;
     p.min_keys = segments * max_keys <= 192ll * 96 ? 96 : 256;

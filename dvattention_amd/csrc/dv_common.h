@@ -269,6 +269,10 @@ hipError_t launch_tree_meta(const TreeMetaParams& p, hipStream_t stream);
 // drafted ones in the merge.  launch_merge_tree merges the segments of a launch
 // of launch_chunk whose parameters carry parents.
 hipError_t launch_merge_tree(int dtype, const DecodeParams& p, int ntb, hipStream_t stream);
+// The whole call in one launch, without a workspace, where few keys and nodes make that
+// the faster way: its list's entries, or 0.
+int tree_entries(int dtype, const DecodeParams& p);
+hipError_t launch_tree_small(int dtype, const DecodeParams& p, hipStream_t stream);
 
 // Key mass: workspace of a call with at most max_rows stream rows and `capacity` outputs
 // per sequence and KV head, and its launches.

@@ -14,9 +14,12 @@
 //
 // Work per node is its depth, not the tree's size: a mask over all drafted rows on
 // the matrix units would multiply S^2 pairs of which a tree of depth d sees S * d.
+//
+// Short sequences take one launch instead (dv_tree_small, below).
 #include "dv_chunk.h"
 
 namespace dv {
+
 namespace chunk {
 
 // Eight elements of a row as fp32.
@@ -34,6 +37,30 @@ struct Run8 {
     }
 };
 
+// Node s and its ancestors, from the node up; their number, or -1 for an absent node (its
+// path leaves the tree at an entry that is no earlier node and not -1).  Every step goes
+// to an earlier node, so the walk ends.
+__device__ inline int walk_path(const int* parents, int s, int* path) {
+    int count = 0;
+    for (;;) {
+        const int up = parents[s];
+        path[count++] = s;
+        if (up == -1) return count;
+        if (up < -1 || up >= s) return -1;
+        s = up;
+    }
+}
+
+// Cache row (without its KV head) of stream row pos of sequence w, or -1 if it lies on no
+// valid page.
+__device__ inline int page_row(const DecodeParams& p, int w, long long pos) {
+    if (pos < 0) return -1;
+    const long long lp = p.bs_shift >= 0 ? pos >> p.bs_shift : (long long)((uint32_t)pos / (uint32_t)p.bs);
+    if (lp >= p.maxB) return -1;
+    const int page = p.bt[(long long)w * p.maxB + lp];
+    return page >= 0 && page < p.nblocks ? (int)(uint32_t)((long long)page * p.bs + (pos - lp * p.bs)) : -1;
+}
+
 // Ancestors, and committed pieces, whose rows are loaded together.  Four: eight would
 // hold 76-100 registers instead of 64, fewer blocks per CU for a kernel that waits for
 // memory (16 trees of 64 nodes: 51 us with eight, 35 with four; few long sequences with
@@ -42,8 +69,7 @@ constexpr int kTreeBatch = 4;
 
 // Block (segment, node of the group): thread t -> head t / 16, dims [(t % 16) * 8, +8).
 // LDS: the sequence's parents, then the node's ancestors as cache rows, which the first
-// wave looks up while the others join the committed pieces.  An absent node (its
-// path leaves the tree at an entry that is no earlier node and not -1) writes zeros.
+// wave looks up while the others join the committed pieces.  An absent node writes zeros.
 template <int DT>
 __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int ntb) {
     using raw = typename Tr<DT>::raw;
@@ -70,18 +96,7 @@ __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int n
     if (tid < kWave) {
         int count = 0;
         if (tid == 0) {
-            // every step goes to an earlier node, so the walk ends
-            int j = s;
-            for (;;) {
-                const int up = s_par[j];
-                s_row[count++] = j;
-                if (up == -1) break;
-                if (up < -1 || up >= j) {
-                    count = -1;
-                    break;
-                }
-                j = up;
-            }
+            count = walk_path(s_par, s, s_row);
             s_count = count;
         }
         count = uniform(count);
@@ -97,15 +112,7 @@ __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int n
         for (int i = tid; i < count; i += kWave) {
             const long long pos = (long long)first + s_row[i];
             const long long l = pos - off;
-            int at = -1;
-            if (l >= 0 && l < len && l > loc && pos >= 0) {
-                const long long lp = p.bs_shift >= 0 ? pos >> p.bs_shift : (long long)((uint32_t)pos / (uint32_t)p.bs);
-                if (lp < p.maxB) {
-                    const int page = p.bt[(long long)w * p.maxB + lp];
-                    if (page >= 0 && page < p.nblocks) at = (int)(uint32_t)((long long)page * p.bs + (pos - lp * p.bs));
-                }
-            }
-            s_row[i] = at;
+            s_row[i] = l >= 0 && l < len && l > loc ? page_row(p, w, pos) : -1;
         }
     }
 
@@ -218,7 +225,278 @@ __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int n
     store_run8<DT>(o, v);
 }
 
+// ---- short sequences -------------------------------------------------------------
+//
+// With few keys per sequence the call above is two launches' fixed times (a view's start
+// alone costs a workgroup of the first 11 - 13 us).  Here it is one: a block of eight
+// waves for each (sequence, KV head, node) goes through the list of the node's keys, the
+// committed ones of each view and then its path, every view's part rounded up to tiles of
+// 16 entries (so a tile has one rotated query):
+//   scores S^T = K Q^T by tiles (the waves take turns), left in LDS with each head's
+//   maximum; weights 2^(x - m) in place with each head's sum; O^T = V^T P by steps of four
+//   keys on 16x16x4 fp32 MFMAs, whatever the cache's type: a lane's 16-byte load of V row
+//   4 * step + g is one element of each of the step's MFMAs, so V needs no transposing
+//   and the weights no rounding.  Last, the waves' sums are joined in order.
+constexpr int kSmallWaves = 8;
+constexpr int kSmallThreads = kSmallWaves * kWave;
+constexpr int kSmallAhead = 4;                // V steps under way together
+// Keys in the list: 640, with which two blocks share a CU; for fp32, whose multi-query kernel
+// takes three times the 16-bit one's time, also 1280 (one block per CU).
+constexpr int kEntries = 640, kManyEntries = 1280;
+constexpr int kSmallQueryBytes = 16 * 1024;   // the views' queries in LDS
+// Read in place of a list entry without a row: loads without branches can be on their way
+// together.
+__device__ __align__(16) unsigned char no_row[kHeadDim * 4];
+template <int DT> constexpr int kQPieces = kHeadDim * Tr<DT>::kBytes / 64;  // 16-byte pieces of a row per lane
+
+template <int DT, int kSmallEntries>
+__global__ __launch_bounds__(kSmallThreads) void dv_tree_small(const DecodeParams p) {
+    using raw = typename Tr<DT>::raw;
+    constexpr int kP = kQPieces<DT>;
+    constexpr int kRowBytes = kHeadDim * Tr<DT>::kBytes;
+    constexpr int kRun = 16 / Tr<DT>::kBytes;     // elements of a piece
+    constexpr int kMaxViews = kSmallQueryBytes / (kP * kWave * 16);
+    __shared__ __align__(16) float s_x[kSmallEntries * kGqa];
+    __shared__ __align__(16) int s_row[kSmallEntries];
+    __shared__ int s_par[kSmallEntries];
+    __shared__ u32x4 s_q[kMaxViews * kP * kWave];
+    __shared__ float s_m[kSmallWaves][kGqa], s_l[kSmallWaves][kGqa];
+    __shared__ int s_count;
+    const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
+    const int g = lane >> 4, n = lane & 15;
+    const int hkv = blockIdx.x % p.Hkv;
+    const int ws = blockIdx.x / p.Hkv;
+    const int w = ws / p.S, s = ws - w * p.S;
+    for (int i = tid; i < p.S; i += kSmallThreads) s_par[i] = p.parents[(long long)w * p.S + i];
+    // per view: its first stream row, and the list's entries before it
+    long long off[kMaxViews];
+    int at[kMaxViews + 1], seen[kMaxViews];
+    const long long rows = (long long)p.maxB * p.bs;
+    const int room = kSmallEntries - (p.S + 15) / 16 * 16;
+    const int tv = p.tree_views[w], first = p.tree_rows[w];
+    long long own_off = 0;
+    int own_len = 0, own_loc = -1;
+    at[0] = 0;
+    {
+        long long o = 0;
+#pragma unroll
+        for (int f = 0; f < kMaxViews; ++f) {
+            off[f] = o;
+            seen[f] = 0;
+            if (f < p.F) {
+                const int len = p.fl[f], loc = p.loc[((long long)f * p.W + w) * p.S + s];
+                const long long most = loc >= len - 1 ? len : (long long)loc + 1;
+                long long here = most < rows - o ? most : rows - o;
+                // (lengths below zero could make views overlap: the list ends where it ends)
+                here = here < room - at[f] ? here : room - at[f];
+                seen[f] = here > 0 ? (int)here : 0;
+                if (f == tv) {
+                    own_off = o;
+                    own_len = len;
+                    own_loc = loc;
+                }
+                o += len;
+            }
+            at[f + 1] = at[f] + (seen[f] + 15) / 16 * 16;
+        }
+    }
+    const int base = at[kMaxViews];
+    const bool has_view = tv >= 0 && tv < p.F;
+    __syncthreads();
+    if (wv == 0) {
+        int count = 0;
+        if (lane == 0) s_count = count = walk_path(s_par, s, s_row + base);
+        count = uniform(count);
+        if (count > 0)
+            for (int i = lane; i < (count + 15) / 16 * 16; i += kWave) {
+                int r = -1;
+                if (has_view && i < count) {
+                    const long long pos = (long long)first + s_row[base + i];
+                    const long long l = pos - own_off;
+                    if (l >= 0 && l < own_len && l > own_loc) r = page_row(p, w, pos);
+                }
+                s_row[base + i] = r;
+            }
+    } else {
+        const int t0 = tid - kWave, nt = kSmallThreads - kWave;
+        for (int i = t0; i < base; i += nt) {
+            int r = -1;
+#pragma unroll
+            for (int f = 0; f < kMaxViews; ++f)
+                if (i >= at[f] && i - at[f] < seen[f]) r = page_row(p, w, off[f] + (i - at[f]));
+            s_row[i] = r;
+        }
+        // the token's 16 heads in the MFMA's operand order, rotated for each view
+        for (int i = t0; i < p.F * kP * kWave; i += nt) {
+            const int f = i / (kP * kWave), piece = i - f * (kP * kWave);
+            const int cc = piece >> 6, h = hkv * kGqa + (piece & 15);
+            const raw* qrow = reinterpret_cast<const raw*>(p.q) + (((long long)w * p.Hq + h) * p.S + s) * kHeadDim;
+            const long long cs = (((long long)f * p.W + w) * p.S + s) * p.R;
+            // (through a register on its way to LDS: kept in LDS, the array is indexed by what
+            // each block would fetch from the launch packet, 5 - 13 us of a call)
+            raw r[kRun];
+            rotate_run<DT, kRun>(qrow, p.cosv + cs, p.sinv + cs, p.R, (cc * 4 + ((piece >> 4) & 3)) * kRun, r);
+            u32x4 v;
+            __builtin_memcpy(&v, r, 16);
+            s_q[i] = v;
+        }
+    }
+    __syncthreads();
+    const int count = s_count;
+    if (count < 0) {
+        raw* o = reinterpret_cast<raw*>(p.out) + (((long long)w * p.Hq + hkv * kGqa) * p.S + s) * kHeadDim;
+        for (int i = tid; i < kGqa * kHeadDim; i += kSmallThreads)
+            o[(long long)(i / kHeadDim) * p.S * kHeadDim + i % kHeadDim] = raw(0);
+        return;
+    }
+    const int tiles = (base + count + 15) / 16;
+
+    // scores
+    float mx = -DV_INF;
+#pragma unroll 2
+    for (int t = wv; t < tiles; t += kSmallWaves) {
+        const int row = s_row[t * 16 + n];
+        u32x4 k[kP];
+        const unsigned char* src = (row != -1 ? reinterpret_cast<const unsigned char*>(p.kc) +
+                                                    ((unsigned long long)(uint32_t)row * p.Hkv + hkv) * kRowBytes
+                                              : no_row) +
+                                   g * 16;
+#pragma unroll
+        for (int cc = 0; cc < kP; ++cc) k[cc] = ld16(src + cc * 64);
+        int f = 0;
+#pragma unroll
+        for (int v = 1; v < kMaxViews; ++v) f = t * 16 >= at[v] ? v : f;
+        if (t * 16 >= base) f = has_view ? tv : 0;
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int cc = 0; cc < kP; ++cc) {
+            const u32x4 q = s_q[(f * kP + cc) * kWave + lane];
+            if constexpr (DT == kF32) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    x = Tr<kF32>::mma1(__builtin_bit_cast(f32x4, k[cc])[j], __builtin_bit_cast(f32x4, q)[j], x);
+            } else {
+                x = Tr<DT>::mma(k[cc], q, x);
+            }
+        }
+        const int4 ids = *reinterpret_cast<const int4*>(s_row + t * 16 + g * 4);
+        x[0] = ids.x != -1 ? x[0] * p.l2scale : -DV_INF;
+        x[1] = ids.y != -1 ? x[1] * p.l2scale : -DV_INF;
+        x[2] = ids.z != -1 ? x[2] * p.l2scale : -DV_INF;
+        x[3] = ids.w != -1 ? x[3] * p.l2scale : -DV_INF;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s_x[(t * 16 + g * 4 + i) * kGqa + n] = x[i];
+            mx = fmaxf(mx, x[i]);
+        }
+    }
+    mx = rows4_max(mx);
+    if (lane < kGqa) s_m[wv][lane] = mx;
+    __syncthreads();
+
+    // weights; every thread meets one head only
+    float m = -DV_INF;
+#pragma unroll
+    for (int v = 0; v < kSmallWaves; ++v) m = fmaxf(m, s_m[v][n]);
+    const float mz = m == -DV_INF ? 0.0f : m;
+    float l = 0.0f;
+    for (int i = tid; i < tiles * 16 * kGqa; i += kSmallThreads) {
+        const float e = __builtin_amdgcn_exp2f(s_x[i] - mz);
+        s_x[i] = e;
+        l += e;
+    }
+    l = rows4_sum(l);
+    if (lane < kGqa) s_l[wv][lane] = l;
+    __syncthreads();
+
+    // the weighted sums: acc[e] holds dims (g * 4 + i) * 8 + e of head n (fp32: two
+    // pieces of four dims, (g * 4 + i) * 4 + e and 64 more)
+    f32x4 acc[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll kSmallAhead
+    for (int st = wv; st < tiles * 4; st += kSmallWaves) {
+        const int row = s_row[st * 4 + g];
+        const float e = s_x[(st * 4 + g) * kGqa + n];
+        u32x4 v[DT == kF32 ? 2 : 1];
+        const unsigned char* src = (row != -1 ? reinterpret_cast<const unsigned char*>(p.vc) +
+                                                    ((unsigned long long)(uint32_t)row * p.Hkv + hkv) * kRowBytes
+                                              : no_row) +
+                                   n * 16;
+        v[0] = ld16(src);
+        if constexpr (DT == kF32) v[1] = ld16(src + 256);
+        raw r[8];
+        __builtin_memcpy(r, v, sizeof(v));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = Tr<kF32>::mma1(Tr<DT>::tof(r[j]), e, acc[j]);
+    }
+    __syncthreads();  // the weights are read; their space takes the waves' sums
+    f32x4* s_acc = reinterpret_cast<f32x4*>(s_x);
+    static_assert(sizeof(s_x) >= kSmallWaves / 2 * 8 * kWave * 16, "half of the waves' sums");
+    if (wv >= kSmallWaves / 2)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s_acc[((wv - kSmallWaves / 2) * 8 + j) * kWave + lane] = acc[j];
+    __syncthreads();
+    if (wv < kSmallWaves / 2)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s_acc[(wv * 8 + j) * kWave + lane] += acc[j];
+    __syncthreads();
+
+    // thread -> head tid / 32, dims [tid % 32 * 4, +4)
+    const int h = tid >> 5, d = (tid & 31) * 4;
+    float sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < kSmallWaves; ++v) sum += s_l[v][h];
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key at all: zeros (a NaN sum stays NaN)
+    float o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int e = DT == kF32 ? (d >> 6) * 4 + j : (d & 7) + j;
+        const int r = DT == kF32 ? (d & 63) >> 2 : d >> 3;
+        float a = 0.0f;
+#pragma unroll
+        for (int v = 0; v < kSmallWaves / 2; ++v)
+            a += s_x[((v * 8 + e) * kWave + (r >> 2) * 16 + h) * 4 + (r & 3)];
+        o[j] = a * inv;
+    }
+    raw* dst = reinterpret_cast<raw*>(p.out) + (((long long)w * p.Hq + hkv * kGqa + h) * p.S + s) * kHeadDim + d;
+    if constexpr (DT == kF32) *reinterpret_cast<f32x4*>(dst) = f32x4{o[0], o[1], o[2], o[3]};
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
+}
+
 }  // namespace chunk
+
+// Keys and nodes up to which one launch is the faster way, 8 KV heads, us here / with two
+// launches.  bf16: 8 nodes on 200 keys 11 / 24, 16 nodes of four sequences on 400 keys
+// 23 / 33, of eight (1024 blocks) 43.5 / 46, 64 nodes of four sequences on 200 (2048
+// blocks) 51 / 49; on 1000 keys 29 / 26 for 8 nodes and 30 / 35 for 32, 65 / 39 for 16 of
+// four sequences.  fp32: 12 / 64, 31 / 92, 56 / 163, 65 / 124; on 1000 keys 34 / 56, 36 /
+// 83, 81 / 144.
+int tree_entries(int dtype, const DecodeParams& p) {
+    const long long blocks = (long long)p.W * p.Hkv * p.S;
+    const long long view = (long long)kGqa * kHeadDim * (dtype == kF32 ? 4 : 2);  // bytes of a view's queries
+    const long long keys = (long long)p.maxB * p.bs + 15ll * p.F + p.S + 15;
+    if (p.F * view > chunk::kSmallQueryBytes) return 0;
+    if (keys <= chunk::kEntries && blocks <= (dtype == kF32 ? 4096 : 1024)) return chunk::kEntries;
+    return dtype == kF32 && keys <= chunk::kManyEntries && blocks <= 1024 ? chunk::kManyEntries : 0;
+}
+
+hipError_t launch_tree_small(int dtype, const DecodeParams& p, hipStream_t stream) {
+    using namespace chunk;
+    const dim3 grid((unsigned)(p.W * p.Hkv * p.S)), block(kSmallThreads);
+    switch (dtype) {
+        case kBF16: hipLaunchKernelGGL((dv_tree_small<kBF16, kEntries>), grid, block, 0, stream, p); break;
+        case kF16: hipLaunchKernelGGL((dv_tree_small<kF16, kEntries>), grid, block, 0, stream, p); break;
+        case kF32:
+            if (tree_entries(dtype, p) == kEntries)
+                hipLaunchKernelGGL((dv_tree_small<kF32, kEntries>), grid, block, 0, stream, p);
+            else
+                hipLaunchKernelGGL((dv_tree_small<kF32, kManyEntries>), grid, block, 0, stream, p);
+            break;
+        default: return hipErrorInvalidValue;
+    }
+    return hipGetLastError();
+}
 
 hipError_t launch_merge_tree(int dtype, const DecodeParams& p, int ntb, hipStream_t stream) {
     const dim3 grid((unsigned)(p.nrows * p.Hkv * ntb)), block(256);

@@ -84,9 +84,24 @@ def tree_case(dtype, W, Hkv, S, fl, bs, R, seed, chain=False, bad=False, absent=
     return d
 
 
+def widened(d, rows):
+    """The same case under a block table of at least so many rows."""
+    W, maxB = d["block_tables"].shape
+    wide = torch.full((W, max(maxB, rows // d["k_cache"].shape[1])), -1, dtype=torch.int32)
+    wide[:, :maxB] = d["block_tables"]
+    return {**d, "block_tables": wide}
+
+
 def check_tree(dv, gpu, d, dtype, scale=SCALE):
+    """Under the given block table, where one launch may take the call, and under a wide one,
+    where pieces of the committed keys are merged."""
     want, size, spread = TO.tree_sdpa(scale, **d)
-    got = dv.dvattn_tree_paged_sdpa(scale=scale, **to(gpu, d)).cpu()
+    for case in (widened(d, 2000), d):
+        got = compare_tree(dv.dvattn_tree_paged_sdpa(scale=scale, **to(gpu, case)).cpu(), d, dtype, want, size, spread)
+    return got, want
+
+
+def compare_tree(got, d, dtype, want, size, spread):
     n = int(d["fragment_lengths"].clamp(min=0).sum())
     e = 2 * (E + 8) * 2.0 ** -24 * spread + (n + 16) * 2.0 ** -24
     tol = size * torch.expm1(2 * e) + 1e-30
@@ -97,7 +112,7 @@ def check_tree(dv, gpu, d, dtype, scale=SCALE):
     assert torch.equal(got.isnan(), want.isnan())
     over = (got.double() - want).abs().nan_to_num(0.0) - tol.nan_to_num(math.inf)
     assert bool((over <= 0).all()), f"largest excess {float(over.max()):.3e}"
-    return got, want
+    return got
 
 
 TREES = [
@@ -110,6 +125,8 @@ TREES = [
     (1, 2, 33, [300], 32, 0),          # no rotation
     (2, 1, 5, [5], 16, 128),           # nothing committed
     (1, 1, 64, [1100], 16, 128),
+    (1, 2, 100, [110], 16, 64),        # a path longer than a wave has lanes; just nodes
+    (2, 1, 3, [25, 1, 40, 60], 24, 64),  # four views
 ]
 
 
@@ -258,9 +275,7 @@ def test_key_mass_narrow_and_wide_tables(dv, gpu, dtype, shape, bad):
     d, mass = mass_case(dtype, W, Hkv, S, fl, bs, R, seed=S + W, bad=bad)
     d["locations"][-1, 0, 0] = -1
     narrow = check_mass(dv, gpu, d, mass, 0.75)
-    wide = torch.full((W, 40000 // bs), -1, dtype=torch.int32)
-    wide[:, :d["block_tables"].shape[1]] = d["block_tables"]
-    d["block_tables"] = wide
+    d = widened(d, 40000)
     again = check_mass(dv, gpu, d, mass, 0.75)
     assert (narrow - again).abs().max() <= 1e-4 * S
     assert torch.equal(again, check_mass(dv, gpu, d, mass, 0.75, in_place=True))
