@@ -858,9 +858,16 @@ dvattn_status dvattn_tree_metadata(int* locations, float* cosines, float* sines,
 }
 
 // ---------------------------------------------------------------------------
+static dv::TreePlan tree_plan_of(int dtype, const dvattn_shape* s) {
+    return dv::tree_plan(dtype, s->F, s->W, s->S, s->Hkv, (long long)s->max_blocks_per_seq * s->block_size);
+}
+
 size_t dvattn_tree_paged_sdpa_workspace_size(int dtype, const dvattn_shape* s, int device) {
     if (!s || !valid_dtype(dtype)) return 0;
-    return dv::chunk_workspace_bytes(s->W, s->S, s->Hkv, current_device(device));
+    if (s->F < 0 || s->W < 0 || s->S < 0 || s->Hkv < 0 || s->max_blocks_per_seq < 0 || s->block_size < 0) return 0;
+    const dv::TreePlan plan = tree_plan_of(dtype, s);
+    return plan.windows > 0 ? dv::tree_workspace_bytes(plan, s->W, s->S, s->Hkv)
+                            : dv::chunk_workspace_bytes(s->W, s->S, s->Hkv, current_device(device));
 }
 
 dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scale, const int* locations, const void* queries,
@@ -920,8 +927,10 @@ dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scale, const in
     p.bs_shift = log2_exact(s->block_size);
     p.maxB = s->max_blocks_per_seq;
     p.nblocks = s->num_blocks;
-    if (dv::tree_entries(dtype, p) > 0) {
-        const hipError_t e = dv::launch_tree_small(dtype, p, (hipStream_t)stream);
+    const dv::TreePlan plan = tree_plan_of(dtype, s);
+    if (plan.windows > 0) {
+        p.part = reinterpret_cast<float*>(workspace);
+        const hipError_t e = dv::launch_tree_small(dtype, plan, p, (hipStream_t)stream);
         if (e != hipSuccess) return hip_fail(e, "dvattn_tree_paged_sdpa launch");
         return ok();
     }

@@ -269,10 +269,14 @@ hipError_t launch_tree_meta(const TreeMetaParams& p, hipStream_t stream);
 // drafted ones in the merge.  launch_merge_tree merges the segments of a launch
 // of launch_chunk whose parameters carry parents.
 hipError_t launch_merge_tree(int dtype, const DecodeParams& p, int ntb, hipStream_t stream);
-// The whole call in one launch, without a workspace, where few keys and nodes make that
-// the faster way: its list's entries, or 0.
-int tree_entries(int dtype, const DecodeParams& p);
-hipError_t launch_tree_small(int dtype, const DecodeParams& p, hipStream_t stream);
+// Short sequences: how the nodes' key lists are cut (no windows: the multi-query kernel
+// and launch_merge_tree are the faster way), the bytes of p.part that takes, the launch.
+struct TreePlan {
+    int windows, window;  // per node and KV head; committed entries of one
+};
+TreePlan tree_plan(int dtype, int F, int W, int S, int Hkv, long long max_keys);
+size_t tree_workspace_bytes(const TreePlan& t, int W, int S, int Hkv);
+hipError_t launch_tree_small(int dtype, const TreePlan& t, const DecodeParams& p, hipStream_t stream);
 
 // Key mass: workspace of a call with at most max_rows stream rows and `capacity` outputs
 // per sequence and KV head, and its launches.

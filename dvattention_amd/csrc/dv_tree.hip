@@ -227,52 +227,59 @@ __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int n
 
 // ---- short sequences -------------------------------------------------------------
 //
-// With few keys per sequence the call above is two launches' fixed times (a view's start
-// alone costs a workgroup of the first 11 - 13 us).  Here it is one: a block of eight
-// waves for each (sequence, KV head, node) goes through the list of the node's keys, the
-// committed ones of each view and then its path, every view's part rounded up to tiles of
-// 16 entries (so a tile has one rotated query):
+// With few keys the call above is two launches' fixed times (a view's start alone costs a
+// workgroup of the first 11 - 13 us).  Here a block of eight waves for each (sequence, KV
+// head, node) goes through the list of the node's keys, the committed ones of each view
+// and then its path, every view's part rounded up to tiles of 16 entries (so a tile has
+// one rotated query):
 //   scores S^T = K Q^T by tiles (the waves take turns), left in LDS with each head's
 //   maximum; weights 2^(x - m) in place with each head's sum; O^T = V^T P by steps of four
 //   keys on 16x16x4 fp32 MFMAs, whatever the cache's type: a lane's 16-byte load of V row
 //   4 * step + g is one element of each of the step's MFMAs, so V needs no transposing
 //   and the weights no rounding.  Last, the waves' sums are joined in order.
+// A list of more than 640 entries, or one that few blocks would have to take in long
+// turns, is cut into windows, a block each, whose sums a second launch joins; the path
+// goes with the first window.
 constexpr int kSmallWaves = 8;
 constexpr int kSmallThreads = kSmallWaves * kWave;
 constexpr int kSmallAhead = 4;                // V steps under way together
-// Keys in the list: 640, with which two blocks share a CU; for fp32, whose multi-query kernel
-// takes three times the 16-bit one's time, also 1280 (one block per CU).
-constexpr int kEntries = 640, kManyEntries = 1280;
+constexpr int kEntries = 640;                 // of a block's list: two blocks share a CU
 constexpr int kSmallQueryBytes = 16 * 1024;   // the views' queries in LDS
 // Read in place of a list entry without a row: loads without branches can be on their way
 // together.
 __device__ __align__(16) unsigned char no_row[kHeadDim * 4];
 template <int DT> constexpr int kQPieces = kHeadDim * Tr<DT>::kBytes / 64;  // 16-byte pieces of a row per lane
 
-template <int DT, int kSmallEntries>
-__global__ __launch_bounds__(kSmallThreads) void dv_tree_small(const DecodeParams p) {
+// A window's sums: [16 heads, 128 dims], then each head's maximum and sum of weights.  A
+// sum below zero marks an absent node.
+constexpr int kSlot = kGqa * kHeadDim + 2 * kGqa;
+
+template <int DT, bool SPLIT>
+__global__ __launch_bounds__(kSmallThreads) void dv_tree_small(const DecodeParams p, int windows, int window) {
     using raw = typename Tr<DT>::raw;
     constexpr int kP = kQPieces<DT>;
     constexpr int kRowBytes = kHeadDim * Tr<DT>::kBytes;
     constexpr int kRun = 16 / Tr<DT>::kBytes;     // elements of a piece
     constexpr int kMaxViews = kSmallQueryBytes / (kP * kWave * 16);
-    __shared__ __align__(16) float s_x[kSmallEntries * kGqa];
-    __shared__ __align__(16) int s_row[kSmallEntries];
-    __shared__ int s_par[kSmallEntries];
+    __shared__ __align__(16) float s_x[kEntries * kGqa];
+    __shared__ __align__(16) int s_row[kEntries];
+    __shared__ int s_par[kEntries];
     __shared__ u32x4 s_q[kMaxViews * kP * kWave];
     __shared__ float s_m[kSmallWaves][kGqa], s_l[kSmallWaves][kGqa];
     __shared__ int s_count;
     const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6);
     const int g = lane >> 4, n = lane & 15;
     const int hkv = blockIdx.x % p.Hkv;
-    const int ws = blockIdx.x / p.Hkv;
+    const int item = blockIdx.x / p.Hkv;
+    const int ws = SPLIT ? item / windows : item;
+    const int part = SPLIT ? item - ws * windows : 0;
     const int w = ws / p.S, s = ws - w * p.S;
     for (int i = tid; i < p.S; i += kSmallThreads) s_par[i] = p.parents[(long long)w * p.S + i];
     // per view: its first stream row, and the list's entries before it
     long long off[kMaxViews];
     int at[kMaxViews + 1], seen[kMaxViews];
     const long long rows = (long long)p.maxB * p.bs;
-    const int room = kSmallEntries - (p.S + 15) / 16 * 16;
+    const int room = windows * window;
     const int tv = p.tree_views[w], first = p.tree_rows[w];
     long long own_off = 0;
     int own_len = 0, own_loc = -1;
@@ -300,12 +307,20 @@ __global__ __launch_bounds__(kSmallThreads) void dv_tree_small(const DecodeParam
             at[f + 1] = at[f] + (seen[f] + 15) / 16 * 16;
         }
     }
-    const int base = at[kMaxViews];
+    // this block's committed entries: [lo, lo + base) of the list
+    const int lo = SPLIT ? part * window : 0;
+    const int rest = at[kMaxViews] - lo;
+    const int base = rest < 0 ? 0 : rest < window ? rest : window;
+    float* slot = SPLIT ? p.part + ((long long)ws * p.Hkv + hkv) * windows * kSlot + part * kSlot : nullptr;
+    if (SPLIT && part > 0 && base == 0) {
+        if (tid < 2 * kGqa) slot[kGqa * kHeadDim + tid] = tid < kGqa ? -DV_INF : 0.0f;
+        return;
+    }
     const bool has_view = tv >= 0 && tv < p.F;
     __syncthreads();
     if (wv == 0) {
         int count = 0;
-        if (lane == 0) s_count = count = walk_path(s_par, s, s_row + base);
+        if (lane == 0) s_count = count = part > 0 ? 0 : walk_path(s_par, s, s_row + base);
         count = uniform(count);
         if (count > 0)
             for (int i = lane; i < (count + 15) / 16 * 16; i += kWave) {
@@ -323,7 +338,7 @@ __global__ __launch_bounds__(kSmallThreads) void dv_tree_small(const DecodeParam
             int r = -1;
 #pragma unroll
             for (int f = 0; f < kMaxViews; ++f)
-                if (i >= at[f] && i - at[f] < seen[f]) r = page_row(p, w, off[f] + (i - at[f]));
+                if (lo + i >= at[f] && lo + i - at[f] < seen[f]) r = page_row(p, w, off[f] + (lo + i - at[f]));
             s_row[i] = r;
         }
         // the token's 16 heads in the MFMA's operand order, rotated for each view
@@ -345,6 +360,10 @@ __global__ __launch_bounds__(kSmallThreads) void dv_tree_small(const DecodeParam
     const int count = s_count;
     if (count < 0) {
         raw* o = reinterpret_cast<raw*>(p.out) + (((long long)w * p.Hq + hkv * kGqa) * p.S + s) * kHeadDim;
+        if constexpr (SPLIT) {
+            if (tid < 2 * kGqa) slot[kGqa * kHeadDim + tid] = tid < kGqa ? -DV_INF : -1.0f;
+            return;
+        }
         for (int i = tid; i < kGqa * kHeadDim; i += kSmallThreads)
             o[(long long)(i / kHeadDim) * p.S * kHeadDim + i % kHeadDim] = raw(0);
         return;
@@ -365,7 +384,7 @@ __global__ __launch_bounds__(kSmallThreads) void dv_tree_small(const DecodeParam
         for (int cc = 0; cc < kP; ++cc) k[cc] = ld16(src + cc * 64);
         int f = 0;
 #pragma unroll
-        for (int v = 1; v < kMaxViews; ++v) f = t * 16 >= at[v] ? v : f;
+        for (int v = 1; v < kMaxViews; ++v) f = lo + t * 16 >= at[v] ? v : f;
         if (t * 16 >= base) f = has_view ? tv : 0;
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -447,7 +466,8 @@ __global__ __launch_bounds__(kSmallThreads) void dv_tree_small(const DecodeParam
     float sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < kSmallWaves; ++v) sum += s_l[v][h];
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key at all: zeros (a NaN sum stays NaN)
+    // no key at all: zeros (a NaN sum stays NaN)
+    const float inv = SPLIT ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
     float o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -459,43 +479,131 @@ __global__ __launch_bounds__(kSmallThreads) void dv_tree_small(const DecodeParam
             a += s_x[((v * 8 + e) * kWave + (r >> 2) * 16 + h) * 4 + (r & 3)];
         o[j] = a * inv;
     }
+    if constexpr (SPLIT) {
+        *reinterpret_cast<f32x4*>(slot + h * kHeadDim + d) = f32x4{o[0], o[1], o[2], o[3]};
+        if (tid < kGqa) slot[kGqa * kHeadDim + tid] = m;
+        if (d == 0) slot[kGqa * kHeadDim + kGqa + h] = sum;
+        return;
+    }
     raw* dst = reinterpret_cast<raw*>(p.out) + (((long long)w * p.Hq + hkv * kGqa + h) * p.S + s) * kHeadDim + d;
     if constexpr (DT == kF32) *reinterpret_cast<f32x4*>(dst) = f32x4{o[0], o[1], o[2], o[3]};
     else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3]));
 }
 
-}  // namespace chunk
-
-// Keys and nodes up to which one launch is the faster way, 8 KV heads, us here / with two
-// launches.  bf16: 8 nodes on 200 keys 11 / 24, 16 nodes of four sequences on 400 keys
-// 23 / 33, of eight (1024 blocks) 43.5 / 46, 64 nodes of four sequences on 200 (2048
-// blocks) 51 / 49; on 1000 keys 29 / 26 for 8 nodes and 30 / 35 for 32, 65 / 39 for 16 of
-// four sequences.  fp32: 12 / 64, 31 / 92, 56 / 163, 65 / 124; on 1000 keys 34 / 56, 36 /
-// 83, 81 / 144.
-int tree_entries(int dtype, const DecodeParams& p) {
-    const long long blocks = (long long)p.W * p.Hkv * p.S;
-    const long long view = (long long)kGqa * kHeadDim * (dtype == kF32 ? 4 : 2);  // bytes of a view's queries
-    const long long keys = (long long)p.maxB * p.bs + 15ll * p.F + p.S + 15;
-    if (p.F * view > chunk::kSmallQueryBytes) return 0;
-    if (keys <= chunk::kEntries && blocks <= (dtype == kF32 ? 4096 : 1024)) return chunk::kEntries;
-    return dtype == kF32 && keys <= chunk::kManyEntries && blocks <= 1024 ? chunk::kManyEntries : 0;
+// Block (sequence, node, KV head): thread t -> head t / 16, dims [(t % 16) * 8, +8).
+template <int DT>
+__global__ __launch_bounds__(256) void dv_tree_join(const DecodeParams p, int windows) {
+    const int n = threadIdx.x >> 4, d = (threadIdx.x & 15) * 8;
+    const int hkv = blockIdx.x % p.Hkv;
+    const int ws = blockIdx.x / p.Hkv;
+    const int w = ws / p.S, s = ws - w * p.S;
+    const float* slots = p.part + ((long long)ws * p.Hkv + hkv) * windows * kSlot;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float m = -DV_INF, sum = 0.0f;
+    const bool absent = slots[kGqa * kHeadDim + kGqa + n] < 0.0f;
+    for (int k0 = 0; k0 < windows && !absent; k0 += kTreeBatch) {
+        float km[kTreeBatch], ks[kTreeBatch];
+        Run8<kF32> x[kTreeBatch];
+#pragma unroll
+        for (int i = 0; i < kTreeBatch; ++i) {
+            const bool in = k0 + i < windows;
+            const float* sp = slots + (long long)(in ? k0 + i : k0) * kSlot;
+            km[i] = in ? sp[kGqa * kHeadDim + n] : -DV_INF;
+            ks[i] = in ? sp[kGqa * kHeadDim + kGqa + n] : 0.0f;
+            x[i].load(sp + n * kHeadDim, d);
+        }
+        float bm = m;
+#pragma unroll
+        for (int i = 0; i < kTreeBatch; ++i) bm = fmaxf(bm, km[i]);
+        const float bz = bm == -DV_INF ? 0.0f : bm;
+        const float sc = __builtin_amdgcn_exp2f(m - bz);
+        sum *= sc;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] *= sc;
+#pragma unroll
+        for (int i = 0; i < kTreeBatch; ++i) {
+            if (ks[i] == 0.0f) continue;  // no key: the rest of the slot holds nothing
+            const float wgt = km[i] == -DV_INF ? 1.0f : __builtin_amdgcn_exp2f(km[i] - bz);
+            sum = __builtin_fmaf(wgt, ks[i], sum);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __builtin_fmaf(wgt, x[i][e], v[e]);
+        }
+        m = bm;
+    }
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] *= inv;
+    store_run8<DT>(reinterpret_cast<typename Tr<DT>::raw*>(p.out) +
+                       (((long long)w * p.Hq + hkv * kGqa + n) * p.S + s) * kHeadDim + d,
+                   v);
 }
 
-hipError_t launch_tree_small(int dtype, const DecodeParams& p, hipStream_t stream) {
+}  // namespace chunk
+
+// Keys and nodes up to which this is the faster way, 8 KV heads of one sequence, us here /
+// with the multi-query kernel.  One launch, bf16: 8 nodes on 200 keys 11 / 24; 16 nodes of
+// four sequences on 400 keys 23 / 33, of eight (1024 blocks) 43.5 / 46; 64 nodes of four
+// sequences on 200 (2048 blocks) 51 / 49.  fp32: 12 / 64, 31 / 92, 56 / 163, 65 / 124.
+// Windows, bf16: 8 nodes on 1000 keys 16.6 / 25.6, on 3000 26 / 30; 32 on 1000 30 / 34;
+// (more entries, nodes times keys:) 64 on 1000 55 / 41.  fp32: 19 / 56, 35 / 81, 39 / 83,
+// 73 / 135; 8 on 8000 84 / 89.
+TreePlan tree_plan(int dtype, int F, int W, int S, int Hkv, long long max_keys) {
     using namespace chunk;
-    const dim3 grid((unsigned)(p.W * p.Hkv * p.S)), block(kSmallThreads);
+    TreePlan t{0, 0};
+    if (S > kEntries / 2 || (long long)W * Hkv > (1 << 20) || max_keys > (1 << 24)) return t;
+    const long long nodes = (long long)W * Hkv * S;
+    const long long view = (long long)kGqa * kHeadDim * (dtype == kF32 ? 4 : 2);  // bytes of a view's queries
+    const long long keys = (max_keys + 15ll * F + 15) / 16 * 16;                  // the committed list at most
+    const long long path = (S + 15ll) / 16 * 16;
+    if (F * view > kSmallQueryBytes) return t;
+    if (keys + path <= kEntries && nodes <= (dtype == kF32 ? 4096 : 1024)) return TreePlan{1, (int)keys};
+    if (nodes * keys > (dtype == kF32 ? 600 : 288) * 1024ll) return t;
+    // Two blocks share a CU and take about as long for entries + 160 (in bf16: 11.7 us for
+    // 128 entries, 15.8 for 224, 23 for 416): as many windows as make the rounds of 512
+    // blocks shortest, fewer ones where that is even.
+    long long best = 0;
+    for (long long n = (keys + kEntries - path - 1) / (kEntries - path); n <= (keys + 127) / 128; ++n) {
+        const long long window = ((keys + n - 1) / n + 15) / 16 * 16;
+        const long long cost = (nodes * n + 511) / 512 * (window + 160);
+        if (t.windows == 0 || cost < best) {
+            best = cost;
+            t = TreePlan{(int)((keys + window - 1) / window), (int)window};
+        }
+    }
+    return t;
+}
+
+size_t tree_workspace_bytes(const TreePlan& t, int W, int S, int Hkv) {
+    return t.windows > 1 ? (size_t)W * S * Hkv * t.windows * chunk::kSlot * sizeof(float) : 0;
+}
+
+namespace {
+
+template <int DT>
+hipError_t tree_go(const TreePlan& t, const DecodeParams& p, hipStream_t stream) {
+    using namespace chunk;
+    const unsigned nodes = (unsigned)(p.W * p.Hkv * p.S);
+    if (t.windows == 1) {
+        hipLaunchKernelGGL((dv_tree_small<DT, false>), dim3(nodes), dim3(kSmallThreads), 0, stream, p, 1, t.window);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL((dv_tree_small<DT, true>), dim3(nodes * t.windows), dim3(kSmallThreads), 0, stream, p,
+                       t.windows, t.window);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(dv_tree_join<DT>, dim3(nodes), dim3(256), 0, stream, p, t.windows);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_tree_small(int dtype, const TreePlan& t, const DecodeParams& p, hipStream_t stream) {
     switch (dtype) {
-        case kBF16: hipLaunchKernelGGL((dv_tree_small<kBF16, kEntries>), grid, block, 0, stream, p); break;
-        case kF16: hipLaunchKernelGGL((dv_tree_small<kF16, kEntries>), grid, block, 0, stream, p); break;
-        case kF32:
-            if (tree_entries(dtype, p) == kEntries)
-                hipLaunchKernelGGL((dv_tree_small<kF32, kEntries>), grid, block, 0, stream, p);
-            else
-                hipLaunchKernelGGL((dv_tree_small<kF32, kManyEntries>), grid, block, 0, stream, p);
-            break;
+        case kBF16: return tree_go<kBF16>(t, p, stream);
+        case kF16: return tree_go<kF16>(t, p, stream);
+        case kF32: return tree_go<kF32>(t, p, stream);
         default: return hipErrorInvalidValue;
     }
-    return hipGetLastError();
 }
 
 hipError_t launch_merge_tree(int dtype, const DecodeParams& p, int ntb, hipStream_t stream) {

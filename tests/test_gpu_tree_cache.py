@@ -93,10 +93,11 @@ def widened(d, rows):
 
 
 def check_tree(dv, gpu, d, dtype, scale=SCALE):
-    """Under the given block table, where one launch may take the call, and under a wide one,
-    where pieces of the committed keys are merged."""
+    """Under the given block table, where one launch may take the call, under a wider one,
+    which cuts the nodes' key lists into windows, and under a wide one, where pieces of the
+    committed keys are merged."""
     want, size, spread = TO.tree_sdpa(scale, **d)
-    for case in (widened(d, 2000), d):
+    for case in (widened(d, 80000), widened(d, 2500), d):
         got = compare_tree(dv.dvattn_tree_paged_sdpa(scale=scale, **to(gpu, case)).cpu(), d, dtype, want, size, spread)
     return got, want
 
@@ -127,6 +128,7 @@ TREES = [
     (1, 1, 64, [1100], 16, 128),
     (1, 2, 100, [110], 16, 64),        # a path longer than a wave has lanes; just nodes
     (2, 1, 3, [25, 1, 40, 60], 24, 64),  # four views
+    (2, 1, 4, [300, 900], 16, 128),    # windows that meet two views
 ]
 
 

@@ -66,9 +66,10 @@ def test_attention_shapes_refused(lib, call, kw, status, needle):
     (mass, ("out", "mass", "loc", "q", "cos", "sin", "fl", "kc", "bt", "ws")),
 ])
 def test_null_and_misaligned_pointers_refused(lib, call, names):
+    s = shape(max_blocks_per_seq=400)  # (short sequences' trees need no workspace)
     for name in names:
-        assert call(lib, shape(), **{name: None}) in (INVALID, WORKSPACE), name
-        assert call(lib, shape(), **{name: P + 2}) == INVALID, name
+        assert call(lib, s, **{name: None}) in (INVALID, WORKSPACE), name
+        assert call(lib, s, **{name: P + 2}) == INVALID, name
         assert "aligned" in error(lib), name
 
 
@@ -76,7 +77,7 @@ def test_workspace_refused(lib):
     for call, size in ((tree, lib.dvattn_tree_paged_sdpa_workspace_size),
                        (mass, lib.dvattn_paged_key_mass_workspace_size)):
         for S in (1, 4):
-            s = shape(S=S)
+            s = shape(S=S, max_blocks_per_seq=400)
             need = size(2, ctypes.byref(s), 64 if call is mass else 0)
             assert need > 0
             assert call(lib, s, ws_bytes=need - 1) == WORKSPACE
@@ -100,6 +101,26 @@ def test_workspace_is_bounded(lib):
     a, b = (shape(S=s, W=1, max_blocks_per_seq=4096) for s in (64, 64 * 32))
     queries = 16 * 128 * 2
     assert size(2, ctypes.byref(b), 0) - size(2, ctypes.byref(a), 0) == (b.S - a.S) * queries
+
+
+def test_tree_workspace(lib):
+    """None where one launch goes through a node's whole key list; windows of the lists, then
+    the pieces of the committed keys, beyond."""
+    size = lib.dvattn_tree_paged_sdpa_workspace_size
+    need = lambda dtype, **kw: size(dtype, ctypes.byref(shape(**kw)), 0)
+    assert need(2) == 0 and need(0, S=100, max_blocks_per_seq=20) == 0
+    slot = (16 * 128 + 32) * 4
+    for kw in (dict(max_blocks_per_seq=100), dict(max_blocks_per_seq=300, S=9), dict(max_blocks_per_seq=500, W=1, S=1)):
+        n = need(2, **kw)
+        s = shape(**kw)
+        nodes = s.W * s.S * s.Hkv
+        assert n > 0 and n % (nodes * slot) == 0
+        windows = n // (nodes * slot)
+        assert windows * 640 >= s.max_blocks_per_seq * 16 and windows <= s.max_blocks_per_seq * 16 / 128 + 1
+    pieces = need(2, S=64, max_blocks_per_seq=10 ** 6)
+    assert pieces > 0 and pieces == need(2, S=64, max_blocks_per_seq=2 ** 20) == need(2, F=60, S=64)
+    assert need(2, W=-1) == need(2, max_blocks_per_seq=-1) == 0
+    assert need(2, W=2 ** 31 - 1, Hkv=2 ** 31 - 1, S=300) >= 0
 
 
 def test_empty_calls_succeed(lib):
