@@ -295,7 +295,7 @@ __global__ __launch_bounds__(256) void dv_tree_meta(const TreeMetaParams tp, int
         s_sum = 0;
     }
     __syncthreads();
-    for (int v = tid; v < p.W; v += 256) {
+    for (int v = tid; v < p.W && p.F > 0; v += 256) {
         const int g = p.order[(long long)v * p.F + p.F - 1];
         if (g >= 0 && g < p.F) s_drafted[g] = 1;
     }
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(256) void dv_tree_meta(const TreeMetaParams tp, int
     }
     if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(&s_sum), (unsigned long long)mine);
     const int s0 = tile * kTreeTile;
-    const int ns = p.S - s0 < kTreeTile ? p.S - s0 : kTreeTile;
+    const int ns = p.F == 0 ? 0 : p.S - s0 < kTreeTile ? p.S - s0 : kTreeTile;
     if (tid < ns) {
         // every step goes to an earlier node, so the walk ends
         int j = s0 + tid, dep = 0;
@@ -379,10 +379,11 @@ __global__ __launch_bounds__(256) void dv_tree_meta(const TreeMetaParams tp, int
 }
 
 hipError_t launch_tree_meta(const TreeMetaParams& p, hipStream_t stream) {
-    const int tiles = (p.m.S + kTreeTile - 1) / kTreeTile;
-    const long long blocks = (long long)p.m.F * p.m.W * tiles;
+    // (without views or nodes a block per sequence still writes the drafted rows' place)
+    const int tiles = p.m.S > 0 ? (p.m.S + kTreeTile - 1) / kTreeTile : 1;
+    const long long blocks = (long long)(p.m.F > 0 ? p.m.F : 1) * p.m.W * tiles;
     if (blocks == 0) return hipSuccess;
-    if (blocks >= (1ll << 31)) return hipErrorInvalidValue;  // the C ABI rejects such calls first
+    if (blocks >= (1ll << 24)) return hipErrorInvalidValue;  // the C ABI rejects such calls first
     const size_t lds = (size_t)(p.m.F + p.m.S + kTreeTile) * sizeof(int);
     auto al = [](const void* ptr) { return ((uintptr_t)ptr & 15) == 0; };
     const bool vec = (p.m.R / 2) % 4 == 0 && al(p.m.cosv) && al(p.m.sinv);

@@ -822,13 +822,14 @@ dvattn_status dvattn_tree_metadata(int* locations, float* cosines, float* sines,
     if (S > dv::kMaxTreeNodes || F > dv::kMaxTreeViews)
         return fail(DVATTN_ERR_UNSUPPORTED, "at most %d drafted nodes and %d views (S=%d, F=%d)", dv::kMaxTreeNodes,
                     dv::kMaxTreeViews, S, F);
-    if ((long long)F * W * S == 0) return ok();
+    if (W == 0) return ok();
     // a launch holds 2^24 blocks of 256 threads: one per (view, sequence) and 64 nodes
-    if ((long long)F * W * ((S + 63) / 64) >= (1ll << 24))
+    if ((long long)(F > 0 ? F : 1) * W * (S > 0 ? (S + 63) / 64 : 1) >= (1ll << 24))
         return fail(DVATTN_ERR_UNSUPPORTED, "%lld (view, sequence) pairs of %d nodes exceed one launch",
                     (long long)F * W, S);
-    if (!locations || !tree_views || !tree_rows || !fragment_lengths || !order || !parents ||
-        (rotary_dim > 0 && (!cosines || !sines || !inv_freq)))
+    const bool nodes = F > 0 && S > 0;
+    if (!tree_views || !tree_rows || (F > 0 && (!fragment_lengths || !order)) || (S > 0 && !parents) ||
+        (nodes && (!locations || (rotary_dim > 0 && (!cosines || !sines || !inv_freq)))))
         return fail(DVATTN_ERR_INVALID, "null pointer");
     const dvattn_status st = check_aligned({{locations, "locations", 4}, {cosines, "cosines", 4}, {sines, "sines", 4},
                                             {tree_views, "tree_views", 4}, {tree_rows, "tree_rows", 4},
@@ -1078,6 +1079,8 @@ dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, c
         return fail(DVATTN_ERR_UNSUPPORTED, "W * Hkv = %lld and N = %d: below 2^15 and at most 2^30",
                     (long long)s->W * s->Hkv, N);
     if (mass && !lengths) return fail(DVATTN_ERR_INVALID, "mass needs lengths");
+    if (mass && capacity > (1ll << 30))
+        return fail(DVATTN_ERR_UNSUPPORTED, "capacity %lld exceeds 2^30 rows", capacity);
     if (N == 0 && !mass) return ok();
     if (!first_rows || (N > 0 && !rows) || (s->max_blocks_per_seq > 0 && !block_tables) ||
         (s->num_blocks > 0 && ((s->E > 0 && !k_cache) || (s->Ev > 0 && !v_cache))))

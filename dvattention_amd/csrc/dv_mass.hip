@@ -526,6 +526,7 @@ __global__ __launch_bounds__(kSmallThreads) void dv_mass_small(const MassParams 
             const float lw = rows4_sum(l * __builtin_amdgcn_exp2f(m - (mw == -DV_INF ? 0.0f : mw)));
             if (lane < kGqa) s_nl[s][n] = minus_lse(mw, lw);
         }
+        lds_wait();  // read by the wave's other lanes
     } else {
         for (int s = wv; s < S; s += kSmallWaves)
             if (lane < kGqa) s_pair[s][n] = make_float2(-DV_INF, 0.0f);

@@ -821,6 +821,8 @@ void dvattn_paged_kv_compact_op(at::Tensor& k_cache, at::Tensor& v_cache, const 
     for (const at::Tensor* c : {&k_cache, &v_cache})
         TORCH_CHECK(c->size(3) <= 1 || c->stride(3) == 1,
                     "dvattn_paged_kv_compact: the last dim of the caches must be contiguous");
+    at::assert_no_internal_overlap(k_cache);
+    at::assert_no_internal_overlap(v_cache);
     TORCH_CHECK(v_cache.size(0) == P && v_cache.size(1) == bs && v_cache.size(2) == Hkv,
                 "dvattn_paged_kv_compact: v_cache must be [num_blocks, block_size, Hkv, Ev], got ", v_cache.sizes());
     TORCH_CHECK(rows.size(1) == Hkv || rows.size(1) == 1, "dvattn_paged_kv_compact: rows must be [W,Hkv|1,N] with Hkv=",

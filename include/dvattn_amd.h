@@ -288,7 +288,8 @@ DVATTN_API dvattn_status dvattn_view_metadata(int* locations, float* cosines, fl
  *                        fragment_lengths before the view; node s is written to
  *                        tree_rows[w] + s (dvattn_paged_kv_append's positions)
  * Absent nodes and views missing from a sequence's order get location -1, cos 1,
- * sin 0.  The other sequences' drafted nodes are neither seen nor counted.  For
+ * sin 0.  Without views (F = 0) or nodes (S = 0) tree_views and tree_rows (0 for no
+ * view) are still written.  The other sequences' drafted nodes are neither seen nor counted.  For
  * one sequence and a chain (parents -1, 0, 1, ...) cos/sin are
  * dvattn_view_metadata's.  S <= 4096, F <= 4096. */
 #define DVATTN_MAX_TREE_NODES 4096
@@ -356,7 +357,8 @@ DVATTN_API dvattn_status dvattn_kv_select(int* rows, const float* mass, const in
  * tree_rows).  Entries may come in any order and more than once; one below its place,
  * past the range, or whose source or destination lies on no valid page moves nothing.
  * With mass [W,Hkv,capacity] f32 (needs lengths) its entries move alike, and those of
- * the rows first_rows[w] + i, i < lengths[w], that nothing moves into become 0.  Uses
+ * the rows first_rows[w] + i, i < lengths[w], that nothing moves into become 0
+ * (capacity <= 2^30).  Uses
  * shape fields W, Hkv, E, Ev, block_size, max_blocks_per_seq, num_blocks and the
  * layout's cache strides.  The pages of the rows moved must each be named once in
  * block_tables (pages shared by sequences or segments lie before first_rows). */

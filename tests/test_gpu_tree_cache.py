@@ -451,6 +451,12 @@ def test_compact_head_dims(dv, gpu, dtype, Ek, Ev):
     check_compact(dv, gpu, *compact_case(dtype, 2, 2, 90, 40, 8, seed=2, Ek=Ek, Ev=Ev))
 
 
+def test_compact_refuses_overlapping_rows(dv, gpu):
+    kc, vc, bt, rows, first, lengths, mass = (t.to(gpu) for t in compact_case(torch.float16, 1, 2, 40, 10, 16, seed=2))
+    with pytest.raises(RuntimeError, match="memory"):
+        dv.dvattn_paged_kv_compact(rows, first, kc[:, :, :1].expand(-1, -1, 2, -1), vc, bt)
+
+
 def test_compact_many_rows(dv, gpu):
     """Several batches of rows, where sources of later batches lie among the
     destinations of earlier ones' neighbours."""
@@ -512,6 +518,20 @@ def test_tree_metadata_orders(dv, gpu):
     check_meta(dv, gpu, fl, order, parents, inv)
 
 
+def test_tree_metadata_without_nodes_or_views(dv, gpu):
+    """The place of the drafted rows is written for S = 0 and F = 0 too."""
+    fl, order, parents, inv = meta_inputs(3, 2, 4, 64, seed=3)
+    loc, cos, _, views, rows = dv.dvattn_tree_metadata(fl.to(gpu), order.to(gpu), parents[:, :0].contiguous().to(gpu),
+                                                       inv.to(gpu))
+    own = order[:, -1].long()
+    want = [int(fl[:o + 1].sum()) if 0 <= o < 2 else 0 for o in own.tolist()]  # S = 0: behind the view's rows
+    assert loc.shape == (2, 3, 0) and cos.shape == (2, 3, 0, 64)
+    assert views.tolist() == [o if 0 <= o < 2 else -1 for o in own.tolist()] and rows.tolist() == want
+    views, rows = dv.dvattn_tree_metadata(fl[:0].to(gpu), order[:, :0].contiguous().to(gpu), parents.to(gpu),
+                                          inv.to(gpu))[3:]
+    assert views.tolist() == [-1] * 3 and rows.tolist() == [0] * 3
+
+
 @pytest.mark.parametrize("round_to", [None, torch.bfloat16, torch.float16])
 def test_tree_metadata_chain_is_view_metadata(dv, gpu, round_to):
     """One sequence drafting a chain: the tables of S ordinary new tokens, bit for bit."""
@@ -528,20 +548,22 @@ def test_tree_metadata_chain_is_view_metadata(dv, gpu, round_to):
 # ---------------------------------------------------------------------------
 def everything(dv, gpu, dtype):
     """One call of each operator on inputs of its own; returns (run, state to restore)."""
-    d = to(gpu, tree_case(dtype, 2, 2, 10, [60, 90], 16, 64, seed=21))
+    trees = [to(gpu, widened(tree_case(dtype, 2, 2, 10, [60, 90], 16, 64, seed=21), n)) for n in (0, 2500, 80000)]
     md, mass = mass_case(dtype, 2, 2, 1, [200], 16, 64, seed=22)
     md3, mass3 = mass_case(dtype, 2, 2, 3, [200], 16, 64, seed=23)
+    mdw = to(gpu, widened(md3, 40000))
     md, md3, mass, mass3 = to(gpu, md), to(gpu, md3), mass.to(gpu), mass3.to(gpu)
     fl, order, parents, inv = (t.to(gpu) for t in meta_inputs(2, 2, 10, 64, seed=24))
     kc, vc, bt, rows, first, lengths, cm = (t.to(gpu) for t in compact_case(dtype, 2, 2, 150, 60, 16, seed=25))
     k0, v0, cm0, mass_out = kc.clone(), vc.clone(), cm.clone(), torch.empty_like(mass)
-    mass3_out = torch.empty_like(mass3)
+    mass3_out, massw_out = torch.empty_like(mass3), torch.empty_like(mass3)
 
     def run():
         kc.copy_(k0), vc.copy_(v0), cm.copy_(cm0)
-        out = [dv.dvattn_tree_paged_sdpa(scale=SCALE, **d)]
+        out = [dv.dvattn_tree_paged_sdpa(scale=SCALE, **d) for d in trees]
         out.append(dv.dvattn_paged_key_mass(mass, scale=SCALE, decay=0.5, out=mass_out, **md))
         out.append(dv.dvattn_paged_key_mass(mass3, scale=SCALE, decay=0.5, out=mass3_out, **md3))
+        out.append(dv.dvattn_paged_key_mass(mass3, scale=SCALE, decay=0.5, out=massw_out, **mdw))
         out += dv.dvattn_tree_metadata(fl, order, parents, inv)
         out.append(dv.dvattn_kv_select(mass, first, lengths, 40, 2, 5))
         dv.dvattn_paged_kv_compact(rows, first, kc, vc, bt, mass=cm, lengths=lengths)
@@ -574,6 +596,40 @@ def test_capture_and_streams(dv, gpu, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(eager, again, captured))
+
+
+def test_pages_beyond_4_gib(dv, gpu):
+    """The same bits from pages whose bytes lie past 2^32 of a cache."""
+    bs, far = 16, (1 << 20) + 100  # pages of 4 KiB
+    big = [torch.empty(far + 300, bs, 1, E, dtype=torch.float16, device=gpu) for _ in range(2)]
+    table = lambda bt: torch.where(bt >= 0, bt + far, bt)
+
+    def place(d):
+        n = d["k_cache"].shape[0]
+        out = dict(d, k_cache=big[0], block_tables=table(d["block_tables"]))
+        big[0][far:far + n] = d["k_cache"]
+        if "v_cache" in d and "parents" in d:
+            big[1][far:far + n] = d["v_cache"]
+            out["v_cache"] = big[1]
+        return out
+
+    tree = tree_case(torch.float16, 2, 1, 6, [60, 90], bs, 64, seed=41)
+    for rows in (0, 2500, 80000):
+        d = to(gpu, widened(tree, rows))
+        assert torch.equal(dv.dvattn_tree_paged_sdpa(scale=SCALE, **d),
+                           dv.dvattn_tree_paged_sdpa(scale=SCALE, **place(d)))
+    for S, rows in ((1, 0), (3, 0), (3, 40000)):
+        md, mass = mass_case(torch.float16, 2, 1, S, [200], bs, 64, seed=42)
+        md = to(gpu, widened(md, rows))
+        out = [dv.dvattn_paged_key_mass(mass.to(gpu), scale=SCALE, **x) for x in (md, place(md))]
+        assert torch.equal(*out)
+    kc, vc, bt, rows, first, lengths, _ = (t.to(gpu) for t in compact_case(torch.float16, 2, 1, 150, 60, bs, seed=43,
+                                                                           heads=1))
+    n = kc.shape[0]
+    big[0][far:far + n], big[1][far:far + n] = kc, vc
+    dv.dvattn_paged_kv_compact(rows, first, kc, vc, bt, lengths=lengths)
+    dv.dvattn_paged_kv_compact(rows, first, big[0], big[1], table(bt), lengths=lengths)
+    assert torch.equal(big[0][far:far + n], kc) and torch.equal(big[1][far:far + n], vc)
 
 
 def test_drafted_and_bounded_decoding(dv, gpu):

@@ -129,7 +129,7 @@ def test_empty_calls_succeed(lib):
     assert tree(lib, shape(S=0)) == 0 and mass(lib, shape(), capacity=0) == 0
     assert select(lib, W=0) == 0 and select(lib, budget=0, kf=0, kl=0) == 0
     assert compact(lib, shape(W=0)) == 0 and compact(lib, shape(), N=0) == 0
-    assert meta(lib, S=0) == 0 and meta(lib, F=0) == 0
+    assert meta(lib, W=0) == 0
 
 
 def select(lib, capacity=100, W=2, Hkv=1, budget=8, kf=1, kl=2, rows=P, m=P, first=P, lengths=P):
@@ -180,6 +180,7 @@ def compact(lib, s, row_heads=1, N=4, dtype=2, capacity=64, layout=True, **ptr):
     (dict(rows=P + 2), INVALID, "aligned"),
     (dict(dtype=9), UNSUPPORTED, "dtype"),
     (dict(layout=False), INVALID, "layout"),
+    (dict(capacity=(1 << 30) + 1), UNSUPPORTED, "2^30"),
 ])
 def test_compact_refused(lib, kw, status, needle):
     assert compact(lib, shape(), **kw) == status
@@ -212,6 +213,10 @@ def meta(lib, F=1, W=2, S=4, R=64, round_dtype=-1, **ptr):
     (dict(loc=None), INVALID, "null"),
     (dict(parents=None), INVALID, "null"),
     (dict(views=None), INVALID, "null"),
+    (dict(views=None, S=0), INVALID, "null"),
+    (dict(rows=None, F=0), INVALID, "null"),
+    (dict(order=None, S=0), INVALID, "null"),
+    (dict(F=0, W=1 << 24), UNSUPPORTED, "one launch"),
     (dict(inv=None), INVALID, "null"),
     (dict(cos=P + 2), INVALID, "aligned"),
 ])
