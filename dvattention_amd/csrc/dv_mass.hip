@@ -482,34 +482,86 @@ __global__ __launch_bounds__(kMassThreads) void dv_mass_apply_scores(const MassP
 
 // S > 1 and few keys in all (a short cache, a single sequence): no launch fills the card,
 // so a call costs the longest chain of one of its waves and not its work.  Here the chain
-// is short: a block of eight waves takes NT * 16 stream rows, every wave holds all of
-// their K rows and takes every eighth token.  The first launch leaves (max, sum) per
-// block, token and head; the second joins them (each wave for its own tokens, eight
-// blocks' pairs loaded together: one after the other took up to 20 us of a call's 49),
-// adds the weights over its tokens, and the waves' shares in order.  The K rows come
-// through LDS: eight waves that each load them into registers cost 0.5 us per wave.
+// is short: a block of eight waves takes up to NT * 16 stream rows of one view (parts cut
+// across views' borders went through them one after the other: 33 tokens on two views of
+// 100 keys 32 us), every wave holds all of their K rows and takes every eighth token.  The
+// first launch leaves (max, sum) per block, token and head; the second joins them (each
+// wave for its own tokens, eight blocks' pairs loaded together: one after the other took
+// up to 20 us of a call's 49), adds the weights over its tokens, and the waves' shares in
+// order.  The K rows come through LDS: eight waves that each load them into registers
+// cost 0.5 us per wave.
 template <int DT, int NT, bool APPLY>
 __global__ __launch_bounds__(kSmallThreads) void dv_mass_small(const MassParams p) {
     constexpr int kRows = NT * 16;
     constexpr int kRowBytes = kHeadDim * Tr<DT>::kBytes;
     constexpr int kLanes = kRowBytes / 16;                       // lanes that copy one row
     __shared__ __align__(256) unsigned char s_keys[kRows * kRowBytes];
-    __shared__ float2 s_pair[APPLY ? 1 : kMassTokens][kGqa];     // (max, sum) of a token: its wave's own
-    __shared__ float s_nl[APPLY ? kMassTokens : 1][kGqa];        // minus its log-sum-exp
+    __shared__ float s_nl[APPLY ? kMassTokens : 1][kGqa];        // minus a token's log-sum-exp: its wave's own
     __shared__ float s_part[APPLY ? kSmallWaves : 1][kRows];
     const int lane = threadIdx.x & 63, wv = uniform((int)threadIdx.x >> 6);
     const int n = lane & 15, S = p.ns;
     const Item it = item_of(p);
-    const long long end = visible_end(p, it.w);
-    const long long b0 = it.chunk * kRows;
-    if (b0 >= end) {
-        if (APPLY && wv == 0) store_decayed(p, it.wh, b0, kRows);
+    // this block's rows: [c0, c0 + here) of view f, which starts at row off (the rows behind
+    // the last view and below the capacity count as one more view)
+    const long long rows = (long long)p.maxB * p.bs;             // keys lie below
+    const long long limit = rows > p.C ? rows : p.C;             // and outputs
+    int f = -1, len = 0, here = 0, count = 0;                    // count: of the views' blocks
+    long long c0 = 0, off = 0, end = 0;
+    for (int g = 0; g <= p.F && end < limit; ++g) {
+        const long long lo = end;
+        const long long all = g < p.F ? view_len(p, g) : limit - end;
+        end += all;
+        const long long left = all < limit - lo ? all : limit - lo;
+        const int blocks = (int)((left + kRows - 1) / kRows);
+        if (it.chunk >= count && it.chunk < count + blocks) {
+            f = g;
+            off = lo;
+            len = (int)all;
+            c0 = lo + (it.chunk - count) * kRows;
+            here = lo + left - c0 < kRows ? (int)(lo + left - c0) : kRows;
+        }
+        if (g < p.F) count += blocks;
+    }
+    if (f < 0) return;
+    float2* part = reinterpret_cast<float2*>(p.part) + it.wh * p.nchunks * S * kGqa;
+    // keys of the block that each token sees, token i in lane i
+    int ends = 0;
+    if (f < p.F) {
+        const long long below = seen_lane(p, f, it.w, len) - (c0 - off);
+        ends = below < 0 ? 0 : below < here ? (int)below : here;
+    }
+    const int most = lanes_max(ends);
+    const uint32_t row = cache_row(p, it.w, it.hkv, c0 + lane, lane < most);
+    const uint64_t valid = ballot(row != 0xffffffffu);
+    if (!valid) {
+        if constexpr (APPLY) {
+            if (wv == 0) store_decayed(p, it.wh, c0, here);
+        } else {
+            for (int i = threadIdx.x; i < S * kGqa && f < p.F; i += kSmallThreads)
+                part[it.chunk * S * kGqa + i] = make_float2(-DV_INF, 0.0f);
+        }
         return;
     }
-    float2* part = reinterpret_cast<float2*>(p.part) + it.wh * p.nchunks * S * kGqa;
+#pragma unroll
+    for (int i = wv; i < kRows * kLanes / kWave; i += kSmallWaves) {
+        const int r = i * (kWave / kLanes) + lane / kLanes;
+        const uint32_t id = (uint32_t)__shfl((int)row, r, kWave);
+        const unsigned char* src = id != 0xffffffffu ? reinterpret_cast<const unsigned char*>(p.kc) +
+                                                           (unsigned long long)id * kRowBytes
+                                                     : zero_row;
+        dma16(src + ((lane % kLanes) ^ (r & 15)) * 16,
+              __builtin_amdgcn_readfirstlane(lds_addr(s_keys) + (uint32_t)(i * 1024)));
+    }
+    u32x4 q[kPieces<DT>];
+    const u32x4* ops = reinterpret_cast<const u32x4*>(p.rq) +
+                       (((long long)f * p.W + it.w) * p.Hkv + it.hkv) * S * (kPieces<DT> * kWave) + lane;
+    auto query = [&](int s) {
+#pragma unroll
+        for (int cc = 0; cc < kPieces<DT>; ++cc) q[cc] = ld16(ops + (s * kPieces<DT> + cc) * kWave);
+    };
+    if (wv < S) query(wv);
     if constexpr (APPLY) {
         constexpr int kBatch = 8;
-        const int count = (int)((end + kRows - 1) / kRows);
         for (int s = wv; s < S; s += kSmallWaves) {
             float m = -DV_INF, l = 0.0f;
             for (int u0 = lane >> 4; u0 < count; u0 += 4 * kBatch) {
@@ -526,95 +578,48 @@ __global__ __launch_bounds__(kSmallThreads) void dv_mass_small(const MassParams 
             const float lw = rows4_sum(l * __builtin_amdgcn_exp2f(m - (mw == -DV_INF ? 0.0f : mw)));
             if (lane < kGqa) s_nl[s][n] = minus_lse(mw, lw);
         }
-        lds_wait();  // read by the wave's other lanes
-    } else {
-        for (int s = wv; s < S; s += kSmallWaves)
-            if (lane < kGqa) s_pair[s][n] = make_float2(-DV_INF, 0.0f);
     }
+    wait_vmcnt<0>();
+    __syncthreads();
+    u32x4 k[NT][kPieces<DT>];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int cc = 0; cc < kPieces<DT>; ++cc)
+            k[t][cc] = *reinterpret_cast<const u32x4*>(s_keys + (t * 16 + n) * kRowBytes +
+                                                       ((cc * 4 + (lane >> 4)) ^ n) * 16);
     f32x4 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    long long off = 0;
-    bool staged = false;
-    for (int f = 0; f < p.F && off < b0 + kRows && off < end; ++f) {
-        const int len = view_len(p, f);
-        const long long lo = off - b0;  // the view's first row in the block
-        off += len;
-        if (off <= b0) continue;
-        // keys of the block below what each token sees, token i in lane i
-        const long long below = seen_lane(p, f, it.w, len) + lo;
-        const int ends = below < 0 ? 0 : below < kRows ? (int)below : kRows;
-        const int most = lanes_max(ends);
-        const uint32_t row = cache_row(p, it.w, it.hkv, b0 + lane, lane >= lo && lane < most);
-        const uint64_t valid = ballot(row != 0xffffffffu);
-        if (!valid) continue;
-        if (staged) __syncthreads();  // the previous view's keys are read
-        staged = true;
-#pragma unroll
-        for (int i = wv; i < kRows * kLanes / kWave; i += kSmallWaves) {
-            const int r = i * (kWave / kLanes) + lane / kLanes;
-            const uint32_t id = (uint32_t)__shfl((int)row, r, kWave);
-            const unsigned char* src = id != 0xffffffffu ? reinterpret_cast<const unsigned char*>(p.kc) +
-                                                               (unsigned long long)id * kRowBytes
-                                                         : zero_row;
-            dma16(src + ((lane % kLanes) ^ (r & 15)) * 16,
-                  __builtin_amdgcn_readfirstlane(lds_addr(s_keys) + (uint32_t)(i * 1024)));
-        }
-        u32x4 q[kPieces<DT>];
-        const u32x4* ops = reinterpret_cast<const u32x4*>(p.rq) +
-                           (((long long)f * p.W + it.w) * p.Hkv + it.hkv) * S * (kPieces<DT> * kWave) + lane;
-        auto query = [&](int s) {
-#pragma unroll
-            for (int cc = 0; cc < kPieces<DT>; ++cc) q[cc] = ld16(ops + (s * kPieces<DT> + cc) * kWave);
-        };
-        if (wv < S) query(wv);
-        wait_vmcnt<0>();
-        __syncthreads();
-        u32x4 k[NT][kPieces<DT>];
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int cc = 0; cc < kPieces<DT>; ++cc)
-                k[t][cc] = *reinterpret_cast<const u32x4*>(s_keys + (t * 16 + n) * kRowBytes +
-                                                           ((cc * 4 + (lane >> 4)) ^ n) * 16);
 #pragma unroll 1
-        for (int s = wv; s < S; s += kSmallWaves) {
-            const uint64_t mask = valid & first_keys<NT>(__builtin_amdgcn_readlane(ends, s));
-            f32x4 x[NT];
-            dot_tiles<DT, NT>(k, q, x);
-            if (s + kSmallWaves < S) query(s + kSmallWaves);
-            scale_masked<NT>(x, mask, p.l2scale);
-            if constexpr (APPLY) {
-                const float nl = s_nl[s][n];
+    for (int s = wv; s < S; s += kSmallWaves) {
+        const uint64_t mask = valid & first_keys<NT>(__builtin_amdgcn_readlane(ends, s));
+        f32x4 x[NT];
+        dot_tiles<DT, NT>(k, q, x);
+        if (s + kSmallWaves < S) query(s + kSmallWaves);
+        scale_masked<NT>(x, mask, p.l2scale);
+        if constexpr (APPLY) {
+            const float nl = s_nl[s][n];
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[t][i] += weight(x[t][i], nl);
-            } else {
-                float mx = -DV_INF;
+                for (int i = 0; i < 4; ++i) acc[t][i] += weight(x[t][i], nl);
+        } else {
+            float mx = -DV_INF;
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    mx = fmaxf(mx, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
-                const float m = rows4_max(mx);
-                const float mz = m == -DV_INF ? 0.0f : m;
-                float l = 0.0f;
+            for (int t = 0; t < NT; ++t) mx = fmaxf(mx, fmaxf(fmaxf(x[t][0], x[t][1]), fmaxf(x[t][2], x[t][3])));
+            const float m = rows4_max(mx);
+            const float mz = m == -DV_INF ? 0.0f : m;
+            float l = 0.0f;
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(x[t][i] - mz);
-                l = rows4_sum(l);
-                if (lane < kGqa) {
-                    float2 e = s_pair[s][n];
-                    join(e.x, e.y, m, l);
-                    s_pair[s][n] = e;
-                }
-            }
+                for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(x[t][i] - mz);
+            l = rows4_sum(l);
+            if (lane < kGqa) part[(it.chunk * S + s) * kGqa + n] = make_float2(m, l);
         }
     }
-    if constexpr (!APPLY) {
-        for (int s = wv; s < S; s += kSmallWaves)
-            if (lane < kGqa) part[(it.chunk * S + s) * kGqa + n] = s_pair[s][n];
-    } else {
+    if constexpr (APPLY) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -623,8 +628,8 @@ __global__ __launch_bounds__(kSmallThreads) void dv_mass_small(const MassParams 
                 if (n == i) s_part[wv][t * 16 + (lane >> 4) * 4 + i] = a;
             }
         __syncthreads();
-        const long long c = b0 + threadIdx.x;
-        if (threadIdx.x < kRows && c < p.C) {
+        const long long c = c0 + threadIdx.x;
+        if (threadIdx.x < (unsigned)here && c < p.C) {
             float sum = 0.0f;
 #pragma unroll
             for (int v = 0; v < kSmallWaves; ++v) sum += s_part[v][threadIdx.x];
@@ -1013,12 +1018,13 @@ MassWs mass_ws(int dtype, int F, int W, int S, int Hkv, long long max_rows, long
     const long long score_bytes = wh * l.chunks * rows * kGqa * 4;
     l.stored = S == 1 && score_bytes <= kMaxScoreBytes;
     const long long all = capacity > max_rows ? capacity : max_rows;
-    l.small = S > 1 && S <= kMassTokens && wh * ((all + unit - 1) / unit) <= (S > kSmallWaves ? 2 * kSmallBlocks : kSmallBlocks);
+    const long long few = (all + unit - 1) / unit + F;  // blocks (at least one: capacity is not 0) of dv_mass_small, per sequence and KV head
+    l.small = S > 1 && S <= kMassTokens && wh * few <= (S > kSmallWaves ? 2 * kSmallBlocks : kSmallBlocks);
     if (l.small) {
         l.units = 1;
         l.rows = unit;
         l.tokens = S;
-        l.chunks = (max_rows + unit - 1) / unit;
+        l.chunks = few;
         l.rq = up256((size_t)F * wh * kGqa * S * kHeadDim * (dtype == kF32 ? 4 : 2));
         l.part = up256((size_t)(wh * l.chunks * S * kGqa * 8));
         l.total = l.rq + l.part;
@@ -1082,9 +1088,9 @@ hipError_t mass_go(MassParams p, const MassWs& l, int device, hipStream_t stream
     if (l.small) {
         p.s0 = 0;
         p.ns = p.S;
-        if (keys.x) hipLaunchKernelGGL((dv_mass_small<DT, NT, false>), keys, dim3(kSmallThreads), 0, stream, p);
+        hipLaunchKernelGGL((dv_mass_small<DT, NT, false>), keys, dim3(kSmallThreads), 0, stream, p);
         if ((e = hipGetLastError()) != hipSuccess) return e;
-        if (outs.x) hipLaunchKernelGGL((dv_mass_small<DT, NT, true>), outs, dim3(kSmallThreads), 0, stream, p);
+        hipLaunchKernelGGL((dv_mass_small<DT, NT, true>), keys, dim3(kSmallThreads), 0, stream, p);
         return hipGetLastError();
     }
     const dim3 parts((unsigned)(wh * l.parts));
