@@ -985,12 +985,14 @@ int tiles_of(int dtype) { return dtype == kF32 ? kTilesOf<kF32> : kTilesOf<kBF16
 // from here on the second pass computes the scores again.
 constexpr long long kMaxScoreBytes = 1ll << 30;
 
-// dv_mass_small up to so many blocks of it: one per CU, two where a wave has more than one
-// token.  Beside the kernels of the plan (16-bit, 4 KV heads, 64-row blocks; fp32 takes
-// 32 rows): 20 blocks, 2 / 33 tokens 13 / 23 us instead of 20 / 55; 252 blocks 15 / 29
-// instead of 21 / 55; 504 blocks 22 / 49 instead of 21 / 55 (fp32 28 / 91 instead of 23 /
-// 111); 1008 blocks 38 / 91 instead of 22 / 58.
-constexpr long long kSmallBlocks = 256;
+// dv_mass_small up to so many blocks of it: two per CU, and four where a sequence has few
+// (each block goes through the pairs of all blocks of its sequence).  Beside the kernels of
+// the plan, bf16, 4 KV heads, 5 / 33 tokens: 20 blocks 13 / 21 us instead of 24 / 55; 252
+// of one sequence 14 / 27 instead of 24 / 55; 400 of 20 sequences 19 / 40 instead of 25 /
+// 62; 576 of 16 21 / 42 instead of 27 / 64; 760 of two 30 / 67 instead of 25 / 60; 1024 of
+// four 35 / 76 instead of 25 / 60.  fp32 (32 rows per block): 640 of 20 31 / 95 instead of
+// 35 / 115; 1056 of 8 34 / 122 instead of 34 / 111.
+constexpr long long kSmallBlocks = 512, kManySmallBlocks = 1024, kFewParts = 34;
 
 struct MassWs {
     bool stored;
@@ -1019,7 +1021,7 @@ MassWs mass_ws(int dtype, int F, int W, int S, int Hkv, long long max_rows, long
     l.stored = S == 1 && score_bytes <= kMaxScoreBytes;
     const long long all = capacity > max_rows ? capacity : max_rows;
     const long long few = (all + unit - 1) / unit + F;  // blocks (at least one: capacity is not 0) of dv_mass_small, per sequence and KV head
-    l.small = S > 1 && S <= kMassTokens && wh * few <= (S > kSmallWaves ? 2 * kSmallBlocks : kSmallBlocks);
+    l.small = S > 1 && S <= kMassTokens && wh * few <= (few <= kFewParts ? kManySmallBlocks : kSmallBlocks);
     if (l.small) {
         l.units = 1;
         l.rows = unit;
