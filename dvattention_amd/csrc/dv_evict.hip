@@ -58,7 +58,9 @@ __device__ inline int block_excl(int v, int* s_wave) {
 // A wave owns a contiguous stretch of rows, so its places follow from one count per
 // wave and a running one inside it, and no pass has a barrier in its loop.  Up to
 // kSelHeld * 1024 rows are read once and held in registers; more are read again
-// (from L2) in each of the five passes.
+// (from L2) in each of the five passes.  Bound by the chain of passes: 1000 rows 7.2
+// us; 128 lists of 32768 rows, a block each, 25.4 (loads 6.4, first digit 8, the list
+// and the other digits 4, counts 3.7, writes 7).
 template <int kSelHeld>
 __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p) {
     __shared__ int s_hist[kBins];

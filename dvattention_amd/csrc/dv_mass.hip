@@ -8,21 +8,21 @@
 // row's (max, sum) over each part of the keys, the second joins them and adds the
 // weights up.
 //
-// K rows are the A operand of S^T = K Q^T (16x16x32 MFMA, 16x16x4 for fp32), loaded
-// into registers by the wave that owns the keys: with no second product there is
-// nothing to share between waves.  Every K row is read once per pass however many
-// tokens vote, and a key's weight is summed by one wave in a fixed order -- no
-// atomics, the same bits from every run.  Scores, maxima, sums and weights are fp32.
+// K rows are the A operand of S^T = K Q^T (16x16x32 MFMA, 16x16x4 for fp32), held in
+// registers while the tokens go by: with no second product there is nothing else to
+// do with them.  Every K row is read once per pass however many tokens vote, and a
+// key's weight is summed in a fixed order -- no atomics, the same bits from every run.
+// Scores, maxima, sums and weights are fp32.
 //
 //  * S = 1 (a decode step; bound by memory): the queries are rotated in the kernel
 //    and the scores stored (64 bytes per key and KV head, a quarter of a 16-bit K row, an
 //    eighth of an fp32 one), so the second pass reads those and not K.
 //  * S > 1 (a window of tokens; bound by the exponentials): a wave holds 64 keys (32
-//    for fp32) and walks the tokens (over few keys, where that walk is all a call's time,
-//    the waves of a block share the tokens instead: dv_mass_small), whose queries one launch beforehand rotated into
+//    for fp32) and walks the tokens, whose queries one launch beforehand rotated into
 //    the MFMA's operand order; the second pass computes the scores again (storing
-//    them would cost more bytes than K from two tokens on).  At most kMassTokens
-//    tokens per launch bound the workspace.
+//    them would cost more bytes than K from two tokens on).  Over few keys, where that
+//    walk is all a call's time, the waves of a block share the tokens (dv_mass_small).
+//    At most kMassTokens tokens per launch bound the workspace.
 #include <type_traits>
 
 #include "dv_common.h"
@@ -868,7 +868,10 @@ __device__ inline void walk_tokens(const MassParams& p, const Part& it, unsigned
 
 }  // namespace
 
-// Per seen part, token of the launch and head, (max, sum).
+// Per seen part, token of the launch and head, (max, sum).  Bound by VALU issue: about 110
+// instructions (maximum, 16 exponentials, sums) beside 16 MFMAs per token and wave.  Four
+// sequences of 9000 keys in two views, 4 KV heads, 32 tokens in fp16: 46 us (0.4 PFLOP/s),
+// dv_mass_apply 43.
 template <int DT, int NT>
 __global__ __launch_bounds__(kMassThreads) void dv_mass_stats(const MassParams p) {
     __shared__ __align__(16) unsigned char ring[kRingBytes<DT>];
