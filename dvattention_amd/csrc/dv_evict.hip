@@ -7,8 +7,6 @@ namespace dv {
 
 namespace {
 
-typedef __attribute__((address_space(1))) u32x4 gw_u32x4;
-
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kBins = 1 << 13;

@@ -1023,7 +1023,8 @@ MassWs mass_ws(int dtype, int F, int W, int S, int Hkv, long long max_rows, long
     const long long score_bytes = wh * l.chunks * rows * kGqa * 4;
     l.stored = S == 1 && score_bytes <= kMaxScoreBytes;
     const long long all = capacity > max_rows ? capacity : max_rows;
-    const long long few = (all + unit - 1) / unit + F;  // blocks (at least one: capacity is not 0) of dv_mass_small, per sequence and KV head
+    // dv_mass_small's blocks per sequence and KV head (at least one: the capacity is not 0)
+    const long long few = (all + unit - 1) / unit + F;
     l.small = S > 1 && S <= kMassTokens && wh * few <= (few <= kFewParts ? kManySmallBlocks : kSmallBlocks);
     if (l.small) {
         l.units = 1;

@@ -556,7 +556,7 @@ TreePlan tree_plan(int dtype, int F, int W, int S, int Hkv, long long max_keys) 
     if (S > kEntries / 2 || (long long)W * Hkv > (1 << 20) || max_keys > (1 << 24)) return t;
     const long long nodes = (long long)W * Hkv * S;
     const long long view = (long long)kGqa * kHeadDim * (dtype == kF32 ? 4 : 2);  // bytes of a view's queries
-    const long long keys = (max_keys + 15ll * F + 15) / 16 * 16;                  // the committed list at most
+    const long long keys = (max_keys + 15ll * F) / 16 * 16 + 16;                  // more than the committed list holds
     const long long path = (S + 15ll) / 16 * 16;
     if (F * view > kSmallQueryBytes) return t;
     if (keys + path <= kEntries && nodes <= (dtype == kF32 ? 4096 : 1024)) return TreePlan{1, (int)keys};
@@ -565,7 +565,7 @@ TreePlan tree_plan(int dtype, int F, int W, int S, int Hkv, long long max_keys) 
     // 128 entries, 15.8 for 224, 23 for 416): as many windows as make the rounds of 512
     // blocks shortest, fewer ones where that is even.
     long long best = 0;
-    for (long long n = (keys + kEntries - path - 1) / (kEntries - path); n <= (keys + 127) / 128; ++n) {
+    for (long long n = (keys + kEntries - path - 1) / (kEntries - path); n == 1 || n <= (keys + 127) / 128; ++n) {
         const long long window = ((keys + n - 1) / n + 15) / 16 * 16;
         const long long cost = (nodes * n + 511) / 512 * (window + 160);
         if (t.windows == 0 || cost < best) {

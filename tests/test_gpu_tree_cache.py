@@ -203,6 +203,25 @@ def test_tree_sdpa_negative_scale_and_empty(dv, gpu):
     assert dv.dvattn_tree_paged_sdpa(scale=SCALE, **to(gpu, e)).shape == (2, 16, 0, E)
 
 
+@pytest.mark.parametrize("W", [2, 150])
+def test_tree_sdpa_without_views(dv, gpu, W):
+    """F = 0, with pages and without: zeros, for few nodes and for more than a launch of
+    short lists takes."""
+    d = tree_case(torch.bfloat16, W, 2, 4, [20], 16, 64, seed=3)
+    for name in ("locations", "cosines", "sines", "fragment_lengths"):
+        d[name] = d[name][:0].contiguous()
+    for pages in (d["block_tables"], d["block_tables"][:, :0].contiguous()):
+        out = torch.full((W, 32, 4, E), math.nan, dtype=torch.bfloat16, device=gpu)
+        dv.dvattn_tree_paged_sdpa(scale=SCALE, out=out, **to(gpu, {**d, "block_tables": pages}))
+        assert not out.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tree_sdpa_many_short_sequences(dv, gpu, dtype):
+    """More nodes than a launch of whole lists takes, few keys each."""
+    check_tree(dv, gpu, tree_case(dtype, 90, 2, 7, [9, 14], 16, 64, seed=8), dtype)
+
+
 # ---------------------------------------------------------------------------
 def mass_case(dtype, W, Hkv, S, fl, bs, R, seed, extra=3, bad=False):
     g = torch.Generator().manual_seed(seed)

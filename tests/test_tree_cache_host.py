@@ -119,6 +119,7 @@ def test_tree_workspace(lib):
         assert windows * 640 >= s.max_blocks_per_seq * 16 and windows <= s.max_blocks_per_seq * 16 / 128 + 1
     pieces = need(2, S=64, max_blocks_per_seq=10 ** 6)
     assert pieces > 0 and pieces == need(2, S=64, max_blocks_per_seq=2 ** 20) == need(2, F=60, S=64)
+    assert need(2, F=0, W=100, Hkv=8, Hq=128, max_blocks_per_seq=0) == 0  # nothing to see, many nodes
     assert need(2, W=-1) == need(2, max_blocks_per_seq=-1) == 0
     assert need(2, W=2 ** 31 - 1, Hkv=2 ** 31 - 1, S=300) >= 0
 
