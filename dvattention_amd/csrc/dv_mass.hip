@@ -640,9 +640,9 @@ __global__ __launch_bounds__(kSmallThreads) void dv_mass_small(const MassParams 
 }
 
 // S > 1: the query operands, [F, W, Hkv, S] of kOperandBytes each, a thread per 16
-// bytes; and, in the first `plans` blocks (W, or none), the plan.  A part is what one block of the
-// kernels below takes: up to part_rows rows of one view (the rows behind the last view
-// and below the capacity count as one more view, F).  The list of a sequence's parts
+// bytes; and, in the first `plans` blocks (W, or none), the plan.  A part is what one
+// block of the kernels below takes: up to part_rows rows of one view (the rows behind the
+// last view and below the capacity count as one more view, F).  The list of a sequence's parts
 // has those that some token sees in front, and they get the first blocks of the
 // launches that follow.  Both matter where a launch is about one block per CU: parts
 // cut across the views' border took twice as long as the others (four sequences of
