@@ -158,6 +158,26 @@ def test_tree_sdpa_chain_is_causal(dv, gpu, dtype, S):
     assert (got.float() - causal.float()).abs().max() <= tol * max(1.0, float(causal.abs().max()))
 
 
+def test_tree_of_the_most_nodes(dv, gpu):
+    """4096 nodes: a chain of all of them is a causal chunk; its metadata counts depths."""
+    S, dt = 4096, torch.float16
+    d = to(gpu, tree_case(dt, 1, 1, S, [S + 30], 16, 64, seed=4, chain=True))
+    got = dv.dvattn_tree_paged_sdpa(scale=SCALE, **d).float()
+    loc = d["locations"] + 1 + torch.arange(S, dtype=torch.int32, device=gpu)
+    causal = dv.dvattn_paged_sdpa(locations=loc, scale=SCALE, **{k: d[k] for k in (
+        "queries", "cosines", "sines", "fragment_lengths", "k_cache", "v_cache", "block_tables")}).float()
+    assert got.isfinite().all()
+    tol = 4 * torch.finfo(dt).eps + 2e-5
+    assert (got - causal).abs().max() <= tol * max(1.0, float(causal.abs().max()))
+    inv = torch.full((2,), 2.0 ** -8, device=gpu)
+    loc, cos, sin, views, rows = dv.dvattn_tree_metadata(d["fragment_lengths"], torch.zeros(1, 1, dtype=torch.int32,
+                                                         device=gpu), d["parents"], inv)
+    angle = (30 + torch.arange(S, device=gpu, dtype=torch.float64)) * 2.0 ** -8
+    assert loc.eq(29).all() and views.tolist() == [0] and rows.tolist() == [30]
+    assert (cos[0, 0].double() - torch.cos(angle)[:, None]).abs().max() <= 2.0 ** -22
+    assert (sin[0, 0].double() - torch.sin(angle)[:, None]).abs().max() <= 2.0 ** -22
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_tree_sdpa_unseen_rows_may_hold_anything(dv, gpu, dtype):
     """NaN and infinity in drafted rows that no node, or only another node, sees:
