@@ -139,6 +139,10 @@ def dvattn_view_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, nu
     int32, cosines [F,W,S,R], sines [F,W,S,R])`` float32, ready for
     ``dvattn_paged_sdpa`` / ``dvattn_fused``.  ``round_to`` rounds cos/sin through
     the model dtype, as the reference's rotary call does.
+
+    Positions are sums of the lengths: the tables are for caches that hold every row.
+    Of a cache that was cut, ``dvattn_tree_metadata`` on a chain (parents -1, 0, 1, ...)
+    gives them with ``dropped``; token s then sees ``locations + 1 + s`` of its own view.
     """
     F = fragment_lengths.numel()
     W = order.size(0)
@@ -154,7 +158,7 @@ def dvattn_view_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, nu
 
 def dvattn_tree_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, parents: torch.Tensor,
                          inv_freq: torch.Tensor, attention_scaling: float = 1.0,
-                         round_to: Optional[torch.dtype] = None):
+                         round_to: Optional[torch.dtype] = None, dropped: Optional[torch.Tensor] = None):
     """Metadata of a step in which every sequence drafts a tree of up to S tokens:
     ``dvattn_view_metadata`` with positions that follow the nodes' depths.
 
@@ -172,9 +176,15 @@ def dvattn_tree_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, pa
 
     The last four and the first are ``dvattn_tree_paged_sdpa``'s arguments.  Another
     sequence's drafted nodes are neither seen nor counted.  S and F are at most 4096.
+
+    A cache that was cut (``dvattn_kv_select``, ``dvattn_paged_kv_compact``) holds
+    fewer rows than its sequence has seen tokens, and kept keys keep the rotation of
+    their own positions: ``dropped [W,F]`` int32 are the tokens of each view that the
+    sequence no longer holds.  They count for the positions and for nothing else.
+    Without them the tables are for caches that hold every row.
     """
     return torch.ops.libdvatt.dvattn_tree_metadata(fragment_lengths, order, parents, inv_freq,
-                                                   float(attention_scaling), round_to)
+                                                   float(attention_scaling), round_to, dropped)
 
 
 def dvattn_tree_paged_sdpa(queries: torch.Tensor, locations: torch.Tensor, cosines: torch.Tensor,
@@ -245,7 +255,8 @@ def dvattn_paged_kv_compact(rows: torch.Tensor, first_rows: torch.Tensor, k_cach
     ``dvattn_paged_kv_append``.  The moved rows' pages must not be named twice in
     ``block_tables``: pages that sequences or segments share lie before first_rows.
     Positions of the kept keys do not change (their rotation stays valid); the
-    caller's locations and lengths count rows from here on."""
+    caller's locations and lengths count rows from here on, and the queries' positions
+    have to count the rows that went (``dropped`` of ``dvattn_tree_metadata``)."""
     torch.ops.libdvatt.dvattn_paged_kv_compact(k_cache, v_cache, block_tables, rows, first_rows, lengths, mass)
     return k_cache, v_cache
 

@@ -261,12 +261,14 @@ hipError_t launch_view_meta(const MetaParams& p, hipStream_t stream) {
 // A step that drafts a tree of S nodes per sequence.  With c(g) the committed tokens
 // of view g -- fl[g] less the S drafted rows where g is some sequence's own (last)
 // view -- and d(s) the depth of node s (0: child of the committed tokens),
-//   position[f, w, s] = sum of c over w's segments from f's place in its order to the
-//                       last one, plus d(s),
+//   position[f, w, s] = sum of c + dropped over w's segments from f's place in its order
+//                       to the last one, plus d(s),
 //   location[f, w, s] = c(f) - 1 (the drafted rows are seen through the tree alone),
 //   cos / sin         = cos / sin(fp32(position) * inv_freq[i]) * scaling, as dv_view_meta.
 // An absent node (parent neither -1 nor an earlier node, or below such a node) and a
 // view missing from the order get location -1 and the identity rotation.
+// dropped[w, g] are tokens that were cut from the view: rows count what a cache holds,
+// positions what it has seen (the keys that stayed keep their rotation).
 //
 // Bound by its writes (F W S (4 + 8 R) bytes) and, for small calls, by the launch: 8 nodes
 // of one sequence 4.1 us, 32 nodes of 16 sequences over 17 views (8.9 MB) 8.4.
@@ -312,7 +314,8 @@ __global__ __launch_bounds__(256) void dv_tree_meta(const TreeMetaParams tp, int
     long long mine = 0;
     for (int j = tid; j < p.F; j += 256) {
         const int g = ord[j];
-        if (j >= place && g >= 0 && g < p.F) mine += committed(g);
+        if (j >= place && g >= 0 && g < p.F)
+            mine += committed(g) + (tp.dropped ? (long long)tp.dropped[(long long)w * p.F + g] : 0ll);
     }
     if (mine) atomicAdd(reinterpret_cast<unsigned long long*>(&s_sum), (unsigned long long)mine);
     const int s0 = tile * kTreeTile;

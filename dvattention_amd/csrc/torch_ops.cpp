@@ -628,13 +628,25 @@ void dvattn_view_metadata_op(at::Tensor& locations, at::Tensor& cosines, at::Ten
 // ---------------------------------------------------------------------------
 // Drafted token trees and bounded caches (no counterpart in the reference).
 
+// A tree call's optional counts [W,F] i32, as order: their pointer, or null.
+const int* counts_of(const std::optional<at::Tensor>& t, const char* name, const at::Tensor& order, const char* op) {
+    if (!t.has_value() || !t->defined()) return nullptr;
+    check_i32(*t, name);
+    check_contig(*t, name);
+    check_dev(*t, order, name);
+    TORCH_CHECK(t->sizes() == order.sizes(), op, ": ", name, " must be [W,F] as order ", order.sizes(), ", got ",
+                t->sizes());
+    return t->data_ptr<int>();
+}
+
 // dvattn_tree_metadata(Tensor fragment_lengths, Tensor order, Tensor parents, Tensor inv_freq,
-//   float attention_scaling, ScalarType? round_to=None)
+//   float attention_scaling, ScalarType? round_to=None, Tensor? dropped=None)
 //   -> (Tensor locations, Tensor cosines, Tensor sines, Tensor tree_views, Tensor tree_rows)
 // The outputs are allocated here: five allocations from Python took longer than the call.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dvattn_tree_metadata_op(
     const at::Tensor& fragment_lengths, const at::Tensor& order, const at::Tensor& parents,
-    const at::Tensor& inv_freq, double attention_scaling, std::optional<at::ScalarType> round_to) {
+    const at::Tensor& inv_freq, double attention_scaling, std::optional<at::ScalarType> round_to,
+    const std::optional<at::Tensor>& dropped) {
     check_dim(fragment_lengths, 1, "fragment_lengths");
     check_dim(order, 2, "order");
     check_dim(parents, 2, "parents");
@@ -650,6 +662,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dvattn_tr
     const int64_t F = fragment_lengths.size(0), W = parents.size(0), S = parents.size(1), R = 2 * inv_freq.size(0);
     TORCH_CHECK(order.size(0) == W && order.size(1) == F, "dvattn_tree_metadata: order must be [W,F] = [", W, ",", F,
                 "], got ", order.sizes());
+    const int* gone = counts_of(dropped, "dropped", order, "dvattn_tree_metadata");
     int rd = -1;
     if (round_to.has_value()) {
         switch (*round_to) {
@@ -664,11 +677,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dvattn_tr
     at::Tensor cosines = at::empty({F, W, S, R}, inv_freq.options());
     at::Tensor sines = at::empty({F, W, S, R}, inv_freq.options());
     at::Tensor views = at::empty({W}, parents.options()), rows = at::empty({W}, parents.options());
-    check_status(dvattn_tree_metadata(locations.data_ptr<int>(), cosines.data_ptr<float>(), sines.data_ptr<float>(),
-                                      views.data_ptr<int>(), rows.data_ptr<int>(), fragment_lengths.data_ptr<int>(),
-                                      order.data_ptr<int>(), parents.data_ptr<int>(), inv_freq.data_ptr<float>(),
-                                      (float)attention_scaling, rd, as_int(F, "F"), as_int(W, "W"), as_int(S, "S"),
-                                      as_int(R, "rotary_dim"), stream_of(parents)),
+    check_status(dvattn_tree_metadata_counts(
+                     locations.data_ptr<int>(), cosines.data_ptr<float>(), sines.data_ptr<float>(),
+                     views.data_ptr<int>(), rows.data_ptr<int>(), fragment_lengths.data_ptr<int>(),
+                     order.data_ptr<int>(), parents.data_ptr<int>(), gone, inv_freq.data_ptr<float>(),
+                     (float)attention_scaling, rd, as_int(F, "F"), as_int(W, "W"), as_int(S, "S"),
+                     as_int(R, "rotary_dim"), stream_of(parents)),
                  "dvattn_tree_metadata");
     return {locations, cosines, sines, views, rows};
 }
@@ -896,8 +910,8 @@ TORCH_LIBRARY(libdvatt, m) {
           "ScalarType? round_to=None) -> ()");
     // drafted token trees and bounded caches
     m.def("dvattn_tree_metadata(Tensor fragment_lengths, Tensor order, Tensor parents, Tensor inv_freq, "
-          "float attention_scaling, ScalarType? round_to=None) -> (Tensor locations, Tensor cosines, Tensor sines, "
-          "Tensor tree_views, Tensor tree_rows)");
+          "float attention_scaling, ScalarType? round_to=None, Tensor? dropped=None) -> (Tensor locations, "
+          "Tensor cosines, Tensor sines, Tensor tree_views, Tensor tree_rows)");
     m.def("dvattn_tree_paged_sdpa(Tensor(a!) output, float scale, Tensor locations, Tensor queries, "
           "Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor v_cache, "
           "Tensor block_tables, Tensor parents, Tensor tree_views, Tensor tree_rows) -> ()");

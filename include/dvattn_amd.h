@@ -291,12 +291,23 @@ DVATTN_API dvattn_status dvattn_view_metadata(int* locations, float* cosines, fl
  * sin 0.  Without views (F = 0) or nodes (S = 0) tree_views and tree_rows (0 for no
  * view) are still written.  The other sequences' drafted nodes are neither seen nor counted.  For
  * one sequence and a chain (parents -1, 0, 1, ...) cos/sin are
- * dvattn_view_metadata's.  S <= 4096, F <= 4096. */
+ * dvattn_view_metadata's.  S <= 4096, F <= 4096.
+ *
+ * A cache that was cut (dvattn_kv_select, dvattn_paged_kv_compact) holds fewer rows than
+ * its sequence has seen tokens, and its keys keep the rotation of their own positions.
+ * dvattn_tree_metadata_counts takes the difference: dropped [W,F] i32 (null: none), the
+ * tokens of view g that sequence w no longer holds, counted by position(f,w,s) beside
+ * c(g) and by nothing else.  The entry without it is for caches that hold every row. */
 #define DVATTN_MAX_TREE_NODES 4096
 DVATTN_API dvattn_status dvattn_tree_metadata(int* locations, float* cosines, float* sines, int* tree_views,
                                    int* tree_rows, const int* fragment_lengths, const int* order,
                                    const int* parents, const float* inv_freq, float attention_scaling,
                                    int round_dtype, int F, int W, int S, int rotary_dim, void* stream);
+DVATTN_API dvattn_status dvattn_tree_metadata_counts(int* locations, float* cosines, float* sines, int* tree_views,
+                                   int* tree_rows, const int* fragment_lengths, const int* order,
+                                   const int* parents, const int* dropped, const float* inv_freq,
+                                   float attention_scaling, int round_dtype, int F, int W, int S, int rotary_dim,
+                                   void* stream);
 
 /* ---- attention of drafted token trees over a paged cache -------------------------
  * dvattn_paged_sdpa's arguments, with S drafted nodes per sequence, and parents
@@ -360,7 +371,8 @@ DVATTN_API dvattn_status dvattn_kv_select(int* rows, const float* mass, const in
  * the rows first_rows[w] + i, i < lengths[w], that nothing moves into become 0
  * (capacity <= 2^30).  Uses
  * shape fields W, Hkv, E, Ev, block_size, max_blocks_per_seq, num_blocks and the
- * layout's cache strides.  The pages of the rows moved must each be named once in
+ * layout's cache strides.  The queries that follow keep counting positions with the rows
+ * that went (dropped above).  The pages of the rows moved must each be named once in
  * block_tables (pages shared by sequences or segments lie before first_rows). */
 DVATTN_API dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, const int* block_tables,
                                       const int* rows, int row_heads, int N, const int* first_rows,

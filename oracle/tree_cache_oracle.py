@@ -177,7 +177,7 @@ def compact(k_cache, v_cache, block_tables, rows, first_rows, lengths=None, mass
     return k, v, m
 
 
-def metadata(fragment_lengths, order, parents, inv_freq, scaling=1.0):
+def metadata(fragment_lengths, order, parents, inv_freq, scaling=1.0, dropped=None):
     """(locations, cos, sin, tree_views, tree_rows); cos/sin float64 of the float32 angle."""
     F, (W, S), R = len(fragment_lengths), parents.shape, 2 * inv_freq.numel()
     fl = [int(x) for x in fragment_lengths]
@@ -195,7 +195,7 @@ def metadata(fragment_lengths, order, parents, inv_freq, scaling=1.0):
         for f in range(F):
             if f not in o:
                 continue
-            base = sum(c[g] for g in o[o.index(f):] if 0 <= g < F)
+            base = sum(c[g] + (0 if dropped is None else int(dropped[w, g])) for g in o[o.index(f):] if 0 <= g < F)
             for s in range(S):
                 nodes = path(parents[w], s)
                 if nodes is None:
