@@ -158,7 +158,8 @@ def dvattn_view_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, nu
 
 def dvattn_tree_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, parents: torch.Tensor,
                          inv_freq: torch.Tensor, attention_scaling: float = 1.0,
-                         round_to: Optional[torch.dtype] = None, dropped: Optional[torch.Tensor] = None):
+                         round_to: Optional[torch.dtype] = None, dropped: Optional[torch.Tensor] = None,
+                         committed: Optional[torch.Tensor] = None):
     """Metadata of a step in which every sequence drafts a tree of up to S tokens:
     ``dvattn_view_metadata`` with positions that follow the nodes' depths.
 
@@ -182,9 +183,14 @@ def dvattn_tree_metadata(fragment_lengths: torch.Tensor, order: torch.Tensor, pa
     their own positions: ``dropped [W,F]`` int32 are the tokens of each view that the
     sequence no longer holds.  They count for the positions and for nothing else.
     Without them the tables are for caches that hold every row.
+
+    Sequences that share a view index share its length, but after their first accepted
+    paths they hold different numbers of rows: ``committed [W,F]`` int32 are then the
+    committed rows of each view (0 and up) in place of those its length gives, and
+    fragment_lengths are at least the most of them and S.
     """
     return torch.ops.libdvatt.dvattn_tree_metadata(fragment_lengths, order, parents, inv_freq,
-                                                   float(attention_scaling), round_to, dropped)
+                                                   float(attention_scaling), round_to, dropped, committed)
 
 
 def dvattn_tree_paged_sdpa(queries: torch.Tensor, locations: torch.Tensor, cosines: torch.Tensor,

@@ -104,7 +104,7 @@ def lib() -> ctypes.CDLL:
         L.dvattn_tree_metadata.restype = _I
         L.dvattn_tree_metadata.argtypes = [_VP] * 9 + [_F, _I, _I, _I, _I, _I, _VP]
         L.dvattn_tree_metadata_counts.restype = _I
-        L.dvattn_tree_metadata_counts.argtypes = [_VP] * 10 + [_F, _I, _I, _I, _I, _I, _VP]
+        L.dvattn_tree_metadata_counts.argtypes = [_VP] * 11 + [_F, _I, _I, _I, _I, _I, _VP]
         L.dvattn_tree_paged_sdpa.restype = _I
         L.dvattn_tree_paged_sdpa.argtypes = [_I, _VP, _F] + [_VP] * 11 + [_SP, _VP, _SZ, _VP]
         L.dvattn_paged_key_mass_workspace_size.restype = _SZ
@@ -305,15 +305,15 @@ def view_metadata(locations, cosines, sines, fragment_lengths, order, inv_freq, 
 
 
 def tree_metadata(locations, cosines, sines, tree_views, tree_rows, fragment_lengths, order, parents, inv_freq,
-                  attention_scaling=1.0, round_to=None, dropped=None):
+                  attention_scaling=1.0, round_to=None, dropped=None, committed=None):
     """dvattn_tree_metadata_counts: locations [F,W,S] i32, cos/sin [F,W,S,R] f32, tree_views/tree_rows [W] i32,
-    dropped [W,F] i32 or None."""
+    dropped and committed [W,F] i32 or None."""
     F, W, S = locations.shape
     rd = -1 if round_to in (None, torch.float32) else dtype_code(round_to)
     _check(lib().dvattn_tree_metadata_counts(_ptr(locations), _ptr(cosines), _ptr(sines), _ptr(tree_views),
                                              _ptr(tree_rows), _ptr(fragment_lengths), _ptr(order), _ptr(parents),
-                                             _ptr(dropped), _ptr(inv_freq), attention_scaling, rd, F, W, S,
-                                             cosines.shape[3], _stream(locations)))
+                                             _ptr(committed), _ptr(dropped), _ptr(inv_freq), attention_scaling, rd,
+                                             F, W, S, cosines.shape[3], _stream(locations)))
     return locations, cosines, sines, tree_views, tree_rows
 
 

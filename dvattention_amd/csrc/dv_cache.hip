@@ -259,8 +259,8 @@ hipError_t launch_view_meta(const MetaParams& p, hipStream_t stream) {
 }
 
 // A step that drafts a tree of S nodes per sequence.  With c(g) the committed tokens
-// of view g -- fl[g] less the S drafted rows where g is some sequence's own (last)
-// view -- and d(s) the depth of node s (0: child of the committed tokens),
+// of view g -- committed[w, g] where given, else fl[g] less the S drafted rows where g is
+// some sequence's own (last) view -- and d(s) the depth of node s (0: child of the committed tokens),
 //   position[f, w, s] = sum of c + dropped over w's segments from f's place in its order
 //                       to the last one, plus d(s),
 //   location[f, w, s] = c(f) - 1 (the drafted rows are seen through the tree alone),
@@ -307,7 +307,8 @@ __global__ __launch_bounds__(256) void dv_tree_meta(const TreeMetaParams tp, int
         if (ord[j] == f) atomicMin(&s_place, j);
     __syncthreads();
     auto committed = [&](int g) {
-        const long long c = (long long)p.fl[g] - (s_drafted[g] ? p.S : 0);
+        const long long c = tp.committed ? (long long)tp.committed[(long long)w * p.F + g]
+                                         : (long long)p.fl[g] - (s_drafted[g] ? p.S : 0);
         return c > 0 ? c : 0ll;
     };
     const int place = s_place;

@@ -815,15 +815,15 @@ dvattn_status dvattn_tree_metadata(int* locations, float* cosines, float* sines,
                                    const float* inv_freq, float attention_scaling, int round_dtype, int F, int W,
                                    int S, int rotary_dim, void* stream) {
     return dvattn_tree_metadata_counts(locations, cosines, sines, tree_views, tree_rows, fragment_lengths, order,
-                                       parents, nullptr, inv_freq, attention_scaling, round_dtype, F, W, S,
+                                       parents, nullptr, nullptr, inv_freq, attention_scaling, round_dtype, F, W, S,
                                        rotary_dim, stream);
 }
 
 dvattn_status dvattn_tree_metadata_counts(int* locations, float* cosines, float* sines, int* tree_views,
                                           int* tree_rows, const int* fragment_lengths, const int* order,
-                                          const int* parents, const int* dropped, const float* inv_freq,
-                                          float attention_scaling, int round_dtype, int F, int W, int S,
-                                          int rotary_dim, void* stream) {
+                                          const int* parents, const int* committed, const int* dropped,
+                                          const float* inv_freq, float attention_scaling, int round_dtype, int F,
+                                          int W, int S, int rotary_dim, void* stream) {
     if (F < 0 || W < 0 || S < 0) return fail(DVATTN_ERR_INVALID, "negative F/W/S");
     if (rotary_dim < 0 || (rotary_dim & 1))
         return fail(DVATTN_ERR_UNSUPPORTED, "rotary_dim must be even and >= 0 (got %d)", rotary_dim);
@@ -844,8 +844,8 @@ dvattn_status dvattn_tree_metadata_counts(int* locations, float* cosines, float*
     const dvattn_status st = check_aligned({{locations, "locations", 4}, {cosines, "cosines", 4}, {sines, "sines", 4},
                                             {tree_views, "tree_views", 4}, {tree_rows, "tree_rows", 4},
                                             {fragment_lengths, "fragment_lengths", 4}, {order, "order", 4},
-                                            {parents, "parents", 4}, {dropped, "dropped", 4},
-                                            {inv_freq, "inv_freq", 4}});
+                                            {parents, "parents", 4}, {committed, "committed", 4},
+                                            {dropped, "dropped", 4}, {inv_freq, "inv_freq", 4}});
     if (st != DVATTN_OK) return st;
     dv::TreeMetaParams p;
     memset(&p, 0, sizeof(p));
@@ -862,6 +862,7 @@ dvattn_status dvattn_tree_metadata_counts(int* locations, float* cosines, float*
     p.m.S = S;
     p.m.R = rotary_dim;
     p.parents = parents;
+    p.committed = committed;
     p.dropped = dropped;
     p.tree_views = tree_views;
     p.tree_rows = tree_rows;

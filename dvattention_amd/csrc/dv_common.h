@@ -150,6 +150,7 @@ constexpr int kMaxTreeViews = 4096;  // views of a tree metadata call (flags and
 struct TreeMetaParams {
     MetaParams m;             // outputs and inputs shared with dv_view_meta
     const int* parents;       // [W, S]
+    const int* committed;     // [W, F] or null: committed rows of a view, in place of those its length gives
     const int* dropped;       // [W, F] or null: tokens of a view that it no longer holds
     int* tree_views;          // [W]
     int* tree_rows;           // [W]

@@ -640,13 +640,13 @@ const int* counts_of(const std::optional<at::Tensor>& t, const char* name, const
 }
 
 // dvattn_tree_metadata(Tensor fragment_lengths, Tensor order, Tensor parents, Tensor inv_freq,
-//   float attention_scaling, ScalarType? round_to=None, Tensor? dropped=None)
+//   float attention_scaling, ScalarType? round_to=None, Tensor? dropped=None, Tensor? committed=None)
 //   -> (Tensor locations, Tensor cosines, Tensor sines, Tensor tree_views, Tensor tree_rows)
 // The outputs are allocated here: five allocations from Python took longer than the call.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dvattn_tree_metadata_op(
     const at::Tensor& fragment_lengths, const at::Tensor& order, const at::Tensor& parents,
     const at::Tensor& inv_freq, double attention_scaling, std::optional<at::ScalarType> round_to,
-    const std::optional<at::Tensor>& dropped) {
+    const std::optional<at::Tensor>& dropped, const std::optional<at::Tensor>& committed) {
     check_dim(fragment_lengths, 1, "fragment_lengths");
     check_dim(order, 2, "order");
     check_dim(parents, 2, "parents");
@@ -663,6 +663,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dvattn_tr
     TORCH_CHECK(order.size(0) == W && order.size(1) == F, "dvattn_tree_metadata: order must be [W,F] = [", W, ",", F,
                 "], got ", order.sizes());
     const int* gone = counts_of(dropped, "dropped", order, "dvattn_tree_metadata");
+    const int* held = counts_of(committed, "committed", order, "dvattn_tree_metadata");
     int rd = -1;
     if (round_to.has_value()) {
         switch (*round_to) {
@@ -680,7 +681,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> dvattn_tr
     check_status(dvattn_tree_metadata_counts(
                      locations.data_ptr<int>(), cosines.data_ptr<float>(), sines.data_ptr<float>(),
                      views.data_ptr<int>(), rows.data_ptr<int>(), fragment_lengths.data_ptr<int>(),
-                     order.data_ptr<int>(), parents.data_ptr<int>(), gone, inv_freq.data_ptr<float>(),
+                     order.data_ptr<int>(), parents.data_ptr<int>(), held, gone, inv_freq.data_ptr<float>(),
                      (float)attention_scaling, rd, as_int(F, "F"), as_int(W, "W"), as_int(S, "S"),
                      as_int(R, "rotary_dim"), stream_of(parents)),
                  "dvattn_tree_metadata");
@@ -910,8 +911,8 @@ TORCH_LIBRARY(libdvatt, m) {
           "ScalarType? round_to=None) -> ()");
     // drafted token trees and bounded caches
     m.def("dvattn_tree_metadata(Tensor fragment_lengths, Tensor order, Tensor parents, Tensor inv_freq, "
-          "float attention_scaling, ScalarType? round_to=None, Tensor? dropped=None) -> (Tensor locations, "
-          "Tensor cosines, Tensor sines, Tensor tree_views, Tensor tree_rows)");
+          "float attention_scaling, ScalarType? round_to=None, Tensor? dropped=None, Tensor? committed=None) "
+          "-> (Tensor locations, Tensor cosines, Tensor sines, Tensor tree_views, Tensor tree_rows)");
     m.def("dvattn_tree_paged_sdpa(Tensor(a!) output, float scale, Tensor locations, Tensor queries, "
           "Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor v_cache, "
           "Tensor block_tables, Tensor parents, Tensor tree_views, Tensor tree_rows) -> ()");

@@ -293,11 +293,16 @@ DVATTN_API dvattn_status dvattn_view_metadata(int* locations, float* cosines, fl
  * one sequence and a chain (parents -1, 0, 1, ...) cos/sin are
  * dvattn_view_metadata's.  S <= 4096, F <= 4096.
  *
- * A cache that was cut (dvattn_kv_select, dvattn_paged_kv_compact) holds fewer rows than
- * its sequence has seen tokens, and its keys keep the rotation of their own positions.
- * dvattn_tree_metadata_counts takes the difference: dropped [W,F] i32 (null: none), the
- * tokens of view g that sequence w no longer holds, counted by position(f,w,s) beside
- * c(g) and by nothing else.  The entry without it is for caches that hold every row. */
+ * fragment_lengths are every sequence's alike, and a view's rows are the tokens it has
+ * seen.  dvattn_tree_metadata_counts lifts both, each by an array [W,F] i32 or null:
+ *   committed[w,g] -- c(g) of sequence w (below 0: 0), in place of what the length gives.
+ *     Of sequences that share a view's length and hold different numbers of rows in it:
+ *     fragment_lengths are then at least the most committed rows and S, and a node's
+ *     row tree_rows[w] + s lies behind its own sequence's.
+ *   dropped[w,g] -- tokens of the view that sequence w no longer holds, counted by
+ *     position(f,w,s) beside c(g) and by nothing else.  A cache that was cut
+ *     (dvattn_kv_select, dvattn_paged_kv_compact) holds fewer rows than its sequence has
+ *     seen tokens, and its keys keep the rotation of their own positions. */
 #define DVATTN_MAX_TREE_NODES 4096
 DVATTN_API dvattn_status dvattn_tree_metadata(int* locations, float* cosines, float* sines, int* tree_views,
                                    int* tree_rows, const int* fragment_lengths, const int* order,
@@ -305,9 +310,9 @@ DVATTN_API dvattn_status dvattn_tree_metadata(int* locations, float* cosines, fl
                                    int round_dtype, int F, int W, int S, int rotary_dim, void* stream);
 DVATTN_API dvattn_status dvattn_tree_metadata_counts(int* locations, float* cosines, float* sines, int* tree_views,
                                    int* tree_rows, const int* fragment_lengths, const int* order,
-                                   const int* parents, const int* dropped, const float* inv_freq,
-                                   float attention_scaling, int round_dtype, int F, int W, int S, int rotary_dim,
-                                   void* stream);
+                                   const int* parents, const int* committed, const int* dropped,
+                                   const float* inv_freq, float attention_scaling, int round_dtype, int F, int W,
+                                   int S, int rotary_dim, void* stream);
 
 /* ---- attention of drafted token trees over a paged cache -------------------------
  * dvattn_paged_sdpa's arguments, with S drafted nodes per sequence, and parents

@@ -177,16 +177,17 @@ def compact(k_cache, v_cache, block_tables, rows, first_rows, lengths=None, mass
     return k, v, m
 
 
-def metadata(fragment_lengths, order, parents, inv_freq, scaling=1.0, dropped=None):
+def metadata(fragment_lengths, order, parents, inv_freq, scaling=1.0, dropped=None, committed=None):
     """(locations, cos, sin, tree_views, tree_rows); cos/sin float64 of the float32 angle."""
     F, (W, S), R = len(fragment_lengths), parents.shape, 2 * inv_freq.numel()
     fl = [int(x) for x in fragment_lengths]
     drafted = {int(order[w, F - 1]) for w in range(W)}
-    c = [max(fl[g] - (S if g in drafted else 0), 0) for g in range(F)]
+    shared = [max(fl[g] - (S if g in drafted else 0), 0) for g in range(F)]
     loc = torch.full((F, W, S), -1, dtype=torch.int32)
     cos, sin = torch.ones(F, W, S, R, dtype=F64), torch.zeros(F, W, S, R, dtype=F64)
     views, rows = torch.empty(W, dtype=torch.int32), torch.empty(W, dtype=torch.int32)
     for w in range(W):
+        c = shared if committed is None else [max(int(x), 0) for x in committed[w]]
         o = [int(x) for x in order[w]]
         own = o[-1]
         ok = 0 <= own < F

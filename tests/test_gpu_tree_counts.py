@@ -42,6 +42,34 @@ def test_dropped_tokens_count_for_positions_only(dv, gpu, W, F, S, R):  # noqa: 
     check_counts(dv, gpu, fl, order, parents, inv, dropped=torch.zeros_like(dropped))
 
 
+@pytest.mark.parametrize("W,F,S,R", [(1, 1, 1, 128), (4, 1, 9, 64), (3, 5, 70, 20)])
+def test_committed_rows_of_each_sequence(dv, gpu, W, F, S, R):  # noqa: F811
+    """Rows below zero count as none; rows of sequences all alike are the lengths' own."""
+    fl, order, parents, inv = meta_inputs(W, F, S, R, seed=S + 1)
+    g = torch.Generator().manual_seed(F)
+    committed = torch.randint(-3, 400, (W, F), generator=g).to(torch.int32)
+    dropped = torch.randint(0, 50, (W, F), generator=g).to(torch.int32)
+    check_counts(dv, gpu, fl, order, parents, inv, committed=committed)
+    check_counts(dv, gpu, fl, order, parents, inv, committed=committed, dropped=dropped)
+    own = torch.zeros(F, dtype=torch.int32)
+    own[order[:, -1].long()] = S
+    alike = (fl - own).clamp(min=0).expand(W, F).contiguous()
+    got = check_counts(dv, gpu, fl, order, parents, inv, committed=alike)
+    plain = dv.dvattn_tree_metadata(*(t.to(gpu) for t in (fl, order, parents, inv)))
+    assert all(torch.equal(a, b.cpu()) for a, b in zip(got, plain))
+
+
+def test_counts_refused(dv, gpu):  # noqa: F811
+    args = [t.to(gpu) for t in meta_inputs(2, 3, 4, 64, seed=1)]
+    good = torch.zeros(2, 3, dtype=torch.int32, device=gpu)
+    for name in ("dropped", "committed"):
+        for bad, text in ((good[:1], "must be"), (good.long(), "int32"), (good.t().contiguous().t(), "contiguous")):
+            with pytest.raises(RuntimeError, match=text):
+                dv.dvattn_tree_metadata(*args, **{name: bad})
+        with pytest.raises(RuntimeError):
+            dv.dvattn_tree_metadata(*args, **{name: good.cpu()})
+
+
 class Loop:
     """Sequences of a prompt (view 0) and tokens of their own (view 1), whose own rows
     each KV head may have cut; `tokens[w][h]` lists what the cache should hold:
@@ -134,7 +162,7 @@ class Loop:
 
     def keep(self, accepted, new, first):
         """Accepted paths (ascending node indices) stay; returns their lengths [W]."""
-        N = max(len(a) for a in accepted)
+        N = max(1, max(len(a) for a in accepted))
         path = torch.tensor([a + [-1] * (N - len(a)) for a in accepted], dtype=torch.int32, device=self.gpu)
         self.dv.dvattn_paged_kv_compact(path[:, None].contiguous(), first, self.kc, self.vc, self.bt)
         for w in range(self.W):
@@ -162,3 +190,20 @@ def test_drafting_on_caches_that_were_cut(dv, gpu):  # noqa: F811
         assert first.tolist() == [37 + n] * 2
         held = held + loop.keep([[0, 3, 5], [0, 1, 3]], new, first)
         position += 3
+
+
+def test_drafting_on_sequences_of_uneven_lengths(dv, gpu):  # noqa: F811
+    """Accepted paths of different lengths, an own view that starts empty, and a cut that
+    only the longer sequences need: each sequence's own rows, not the shared length."""
+    loop = Loop(dv, gpu, prompt=20, seed=9)
+    loop.fill(0, 20, 0)
+    S = PARENTS.shape[1]
+    held, position = torch.tensor([0, 0]), [20, 20]
+    for accepted in ([[0, 3, 5], [0]], [[1, 4], [0, 1, 3, 5]], [[0], [0, 4]], [[], [0, 1, 2]], [[0, 2], [0, 1]]):
+        if int(held.max()) > 8:
+            held = loop.cut(held, 8)
+        committed = torch.tensor([[20, int(n)] for n in held], dtype=torch.int32, device=gpu)
+        new, first, *_ = loop.draft(PARENTS, [20, int(held.max()) + S], position, committed=committed)
+        assert first.tolist() == [20 + int(n) for n in held]
+        held = held + loop.keep(accepted, new, first)
+        position = [p + len(a) for p, a in zip(position, accepted)]

@@ -13,13 +13,14 @@ def lib():
 
 
 def meta(lib, F=1, W=2, S=4, R=64, **ptr):
-    names = ("loc", "cos", "sin", "views", "rows", "fl", "order", "parents", "dropped", "inv")
+    names = ("loc", "cos", "sin", "views", "rows", "fl", "order", "parents", "committed", "dropped", "inv")
     a = {n: ptr.get(n, P) for n in names}
     return lib.dvattn_tree_metadata_counts(*(a[n] for n in names), 1.0, -1, F, W, S, R, None)
 
 
 @pytest.mark.parametrize("kw,status,needle", [
     (dict(dropped=P + 2), INVALID, "dropped"),
+    (dict(committed=P + 1), INVALID, "committed"),
     (dict(dropped=None, loc=None), INVALID, "null"),
     (dict(W=-1), INVALID, "negative"),
     (dict(S=4097), UNSUPPORTED, "drafted nodes"),
@@ -30,10 +31,10 @@ def test_counts_refused(lib, kw, status, needle):
 
 
 def test_empty_calls_succeed(lib):
-    assert meta(lib, W=0) == 0 and meta(lib, W=0, dropped=None) == 0
+    assert meta(lib, W=0) == 0 and meta(lib, W=0, dropped=None, committed=None) == 0
 
 
 def test_schema_keeps_the_earlier_calls():
     import dvattention_amd  # noqa: F401
     schema = str(torch.ops.libdvatt.dvattn_tree_metadata.default._schema)
-    assert "ScalarType? round_to=None, Tensor? dropped=None" in schema
+    assert "ScalarType? round_to=None, Tensor? dropped=None, Tensor? committed=None" in schema
