@@ -222,7 +222,12 @@ def dvattn_paged_key_mass(mass: Optional[torch.Tensor], queries: torch.Tensor, l
     mass ``[W,Hkv,capacity]`` float32, by row of each sequence's page stream (views
     one after the other); ``out`` defaults to ``mass`` itself (accumulation in place).
     With ``decay=0`` mass is not read and may be None if ``out`` is given.  Rows at or
-    past the capacity take part in the softmax and are not stored."""
+    past the capacity take part in the softmax and are not stored.  Lengths below zero
+    count as 0.
+
+    Every query votes, and its locations say all that it sees: the tables of a tree step
+    would leave out the drafted rows.  The weights of its accepted tokens are those of
+    the causal chain that they are once ``dvattn_paged_kv_compact`` has kept them."""
     if out is None:
         out = mass
     if out is None:

@@ -340,7 +340,10 @@ DVATTN_API dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scal
  *                query heads of KV head h give to the key in row c
  * with the weights of dvattn_paged_sdpa (same queries, locations, cos/sin, scale), in
  * fp32.  Rows no query sees only decay; rows from capacity on take part in the
- * softmax and are not stored.  out may be mass (accumulation in place), else they
+ * softmax and are not stored.  All S queries take part and see what their locations say:
+ * those of a drafted tree (dvattn_tree_metadata) leave out its own rows, so a tree's
+ * accepted tokens are passed as the causal chain they are once they are kept.  out may be
+ * mass (accumulation in place), else they
  * must not overlap; with decay 0 mass is not read and may be null.  Every key is
  * summed in a fixed order: the same call gives the same bits.  Workspace of a single
  * token: about a quarter of a 16-bit K cache of W * max_blocks_per_seq pages, at most

@@ -207,3 +207,40 @@ def test_drafting_on_sequences_of_uneven_lengths(dv, gpu):  # noqa: F811
         assert first.tolist() == [20 + int(n) for n in held]
         held = held + loop.keep(accepted, new, first)
         position = [p + len(a) for p, a in zip(position, accepted)]
+
+
+def test_key_mass_of_accepted_tokens(dv, gpu):  # noqa: F811
+    """The accepted tokens of a tree, passed as a causal chain once they are kept: every
+    key collects the weights that the tree attention gave it.  A weight is off by a factor
+    exp(2 * 1.1e-3), as above."""
+    loop = Loop(dv, gpu, prompt=20, seed=3)
+    loop.fill(0, 20, 0)
+    loop.fill(20, 40, 20)
+    W, S = PARENTS.shape
+    held = loop.cut(torch.tensor([40, 40]), 25)
+    committed = torch.tensor([[20, 25]] * W, dtype=torch.int32, device=gpu)
+    for accepted in ([[0, 3, 5], [0]], [[1], [0, 1, 2]]):
+        position = [20 + int(c) + int(d) for c, d in zip(committed[:, 1], loop.dropped[:, 1])]
+        before = [len(loop.tokens[w][0]) for w in range(W)]
+        new, first, q, (loc, cos, sin, views, fl), weights = loop.draft(
+            PARENTS, [20, int(committed[:, 1].max()) + S], position, committed=committed)
+        committed[:, 1] += loop.keep(accepted, new, first).to(torch.int32).to(gpu)
+        F, N, R, Hq = 2, max(map(len, accepted)), cos.shape[3], q.shape[1]
+        path = torch.tensor([a + [-1] * (N - len(a)) for a in accepted], dtype=torch.int32, device=gpu)[:, None]
+        taken, take = path[:, 0] >= 0, path[:, 0].clamp(min=0).long()
+        of = lambda t: t.gather(2, take.view(1, W, N, 1).expand(F, W, N, t.size(3)))  # noqa: E731
+        seen = loc.gather(2, take.expand(F, W, N))
+        seen[views.long(), torch.arange(W, device=gpu)] += 1 + torch.arange(N, dtype=torch.int32, device=gpu)
+        seen = torch.where(taken, seen, -1)
+        voters = q.to(gpu).gather(2, take.view(W, 1, N, 1).expand(W, Hq, N, E))
+        mass = torch.rand(W, loop.Hkv, 80, generator=loop.g)
+        got = dv.dvattn_paged_key_mass(mass.to(gpu), voters, seen, of(cos), of(sin), fl, loop.kc, loop.bt, SCALE,
+                                       decay=0.5).cpu()
+        want = mass.double() * 0.5
+        for w in range(W):
+            for h in range(loop.Hkv):
+                for s in accepted[w]:
+                    p = weights[w, h, s]
+                    assert len(p) <= before[w] + len(accepted[w])
+                    want[w, h, :len(p)] += p
+        assert ((got - want).abs() <= 2.3e-3 * want).all()
