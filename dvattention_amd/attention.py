@@ -263,7 +263,7 @@ def dvattn_paged_kv_compact(rows: torch.Tensor, first_rows: torch.Tensor, k_cach
     alike: the accepted path of a drafted tree, with ``first_rows = tree_rows``.
     ``mass [W,Hkv,capacity]`` moves along (needs lengths); entries of the range's
     rows that nothing moves into become 0.  The caches may be strided views as in
-    ``dvattn_paged_kv_append``.  The moved rows' pages must not be named twice in
+    ``dvattn_paged_kv_append``, and may not share rows.  The moved rows' pages must not be named twice in
     ``block_tables``: pages that sequences or segments share lie before first_rows.
     Positions of the kept keys do not change (their rotation stays valid); the
     caller's locations and lengths count rows from here on, and the queries' positions

@@ -1103,6 +1103,9 @@ dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, c
                                             {block_tables, "block_tables", 4}, {first_rows, "first_rows", 4},
                                             {lengths, "lengths", 4}, {mass, "mass", 4}});
     if (st != DVATTN_OK) return st;
+    // keys and values are moved by blocks of their own, unordered: one array would be moved twice
+    if (k_cache == v_cache && s->num_blocks > 0 && s->E > 0 && s->Ev > 0)
+        return fail(DVATTN_ERR_INVALID, "k_cache and v_cache are the same array");
     dv::CompactParams p;
     memset(&p, 0, sizeof(p));
     p.kc = k_cache;

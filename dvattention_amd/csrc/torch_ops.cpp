@@ -808,6 +808,15 @@ void dvattn_kv_select_op(at::Tensor& rows, const at::Tensor& mass, const at::Ten
                  "dvattn_kv_select");
 }
 
+// Whether the two caches certainly share rows: they start at the same element, or both are
+// dense and their memory overlaps.  (Keys and values side by side in one tensor, strided,
+// are two caches.)
+bool caches_share_rows(const at::Tensor& k, const at::Tensor& v) {
+    if (k.numel() == 0 || v.numel() == 0) return false;
+    const at::MemOverlapStatus o = at::get_overlap_status(k, v);
+    return k.data_ptr() == v.data_ptr() || o == at::MemOverlapStatus::Full || o == at::MemOverlapStatus::Partial;
+}
+
 // dvattn_paged_kv_compact(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_tables, Tensor rows,
 //   Tensor first_rows, Tensor? lengths=None, Tensor(c!)? mass=None)
 void dvattn_paged_kv_compact_op(at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& block_tables,
@@ -838,6 +847,8 @@ void dvattn_paged_kv_compact_op(at::Tensor& k_cache, at::Tensor& v_cache, const 
                     "dvattn_paged_kv_compact: the last dim of the caches must be contiguous");
     at::assert_no_internal_overlap(k_cache);
     at::assert_no_internal_overlap(v_cache);
+    TORCH_CHECK(!caches_share_rows(k_cache, v_cache),
+                "dvattn_paged_kv_compact: k_cache and v_cache overlap: their rows are moved separately");
     TORCH_CHECK(v_cache.size(0) == P && v_cache.size(1) == bs && v_cache.size(2) == Hkv,
                 "dvattn_paged_kv_compact: v_cache must be [num_blocks, block_size, Hkv, Ev], got ", v_cache.sizes());
     TORCH_CHECK(rows.size(1) == Hkv || rows.size(1) == 1, "dvattn_paged_kv_compact: rows must be [W,Hkv|1,N] with Hkv=",

@@ -381,7 +381,8 @@ DVATTN_API dvattn_status dvattn_kv_select(int* rows, const float* mass, const in
  * shape fields W, Hkv, E, Ev, block_size, max_blocks_per_seq, num_blocks and the
  * layout's cache strides.  The queries that follow keep counting positions with the rows
  * that went (dropped above).  The pages of the rows moved must each be named once in
- * block_tables (pages shared by sequences or segments lie before first_rows). */
+ * block_tables (pages shared by sequences or segments lie before first_rows), and k_cache
+ * and v_cache may not share rows (the same array is refused). */
 DVATTN_API dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, const int* block_tables,
                                       const int* rows, int row_heads, int N, const int* first_rows,
                                       const int* lengths, float* mass, long long capacity,

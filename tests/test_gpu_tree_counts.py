@@ -244,3 +244,22 @@ def test_key_mass_of_accepted_tokens(dv, gpu):  # noqa: F811
                     assert len(p) <= before[w] + len(accepted[w])
                     want[w, h, :len(p)] += p
         assert ((got - want).abs() <= 2.3e-3 * want).all()
+
+
+def test_compaction_of_caches_that_share_rows(dv, gpu):  # noqa: F811
+    """Refused where both certainly hold the same rows; keys and values side by side in one
+    tensor are two caches."""
+    rows = torch.tensor([[[1, 3]]], dtype=torch.int32, device=gpu)
+    first, bt = torch.zeros(1, dtype=torch.int32, device=gpu), torch.tensor([[1, 0]], dtype=torch.int32, device=gpu)
+    kv = torch.randn(2, 4, 2, 2, 64, generator=torch.Generator().manual_seed(1)).to(gpu)
+    before = kv.clone()
+    flat = kv.view(-1)
+    one, behind = flat[:1024].view(2, 4, 1, 128), flat[512:1536].view(2, 4, 1, 128)
+    for k, v in ((one, one), (one, behind), (kv[:, :, 0], kv[:, :, 0]), (kv[:, :, 0], kv[:, :, 0, :, :32])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            dv.dvattn_paged_kv_compact(rows, first, k, v, bt)
+    assert torch.equal(kv, before)
+    dv.dvattn_paged_kv_compact(rows, first, kv[:, :, 0], kv[:, :, 1], bt)
+    want = before.clone()
+    want[1, 0], want[1, 1] = before[1, 1], before[1, 3]
+    assert torch.equal(kv, want)

@@ -38,3 +38,17 @@ def test_schema_keeps_the_earlier_calls():
     import dvattention_amd  # noqa: F401
     schema = str(torch.ops.libdvatt.dvattn_tree_metadata.default._schema)
     assert "ScalarType? round_to=None, Tensor? dropped=None, Tensor? committed=None" in schema
+
+
+def test_compaction_refuses_one_array_as_both_caches(lib):
+    """Keys and values are moved separately: rows of an array that is both would be moved twice."""
+    import ctypes
+
+    from dvattention_amd import capi
+    s = capi.Shape(F=0, W=2, Hq=0, Hkv=1, E=128, Ev=128, S=0, block_size=16, max_blocks_per_seq=4, total_q_tokens=0,
+                   num_blocks=8, rotary_dim=0)
+    lay = capi.KvLayout()
+    p = ctypes.c_void_p(P)
+    assert lib.dvattn_paged_kv_compact(2, p, p, p, p, 1, 4, p, None, None, 0, ctypes.byref(s), ctypes.byref(lay),
+                                       None) == INVALID
+    assert "same array" in lib.dvattn_last_error().decode()
