@@ -986,10 +986,11 @@ dvattn_status dvattn_paged_key_mass(int dtype, float* out, const float* mass, fl
     const long long rows = max_rows > capacity ? max_rows : capacity;
     if (max_rows >= (1ll << 32))
         return fail(DVATTN_ERR_UNSUPPORTED, "block tables of %lld rows exceed 2^32", max_rows);
-    // a launch holds 2^24 blocks of 256 threads: one per 128 rows and view at least, two per token's query operand
-    const long long wh = (long long)s->W * s->Hkv;
-    if (wh >= (1ll << 24) || wh * (rows / 128 + s->F + 2) >= (1ll << 24) ||
-        wh * s->S * (s->F > 0 ? s->F : 1) >= (1ll << 23))
+    // a launch holds 2^24 blocks of 256 threads: one per 128 rows and view at least; two per token's
+    // query operand and one per sequence.  (Each factor is bounded before a product that it is in.)
+    const long long limit = 1ll << 24, wh = (long long)s->W * s->Hkv, sf = (long long)s->S * (s->F > 0 ? s->F : 1);
+    if (wh >= limit || rows >= limit * 128 || sf >= limit || wh * (rows / 128 + s->F + 2) >= limit ||
+        wh * sf * 2 + s->W > limit)
         return fail(DVATTN_ERR_UNSUPPORTED, "W=%d, Hkv=%d, S=%d, %lld rows: too many blocks for one launch", s->W,
                     s->Hkv, s->S, rows);
     if (!out || (s->S > 0 && !queries) || (decay != 0.0f && !mass))

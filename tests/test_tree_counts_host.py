@@ -52,3 +52,25 @@ def test_compaction_refuses_one_array_as_both_caches(lib):
     assert lib.dvattn_paged_kv_compact(2, p, p, p, p, 1, 4, p, None, None, 0, ctypes.byref(s), ctypes.byref(lay),
                                        None) == INVALID
     assert "same array" in lib.dvattn_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,capacity", [
+    (dict(W=256, Hkv=1, Hq=16, S=4), 1 << 62),                   # W * Hkv * rows past 2^63
+    (dict(W=256, Hkv=1, Hq=16, S=1), (1 << 63) - 1),
+    (dict(W=1 << 20, S=1 << 22, F=1 << 21), 64),                  # W * S * F past 2^62
+    (dict(W=1 << 22, S=2, F=0, max_blocks_per_seq=0), 64),        # one block of the plan too many
+    (dict(W=(1 << 22) - 1, S=2, F=1, max_blocks_per_seq=0), 64),
+])
+def test_key_mass_beyond_a_launch_refused(lib, kw, capacity):
+    """Sizes whose products leave 63 bits, and calls one launch cannot hold."""
+    import ctypes
+
+    from dvattention_amd import capi
+    base = dict(F=1, W=2, Hq=16, Hkv=1, E=128, Ev=128, S=4, block_size=16, max_blocks_per_seq=4, total_q_tokens=0,
+                num_blocks=8, rotary_dim=64)
+    s = capi.Shape(**{**base, **kw})
+    p = ctypes.c_void_p(P)
+    for dtype in (0, 2):
+        got = lib.dvattn_paged_key_mass(dtype, p, p, 1.0, capacity, 0.1, p, p, p, p, p, p, p, ctypes.byref(s), p,
+                                        (1 << 64) - 1, None)
+        assert got == UNSUPPORTED and "too many blocks" in lib.dvattn_last_error().decode()
