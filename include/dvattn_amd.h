@@ -375,8 +375,9 @@ DVATTN_API dvattn_status dvattn_kv_select(int* rows, const float* mass, const in
  * Hkv or 1 (the same rows for every KV head: a tree's accepted path, with first_rows =
  * tree_rows).  Entries may come in any order and more than once; one below its place,
  * past the range, or whose source or destination lies on no valid page moves nothing.
- * With mass [W,Hkv,capacity] f32 (needs lengths) its entries move alike, and those of
- * the rows first_rows[w] + i, i < lengths[w], that nothing moves into become 0
+ * With mass [W,Hkv,capacity] f32 (needs lengths) its entries move by the rows and the
+ * range alone (row first_rows[w] + i takes the entry of rows[w,h,i], whatever the pages), and
+ * those of the rows first_rows[w] + i, i < lengths[w], that nothing moves into become 0
  * (capacity <= 2^30).  Uses
  * shape fields W, Hkv, E, Ev, block_size, max_blocks_per_seq, num_blocks and the
  * layout's cache strides.  The queries that follow keep counting positions with the rows
