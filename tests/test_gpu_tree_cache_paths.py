@@ -1,0 +1,113 @@
+"""GPU tests of the tree and bounded-cache operators at the sizes that choose the
+less common ways through their kernels (marked ``gpu``): one token's key mass with
+several units of keys per wave, lists of more rows than a block's registers hold, one
+node per sequence through the multi-query kernel, many views, and every key's weight
+read off the output.  Oracles and tolerances: test_gpu_tree_cache."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_tree_cache import (DTYPES, E, SCALE, check_mass, check_tree, compare_tree, dv, mass_case,  # noqa: F401
+                                 run_select, to, tree_case, widened)
+from oracle import tree_cache_oracle as TO
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------
+# Key mass of one token: two and four units of 64 keys (fp32: 32) per wave from 2^20
+# and 2^21 (fp32: 2^19 and 2^20) rows of block tables on.
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("units", [2, 4])
+@pytest.mark.parametrize("fl,bs,bad", [
+    ([2050], 16, False),             # whole units and a ragged end
+    ([700, 450, 900, 3], 16, True),  # views that meet inside a wave's later units; missing pages
+    ([100] * 9 + [0, 61], 24, False),
+])
+def test_key_mass_several_units(dv, gpu, dtype, units, fl, bs, bad):  # noqa: F811
+    d, mass = mass_case(dtype, 2, 2, 1, fl, bs, 64, seed=len(fl), bad=bad)
+    d["locations"][0, 0] = 10 ** 6  # one sequence sees a whole view
+    narrow = check_mass(dv, gpu, d, mass, 0.75)
+    rows = units * (1 << 17) // (2 if dtype == torch.float32 else 1)
+    wide = widened(d, -(-rows // bs) * bs)
+    again = check_mass(dv, gpu, wide, mass, 0.75)
+    assert (narrow - again).abs().max() <= 1e-4
+    assert torch.equal(again, check_mass(dv, gpu, wide, mass, 0.75, in_place=True))
+    check_mass(dv, gpu, wide, mass, 0.0, scale=-SCALE)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("S,rows", [(1, 0), (4, 0), (4, 60000)])
+def test_key_mass_many_views(dv, gpu, dtype, S, rows):  # noqa: F811
+    """Seventeen short views, empty ones among them, for each way through the kernels."""
+    fl = [33, 0, 70, 15, 16, 17, 1, 64, 0, 40, 90, 5, 31, 32, 48, 60, 7]
+    d, mass = mass_case(dtype, 2, 1, S, fl, 16, 64, seed=S)
+    d["locations"][5:9, 1] = -1
+    check_mass(dv, gpu, widened(d, rows), mass, 0.5)
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fl", [[1], [90], [30, 0, 50, 7]])
+def test_tree_sdpa_one_node(dv, gpu, dtype, fl):  # noqa: F811
+    """One node per sequence under a table so wide that the multi-query kernel takes it."""
+    d = tree_case(dtype, 3, 2, 1, fl, 16, 64, seed=7, absent=0.0)
+    want, size, spread = TO.tree_sdpa(SCALE, **d)
+    got = dv.dvattn_tree_paged_sdpa(scale=SCALE, **to(gpu, widened(d, 1 << 20))).cpu()
+    compare_tree(got, d, dtype, want, size, spread)
+    d["parents"][1] = -2
+    out = dv.dvattn_tree_paged_sdpa(scale=SCALE, **to(gpu, widened(d, 1 << 20))).cpu()
+    assert not out[1].any() and torch.equal(out[0], got[0])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("F", [5, 17])
+@pytest.mark.parametrize("S", [1, 6, 20])
+def test_tree_sdpa_many_views(dv, gpu, dtype, F, S):  # noqa: F811
+    """More views than the short-list kernel holds the queries of."""
+    fl = [S + 3 + 7 * (f % 4) if f % 5 else 2 * S for f in range(F)]
+    check_tree(dv, gpu, tree_case(dtype, 2, 1, S, fl, 16, 64, seed=F + S), dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("S,fl", [(9, [120]), (20, [60, 40]), (1, [100])])
+def test_tree_sdpa_weight_of_every_key(dv, gpu, dtype, S, fl):  # noqa: F811
+    """The value of stream row l is the l-th unit vector, so an output's elements are its
+    keys' weights: in float32 each is held to its own size, however small, and a key lost
+    or counted twice is off by all of it."""
+    d = tree_case(dtype, 2, 2, S, fl, 16, 64, seed=S)
+    P, bs = d["k_cache"].shape[:2]
+    d["v_cache"].zero_()
+    for w in range(2):
+        for pos in range(sum(fl)):
+            page, row = TO.cache_row(d["block_tables"], w, pos, P, bs)
+            d["v_cache"][page, row, :, pos] = 1.0
+    got, want = check_tree(dv, gpu, d, dtype)
+    if dtype == torch.float32:
+        assert torch.equal(got != 0, want != 0)
+    sums = got.double().sum(-1)
+    assert ((sums - (want.sum(-1) > 0).double()).abs() <= 2.0 ** -6).all()
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("m", [32767, 32768, 32769, 40001, 70000])
+@pytest.mark.parametrize("kind", ["wide", "narrow", "few", "special"])
+def test_select_long_lists(dv, gpu, m, kind):  # noqa: F811
+    """Up to and past the 32768 competing rows that a block's registers hold: weights of
+    many sizes (few share the deciding digit), of one size (more than the short list
+    holds do), few distinct ones, and specials."""
+    g = torch.Generator().manual_seed(m)
+    kf, kl, first = 3, 21, 1000
+    n = m + kf + kl
+    if kind == "wide":
+        mass = torch.exp(3 * torch.randn(2, 1, first + n + 17, generator=g))
+    elif kind == "narrow":
+        mass = 1.0 + torch.rand(2, 1, first + n + 17, generator=g) * 2.0 ** -5
+    elif kind == "few":
+        mass = torch.randint(0, 3, (2, 1, first + n + 17), generator=g).float()
+    else:
+        mass = torch.tensor([math.nan, math.inf, -math.inf, -1.0, 0.0, -0.0, 1e-42, 7.0])[
+            torch.randint(0, 8, (2, 1, first + n + 17), generator=g)]
+    for budget in (kf + kl + 1, n // 4, n - 1):
+        run_select(dv, gpu, mass, [0, first], [n, n], budget, kf, kl)
