@@ -1088,7 +1088,8 @@ dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, c
         return fail(DVATTN_ERR_INVALID, "max_blocks_per_seq / num_blocks must be >= 0");
     if (s->E > 8192 || s->Ev > 8192)
         return fail(DVATTN_ERR_UNSUPPORTED, "head dims up to 8192 (E=%d, Ev=%d)", s->E, s->Ev);
-    // blocks of 1024 threads of one launch: up to 65 per (sequence, KV head)
+    // blocks of 512 threads of one launch: fewer than 1024 for the slices of small calls, else up
+    // to 33 per (sequence, KV head): 16 slices of 8192 elements, K and V, and mass
     if ((long long)s->W * s->Hkv >= (1ll << 15) || N > (1 << 30))
         return fail(DVATTN_ERR_UNSUPPORTED, "W * Hkv = %lld and N = %d: below 2^15 and at most 2^30",
                     (long long)s->W * s->Hkv, N);

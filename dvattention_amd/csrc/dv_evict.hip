@@ -56,9 +56,8 @@ __device__ inline int block_excl(int v, int* s_wave) {
 // A wave owns a contiguous stretch of rows, so its places follow from one count per
 // wave and a running one inside it, and no pass has a barrier in its loop.  Up to
 // kSelHeld * 1024 rows are read once and held in registers; more are read again
-// (from L2) in each of the five passes.  Bound by the chain of passes: 1000 rows 7.2
-// us; 128 lists of 32768 rows, a block each, 25.4 (loads 6.4, first digit 8, the list
-// and the other digits 4, counts 3.7, writes 7).
+// (from L2) in each of the five passes.  Bound by the chain of passes, and a list has one
+// block: 1000 rows 7.2 us; 128 lists of 32768 rows 25.4, with half of the CUs idle.
 template <int kSelHeld>
 __global__ __launch_bounds__(kSelThreads) void dv_kv_select(const SelectParams p) {
     __shared__ int s_hist[kBins];
@@ -380,9 +379,10 @@ hipError_t launch_kv_compact(int dtype, const CompactParams& base, hipStream_t s
     const int elems = vec ? 16 / es : 1;
     const int kv = p.E / elems, vv = p.Ev / elems;
     const int widest = kv > vv ? kv : vv;
-    // slices of at least 128 bytes until the call has 512 blocks, two per CU (16 sequences,
-    // 8 KV heads, 4096 of 8100 rows kept: 118 us, with 256 blocks 132, of 1024 threads 132),
-    // and as many as a block's threads need
+    // slices of at least 128 bytes while the call has fewer than 512 blocks, two per CU (16
+    // sequences, 8 KV heads, 4096 of 8100 rows kept: 112-118 us, with 256 blocks 132, of 1024
+    // threads 132) -- a 16-bit row of 128 is two slices at most, so fewer than 128 (sequence,
+    // KV head) pairs stay below that -- and as many as a block's threads need
     int slices = 1;
     while (slices < widest && ((long long)p.W * p.Hkv * 2 * slices < 512 && widest * elems * es / (2 * slices) >= 128))
         slices *= 2;

@@ -17,12 +17,13 @@
 //  * S = 1 (a decode step; bound by memory): the queries are rotated in the kernel
 //    and the scores stored (64 bytes per key and KV head, a quarter of a 16-bit K row, an
 //    eighth of an fp32 one), so the second pass reads those and not K.
-//  * S > 1 (a window of tokens; bound by the exponentials): a wave holds 64 keys (32
+//  * S > 1 (a window of tokens; bound by waits and issue, see dv_mass_stats): a wave holds 64 keys (32
 //    for fp32) and walks the tokens, whose queries one launch beforehand rotated into
 //    the MFMA's operand order; the second pass computes the scores again (storing
 //    them would cost more bytes than K from two tokens on).  Over few keys, where that
 //    walk is all a call's time, the waves of a block share the tokens (dv_mass_small).
-//    At most kMassTokens tokens per launch bound the workspace.
+//    A launch takes at most kMassTokens tokens, which bounds the pairs (max, sum) in the
+//    workspace; the rotated queries in it are those of all tokens and views.
 #include <type_traits>
 
 #include "dv_common.h"
@@ -868,10 +869,12 @@ __device__ inline void walk_tokens(const MassParams& p, const Part& it, unsigned
 
 }  // namespace
 
-// Per seen part, token of the launch and head, (max, sum).  Bound by VALU issue: about 110
-// instructions (maximum, 16 exponentials, sums) beside 16 MFMAs per token and wave.  Four
-// sequences of 9000 keys in two views, 4 KV heads, 32 tokens in fp16: 46 us (0.4 PFLOP/s),
-// dv_mass_apply 43.
+// Per seen part, token of the launch and head, (max, sum): about 110 VALU instructions
+// (maximum, 16 exponentials, sums) beside 16 MFMAs per token and wave.  Four sequences of
+// 9000 keys in two views, 4 KV heads, 32 tokens in fp16: 46 us (0.4 PFLOP/s), dv_mass_apply
+// 43.  By its counters a SIMD issues VALU instructions for 15 us of that and its matrix unit
+// runs for 8.5; the waves wait for 41 % of their time (apply: 45 %), at the end of every
+// group of four tokens and its barriers, and the 587 parts are two or three per CU.
 template <int DT, int NT>
 __global__ __launch_bounds__(kMassThreads) void dv_mass_stats(const MassParams p) {
     __shared__ __align__(16) unsigned char ring[kRingBytes<DT>];
@@ -989,7 +992,8 @@ int tiles_of(int dtype) { return dtype == kF32 ? kTilesOf<kF32> : kTilesOf<kBF16
 constexpr long long kMaxScoreBytes = 1ll << 30;
 
 // dv_mass_small up to so many blocks of it: two per CU, and four where a sequence has few
-// (each block goes through the pairs of all blocks of its sequence).  Beside the kernels of
+// (each block goes through the pairs of all blocks of its sequence: 33 parts are about as fast either
+// way at 1056 blocks, 64 parts slower at 1024).  Beside the kernels of
 // the plan, bf16, 4 KV heads, 5 / 33 tokens: 20 blocks 13 / 21 us instead of 24 / 55; 252
 // of one sequence 14 / 27 instead of 24 / 55; 400 of 20 sequences 19 / 40 instead of 25 /
 // 62; 576 of 16 21 / 42 instead of 27 / 64; 760 of two 30 / 67 instead of 25 / 60; 1024 of

@@ -15,8 +15,8 @@
 // Work per node is its depth, not the tree's size: a mask over all drafted rows on
 // the matrix units would multiply S^2 pairs of which a tree of depth d sees S * d.
 //
-// 16 trees of 64 nodes over 8192 keys, 8 KV heads in bf16: the multi-query kernel 585 us
-// (650 TFLOP/s), the merge 35.
+// 16 trees of 64 nodes over 8192 keys, 8 KV heads in bf16: 621 us a call (650 TFLOP/s), of
+// which the merge is 32-35 and the multi-query kernel the rest (685 TFLOP/s).
 //
 // Short sequences take one launch instead (dv_tree_small, below).
 #include "dv_chunk.h"

@@ -324,7 +324,10 @@ DVATTN_API dvattn_status dvattn_tree_metadata_counts(int* locations, float* cosi
  * each key once.  An absent node's output is zeros.  A drafted row that a node
  * does not see is not read for it, whatever it holds; a committed key past a
  * node's location but within that of another node of its sequence takes part with
- * weight 0 and must be finite, as in dvattn_paged_sdpa.  S <= 4096. */
+ * weight 0 and must be finite, as in dvattn_paged_sdpa.  S <= 4096.
+ * Weights of bf16 calls are rounded to bf16 for the product with V, as in
+ * dvattn_paged_sdpa, where the block tables are wide; under narrow ones (and in the other
+ * types) they are not: the same keys may round differently under another table. */
 DVATTN_API size_t dvattn_tree_paged_sdpa_workspace_size(int dtype, const dvattn_shape* shape, int device);
 DVATTN_API dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scale, const int* locations,
                                      const void* queries, const float* cosines, const float* sines,
@@ -347,7 +350,9 @@ DVATTN_API dvattn_status dvattn_tree_paged_sdpa(int dtype, void* out, float scal
  * must not overlap; with decay 0 mass is not read and may be null.  Every key is
  * summed in a fixed order: the same call gives the same bits.  Workspace of a single
  * token: about a quarter of a 16-bit K cache of W * max_blocks_per_seq pages, at most
- * 1 GiB of scores. */
+ * 1 GiB of scores; of several: the rotated queries of all of them, [F,W,Hq,S,E] in dtype,
+ * and 128 bytes per KV head, part of the keys (32 to 256 rows) and token, of at most 64
+ * tokens at a time. */
 DVATTN_API size_t dvattn_paged_key_mass_workspace_size(int dtype, const dvattn_shape* shape, long long capacity);
 DVATTN_API dvattn_status dvattn_paged_key_mass(int dtype, float* out, const float* mass, float decay,
                                     long long capacity, float scale, const int* locations, const void* queries,
