@@ -683,7 +683,7 @@ __device__ void chunk_piece(const DecodeParams& p, unsigned char* smem, int* pag
         } else {
             const int tb = tok0 + t;  // token within the block
             store_partial<DT>(p.part + (long long)slot * p.slot_floats, kTokBlk * kGqa, tb * kGqa + n, g, tl[t].o,
-                              inv, lt > 0.0f ? tl[t].m + log2f(lt) : -DV_INF);
+                              inv, row_lse(tl[t].m, lt));
         }
     }
     }

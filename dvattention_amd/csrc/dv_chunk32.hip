@@ -289,7 +289,7 @@ __device__ void chunk32_piece(const DecodeParams& p, unsigned char* smem, int* p
             for (int c = 0; c < 8; ++c) *reinterpret_cast<f32x4*>(o + c * 16 + g * 4) = tl[t].o[c] * inv;
         } else {
             store_partial<kF32>(p.part + (long long)slot * p.slot_floats, kTokBlk * kGqa, tb * kGqa + n, g, tl[t].o,
-                                inv, lt > 0.0f ? tl[t].m + log2f(lt) : -DV_INF);
+                                inv, row_lse(tl[t].m, lt));
         }
     }
 }

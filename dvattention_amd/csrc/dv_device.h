@@ -435,6 +435,13 @@ __device__ inline int partial_exp(float amax) {
     return k < 100 ? k : 100;
 }
 
+// Base-2 log-sum-exp of a row of maximum m and weight sum l: -inf for a row that saw no
+// key, and NaN where a NaN score went into the sum, so that a merge cannot take the one for
+// the other.
+__device__ inline float row_lse(float m, float l) {
+    return l > 0.0f ? m + log2f(l) : l == 0.0f ? -DV_INF : l;
+}
+
 // Lane (g, n) holds dims c*16 + g*4 + e (c < 8, e < 4) of slot row j in o
 // (unnormalised; inv = 1 / row sum); the four lanes of a row are n + 16g, and
 // every lane of the wave takes part (cross-lane maximum).  g == 0 also writes

@@ -120,7 +120,8 @@ __global__ __launch_bounds__(256) void dv_merge_tree(const DecodeParams p, int n
     }
 
     // the committed keys' pieces: running base-2 maximum m, weight sum, weighted sum.
-    // A piece that saw no key (-inf) holds nothing, whatever its values are.
+    // A piece that saw no key (-inf) holds nothing, whatever its values are; one with a NaN
+    // score has a NaN log-sum-exp (row_lse), which reaches the output.
     float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     float m = -DV_INF, wsum = 0.0f;
     for (int k0 = 0; k0 < cnt; k0 += kTreeBatch) {

@@ -111,3 +111,37 @@ def test_select_long_lists(dv, gpu, m, kind):  # noqa: F811
             torch.randint(0, 8, (2, 1, first + n + 17), generator=g)]
     for budget in (kf + kl + 1, n // 4, n - 1):
         run_select(dv, gpu, mass, [0, first], [n, n], budget, kf, kl)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("S", [1, 2, 5, 17])
+@pytest.mark.parametrize("what", ["nan key", "inf key", "nan query", "every key"])
+def test_tree_sdpa_nan_reaches_the_output(dv, gpu, dtype, S, what):  # noqa: F811
+    """A NaN score among the committed keys makes a node's output NaN, whichever piece of
+    the keys it is in and whatever the others hold; heads whose query turns an infinite
+    key to -infinity only lose that key."""
+    fl = [1500]
+    d = tree_case(dtype, 2, 1, S, fl, 16, 64, seed=S, absent=0.0)
+    d["parents"][:] = -1  # (the drafted rows alone would hide a lost piece)
+    P, bs = d["k_cache"].shape[:2]
+    if what == "nan query":
+        d["queries"][0, 3] = math.nan
+    elif what == "every key":
+        for pos in range(1500 - S - 1):
+            page, row = TO.cache_row(d["block_tables"], 0, pos, P, bs)
+            d["k_cache"][page, row] = math.nan
+    else:
+        page, row = TO.cache_row(d["block_tables"], 0, 700, P, bs)
+        if what == "nan key":
+            d["k_cache"][page, row] = math.nan
+        else:
+            d["k_cache"][page, row, :, 100] = math.inf  # (a dim that is not rotated)
+    want, size, spread = TO.tree_sdpa(SCALE, **d)
+    spread = spread.nan_to_num(0.0, posinf=0.0).clamp(max=1e6)
+    if what == "inf key":  # e as without the key: its weight is 0 where the row is finite
+        spread = TO.tree_sdpa(SCALE, **{**d, "k_cache": d["k_cache"].clamp(max=100.0)})[2]
+    assert want[0].isnan().any() and not want[1].isnan().any()
+    for rows in (0, 2500, 80000, 1 << 20):
+        got = dv.dvattn_tree_paged_sdpa(scale=SCALE, **to(gpu, widened(d, rows))).cpu()
+        assert torch.equal(got.isnan(), want.isnan()), f"table of {rows} rows"
+        compare_tree(got, d, dtype, want, size, spread)
