@@ -145,3 +145,21 @@ def test_tree_sdpa_nan_reaches_the_output(dv, gpu, dtype, S, what):  # noqa: F81
         got = dv.dvattn_tree_paged_sdpa(scale=SCALE, **to(gpu, widened(d, rows))).cpu()
         assert torch.equal(got.isnan(), want.isnan()), f"table of {rows} rows"
         compare_tree(got, d, dtype, want, size, spread)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("S,rows", [(1, 0), (1, 1 << 18), (3, 0), (3, 60000), (70, 0)])
+@pytest.mark.parametrize("what", [math.nan, math.inf])
+def test_key_mass_of_nan_and_infinite_keys(dv, gpu, dtype, S, rows, what):  # noqa: F811
+    """A NaN score makes every weight of its (token, head) NaN, an infinite key does so for
+    the heads that score it +infinity and weighs nothing for the others; other sequences
+    and rows past what is seen keep their own."""
+    d, mass = mass_case(dtype, 2, 1, S, [300], 16, 64, seed=S)
+    d["locations"][0, 0] = 250
+    page, row = TO.cache_row(d["block_tables"], 0, 100, d["k_cache"].shape[0], 16)
+    d["k_cache"][page, row, :, 100] = what
+    want, _ = TO.key_mass(mass, 0.5, SCALE, **d)
+    assert want[0, 0, :251].isnan().all() and want[0, 0, 251:].isfinite().all() and want[1].isfinite().all()
+    got = dv.dvattn_paged_key_mass(mass.to(gpu), scale=SCALE, decay=0.5, **to(gpu, widened(d, rows))).cpu()
+    assert torch.equal(got.isnan(), want.isnan())
+    check_mass(dv, gpu, widened({**d, "locations": d["locations"].clamp(max=99)}, rows), mass, 0.5)
