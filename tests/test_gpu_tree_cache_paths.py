@@ -163,3 +163,41 @@ def test_key_mass_of_nan_and_infinite_keys(dv, gpu, dtype, S, rows, what):  # no
     got = dv.dvattn_paged_key_mass(mass.to(gpu), scale=SCALE, decay=0.5, **to(gpu, widened(d, rows))).cpu()
     assert torch.equal(got.isnan(), want.isnan())
     check_mass(dv, gpu, widened({**d, "locations": d["locations"].clamp(max=99)}, rows), mass, 0.5)
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_ctypes_entries(dv, gpu, dtype):  # noqa: F811
+    """The C entries through dvattention_amd.capi give the operators' bits, with a workspace
+    of the caller's and without."""
+    from dvattention_amd import capi
+    from test_gpu_tree_cache import compact_case, meta_inputs
+
+    names = ("locations", "queries", "cosines", "sines", "fragment_lengths", "k_cache", "v_cache", "block_tables",
+             "parents", "tree_views", "tree_rows")
+    for rows in (0, 2500, 80000):
+        d = to(gpu, widened(tree_case(dtype, 2, 2, 6, [60, 90], 16, 64, seed=2), rows))
+        want = dv.dvattn_tree_paged_sdpa(scale=SCALE, **d)
+        for ws in (None, torch.empty(64 << 20, dtype=torch.uint8, device=gpu)):
+            out = torch.full_like(want, math.nan)
+            assert torch.equal(capi.tree_paged_sdpa(out, SCALE, *(d[n] for n in names), workspace=ws), want)
+    for S in (1, 3):
+        d, mass = mass_case(dtype, 2, 2, S, [90, 40], 16, 64, seed=2)
+        d, mass = to(gpu, d), mass.to(gpu)
+        want = dv.dvattn_paged_key_mass(mass, scale=SCALE, decay=0.5, out=torch.empty_like(mass), **d)
+        out = capi.paged_key_mass(torch.empty_like(mass), mass, 0.5, SCALE, *(d[n] for n in names[:6]), d["block_tables"])
+        assert torch.equal(out, want)
+    kc, vc, bt, rows, first, lengths, mass = (t.to(gpu) for t in compact_case(dtype, 2, 2, 150, 60, 16, seed=3))
+    want = dv.dvattn_kv_select(mass, first, lengths, 40, 2, 5)
+    assert torch.equal(capi.kv_select(torch.empty_like(want), mass, first, lengths, 2, 5), want)
+    a, b = [t.clone() for t in (kc, vc, mass)], [t.clone() for t in (kc, vc, mass)]
+    dv.dvattn_paged_kv_compact(rows, first, a[0], a[1], bt, mass=a[2], lengths=lengths)
+    capi.kv_compact(b[0], b[1], bt, rows, first, lengths=lengths, mass=b[2])
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    fl, order, parents, inv = (t.to(gpu) for t in meta_inputs(2, 3, 9, 64, seed=4))
+    counts = torch.arange(6, dtype=torch.int32, device=gpu).view(2, 3)
+    for kw in ({}, dict(committed=counts * 11, dropped=counts)):
+        want = dv.dvattn_tree_metadata(fl, order, parents, inv, 1.5, torch.bfloat16, **kw)
+        got = capi.tree_metadata(*(torch.empty_like(t) for t in want), fl, order, parents, inv, 1.5, torch.bfloat16,
+                                 **kw)
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
