@@ -35,18 +35,22 @@ _load_ops()
 
 from .attention import (  # noqa: E402
     apply_rotary_pos_emb,
+    dvattn_block_tables,
     dvattn_fused,
     dvattn_kv_select,
     dvattn_paged_key_mass,
     dvattn_paged_kv_append,
+    dvattn_paged_kv_append_q8,
     dvattn_paged_kv_compact,
     dvattn_paged_sdpa,
+    dvattn_paged_sdpa_q8,
     dvattn_rope,
     dvattn_sdpa,
     dvattn_sdpa_pt,
     dvattn_tree_metadata,
     dvattn_tree_paged_sdpa,
     dvattn_varlen_paged_sdpa,
+    dvattn_varlen_paged_sdpa_q8,
     dvattn_varlen_rope,
     dvattn_view_metadata,
     merge_caches_paged,
@@ -55,18 +59,22 @@ from .attention import (  # noqa: E402
 
 __all__ = [
     "apply_rotary_pos_emb",
+    "dvattn_block_tables",
     "dvattn_fused",
     "dvattn_kv_select",
     "dvattn_paged_key_mass",
     "dvattn_paged_kv_append",
+    "dvattn_paged_kv_append_q8",
     "dvattn_paged_kv_compact",
     "dvattn_paged_sdpa",
+    "dvattn_paged_sdpa_q8",
     "dvattn_rope",
     "dvattn_sdpa",
     "dvattn_sdpa_pt",
     "dvattn_tree_metadata",
     "dvattn_tree_paged_sdpa",
     "dvattn_varlen_paged_sdpa",
+    "dvattn_varlen_paged_sdpa_q8",
     "dvattn_varlen_rope",
     "dvattn_view_metadata",
     "merge_caches_paged",

@@ -272,6 +272,97 @@ def dvattn_paged_kv_compact(rows: torch.Tensor, first_rows: torch.Tensor, k_cach
     return k_cache, v_cache
 
 
+def dvattn_block_tables(lengths: torch.Tensor, new_tokens: torch.Tensor, block_tables: torch.Tensor,
+                        free_pages: torch.Tensor, free_count: torch.Tensor, block_size: int, max_tokens: int,
+                        in_place: bool = False):
+    """Where a step's tokens go in a paged cache, on the device, from request lengths.
+
+    lengths ``[W]`` int32: tokens that each sequence holds; new_tokens ``[W]`` int32:
+    tokens it adds in this step (0: none; negative: the sequence has ended and gives its
+    pages back).  block_tables ``[W,max_blocks]`` int32 are extended in place by the
+    pages that the new tokens need, taken from free_pages ``[num_blocks]`` int32, a stack
+    whose first ``free_count [1]`` int32 entries are the free pages.  Returns
+
+    * ``cu_seqlens [W+1]``: the packed tokens' bounds, sequence after sequence;
+    * ``starts [W]``: the position of each sequence's first new token; -1 for one that has
+      ended, or was refused: the stack, its table row or the ``max_tokens`` packed tokens
+      have no room for it.  A refused sequence takes no page and its length stays;
+    * ``positions [max_tokens]`` int32 and ``slots [max_tokens]`` int64 of the packed
+      tokens (slot = page * block_size + row), -1 for tokens of refused sequences and
+      behind the last;
+    * ``lengths [W]`` and ``free_count [1]`` after the step: new tensors, or with
+      ``in_place`` the ones given (a captured step then carries its state on).
+
+    ``slots`` are ``dvattn_paged_kv_append_q8``'s; ``positions[None]`` are locations of
+    the varlen operators with one view.  Pages that an ending sequence holds may not be
+    shared.  At most 8192 sequences."""
+    lengths_out = lengths if in_place else torch.empty_like(lengths)
+    count_out = free_count if in_place else torch.empty_like(free_count)
+    cu, starts, positions, slots = torch.ops.libdvatt.dvattn_block_tables(
+        block_tables, free_pages, lengths_out, count_out, lengths, new_tokens, free_count, block_size, max_tokens)
+    return cu, starts, positions, slots, lengths_out, count_out
+
+
+def dvattn_paged_kv_append_q8(keys: torch.Tensor, values: torch.Tensor, slots: torch.Tensor, cosines: torch.Tensor,
+                              sines: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                              k_scales: torch.Tensor, v_scales: torch.Tensor):
+    """``dvattn_paged_kv_append`` into a cache held in 8 bits: rotated keys and values are
+    rounded to E4M3 under a power of two for each page and KV head.
+
+    keys/values ``[T,Hkv,E]`` (packed tokens) or ``[W,Hkv,S,E]``, strided views alike;
+    slots ``[T]`` or ``[W,S]`` int64: page * block_size + row (negative: not written), as
+    ``dvattn_block_tables`` gives them; cosines/sines ``[T,R]`` / ``[R]`` or ``[W,S,R]`` /
+    ``[S,R]`` / ``[R]`` in float32 or the model dtype.  Caches
+    ``[num_blocks,block_size,Hkv,E]`` float8_e4m3fn (or uint8) and scales
+    ``[num_blocks,Hkv]`` float8_e8m0fnu (or uint8 exponents) are updated in place; all
+    cleared to zero they are an empty cache.
+
+    A page takes the smallest power of two that holds the largest element written, or
+    keeps its own if that is larger; rows that it holds under a smaller one are
+    rounded again.  Writing row 0 of a page starts it anew: what its other rows held
+    before is gone.  A slot given more than once holds its last token."""
+    if keys.dim() == 3:
+        keys, values, slots = keys.transpose(0, 1)[None], values.transpose(0, 1)[None], slots[None]
+    W, _, S, _ = keys.shape
+    R = cosines.size(-1)
+    cos = cosines.reshape((1,) * (3 - cosines.dim()) + tuple(cosines.shape)) if cosines.dim() < 3 else cosines
+    sin = sines.reshape((1,) * (3 - sines.dim()) + tuple(sines.shape)) if sines.dim() < 3 else sines
+    torch.ops.libdvatt.dvattn_paged_kv_append_q8(k_cache, v_cache, k_scales, v_scales, slots, keys, values,
+                                                 cos.expand(W, S, R), sin.expand(W, S, R))
+    return k_cache, v_cache, k_scales, v_scales
+
+
+def dvattn_paged_sdpa_q8(queries: torch.Tensor, locations: torch.Tensor, cosines: torch.Tensor, sines: torch.Tensor,
+                         fragment_lengths: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                         k_scales: torch.Tensor, v_scales: torch.Tensor, block_tables: torch.Tensor, scale: float,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dvattn_paged_sdpa`` over a cache held in 8 bits (``dvattn_paged_kv_append_q8``):
+    the same queries, views and tables, in float32, float16 or bfloat16, with the caches'
+    scales.  queries ``[W,Hq,S,E]`` -> out ``[W,Hq,S,Ev]``."""
+    if out is None:
+        out = torch.empty(tuple(queries.shape[:3]) + (v_cache.size(-1),), dtype=queries.dtype,
+                          device=queries.device)
+    torch.ops.libdvatt.dvattn_paged_sdpa_q8(out, scale, locations, queries, cosines, sines, fragment_lengths,
+                                            k_cache, v_cache, k_scales, v_scales, block_tables)
+    return out
+
+
+def dvattn_varlen_paged_sdpa_q8(queries: torch.Tensor, locations: torch.Tensor, cosines: torch.Tensor,
+                                sines: torch.Tensor, fragment_lengths: torch.Tensor, k_cache: torch.Tensor,
+                                v_cache: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor,
+                                block_tables: torch.Tensor, cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor,
+                                scale: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``dvattn_varlen_paged_sdpa`` over a cache held in 8 bits.  queries ``[T,Hq,E]`` ->
+    out ``[T,Hq,Ev]``; cu_seqlens_k is not read."""
+    if out is None:
+        out = torch.empty(tuple(queries.shape[:2]) + (v_cache.size(-1),), dtype=queries.dtype,
+                          device=queries.device)
+    torch.ops.libdvatt.dvattn_varlen_paged_sdpa_q8(out, scale, locations, queries, cosines, sines, fragment_lengths,
+                                                   k_cache, v_cache, k_scales, v_scales, block_tables, cu_seqlens_q,
+                                                   cu_seqlens_k)
+    return out
+
+
 def dvattn_sdpa_pt(queries: torch.Tensor, locations: torch.Tensor, keys: list, values: list,
                    scale: float, return_intermediate_results: bool = False):
     """Pure-PyTorch attention over already-rotated queries and contiguous views,
@@ -344,4 +435,5 @@ __all__ = [
     "dvattn_varlen_paged_sdpa", "dvattn_sdpa_pt", "rotate_half", "apply_rotary_pos_emb",
     "dvattn_paged_kv_append", "merge_caches_paged", "dvattn_view_metadata", "dvattn_tree_metadata",
     "dvattn_tree_paged_sdpa", "dvattn_paged_key_mass", "dvattn_kv_select", "dvattn_paged_kv_compact",
+    "dvattn_block_tables", "dvattn_paged_kv_append_q8", "dvattn_paged_sdpa_q8", "dvattn_varlen_paged_sdpa_q8",
 ]

@@ -77,7 +77,8 @@ def lib() -> ctypes.CDLL:
         L.dvattn_abi_version.restype = _I
         L.dvattn_abi_version.argtypes = []
         for n in ("dvattn_paged_sdpa_workspace_size", "dvattn_varlen_paged_sdpa_workspace_size",
-                  "dvattn_sdpa_workspace_size", "dvattn_tree_paged_sdpa_workspace_size"):
+                  "dvattn_sdpa_workspace_size", "dvattn_tree_paged_sdpa_workspace_size",
+                  "dvattn_paged_sdpa_q8_workspace_size", "dvattn_varlen_paged_sdpa_q8_workspace_size"):
             getattr(L, n).restype = _SZ
             getattr(L, n).argtypes = [_I, _SP, _I]
         L.dvattn_paged_sdpa.restype = _I
@@ -116,6 +117,14 @@ def lib() -> ctypes.CDLL:
         L.dvattn_paged_kv_compact.restype = _I
         L.dvattn_paged_kv_compact.argtypes = [_I, _VP, _VP, _VP, _VP, _I, _I, _VP, _VP, _VP, _LL, _SP,
                                               ctypes.POINTER(KvLayout), _VP]
+        L.dvattn_block_tables.restype = _I
+        L.dvattn_block_tables.argtypes = [_VP] * 11 + [_I, _SP, _VP]
+        L.dvattn_paged_kv_append_q8.restype = _I
+        L.dvattn_paged_kv_append_q8.argtypes = [_I, _I] + [_VP] * 9 + [_SP, ctypes.POINTER(KvLayout), _VP]
+        L.dvattn_paged_sdpa_q8.restype = _I
+        L.dvattn_paged_sdpa_q8.argtypes = [_I, _VP, _F] + [_VP] * 10 + [_SP, _VP, _SZ, _VP]
+        L.dvattn_varlen_paged_sdpa_q8.restype = _I
+        L.dvattn_varlen_paged_sdpa_q8.argtypes = [_I, _VP, _F] + [_VP] * 11 + [_SP, _VP, _SZ, _VP]
         L.dvattn_set_option.restype = _I
         L.dvattn_set_option.argtypes = [ctypes.c_char_p, _I]
         L.dvattn_get_option.restype = _I
@@ -365,3 +374,69 @@ def kv_compact(k_cache, v_cache, block_tables, rows, first_rows, lengths=None, m
                                          _ptr(mass), 0 if mass is None else mass.shape[2], ctypes.byref(s),
                                          ctypes.byref(lay), _stream(k_cache)))
     return k_cache, v_cache
+
+
+def block_tables(block_tables, free_pages, lengths, new_tokens, free_count, block_size, max_tokens):
+    """dvattn_block_tables: (cu_seqlens, starts, positions, slots, lengths, free_count) of the step."""
+    W = lengths.shape[0]
+    s = Shape(F=0, W=W, Hq=0, Hkv=0, E=0, Ev=0, S=0, block_size=block_size, max_blocks_per_seq=block_tables.shape[1],
+              total_q_tokens=0, num_blocks=free_pages.shape[0], rotary_dim=0)
+    cu, starts = lengths.new_empty(W + 1), lengths.new_empty(W)
+    positions = lengths.new_empty(max_tokens)
+    slots = torch.empty(max_tokens, dtype=torch.int64, device=lengths.device)
+    new_lengths, count = torch.empty_like(lengths), torch.empty_like(free_count)
+    _check(lib().dvattn_block_tables(_ptr(cu), _ptr(starts), _ptr(positions), _ptr(slots), _ptr(new_lengths),
+                                     _ptr(count), _ptr(block_tables), _ptr(free_pages), _ptr(lengths),
+                                     _ptr(new_tokens), _ptr(free_count), max_tokens, ctypes.byref(s),
+                                     _stream(lengths)))
+    return cu, starts, positions, slots, new_lengths, count
+
+
+def kv_append_q8(k_cache, v_cache, k_scales, v_scales, slots, keys, values, cosines, sines):
+    """dvattn_paged_kv_append_q8: keys/values [W,Hkv,S,E] (any strides, last dim contiguous), slots [W,S] int64,
+    cos/sin [W|1, S|1, R], caches [P,bs,Hkv,E] and scales [P,Hkv] of one byte per element."""
+    W, Hkv, S, E = keys.shape
+    s = Shape(F=0, W=W, Hq=0, Hkv=Hkv, E=E, Ev=values.shape[3], S=S, block_size=k_cache.shape[1],
+              max_blocks_per_seq=0, total_q_tokens=0, num_blocks=k_cache.shape[0], rotary_dim=cosines.shape[2])
+    lay = KvLayout()
+    for i in range(3):
+        lay.key_strides[i] = keys.stride(i)
+        lay.value_strides[i] = values.stride(i)
+    lay.rope_strides[0] = 0 if cosines.shape[0] == 1 else cosines.stride(0)
+    lay.rope_strides[1] = 0 if cosines.shape[1] == 1 else cosines.stride(1)
+    rdt = DVATTN_F32 if cosines.dtype == torch.float32 else dtype_code(cosines.dtype)
+    _check(lib().dvattn_paged_kv_append_q8(dtype_code(keys.dtype), rdt, _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
+                                           _ptr(v_scales), _ptr(slots), _ptr(keys), _ptr(values), _ptr(cosines),
+                                           _ptr(sines), ctypes.byref(s), ctypes.byref(lay), _stream(k_cache)))
+    return k_cache, v_cache, k_scales, v_scales
+
+
+def paged_sdpa_q8(out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, k_scales,
+                  v_scales, block_tables, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    L = lib()
+    s = paged_shape(queries, locations, cosines, k_cache, v_cache, block_tables)
+    dt = dtype_code(out.dtype)
+    need = L.dvattn_paged_sdpa_q8_workspace_size(dt, ctypes.byref(s), out.device.index or 0)
+    ws = workspace if workspace is not None and workspace.numel() >= need else _workspace(need, out)
+    _check(L.dvattn_paged_sdpa_q8(dt, _ptr(out), scale, _ptr(locations), _ptr(queries), _ptr(cosines), _ptr(sines),
+                                  _ptr(fragment_lengths), _ptr(k_cache), _ptr(v_cache), _ptr(k_scales),
+                                  _ptr(v_scales), _ptr(block_tables), ctypes.byref(s), _ptr(ws), ws.numel(),
+                                  _stream(out)))
+    return out
+
+
+def varlen_paged_sdpa_q8(out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, k_scales,
+                         v_scales, block_tables, cu_seqlens_q, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    L = lib()
+    T, Hq, E = queries.shape
+    s = Shape(F=locations.shape[0], W=cu_seqlens_q.shape[0] - 1, Hq=Hq, Hkv=k_cache.shape[2], E=E,
+              Ev=v_cache.shape[3], S=1, block_size=k_cache.shape[1], max_blocks_per_seq=block_tables.shape[1],
+              total_q_tokens=T, num_blocks=k_cache.shape[0], rotary_dim=2 * cosines.shape[2])
+    dt = dtype_code(out.dtype)
+    need = L.dvattn_varlen_paged_sdpa_q8_workspace_size(dt, ctypes.byref(s), out.device.index or 0)
+    ws = workspace if workspace is not None and workspace.numel() >= need else _workspace(need, out)
+    _check(L.dvattn_varlen_paged_sdpa_q8(dt, _ptr(out), scale, _ptr(locations), _ptr(queries), _ptr(cosines),
+                                         _ptr(sines), _ptr(fragment_lengths), _ptr(k_cache), _ptr(v_cache),
+                                         _ptr(k_scales), _ptr(v_scales), _ptr(block_tables), _ptr(cu_seqlens_q),
+                                         ctypes.byref(s), _ptr(ws), ws.numel(), _stream(out)))
+    return out

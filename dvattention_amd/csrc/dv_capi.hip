@@ -1137,4 +1137,219 @@ dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void* v_cache, c
     return ok();
 }
 
+// ---------------------------------------------------------------------------
+static_assert(dv::kMaxTableSeqs == DVATTN_MAX_TABLE_SEQS, "header and kernels agree");
+
+dvattn_status dvattn_block_tables(int* cu_seqlens, int* starts, int* positions, long long* slots, int* new_lengths,
+                                  int* new_free_count, int* block_tables, int* free_pages, const int* lengths,
+                                  const int* new_tokens, const int* free_count, int max_tokens, const dvattn_shape* s,
+                                  void* stream) {
+    if (!s) return fail(DVATTN_ERR_INVALID, "shape is null");
+    if (s->W < 0 || max_tokens < 0) return fail(DVATTN_ERR_INVALID, "negative W / max_tokens");
+    if (s->W > DVATTN_MAX_TABLE_SEQS)
+        return fail(DVATTN_ERR_UNSUPPORTED, "%d sequences in one call exceed %d", s->W, DVATTN_MAX_TABLE_SEQS);
+    if (s->block_size <= 0) return fail(DVATTN_ERR_INVALID, "block_size must be positive (got %d)", s->block_size);
+    if (s->max_blocks_per_seq < 0 || s->num_blocks < 0)
+        return fail(DVATTN_ERR_INVALID, "max_blocks_per_seq / num_blocks must be >= 0");
+    if (!cu_seqlens || !new_free_count || !free_count || (max_tokens > 0 && (!positions || !slots)) ||
+        (s->W > 0 && (!starts || !new_lengths || !lengths || !new_tokens)) || (s->num_blocks > 0 && !free_pages) ||
+        ((long long)s->W * s->max_blocks_per_seq > 0 && !block_tables))
+        return fail(DVATTN_ERR_INVALID, "null pointer");
+    dvattn_status st;
+    if ((st = check_aligned({{cu_seqlens, "cu_seqlens", 4}, {starts, "starts", 4}, {positions, "positions", 4},
+                             {slots, "slots", 8}, {new_lengths, "new_lengths", 4},
+                             {new_free_count, "new_free_count", 4}, {block_tables, "block_tables", 4},
+                             {free_pages, "free_pages", 4}, {lengths, "lengths", 4}, {new_tokens, "new_tokens", 4},
+                             {free_count, "free_count", 4}})) != DVATTN_OK)
+        return st;
+    dv::TablesParams p;
+    memset(&p, 0, sizeof(p));
+    p.cu = cu_seqlens;
+    p.starts = starts;
+    p.positions = positions;
+    p.slots = slots;
+    p.lengths_out = new_lengths;
+    p.count_out = new_free_count;
+    p.bt = block_tables;
+    p.stack = free_pages;
+    p.lengths = lengths;
+    p.new_tokens = new_tokens;
+    p.count = free_count;
+    p.W = s->W;
+    p.maxB = s->max_blocks_per_seq;
+    p.nblocks = s->num_blocks;
+    p.bs = s->block_size;
+    p.T = max_tokens;
+    const hipError_t e = dv::launch_block_tables(p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "dvattn_block_tables launch");
+    return ok();
+}
+
+// ---------------------------------------------------------------------------
+dvattn_status dvattn_paged_kv_append_q8(int dtype, int rope_dtype, void* k_cache, void* v_cache,
+                                        unsigned char* k_scales, unsigned char* v_scales, const long long* slots,
+                                        const void* keys, const void* values, const void* cosines, const void* sines,
+                                        const dvattn_shape* s, const dvattn_kv_layout* lay, void* stream) {
+    if (!s || !lay) return fail(DVATTN_ERR_INVALID, "shape or layout is null");
+    if (!valid_dtype(dtype)) return fail(DVATTN_ERR_UNSUPPORTED, "unsupported dtype code %d", dtype);
+    if (rope_dtype != DVATTN_F32 && rope_dtype != dtype)
+        return fail(DVATTN_ERR_UNSUPPORTED, "cos/sin dtype code %d must be float32 or the storage dtype %d",
+                    rope_dtype, dtype);
+    if (s->W < 0 || s->S < 0 || s->Hkv < 0) return fail(DVATTN_ERR_INVALID, "negative W/S/Hkv");
+    dvattn_status st;
+    if (s->E != 128 || s->Ev != 128)
+        return fail(DVATTN_ERR_UNSUPPORTED, "only head dims E == Ev == 128 are implemented (E=%d, Ev=%d)", s->E,
+                    s->Ev);
+    if ((st = check_rotary(s->rotary_dim, s->E)) != DVATTN_OK) return st;
+    if ((st = check_pages(s)) != DVATTN_OK) return st;
+    if ((long long)s->W * s->S * s->Hkv == 0) return ok();
+    if ((long long)s->W * s->S >= (1ll << 30) || s->Hkv >= (1 << 16))
+        return fail(DVATTN_ERR_UNSUPPORTED, "%lld tokens / %d KV heads in one call", (long long)s->W * s->S, s->Hkv);
+    if (!slots || !keys || !values || (s->num_blocks > 0 && (!k_cache || !v_cache || !k_scales || !v_scales)) ||
+        (s->rotary_dim > 0 && (!cosines || !sines)))
+        return fail(DVATTN_ERR_INVALID, "null pointer");
+    if (s->num_blocks > 0 && (k_cache == v_cache || k_scales == v_scales))
+        return fail(DVATTN_ERR_INVALID, "one array as both caches (or both scales)");
+    if ((st = check_aligned({{k_cache, "k_cache", 16}, {v_cache, "v_cache", 16}, {slots, "slots", 8},
+                             {keys, "keys", elem_bytes(dtype)}, {values, "values", elem_bytes(dtype)},
+                             {cosines, "cosines", elem_bytes(rope_dtype)},
+                             {sines, "sines", elem_bytes(rope_dtype)}})) != DVATTN_OK)
+        return st;
+    dv::Append8Params p;
+    memset(&p, 0, sizeof(p));
+    p.kc = (unsigned char*)k_cache;
+    p.vc = (unsigned char*)v_cache;
+    p.ks = k_scales;
+    p.vs = v_scales;
+    p.slots = slots;
+    p.k = keys;
+    p.v = values;
+    for (int i = 0; i < 3; ++i) {
+        p.kst[i] = lay->key_strides[i];
+        p.vst[i] = lay->value_strides[i];
+    }
+    p.cosv = cosines;
+    p.sinv = sines;
+    p.cs[0] = lay->rope_strides[0];
+    p.cs[1] = lay->rope_strides[1];
+    p.W = s->W;
+    p.S = s->S;
+    p.Hkv = s->Hkv;
+    p.R = s->rotary_dim;
+    p.bs = s->block_size;
+    p.nblocks = s->num_blocks;
+    const hipError_t e = dv::launch_kv_append8(dtype, rope_dtype, p, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, "dvattn_paged_kv_append_q8 launch");
+    return ok();
+}
+
+// ---------------------------------------------------------------------------
+size_t dvattn_paged_sdpa_q8_workspace_size(int dtype, const dvattn_shape* s, int device) {
+    if (!s || !valid_dtype(dtype)) return 0;
+    return dv::decode_workspace_bytes(s->W * s->S, s->Hkv, current_device(device), dtype);
+}
+
+size_t dvattn_varlen_paged_sdpa_q8_workspace_size(int dtype, const dvattn_shape* s, int device) {
+    if (!s || !valid_dtype(dtype)) return 0;
+    return dv::decode_workspace_bytes(s->total_q_tokens, s->Hkv, current_device(device), dtype);
+}
+
+}  // extern "C"
+
+namespace {
+
+// Checks and launch of both attentions over 8-bit caches.
+dvattn_status sdpa_q8(bool varlen, int dtype, void* out, float scale, const int* locations, const void* queries,
+                      const float* cosines, const float* sines, const int* fragment_lengths, const void* k_cache,
+                      const void* v_cache, const unsigned char* k_scales, const unsigned char* v_scales,
+                      const int* block_tables, const int* cu_seqlens_q, const dvattn_shape* s, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    const char* op = varlen ? "dvattn_varlen_paged_sdpa_q8 launch" : "dvattn_paged_sdpa_q8 launch";
+    if (!s) return fail(DVATTN_ERR_INVALID, "shape is null");
+    if (!valid_dtype(dtype)) return fail(DVATTN_ERR_UNSUPPORTED, "unsupported dtype code %d", dtype);
+    if (s->F < 0 || s->W < 0 || (varlen ? s->total_q_tokens : s->S) < 0)
+        return fail(DVATTN_ERR_INVALID, "negative F / W / number of tokens");
+    const long long rows = varlen ? s->total_q_tokens : (long long)s->W * s->S;
+    if (rows == 0 || s->Hkv == 0) return ok();
+    if (rows >= (1ll << 31)) return fail(DVATTN_ERR_UNSUPPORTED, "%lld query rows exceed 2^31", rows);
+    dvattn_status st;
+    if ((st = check_heads(s)) != DVATTN_OK) return st;
+    if ((st = check_rotary(s->rotary_dim, s->E)) != DVATTN_OK) return st;
+    if ((st = check_pages(s)) != DVATTN_OK) return st;
+    if (!out || !queries) return fail(DVATTN_ERR_INVALID, "null output or query pointer");
+    if (varlen && s->W > 0 && !cu_seqlens_q) return fail(DVATTN_ERR_INVALID, "null cu_seqlens_q pointer");
+    if (varlen && s->W == 0) return fail(DVATTN_ERR_INVALID, "tokens without any sequence");
+    if (s->F > 0 && (!locations || !fragment_lengths || ((!cosines || !sines) && s->rotary_dim > 0)))
+        return fail(DVATTN_ERR_INVALID, "null locations / fragment_lengths / cos / sin pointer");
+    if (s->num_blocks > 0 && (!k_cache || !v_cache || !k_scales || !v_scales))
+        return fail(DVATTN_ERR_INVALID, "null k/v cache or scales pointer");
+    if (s->max_blocks_per_seq > 0 && !block_tables) return fail(DVATTN_ERR_INVALID, "null block_tables pointer");
+    if ((st = check_aligned({{out, "out", 16}, {queries, "queries", 16}, {k_cache, "k_cache", 16},
+                             {v_cache, "v_cache", 16}, {workspace, "workspace", 16}, {locations, "locations", 4},
+                             {fragment_lengths, "fragment_lengths", 4}, {cosines, "cosines", 4},
+                             {sines, "sines", 4}, {block_tables, "block_tables", 4},
+                             {cu_seqlens_q, "cu_seqlens_q", 4}})) != DVATTN_OK)
+        return st;
+    const size_t need = varlen ? dvattn_varlen_paged_sdpa_q8_workspace_size(dtype, s, -1)
+                               : dvattn_paged_sdpa_q8_workspace_size(dtype, s, -1);
+    if (workspace_bytes < need || (need && !workspace))
+        return fail(DVATTN_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
+    dv::DecodeParams p;
+    memset(&p, 0, sizeof(p));
+    p.out = out;
+    p.loc = locations;
+    p.q = queries;
+    p.cosv = cosines;
+    p.sinv = sines;
+    p.fl = fragment_lengths;
+    p.kc = k_cache;
+    p.vc = v_cache;
+    p.ks = k_scales;
+    p.vs = v_scales;
+    p.bt = block_tables;
+    p.cu_q = cu_seqlens_q;
+    p.l2scale = scale * 1.4426950408889634f;  // scale / ln 2
+    p.F = s->F;
+    p.W = s->W;
+    p.S = varlen ? 1 : s->S;
+    p.T = varlen ? s->total_q_tokens : 0;
+    p.Hq = s->Hq;
+    p.Hkv = s->Hkv;
+    p.R = s->rotary_dim;
+    p.bs = s->block_size;
+    p.bs_shift = log2_exact(s->block_size);
+    p.maxB = s->max_blocks_per_seq;
+    p.nblocks = s->num_blocks;
+    p.min_keys = dv::kDecodeMinKeys;
+    const long long max_keys = (long long)s->max_blocks_per_seq * s->block_size;
+    const hipError_t e = dv::launch_decode8(dtype, varlen ? dv::kQRotHalf : dv::kQRotFull,
+                                            varlen ? dv::kRowVarlen : dv::kRowWS, p, (int)rows, max_keys, workspace,
+                                            workspace_bytes, (hipStream_t)stream);
+    if (e != hipSuccess) return hip_fail(e, op);
+    return ok();
+}
+
+}  // namespace
+
+extern "C" {
+
+dvattn_status dvattn_paged_sdpa_q8(int dtype, void* out, float scale, const int* locations, const void* queries,
+                                   const float* cosines, const float* sines, const int* fragment_lengths,
+                                   const void* k_cache, const void* v_cache, const unsigned char* k_scales,
+                                   const unsigned char* v_scales, const int* block_tables, const dvattn_shape* s,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+    return sdpa_q8(false, dtype, out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache,
+                   k_scales, v_scales, block_tables, nullptr, s, workspace, workspace_bytes, stream);
+}
+
+dvattn_status dvattn_varlen_paged_sdpa_q8(int dtype, void* out, float scale, const int* locations,
+                                          const void* queries, const float* cosines, const float* sines,
+                                          const int* fragment_lengths, const void* k_cache, const void* v_cache,
+                                          const unsigned char* k_scales, const unsigned char* v_scales,
+                                          const int* block_tables, const int* cu_seqlens_q, const dvattn_shape* s,
+                                          void* workspace, size_t workspace_bytes, void* stream) {
+    return sdpa_q8(true, dtype, out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache,
+                   k_scales, v_scales, block_tables, cu_seqlens_q, s, workspace, workspace_bytes, stream);
+}
+
 }  // extern "C"

@@ -82,6 +82,9 @@ struct DecodeParams {
     const int* tree_views;
     const int* tree_rows;
     FragDesc frags[kMaxFragArgs];
+    // 8-bit caches (dv_decode8.hip, dv_chunk8.hip): exponent bytes [num_blocks, Hkv] of K and V
+    const unsigned char* ks;
+    const unsigned char* vs;
 };
 
 // Single-launch path for short contiguous views (dv_small.hip): one workgroup
@@ -211,6 +214,42 @@ struct CompactParams {
     int slices;               // column slices of a row, a workgroup each
 };
 
+// Block tables, positions and slots of a step from the sequences' lengths (dv_pages.hip).
+constexpr int kMaxTableSeqs = 8192;  // sequences of a call (their counts live in LDS)
+struct TablesParams {
+    int* cu;                  // [W + 1]
+    int* starts;              // [W]
+    int* positions;           // [T]
+    long long* slots;         // [T]
+    int* lengths_out;         // [W], may be lengths
+    int* count_out;           // [1], may be count
+    int* bt;                  // [W, maxB]
+    int* stack;               // [nblocks]
+    const int* lengths;       // [W]
+    const int* new_tokens;    // [W]
+    const int* count;         // [1]
+    int W, maxB, nblocks, bs, T;
+};
+
+// Quantising append to an 8-bit cache (dv_pages.hip).
+struct Append8Params {
+    unsigned char* kc;        // [num_blocks, block_size, Hkv, E] E4M3
+    unsigned char* vc;
+    unsigned char* ks;        // [num_blocks, Hkv] exponent bytes
+    unsigned char* vs;
+    const long long* slots;   // [W, S]
+    const void* k;            // keys [W, Hkv, S, E], element strides (w, h, s)
+    const void* v;
+    long long kst[3], vst[3];
+    const void* cosv;         // cos/sin [W, S, R], element strides (w, s)
+    const void* sinv;
+    long long cs[2];
+    int W, S, Hkv, R;
+    int bs, nblocks;
+    int tile;                 // tokens of a workgroup
+    int vec;                  // 1: rows, tables and strides allow 16-byte loads
+};
+
 // CU count of a device, queried once per device (thread-safe; 256 if unknown).
 inline int device_cu_count(int device) {
     static std::atomic<int> cache[64];
@@ -284,6 +323,16 @@ hipError_t launch_tree_small(int dtype, const TreePlan& t, const DecodeParams& p
 // per sequence and KV head, and its launches.
 size_t mass_workspace_bytes(int dtype, int F, int W, int S, int Hkv, long long max_rows, long long capacity);
 hipError_t launch_key_mass(int dtype, const MassParams& p, void* workspace, hipStream_t stream);
+
+hipError_t launch_block_tables(const TablesParams& p, hipStream_t stream);
+hipError_t launch_kv_append8(int dtype, int rope_dtype, const Append8Params& p, hipStream_t stream);
+
+// Decode over an 8-bit cache: launch_decode's arguments and workspace
+// (decode_workspace_bytes), paged caches only.
+hipError_t launch_decode8(int dtype, int qmode, int rowmode, const DecodeParams& base, int nrows_total,
+                          long long max_keys_per_row, void* workspace, size_t ws_bytes, hipStream_t stream);
+// The merge of a decode launch's partial slots (rowmode: kRowWS or kRowVarlen).
+hipError_t launch_merge(int dtype, int rowmode, const DecodeParams& p, hipStream_t stream);
 
 hipError_t launch_kv_select(const SelectParams& p, hipStream_t stream);
 hipError_t launch_kv_compact(int dtype, const CompactParams& p, hipStream_t stream);

@@ -855,6 +855,15 @@ int resident_wgs(int hpw, size_t lds) {
     return nb;
 }
 
+template <int DT, int RM>
+hipError_t merge_one(const DecodeParams& p, hipStream_t stream) {
+    const int nseg = p.nrows * (p.Hkv / p.hpw);
+    hipLaunchKernelGGL((dv_merge<DT, RM>), dim3(nseg * p.hpw * kMergeQuarters), dim3(kMergeWaves * kWave), 0,
+                       stream, p);
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? e : note_site(e, "launch dv_merge");
+}
+
 template <int DT, int QM, int KVM, int RM, bool MV, bool P2>
 hipError_t launch_one(DecodeParams p, int device, long long max_wg, long long cap, int cus, hipStream_t stream) {
     const size_t lds = (size_t)p.hpw * wave_lds<DT>() + (size_t)(p.nrows + 1) * sizeof(long long);
@@ -877,12 +886,7 @@ hipError_t launch_one(DecodeParams p, int device, long long max_wg, long long ca
         hipLaunchKernelGGL((dv_stream<DT, QM, KVM, RM, MV, P2>), dim3(p.nwg), dim3(p.hpw * kWave), lds, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return note_site(e, "launch decode");
-    const int nseg = p.nrows * (p.Hkv / p.hpw);
-    hipLaunchKernelGGL((dv_merge<DT, RM>), dim3(nseg * p.hpw * kMergeQuarters), dim3(kMergeWaves * kWave), 0,
-                       stream, p);
-    e = hipGetLastError();
-    if (e != hipSuccess) return note_site(e, "launch dv_merge");
-    return hipSuccess;
+    return merge_one<DT, RM>(p, stream);
 }
 
 template <int DT, int QM, int RM>
@@ -910,6 +914,16 @@ hipError_t dispatch_modes(int qmode, int kvmode, int rowmode, const DecodeParams
 }  // namespace
 
 const char* last_hip_site() { return g_site; }
+
+hipError_t launch_merge(int dtype, int rowmode, const DecodeParams& p, hipStream_t stream) {
+    const bool varlen = rowmode == kRowVarlen;
+    switch (dtype) {
+        case kBF16: return varlen ? merge_one<kBF16, kRowVarlen>(p, stream) : merge_one<kBF16, kRowWS>(p, stream);
+        case kF16: return varlen ? merge_one<kF16, kRowVarlen>(p, stream) : merge_one<kF16, kRowWS>(p, stream);
+        case kF32: return varlen ? merge_one<kF32, kRowVarlen>(p, stream) : merge_one<kF32, kRowWS>(p, stream);
+        default: return hipErrorInvalidValue;
+    }
+}
 
 // Workspace per segment after the partial slots: merge directory {first slot,
 // pieces}.

@@ -890,6 +890,261 @@ void dvattn_paged_kv_compact_op(at::Tensor& k_cache, at::Tensor& v_cache, const 
                  "dvattn_paged_kv_compact");
 }
 
+// ---------------------------------------------------------------------------
+// Caches held in 8 bits: E4M3 bytes (float8_e4m3fn or uint8) with an exponent byte
+// (float8_e8m0fnu or uint8) per page and KV head.
+void check_cache8(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scales,
+                  const at::Tensor& v_scales, const at::Tensor& like, const char* op) {
+    const at::Tensor* all[] = {&k_cache, &v_cache, &k_scales, &v_scales};
+    const char* names[] = {"k_cache", "v_cache", "k_scales", "v_scales"};
+    for (int i = 0; i < 4; ++i) {
+        check_dim(*all[i], i < 2 ? 4 : 2, names[i]);
+        const auto t = all[i]->scalar_type();
+        TORCH_CHECK(t == at::kByte || t == (i < 2 ? at::kFloat8_e4m3fn : at::kFloat8_e8m0fnu), op, ": ", names[i],
+                    " must be ", i < 2 ? "float8_e4m3fn" : "float8_e8m0fnu", " or uint8, got ", t);
+        check_contig(*all[i], names[i]);
+        check_dev(*all[i], like, names[i]);
+    }
+    TORCH_CHECK(v_cache.sizes().slice(0, 3) == k_cache.sizes().slice(0, 3), op,
+                ": v_cache must be [num_blocks, block_size, Hkv, Ev], got ", v_cache.sizes());
+    for (int i = 2; i < 4; ++i)
+        TORCH_CHECK(all[i]->size(0) == k_cache.size(0) && all[i]->size(1) == k_cache.size(2), op, ": ", names[i],
+                    " must be [num_blocks, Hkv], got ", all[i]->sizes());
+}
+
+// dvattn_paged_sdpa_q8 / dvattn_varlen_paged_sdpa_q8: the arguments of the operators without
+// _q8, the 8-bit caches and their scales.
+void sdpa_q8(bool varlen, at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
+             const at::Tensor& cosines, const at::Tensor& sines, const at::Tensor& fragment_lengths,
+             const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scales,
+             const at::Tensor& v_scales, const at::Tensor& block_tables, const at::Tensor* cu_seqlens_q) {
+    const char* op = varlen ? "dvattn_varlen_paged_sdpa_q8" : "dvattn_paged_sdpa_q8";
+    const int dt = dtype_code(out);
+    const int nd = varlen ? 3 : 4;  // dims of queries, cos/sin and the output
+    check_dim(out, nd, "output");
+    check_dim(queries, nd, "queries");
+    check_dim(locations, nd - 1, "locations");
+    check_dim(cosines, nd, "cosines");
+    check_dim(sines, nd, "sines");
+    check_dim(fragment_lengths, 1, "fragment_lengths");
+    check_dim(block_tables, 2, "block_tables");
+    check_same(queries, out, "queries");
+    check_i32(locations, "locations");
+    check_i32(fragment_lengths, "fragment_lengths");
+    check_i32(block_tables, "block_tables");
+    check_f32(cosines, "cosines");
+    check_f32(sines, "sines");
+    const at::Tensor* all[] = {&out, &locations, &queries, &cosines, &sines, &fragment_lengths, &block_tables};
+    const char* names[] = {"output", "locations", "queries", "cosines", "sines", "fragment_lengths", "block_tables"};
+    for (int i = 0; i < 7; ++i) {
+        check_contig(*all[i], names[i]);
+        check_dev(*all[i], out, names[i]);
+    }
+    if (varlen) {
+        check_dim(*cu_seqlens_q, 1, "cu_seqlens_q");
+        check_i32(*cu_seqlens_q, "cu_seqlens_q");
+        check_contig(*cu_seqlens_q, "cu_seqlens_q");
+        check_dev(*cu_seqlens_q, out, "cu_seqlens_q");
+        TORCH_CHECK(cu_seqlens_q->size(0) >= 1, op, ": cu_seqlens_q must have W+1 >= 1 entries");
+    }
+    check_cache8(k_cache, v_cache, k_scales, v_scales, out, op);
+    const int64_t F = locations.size(0), N = queries.size(0), Hq = queries.size(1), E = queries.size(nd - 1);
+    const int64_t W = varlen ? cu_seqlens_q->size(0) - 1 : N;
+    for (int i = 0; i + 1 < nd; ++i)
+        TORCH_CHECK(out.size(i) == queries.size(i), op, ": output must be ", varlen ? "[T,Hq,Ev]" : "[W,Hq,S,Ev]",
+                    ", got ", out.sizes());
+    TORCH_CHECK(out.size(nd - 1) == v_cache.size(3), op, ": output must be ", varlen ? "[T,Hq,Ev]" : "[W,Hq,S,Ev]",
+                ", got ", out.sizes());
+    TORCH_CHECK(locations.size(1) == N && (varlen || locations.size(2) == queries.size(2)), op,
+                ": locations must be ", varlen ? "[F,T]" : "[F,W,S]", ", got ", locations.sizes());
+    TORCH_CHECK(cosines.size(0) == F && cosines.size(1) == N && (varlen || cosines.size(2) == queries.size(2)), op,
+                ": cosines must be ", varlen ? "[F,T,R/2]" : "[F,W,S,R]", ", got ", cosines.sizes());
+    TORCH_CHECK(sines.sizes() == cosines.sizes(), op, ": sines must match cosines");
+    TORCH_CHECK(fragment_lengths.size(0) == F, op, ": fragment_lengths must be [F], got ", fragment_lengths.sizes());
+    TORCH_CHECK(k_cache.size(3) == E, op, ": k_cache head dim ", k_cache.size(3), " != query dim ", E);
+    TORCH_CHECK(block_tables.size(0) >= W || N == 0, op, ": block_tables needs a row per sequence (", W, "), got ",
+                block_tables.sizes());
+    TORCH_CHECK(W > 0 || N == 0, op, ": tokens without any sequence (cu_seqlens_q has 1 entry)");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(out.device());
+    dvattn_shape s{};
+    s.F = as_int(F, "F");
+    s.W = as_int(W, "W");
+    s.Hq = as_int(Hq, "Hq");
+    s.Hkv = as_int(k_cache.size(2), "Hkv");
+    s.E = as_int(E, "E");
+    s.Ev = as_int(v_cache.size(3), "Ev");
+    s.S = varlen ? 1 : as_int(queries.size(2), "S");
+    s.total_q_tokens = varlen ? as_int(N, "T") : 0;
+    s.block_size = as_int(k_cache.size(1), "block_size");
+    s.max_blocks_per_seq = as_int(block_tables.size(1), "max_blocks_per_seq");
+    s.num_blocks = as_int(k_cache.size(0), "num_blocks");
+    s.rotary_dim = as_int(cosines.size(nd - 1) * (varlen ? 2 : 1), "rotary_dim");
+    const size_t ws = varlen ? dvattn_varlen_paged_sdpa_q8_workspace_size(dt, &s, out.device().index())
+                             : dvattn_paged_sdpa_q8_workspace_size(dt, &s, out.device().index());
+    at::Tensor w = workspace(ws, out);
+    const auto* ksp = static_cast<const unsigned char*>(k_scales.data_ptr());
+    const auto* vsp = static_cast<const unsigned char*>(v_scales.data_ptr());
+    const dvattn_status st =
+        varlen ? dvattn_varlen_paged_sdpa_q8(dt, out.data_ptr(), (float)scale, locations.data_ptr<int>(),
+                                             queries.data_ptr(), cosines.data_ptr<float>(), sines.data_ptr<float>(),
+                                             fragment_lengths.data_ptr<int>(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                             ksp, vsp, block_tables.data_ptr<int>(), cu_seqlens_q->data_ptr<int>(),
+                                             &s, w.data_ptr(), ws, stream_of(out))
+               : dvattn_paged_sdpa_q8(dt, out.data_ptr(), (float)scale, locations.data_ptr<int>(), queries.data_ptr(),
+                                      cosines.data_ptr<float>(), sines.data_ptr<float>(),
+                                      fragment_lengths.data_ptr<int>(), k_cache.data_ptr(), v_cache.data_ptr(), ksp,
+                                      vsp, block_tables.data_ptr<int>(), &s, w.data_ptr(), ws, stream_of(out));
+    check_status(st, op);
+}
+
+void dvattn_paged_sdpa_q8_op(at::Tensor& out, double scale, const at::Tensor& locations, const at::Tensor& queries,
+                             const at::Tensor& cosines, const at::Tensor& sines, const at::Tensor& fragment_lengths,
+                             const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scales,
+                             const at::Tensor& v_scales, const at::Tensor& block_tables) {
+    sdpa_q8(false, out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, k_scales,
+            v_scales, block_tables, nullptr);
+}
+
+// cu_seqlens_k: accepted and not read, as in dvattn_varlen_paged_sdpa
+void dvattn_varlen_paged_sdpa_q8_op(at::Tensor& out, double scale, const at::Tensor& locations,
+                                    const at::Tensor& queries, const at::Tensor& cosines, const at::Tensor& sines,
+                                    const at::Tensor& fragment_lengths, const at::Tensor& k_cache,
+                                    const at::Tensor& v_cache, const at::Tensor& k_scales, const at::Tensor& v_scales,
+                                    const at::Tensor& block_tables, const at::Tensor& cu_seqlens_q,
+                                    const at::Tensor& cu_seqlens_k) {
+    (void)cu_seqlens_k;
+    sdpa_q8(true, out, scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, k_scales,
+            v_scales, block_tables, &cu_seqlens_q);
+}
+
+// dvattn_paged_kv_append_q8(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scales,
+//   Tensor(d!) v_scales, Tensor slots, Tensor keys, Tensor values, Tensor cosines, Tensor sines)
+// keys/values [W,Hkv,S,E] strided (last dim contiguous), slots [W,S] int64, cos/sin
+// [W|1, S|1, R].
+void dvattn_paged_kv_append_q8_op(at::Tensor& k_cache, at::Tensor& v_cache, at::Tensor& k_scales,
+                                  at::Tensor& v_scales, const at::Tensor& slots, const at::Tensor& keys,
+                                  const at::Tensor& values, const at::Tensor& cosines, const at::Tensor& sines) {
+    const char* op = "dvattn_paged_kv_append_q8";
+    const int dt = dtype_code(keys);
+    check_dim(keys, 4, "keys");
+    check_dim(values, 4, "values");
+    check_dim(slots, 2, "slots");
+    check_dim(cosines, 3, "cosines");
+    check_dim(sines, 3, "sines");
+    check_same(values, keys, "values");
+    check_cache8(k_cache, v_cache, k_scales, v_scales, keys, op);
+    TORCH_CHECK(slots.scalar_type() == at::kLong, op, ": slots must be int64, got ", slots.scalar_type());
+    TORCH_CHECK(cosines.scalar_type() == at::kFloat || cosines.scalar_type() == keys.scalar_type(), op,
+                ": cosines must be float32 or ", keys.scalar_type(), ", got ", cosines.scalar_type());
+    check_same(sines, cosines, "sines");
+    const at::Tensor* all[] = {&slots, &keys, &values, &cosines, &sines};
+    const char* names[] = {"slots", "keys", "values", "cosines", "sines"};
+    for (int i = 0; i < 5; ++i) check_dev(*all[i], k_cache, names[i]);
+    check_contig(slots, "slots");
+    for (int i = 1; i < 5; ++i)
+        TORCH_CHECK(all[i]->size(-1) <= 1 || all[i]->stride(-1) == 1, op, ": the last dim of ", names[i],
+                    " must be contiguous");
+    const int64_t W = keys.size(0), Hkv = keys.size(1), S = keys.size(2), E = keys.size(3);
+    TORCH_CHECK(values.size(0) == W && values.size(1) == Hkv && values.size(2) == S, op,
+                ": values must be [W,Hkv,S,Ev] = [", W, ",", Hkv, ",", S, ",Ev], got ", values.sizes());
+    TORCH_CHECK(k_cache.size(2) == Hkv && k_cache.size(3) == E, op,
+                ": k_cache must be [num_blocks, block_size, Hkv, E] with Hkv=", Hkv, ", E=", E, ", got ",
+                k_cache.sizes());
+    TORCH_CHECK(v_cache.size(3) == values.size(3), op, ": v_cache head dim ", v_cache.size(3), " != value dim ",
+                values.size(3));
+    TORCH_CHECK(slots.size(0) == W && slots.size(1) == S, op, ": slots must be [W,S] = [", W, ",", S, "], got ",
+                slots.sizes());
+    TORCH_CHECK((cosines.size(0) == W || cosines.size(0) == 1) && (cosines.size(1) == S || cosines.size(1) == 1), op,
+                ": cosines must be [W|1, S|1, R], got ", cosines.sizes());
+    TORCH_CHECK(sines.sizes() == cosines.sizes(), op, ": sines must match cosines, got ", sines.sizes());
+    TORCH_CHECK(cosines.stride(0) == sines.stride(0) && cosines.stride(1) == sines.stride(1), op,
+                ": cosines and sines must have the same strides");
+    const int64_t R = cosines.size(2);
+    TORCH_CHECK(R <= E && R % 2 == 0, op, ": rotary dim ", R, " must be even and <= E=", E);
+    at::assert_no_overlap(k_cache, keys);
+    at::assert_no_overlap(v_cache, values);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
+    dvattn_shape s{};
+    s.W = as_int(W, "W");
+    s.S = as_int(S, "S");
+    s.Hkv = as_int(Hkv, "Hkv");
+    s.E = as_int(E, "E");
+    s.Ev = as_int(values.size(3), "Ev");
+    s.block_size = as_int(k_cache.size(1), "block_size");
+    s.num_blocks = as_int(k_cache.size(0), "num_blocks");
+    s.rotary_dim = as_int(R, "rotary_dim");
+    dvattn_kv_layout lay{};
+    for (int i = 0; i < 3; ++i) {
+        lay.key_strides[i] = keys.stride(i);
+        lay.value_strides[i] = values.stride(i);
+    }
+    lay.rope_strides[0] = cosines.size(0) == 1 ? 0 : cosines.stride(0);
+    lay.rope_strides[1] = cosines.size(1) == 1 ? 0 : cosines.stride(1);
+    const int rope_dt = cosines.scalar_type() == at::kFloat ? DVATTN_F32 : dt;
+    check_status(dvattn_paged_kv_append_q8(dt, rope_dt, k_cache.data_ptr(), v_cache.data_ptr(),
+                                           static_cast<unsigned char*>(k_scales.data_ptr()),
+                                           static_cast<unsigned char*>(v_scales.data_ptr()),
+                                           reinterpret_cast<const long long*>(slots.data_ptr<int64_t>()),
+                                           keys.data_ptr(), values.data_ptr(), cosines.data_ptr(), sines.data_ptr(),
+                                           &s, &lay, stream_of(k_cache)),
+                 op);
+}
+
+// dvattn_block_tables(Tensor(a!) block_tables, Tensor(b!) free_pages, Tensor(c!) new_lengths,
+//   Tensor(d!) new_free_count, Tensor lengths, Tensor new_tokens, Tensor free_count,
+//   int block_size, int max_tokens) -> (cu_seqlens, starts, positions, slots)
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> dvattn_block_tables_op(
+    at::Tensor& block_tables, at::Tensor& free_pages, at::Tensor& new_lengths, at::Tensor& new_free_count,
+    const at::Tensor& lengths, const at::Tensor& new_tokens, const at::Tensor& free_count, int64_t block_size,
+    int64_t max_tokens) {
+    const char* op = "dvattn_block_tables";
+    const at::Tensor* all[] = {&block_tables, &free_pages, &new_lengths, &new_free_count,
+                               &lengths, &new_tokens, &free_count};
+    const char* names[] = {"block_tables", "free_pages", "new_lengths", "new_free_count",
+                           "lengths", "new_tokens", "free_count"};
+    for (int i = 0; i < 7; ++i) {
+        check_dim(*all[i], i == 0 ? 2 : 1, names[i]);
+        check_i32(*all[i], names[i]);
+        check_contig(*all[i], names[i]);
+        check_dev(*all[i], block_tables, names[i]);
+    }
+    const int64_t W = lengths.size(0);
+    TORCH_CHECK(new_tokens.size(0) == W && new_lengths.size(0) == W, op,
+                ": lengths, new_tokens and new_lengths must be [W], got ", lengths.sizes(), ", ", new_tokens.sizes(),
+                " and ", new_lengths.sizes());
+    TORCH_CHECK(block_tables.size(0) >= W, op, ": block_tables needs a row per sequence (", W, "), got ",
+                block_tables.sizes());
+    TORCH_CHECK(free_count.size(0) == 1 && new_free_count.size(0) == 1, op, ": free_count must have one entry");
+    TORCH_CHECK(block_size > 0, op, ": block_size must be positive, got ", block_size);
+    const at::Tensor* out[] = {&block_tables, &free_pages, &new_lengths, &new_free_count};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 7; ++j) {
+            // new_lengths may be lengths and new_free_count free_count, as a whole
+            const bool own = i == j || (((i == 2 && j == 4) || (i == 3 && j == 6)) &&
+                                        out[i]->data_ptr() == all[j]->data_ptr());
+            if (!own) at::assert_no_overlap(*out[i], *all[j]);
+        }
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(block_tables.device());
+    dvattn_shape s{};
+    s.W = as_int(W, "W");
+    s.block_size = as_int(block_size, "block_size");
+    s.max_blocks_per_seq = as_int(block_tables.size(1), "max_blocks_per_seq");
+    s.num_blocks = as_int(free_pages.size(0), "num_blocks");
+    const int T = as_int(max_tokens, "max_tokens");
+    at::Tensor cu = at::empty({W + 1}, lengths.options());
+    at::Tensor starts = at::empty({W}, lengths.options());
+    at::Tensor positions = at::empty({max_tokens}, lengths.options());
+    at::Tensor slots = at::empty({max_tokens}, lengths.options().dtype(at::kLong));
+    check_status(dvattn_block_tables(cu.data_ptr<int>(), starts.data_ptr<int>(), positions.data_ptr<int>(),
+                                     reinterpret_cast<long long*>(slots.data_ptr<int64_t>()),
+                                     new_lengths.data_ptr<int>(), new_free_count.data_ptr<int>(),
+                                     block_tables.data_ptr<int>(), free_pages.data_ptr<int>(),
+                                     lengths.data_ptr<int>(), new_tokens.data_ptr<int>(), free_count.data_ptr<int>(),
+                                     T, &s, stream_of(block_tables)),
+                 op);
+    return {cu, starts, positions, slots};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(libdvatt, m) {
@@ -934,6 +1189,18 @@ TORCH_LIBRARY(libdvatt, m) {
           "int keep_last) -> ()");
     m.def("dvattn_paged_kv_compact(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_tables, Tensor rows, "
           "Tensor first_rows, Tensor? lengths=None, Tensor(c!)? mass=None) -> ()");
+    // caches held in 8 bits
+    m.def("dvattn_block_tables(Tensor(a!) block_tables, Tensor(b!) free_pages, Tensor(c!) new_lengths, "
+          "Tensor(d!) new_free_count, Tensor lengths, Tensor new_tokens, Tensor free_count, int block_size, "
+          "int max_tokens) -> (Tensor cu_seqlens, Tensor starts, Tensor positions, Tensor slots)");
+    m.def("dvattn_paged_kv_append_q8(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scales, "
+          "Tensor(d!) v_scales, Tensor slots, Tensor keys, Tensor values, Tensor cosines, Tensor sines) -> ()");
+    m.def("dvattn_paged_sdpa_q8(Tensor(a!) output, float scale, Tensor locations, Tensor queries, "
+          "Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor v_cache, "
+          "Tensor k_scales, Tensor v_scales, Tensor block_tables) -> ()");
+    m.def("dvattn_varlen_paged_sdpa_q8(Tensor(a!) output, float scale, Tensor locations, Tensor queries, "
+          "Tensor cosines, Tensor sines, Tensor fragment_lengths, Tensor k_cache, Tensor v_cache, "
+          "Tensor k_scales, Tensor v_scales, Tensor block_tables, Tensor cu_seqlens_q, Tensor cu_seqlens_k) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(libdvatt, CUDA, m) {
@@ -950,4 +1217,8 @@ TORCH_LIBRARY_IMPL(libdvatt, CUDA, m) {
     m.impl("dvattn_paged_key_mass", dvattn_paged_key_mass_op);
     m.impl("dvattn_kv_select", dvattn_kv_select_op);
     m.impl("dvattn_paged_kv_compact", dvattn_paged_kv_compact_op);
+    m.impl("dvattn_block_tables", dvattn_block_tables_op);
+    m.impl("dvattn_paged_kv_append_q8", dvattn_paged_kv_append_q8_op);
+    m.impl("dvattn_paged_sdpa_q8", dvattn_paged_sdpa_q8_op);
+    m.impl("dvattn_varlen_paged_sdpa_q8", dvattn_varlen_paged_sdpa_q8_op);
 }

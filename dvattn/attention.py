@@ -19,18 +19,22 @@ library raises ``ImportError``.  The names are the reference's:
 """
 from dvattention_amd.attention import (  # noqa: F401  (importing dvattention_amd registers the ops)
     apply_rotary_pos_emb,
+    dvattn_block_tables,
     dvattn_fused,
     dvattn_kv_select,
     dvattn_paged_key_mass,
     dvattn_paged_kv_append,
+    dvattn_paged_kv_append_q8,
     dvattn_paged_kv_compact,
     dvattn_paged_sdpa,
+    dvattn_paged_sdpa_q8,
     dvattn_rope,
     dvattn_sdpa,
     dvattn_sdpa_pt,
     dvattn_tree_metadata,
     dvattn_tree_paged_sdpa,
     dvattn_varlen_paged_sdpa,
+    dvattn_varlen_paged_sdpa_q8,
     dvattn_varlen_rope,
     dvattn_view_metadata,
     merge_caches_paged,
@@ -51,7 +55,8 @@ __all__ = [
     "apply_rotary_pos_emb", "dvattn_fused", "dvattn_paged_kv_append", "dvattn_paged_sdpa", "dvattn_rope",
     "dvattn_sdpa", "dvattn_sdpa_pt", "dvattn_varlen_paged_sdpa", "dvattn_varlen_rope", "dvattn_view_metadata",
     "dvattn_tree_metadata", "dvattn_tree_paged_sdpa", "dvattn_paged_key_mass", "dvattn_kv_select",
-    "dvattn_paged_kv_compact",
+    "dvattn_paged_kv_compact", "dvattn_block_tables", "dvattn_paged_kv_append_q8", "dvattn_paged_sdpa_q8",
+    "dvattn_varlen_paged_sdpa_q8",
     "merge_caches_paged", "rotate_half", "AttentionModule", "CacheStructure", "DVAttnCache", "Segment",
     "SegmentPool", "merge_caches", "model_surgery", "segments_from_caches",
 ]

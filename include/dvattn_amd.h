@@ -28,7 +28,10 @@
  *                               cos/sin)
  * and, with no counterpart there, for drafted token trees and bounded caches:
  *   dvattn_tree_metadata, dvattn_tree_paged_sdpa, dvattn_paged_key_mass,
- *   dvattn_kv_select, dvattn_paged_kv_compact.
+ *   dvattn_kv_select, dvattn_paged_kv_compact;
+ * and for caches held in 8 bits:
+ *   dvattn_block_tables, dvattn_paged_kv_append_q8, dvattn_paged_sdpa_q8,
+ *   dvattn_varlen_paged_sdpa_q8.
  *
  * Semantics (identical to the reference operators):
  *   - GQA factor 16 (Hq == 16*Hkv) and head dims E == Ev == 128 only; other
@@ -52,11 +55,13 @@
  * Alignment (checked; the reference's kernels assumed 16-byte vectors,
  * paged_kernel_v21.cuh:58-62, without checking): the attention entry points
  * (dvattn_paged_sdpa[_noalloc], dvattn_varlen_paged_sdpa, dvattn_sdpa,
- * dvattn_fused, dvattn_tree_paged_sdpa, dvattn_paged_key_mass) need out, queries, rotated_queries, k_cache, v_cache, every
+ * dvattn_fused, dvattn_tree_paged_sdpa, dvattn_paged_key_mass, dvattn_paged_sdpa_q8,
+ * dvattn_varlen_paged_sdpa_q8) need out, queries, rotated_queries, k_cache, v_cache, every
  * key/value fragment and the workspace 16-byte aligned and the int32 / fp32
  * arrays 4-byte aligned; dvattn_rope, dvattn_varlen_rope,
- * dvattn_paged_kv_append, the metadata entries, dvattn_kv_select and
- * dvattn_paged_kv_compact need each array aligned to its element size.  A
+ * dvattn_paged_kv_append, the metadata entries, dvattn_kv_select,
+ * dvattn_paged_kv_compact and dvattn_block_tables need each array aligned to its element
+ * size, and so does dvattn_paged_kv_append_q8, but for its caches (16 bytes).  A
  * pointer off its alignment returns DVATTN_ERR_INVALID, naming the argument.
  * Tensors from a device allocator, and views of them that start on a row of
  * the last dimension, always qualify.
@@ -393,6 +398,87 @@ DVATTN_API dvattn_status dvattn_paged_kv_compact(int dtype, void* k_cache, void*
                                       const int* rows, int row_heads, int N, const int* first_rows,
                                       const int* lengths, float* mass, long long capacity,
                                       const dvattn_shape* shape, const dvattn_kv_layout* layout, void* stream);
+
+/* ---- block tables, positions and slots of a step ---------------------------------------
+ * From the tokens each sequence holds, lengths [W] i32, and those it adds in this step,
+ * new_tokens [W] i32 (0: none; below 0: the sequence has ended):
+ *   - an ended sequence's pages, block_tables[w, 0 .. ceil(lengths[w] / block_size)), are
+ *     pushed on the stack free_pages [num_blocks] i32, whose first *free_count entries are
+ *     free pages, in order of w and page; its length becomes 0 (its row is left as it is);
+ *   - every other sequence takes the pages that lengths[w] + new_tokens[w] tokens need
+ *     beyond those it holds, from the top of that stack down, in order of w, and they are
+ *     written to its row.  A sequence is refused if its row or the max_tokens packed
+ *     tokens have no room for it, or if the stack does not hold the pages that it and all
+ *     sequences before it that were not refused for room need: it takes no page and its
+ *     length stays;
+ *   - the step's tokens are packed in order of w: cu_seqlens [W+1] i32 are the sums of the
+ *     new tokens (refused sequences keep their places), starts [W] i32 the position of
+ *     each sequence's first new token (-1: refused or ended), positions [max_tokens] i32
+ *     and slots [max_tokens] i64 those of each packed token: position p lies in slot
+ *     block_tables[w, p / block_size] * block_size + p % block_size (-1 for both: a
+ *     token of a refused sequence, or behind the last; slot -1 too where the table names
+ *     no page);
+ *   - new_lengths [W] and new_free_count [1] hold the state after the step; they may be
+ *     lengths and free_count.  The same call on the same lengths and count gives the same.
+ * A page must be held by one sequence when it ends (pages that sequences share would be
+ * pushed twice).  Lengths outside [0, max_blocks_per_seq * block_size] and counts outside
+ * [0, num_blocks] are brought into the range.  Uses W, max_blocks_per_seq, num_blocks and
+ * block_size; W <= DVATTN_MAX_TABLE_SEQS.  One launch, two from 4097 tokens on. */
+#define DVATTN_MAX_TABLE_SEQS 8192
+DVATTN_API dvattn_status dvattn_block_tables(int* cu_seqlens, int* starts, int* positions, long long* slots,
+                                  int* new_lengths, int* new_free_count, int* block_tables, int* free_pages,
+                                  const int* lengths, const int* new_tokens, const int* free_count, int max_tokens,
+                                  const dvattn_shape* shape, void* stream);
+
+/* ---- caches held in 8 bits --------------------------------------------------------------
+ * k_cache [num_blocks,block_size,Hkv,E], v_cache [num_blocks,block_size,Hkv,Ev] hold OCP E4M3
+ * bytes and k_scales, v_scales [num_blocks,Hkv] an exponent byte b (E8M0) for each page
+ * and KV head: an element is byte * 2^(b - 127).  b = 0 is an empty page (its elements count
+ * as zeros), so caches and scales cleared to zero are a valid cache; b = 255 is no number.
+ *
+ * dvattn_paged_kv_append_q8 rounds new tokens to that form.  Token (w, s) is written to
+ * slots[w,s] i64 (slot = page * block_size + row; negative or past the cache: not
+ * written): the key rotated as dvattn_paged_kv_append rotates it and rounded to the storage type, and
+ * the value, as that cache would hold them.  For each page, KV head, and keys and
+ * values apart, with amax the largest finite magnitude written to the page:
+ *   - the exponent that amax asks for is the smallest b >= 1 with amax <= 448 * 2^(b - 127);
+ *   - if row 0 of the page is written (or b was 255), the page starts anew: it takes
+ *     that exponent, and its rows that are not written hold nothing any more;
+ *   - else it takes the larger of that and its own, and if its own was smaller, all
+ *     rows that are not written are rounded again under the new one (exact but for elements
+ *     that become less than 2^-6 of the new unit);
+ *   - elements are rounded to E4M3, ties to even.  NaN and infinities become NaN; finite fp16
+ *     magnitudes above 61440 are held as 61440.
+ * A sequence that fills its pages in order thus never reads what a page held before.  Slots
+ * may come in any order and more than once (the last token of a slot is the one that is
+ * held); tokens in consecutive slots are the fast case.  Keys and values must not overlap
+ * the caches.  Strides as in dvattn_kv_layout (its cache strides are not read: caches and
+ * scales are contiguous).  Uses W, Hkv, S, E = Ev = 128, block_size, num_blocks, rotary_dim. */
+DVATTN_API dvattn_status dvattn_paged_kv_append_q8(int dtype, int rope_dtype, void* k_cache, void* v_cache,
+                                        unsigned char* k_scales, unsigned char* v_scales, const long long* slots,
+                                        const void* keys, const void* values, const void* cosines,
+                                        const void* sines, const dvattn_shape* shape, const dvattn_kv_layout* layout,
+                                        void* stream);
+
+/* dvattn_paged_sdpa and dvattn_varlen_paged_sdpa over such caches: the same arguments, the
+ * caches' bytes and their scales.  dtype is that of queries and out; every element of a
+ * cache is exact in the products, queries are rounded to dtype after their rotation,
+ * and weights to bf16 in bf16 calls (fp16 calls carry 16 bits of them, fp32 calls
+ * 24). */
+DVATTN_API size_t dvattn_paged_sdpa_q8_workspace_size(int dtype, const dvattn_shape* shape, int device);
+DVATTN_API dvattn_status dvattn_paged_sdpa_q8(int dtype, void* out, float scale, const int* locations,
+                                   const void* queries, const float* cosines, const float* sines,
+                                   const int* fragment_lengths, const void* k_cache, const void* v_cache,
+                                   const unsigned char* k_scales, const unsigned char* v_scales,
+                                   const int* block_tables, const dvattn_shape* shape, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+DVATTN_API size_t dvattn_varlen_paged_sdpa_q8_workspace_size(int dtype, const dvattn_shape* shape, int device);
+DVATTN_API dvattn_status dvattn_varlen_paged_sdpa_q8(int dtype, void* out, float scale, const int* locations,
+                                          const void* queries, const float* cosines, const float* sines,
+                                          const int* fragment_lengths, const void* k_cache, const void* v_cache,
+                                          const unsigned char* k_scales, const unsigned char* v_scales,
+                                          const int* block_tables, const int* cu_seqlens_q, const dvattn_shape* shape,
+                                          void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
