@@ -31,7 +31,9 @@ EXPORTED = [
     "dvattn_paged_kv_append", "dvattn_view_metadata",
     "dvattn_tree_metadata", "dvattn_tree_metadata_counts", "dvattn_tree_paged_sdpa_workspace_size", "dvattn_tree_paged_sdpa",
     "dvattn_paged_key_mass_workspace_size", "dvattn_paged_key_mass", "dvattn_kv_select",
-    "dvattn_paged_kv_compact",
+    "dvattn_paged_kv_compact", "dvattn_block_tables", "dvattn_paged_kv_append_q8",
+    "dvattn_paged_sdpa_q8_workspace_size", "dvattn_paged_sdpa_q8",
+    "dvattn_varlen_paged_sdpa_q8_workspace_size", "dvattn_varlen_paged_sdpa_q8",
 ]
 
 
