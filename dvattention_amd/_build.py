@@ -31,7 +31,8 @@ TORCH_SO = os.path.join(HERE, "_libdvatt.so")
 PROBE_SO = os.path.join(HERE, "libdvattn_probe.so")
 
 HIP_SOURCES = ["dv_decode.hip", "dv_chunk.hip", "dv_chunk32.hip", "dv_small.hip", "dv_rope.hip", "dv_cache.hip",
-               "dv_tree.hip", "dv_mass.hip", "dv_evict.hip", "dv_pages.hip", "dv_decode8.hip", "dv_capi.hip"]
+               "dv_tree.hip", "dv_mass.hip", "dv_evict.hip", "dv_pages.hip", "dv_decode8.hip",
+               "dv_decode8m.hip", "dv_chunk8.hip", "dv_capi.hip"]
 
 # gfx950 code only; packed-fp32 instructions are disabled (the host pass of
 # hipcc warns that it does not know the feature, which is harmless).
@@ -60,7 +61,10 @@ def _run(cmd: list[str]) -> None:
 # where the compiler's default choice moved accumulators between VGPRs and
 # AGPRs around every MFMA.
 # dv_mass.hip: every score of an MFMA goes straight to the VALU.
-SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=true"] for name in ("dv_chunk.hip", "dv_mass.hip")}
+# dv_decode8.hip: two waves per SIMD share its registers, which a fixed half of AGPRs
+# would leave too few of for the rest.
+SOURCE_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=true"] for name in ("dv_chunk.hip", "dv_mass.hip", "dv_decode8.hip",
+                                                                                "dv_chunk8.hip")}
 
 
 def build_capi() -> str:

@@ -1246,12 +1246,12 @@ dvattn_status dvattn_paged_kv_append_q8(int dtype, int rope_dtype, void* k_cache
 // ---------------------------------------------------------------------------
 size_t dvattn_paged_sdpa_q8_workspace_size(int dtype, const dvattn_shape* s, int device) {
     if (!s || !valid_dtype(dtype)) return 0;
-    return dv::decode_workspace_bytes(s->W * s->S, s->Hkv, current_device(device), dtype);
+    return dv::sdpa8_workspace_bytes(dtype, false, s->W, s->S, s->Hkv, current_device(device));
 }
 
 size_t dvattn_varlen_paged_sdpa_q8_workspace_size(int dtype, const dvattn_shape* s, int device) {
     if (!s || !valid_dtype(dtype)) return 0;
-    return dv::decode_workspace_bytes(s->total_q_tokens, s->Hkv, current_device(device), dtype);
+    return dv::sdpa8_workspace_bytes(dtype, true, s->W, s->total_q_tokens, s->Hkv, current_device(device));
 }
 
 }  // extern "C"
@@ -1320,11 +1320,9 @@ dvattn_status sdpa_q8(bool varlen, int dtype, void* out, float scale, const int*
     p.bs_shift = log2_exact(s->block_size);
     p.maxB = s->max_blocks_per_seq;
     p.nblocks = s->num_blocks;
-    p.min_keys = dv::kDecodeMinKeys;
     const long long max_keys = (long long)s->max_blocks_per_seq * s->block_size;
-    const hipError_t e = dv::launch_decode8(dtype, varlen ? dv::kQRotHalf : dv::kQRotFull,
-                                            varlen ? dv::kRowVarlen : dv::kRowWS, p, (int)rows, max_keys, workspace,
-                                            workspace_bytes, (hipStream_t)stream);
+    const hipError_t e =
+        dv::launch_sdpa8(dtype, varlen, p, max_keys, workspace, workspace_bytes, (hipStream_t)stream);
     if (e != hipSuccess) return hip_fail(e, op);
     return ok();
 }

@@ -248,7 +248,8 @@ __device__ inline uint32_t token_mask(int vis, int kb0) {
 // Block (segment, token of the block; ntb tokens at most): thread t -> head t/16,
 // dims [(t%16)*8, +8).
 // A segment without pieces (no visible key) writes zeros, as the decode merge does.
-template <int DT, int RM>
+// kMany: groups of at most kFewTok tokens are left alone.
+template <int DT, int RM, bool kMany = false>
 __global__ __launch_bounds__(256) void dv_merge_chunk(const DecodeParams p, int ntb) {
     using raw = typename Tr<DT>::raw;
     const int sg = blockIdx.x / ntb;
@@ -258,7 +259,7 @@ __global__ __launch_bounds__(256) void dv_merge_chunk(const DecodeParams p, int 
     const int NHG = p.Hkv;
     const int r = sg / NHG, hkv = sg - (sg / NHG) * NHG;
     const Grp gr = group_of<RM>(p, p.row_begin + r);
-    if (tb >= gr.ntok) return;
+    if (tb >= gr.ntok || (kMany && gr.ntok <= kFewTok)) return;
     const int tid = threadIdx.x;
     const int n = tid >> 4;
     const int d[1] = {(tid & 15) * 8};

@@ -85,6 +85,7 @@ struct DecodeParams {
     // 8-bit caches (dv_decode8.hip, dv_chunk8.hip): exponent bytes [num_blocks, Hkv] of K and V
     const unsigned char* ks;
     const unsigned char* vs;
+    int sub;              // varlen groups of several tokens: blocks that a table entry is cut into
 };
 
 // Single-launch path for short contiguous views (dv_small.hip): one workgroup
@@ -327,10 +328,23 @@ hipError_t launch_key_mass(int dtype, const MassParams& p, void* workspace, hipS
 hipError_t launch_block_tables(const TablesParams& p, hipStream_t stream);
 hipError_t launch_kv_append8(int dtype, int rope_dtype, const Append8Params& p, hipStream_t stream);
 
-// Decode over an 8-bit cache: launch_decode's arguments and workspace
-// (decode_workspace_bytes), paged caches only.
-hipError_t launch_decode8(int dtype, int qmode, int rowmode, const DecodeParams& base, int nrows_total,
-                          long long max_keys_per_row, void* workspace, size_t ws_bytes, hipStream_t stream);
+// Attention over an 8-bit cache (dv_decode8.hip: a wave per KV head and up to four tokens;
+// dv_chunk8.hip: workgroups of 16 tokens): workspace of a [W, S] call and of T packed
+// tokens, and the launches.
+size_t sdpa8_workspace_bytes(int dtype, bool varlen, int W, int S_or_T, int Hkv, int device);
+hipError_t launch_sdpa8(int dtype, bool varlen, const DecodeParams& base, long long max_keys_per_row, void* workspace,
+                        size_t ws_bytes, hipStream_t stream);
+// Parts of it.  groups: rows of the launch's schedule, of nt tokens each (varlen and nt >
+// 1: blocks of the entries of p.vgroups).
+size_t decode8_workspace_bytes(long long groups, int nt, int Hkv, int device);
+hipError_t launch_decode8(int dtype, bool varlen, int nt, const DecodeParams& base, long long groups,
+                          long long max_keys_per_row, void* workspace, hipStream_t stream);
+size_t chunk8_workspace_bytes(long long groups, int Hkv, int device);
+hipError_t launch_chunk8(int dtype, bool varlen, const DecodeParams& base, long long groups,
+                         long long max_keys_per_group, void* workspace, hipStream_t stream);
+// The table of row groups of a varlen call (dv_chunk.hip): entries {first token, tokens,
+// sequence, 0}, gmax = T / 16 + W + 1 of them.
+hipError_t launch_varlen_groups(const int* cu, int W, int T, int gmax, int* groups, hipStream_t stream);
 // The merge of a decode launch's partial slots (rowmode: kRowWS or kRowVarlen).
 hipError_t launch_merge(int dtype, int rowmode, const DecodeParams& p, hipStream_t stream);
 

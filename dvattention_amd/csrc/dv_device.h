@@ -152,6 +152,12 @@ __device__ inline void dma16(const void* gptr, uint32_t lds_base) {
                  : "memory", "m0");
 }
 
+// A byte per lane from global memory into the LDS word at lds_base + 4 * lane.
+__device__ inline void dma1(const void* gptr, uint32_t lds_base) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_ubyte %0, off" ::"v"(gptr), "s"(lds_base)
+                 : "memory", "m0");
+}
+
 // dma16 of a K and a V piece, each with a wave-uniform base address and a 32-bit
 // byte offset per lane.  A vector-memory instruction may read a scalar register
 // only five wait states after a vector instruction (v_readfirstlane, v_readlane)
