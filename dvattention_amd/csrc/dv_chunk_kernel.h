@@ -32,6 +32,8 @@
 // (dv_chunk8.hip), as templates.
 #pragma once
 
+#include <type_traits>
+
 #include "dv_chunk.h"
 
 namespace dv {
@@ -52,30 +54,49 @@ __device__ inline int swz_v(int key, int piece) { return piece ^ ((key & 7) << 1
 // ---- 8-bit caches (KV8) ---------------------------------------------------------
 //
 // The stage loop computes on 16-bit tiles, as for a 16-bit cache; they are made from the
-// 8-bit rows in LDS, once per workgroup: a byte that every wave widened for itself would
-// cost 64 conversions per wave and stage, and an operand read of 16-bit tiles is what the
-// MFMAs take.  A wave brings its eighth of a stage (four rows of K, four of V, 16 bytes
-// per lane, and the exponent byte of the lane's row) into a raw ring of its own, seven
-// stages ahead; one stage before its turn it widens them -- E4M3 times a power of two,
-// exact in bf16 -- into one of three 16-bit slots.  Three, so that a slot outlives its
-// stage by a barrier and V can be read from it again (mask_v).
+// 8-bit rows in LDS, once per workgroup: bytes that every wave widened for itself would
+// cost 64 conversions per wave and stage, this takes eight.  Waves 0 .. 3 bring eight rows
+// of K each, waves 4 .. 7 of V (16 bytes per lane, and the exponent byte of the lane's
+// row), into a raw ring of their own, seven stages ahead; one stage before its turn a
+// wave widens its rows -- E4M3 times a power of two, exact in bf16 -- into one of three
+// 16-bit slots.  Three, so that a slot outlives its stage by a barrier and V can be read
+// from it again (mask_v).
 constexpr int kWideSlots = 3;
 constexpr int kRawStages = 8;
 constexpr int kRawWave = 64 * 16 + 64 * 4;  // a wave's share of a raw stage: rows, then exponents
 constexpr int kRawBytes = kWaves * kRawWave;
-template <bool KV8> constexpr int kSlots = KV8 ? kWideSlots : kStages;
 template <bool KV8> constexpr int kLdsRing = KV8 ? kWideSlots * kStageBytes + kRawStages * kRawBytes : kRingBytes;
 
-// This wave's share of raw stage st (keys kb0 .. kb0 + 31 of the range): lane -> K or V
-// (lane / 32), row 4 * wave + lane / 8 % 4, 16-byte piece lane % 8.
+// Per-lane constants of the loop, held in a register each (what derives from them is
+// computed where it is used): the LDS offsets of this lane's K and V^T operands in a slot
+// and of its widened piece, and 16 * lane.
+struct Off8 {
+    uint32_t k, v, w, lane16;
+};
+__device__ inline Off8 offsets8() {
+    const int lane = threadIdx.x & 63, wv = uniform((int)(threadIdx.x >> 6));
+    const int g = lane >> 4, n = lane & 15;
+    const int k0 = g * 4 + (n >> 2);
+    const int kl = (wv & 3) * 8 + (lane >> 3), piece = (lane & 7) * 2;
+    Off8 o;
+    o.k = (uint32_t)(n * 256 + 16 * (g ^ (n & 3)) + 64 * (n >> 2));
+    o.v = (uint32_t)(kKvBytes + k0 * 256 + 16 * ((n & 3) >> 1) + (n & 1) * 8 + 32 * (k0 & 7));
+    o.w = (uint32_t)((wv < 4 ? 0 : kKvBytes) + kl * 256 + (wv < 4 ? swz_k(kl, piece) : swz_v(kl, piece)) * 16);
+    o.lane16 = (uint32_t)lane * 16;
+    asm volatile("" : "+v"(o.k), "+v"(o.v), "+v"(o.w), "+v"(o.lane16));
+    return o;
+}
+
+// This wave's share of raw stage st (keys kb0 .. kb0 + 31 of the range): lane -> row 8 *
+// (wave % 4) + lane / 8, 16-byte piece lane % 8.
 template <bool P2>
 __device__ inline void issue_raw(const DecodeParams& p, const Range& r, const int* pages, uint32_t raw, int st,
-                                 int kb0) {
-    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const int kl = wv * 4 + ((lane >> 3) & 3);
+                                 int kb0, const Off8& o) {
+    const int wv = uniform((int)(threadIdx.x >> 6));
     const uint32_t base = raw + (uint32_t)((st % kRawStages) * kRawBytes + wv * kRawWave);
-    const int l = kb0 + kl;
-    const uint32_t pos = (uint32_t)(r.off + l);
+    const int lrow = (int)(o.lane16 >> 7);
+    const int l = kb0 + (wv & 3) * 8 + lrow;
+    const uint32_t pos = (uint32_t)(r.off + kb0 + (wv & 3) * 8) + (uint32_t)lrow;
     uint32_t lp, rr;
     if (P2) {
         lp = pos >> p.bs_shift;
@@ -85,60 +106,56 @@ __device__ inline void issue_raw(const DecodeParams& p, const Range& r, const in
         rr = pos - lp * (uint32_t)p.bs;
     }
     const uint32_t idx = lp - r.lp0;
+    const unsigned char* c = wv < 4 ? r.k : r.v;
+    const unsigned char* e = wv < 4 ? p.ks : p.vs;
+    // (one path: a branch here would part the MFMAs that this is computed beside)
     const int pg = pages[idx < (uint32_t)kPageCap ? idx : (uint32_t)(kPageCap - 1)];
     const bool ok = l < r.b && idx < (uint32_t)kPageCap && pg >= 0;
-    const uint32_t hrow = (uint32_t)pg * (uint32_t)p.Hkv + (uint32_t)r.hkv;
-    const uint32_t rowidx = ((uint32_t)pg * (uint32_t)p.bs + rr) * (uint32_t)p.Hkv + (uint32_t)r.hkv;
-    const unsigned char* c = lane < 32 ? r.k : r.v;
-    const unsigned char* e = lane < 32 ? p.ks : p.vs;
-    const unsigned char* a = ok ? c + ((unsigned long long)rowidx << 7) : zrow;
-    dma16(a + (lane & 7) * 16, __builtin_amdgcn_readfirstlane(base));
-    dma1(ok ? e + hrow : zrow, __builtin_amdgcn_readfirstlane(base + 64 * 16));
+    const uint32_t h = ((uint32_t)pg * (uint32_t)p.bs + rr) * (uint32_t)p.Hkv + (uint32_t)r.hkv;
+    const unsigned char* a = (ok ? c + ((unsigned long long)h << 7) : zrow) + (o.lane16 & 127u);
+    const unsigned char* s = ok ? e + ((uint32_t)pg * (uint32_t)p.Hkv + (uint32_t)r.hkv) : zrow;
+    dma16(a, __builtin_amdgcn_readfirstlane(base));
+    dma1(s, __builtin_amdgcn_readfirstlane(base + 64 * 16));
 }
 
-// The wave's share of a landed raw stage: 16 bytes of the lane's row and its exponent.
-struct Raw {
-    u32x4 b;
-    uint32_t e;
-};
-__device__ inline Raw read_raw(const unsigned char* raw, int st) {
-    const int lane = opaque_tid() & 63, wv = threadIdx.x >> 6;
-    const unsigned char* base = raw + (st % kRawStages) * kRawBytes + wv * kRawWave;
-    Raw x;
-    x.b = *reinterpret_cast<const u32x4*>(base + lane * 16);
-    x.e = *reinterpret_cast<const uint32_t*>(base + 64 * 16 + lane * 4);
-    return x;
-}
-
-// ... widened into the 16-bit slot, at the places where a 16-bit stage has its pieces: K in
-// the queries' type, V in bf16.  (b = 0 is a page of zeros.)
+// The wave's share of landed raw stage st, widened into the 16-bit slot at LDS address
+// `slot`, at the places where a 16-bit stage has its pieces: K in the queries' type, V in
+// bf16.
 template <int DT>
-__device__ inline void widen(unsigned char* slot, const Raw& x) {
-    const int lane = opaque_tid() & 63, wv = threadIdx.x >> 6;
-    const int kl = wv * 4 + ((lane >> 3) & 3), piece = (lane & 7) * 2;
-    const float s = __uint_as_float(x.e << 23);
-    const uint32_t keep = x.e ? 0xffffffffu : 0u;
+__device__ inline void widen(uint32_t slot, uint32_t raw, int st, const Off8& o) {
+    const int wv = uniform((int)(threadIdx.x >> 6));
+    const uint32_t base = raw + (uint32_t)((st % kRawStages) * kRawBytes + wv * kRawWave);
+    typedef __attribute__((address_space(3))) const uint32_t lds_u32;
+    u32x4 x = lds_read16_at(base + o.lane16);
+    const uint32_t e = *(lds_u32*)(uintptr_t)(base + 64 * 16 + (o.lane16 >> 2));
+    if (ballot(e == 0)) {  // an exponent of 0: a page of zeros (or no page)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = e ? x[i] : 0u;
+    }
+    const float s = __uint_as_float(e << 23);
     u32x4 w[2];
+    if (DT == kF16 && wv < 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int b = (int)(x.b[i] & keep);
-        uint32_t lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, false));
-        uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, s, true));
-        if constexpr (DT == kF16) {
-            const uint32_t klo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, s, false));
-            const uint32_t khi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, s, true));
-            lo = lane < 32 ? klo : lo;
-            hi = lane < 32 ? khi : hi;
+        for (int i = 0; i < 4; ++i) {
+            w[i >> 1][(i & 1) * 2] =
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x[i], s, false));
+            w[i >> 1][(i & 1) * 2 + 1] =
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)x[i], s, true));
         }
-        w[i >> 1][(i & 1) * 2] = lo;
-        w[i >> 1][(i & 1) * 2 + 1] = hi;
-    }
-    unsigned char* row = slot + (lane < 32 ? 0 : kKvBytes) + kl * 256;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int at = lane < 32 ? swz_k(kl, piece + i) : swz_v(kl, piece + i);
-        *reinterpret_cast<u32x4*>(row + at * 16) = w[i];
+        for (int i = 0; i < 4; ++i) {
+            w[i >> 1][(i & 1) * 2] =
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x[i], s, false));
+            w[i >> 1][(i & 1) * 2 + 1] =
+                __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)x[i], s, true));
+        }
     }
+    // (both swizzles keep a row's pieces 2i and 2i + 1 side by side, in one order or the other)
+    typedef __attribute__((address_space(3))) u32x4 lds_w;
+    const uint32_t at = slot + o.w;
+    *(lds_w*)(uintptr_t)at = w[0];
+    *(lds_w*)(uintptr_t)(at ^ 16u) = w[1];
 }
 
 // fp16 calls over 8-bit caches: the weights as two bf16 numbers, 16 bits of each whatever
@@ -329,10 +346,7 @@ struct VOp {
     u32x4 v[8];
 };
 
-__device__ inline void read_k(const unsigned char* kt, KOp& k) {
-    const int lane = threadIdx.x & 63;
-    const int g = lane >> 4, n = lane & 15;
-    const uint32_t kbase = lds_addr(kt) + (uint32_t)(n * 256 + 16 * (g ^ (n & 3)) + 64 * (n >> 2));
+__device__ inline void read_k_at(uint32_t kbase, KOp& k) {
 #pragma unroll
     for (int cc = 0; cc < 4; ++cc) {
         k.lo[cc] = lds_read16_at(kbase ^ (uint32_t)(64 * cc));
@@ -340,12 +354,13 @@ __device__ inline void read_k(const unsigned char* kt, KOp& k) {
     }
 }
 
-__device__ inline void read_v(const unsigned char* vt, VOp& v) {
+__device__ inline void read_k(const unsigned char* kt, KOp& k) {
     const int lane = threadIdx.x & 63;
-    const int g = lane >> 4, sl = lane & 15;
-    const int k0 = g * 4 + (sl >> 2);
-    const uint32_t vbase =
-        lds_addr(vt) + (uint32_t)(k0 * 256 + 16 * ((sl & 3) >> 1) + (sl & 1) * 8 + 32 * (k0 & 7));
+    const int g = lane >> 4, n = lane & 15;
+    read_k_at(lds_addr(kt) + (uint32_t)(n * 256 + 16 * (g ^ (n & 3)) + 64 * (n >> 2)), k);
+}
+
+__device__ inline void read_v_at(uint32_t vbase, VOp& v) {
 #pragma unroll
     for (int cc = 0; cc < 8; ++cc) {
         const u32x2 a0 = lds_read_tr16_at(vbase ^ (uint32_t)(32 * cc));
@@ -394,17 +409,25 @@ __device__ inline uint32_t stage_mask(const DecodeParams& p, const Range& r, con
     return m;
 }
 
+__device__ inline void read_v(const unsigned char* vt, VOp& v) {
+    const int lane = threadIdx.x & 63;
+    const int g = lane >> 4, sl = lane & 15;
+    const int k0 = g * 4 + (sl >> 2);
+    read_v_at(lds_addr(vt) + (uint32_t)(k0 * 256 + 16 * ((sl & 3) >> 1) + (sl & 1) * 8 + 32 * (k0 & 7)), v);
+}
+
 // V^T operand with the keys cleared that a tile does not see (bit k of mask: key k): their
 // weight is 0, which a NaN of another token's row would survive.  A lane holds keys
 // g*4 + i and 16 + g*4 + i, 16 bits each.
 __device__ inline void mask_v(VOp& v, uint32_t mask) {
-    const int lane = threadIdx.x & 63;
+    const int lane = opaque_tid() & 63;
     const uint32_t mg = mask >> ((lane >> 4) * 4);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t b = mg >> ((i >> 1) * 16 + (i & 1) * 2);
         w[i] = ((b & 1u) ? 0xffffu : 0u) | ((b & 2u) ? 0xffff0000u : 0u);
+        asm volatile("" : "+v"(w[i]));  // (a branch around it stays one)
     }
 #pragma unroll
     for (int cc = 0; cc < 8; ++cc)
@@ -525,17 +548,13 @@ template <int KS> constexpr int lead() { return KS == 1 ? kAhead : kStages / KS;
 // writes; mfma_settle before each softmax covers the MFMA -> VALU dependence
 // across the half-stage boundary.  Invisible keys get -inf scores only on a
 // partially visible stage (a uniform branch between the interleaved regions).
-template <int DT, int KVM, bool P2, int KS, bool KV8>
+template <int DT, int KVM, bool P2, int KS>
 __device__ inline void stream_range(const DecodeParams& p, const Range& r, const int* pages, unsigned char* smem,
                                     int sa, int sbnd, int kg, const int (&vis_t)[kTiles],
                                     const u32x4 (&qB)[kTiles][4], Tile (&tl)[kTiles]) {
     constexpr int kLead = lead<KS>();
     constexpr int kDma = kDmaPerStage * KS;  // loads per wave and step
-    static_assert(!KV8 || (KS == 1 && KVM == kKvPaged), "8-bit caches: paged, no key split");
     const uint32_t ring = lds_addr(smem);
-    unsigned char* raw8 = smem + kWideSlots * kStageBytes;  // KV8: the raw ring
-    // (the loads of a raw stage are two as well: rows and exponents)
-    constexpr int kNs = kSlots<KV8>;
     const int nsteps = (sbnd - sa + KS * kStep - 1) / (KS * kStep);
     const float l2 = p.l2scale;
     // prologue: steps 0 .. kLead-1.  Past the end, KS = 1 issues rows of zeros; with a
@@ -546,17 +565,10 @@ __device__ inline void stream_range(const DecodeParams& p, const Range& r, const
     for (int s = 0; s < kLead; ++s) {
         if (KS > 1 && s >= nsteps) break;
 #pragma unroll
-        for (int st = s * KS; st < (s + 1) * KS; ++st) {
-            if constexpr (KV8) issue_raw<P2>(p, r, pages, lds_addr(raw8), st, sa + st * kStep);
-            else issue_stage<KVM, P2>(p, r, pages, ring, st, sa + st * kStep);
-        }
+        for (int st = s * KS; st < (s + 1) * KS; ++st) issue_stage<KVM, P2>(p, r, pages, ring, st, sa + st * kStep);
     }
     if (KS == 1 || nsteps >= kLead) wait_vmcnt<kDma * (kLead - 1)>();  // own share of step 0 landed
     else wait_vmcnt<0>();
-    if constexpr (KV8) {
-        widen<DT>(smem, read_raw(raw8, 0));
-        lds_wait();
-    }
     wg_barrier();
 
     KOp kop;
@@ -568,27 +580,17 @@ __device__ inline void stream_range(const DecodeParams& p, const Range& r, const
     read_k(smem + kg * kStageBytes, kop);
     qk_tile<DT>(kop, qB[0], sa0, sa1);
 
-    uint32_t mkb_last = 0xffffffffu;  // KV8: what B saw of the stage whose P V is still to come
     for (int i = 0; i < nsteps; ++i) {
         const int st = i * KS + kg;  // this wave's stage of the step
         const int kb0 = sa + st * kStep;
-        const unsigned char* slot = smem + (st % kNs) * kStageBytes;
+        const unsigned char* slot = smem + (st % kStages) * kStageBytes;
         const uint32_t okm = stage_mask<KVM, P2, KS>(p, r, pages, sbnd, kb0);
         const uint32_t mka = okm & token_mask(vis_t[0], kb0), mkb = okm & token_mask(vis_t[1], kb0);
         float pr[8];
         // ---- H1(i)
-        Raw rw;
-        if constexpr (KV8) {
-            // own share of stage i + 1 landed: widened in this half-stage, complete
-            // before the barrier after which K(i + 1) is read
-            wait_vmcnt<kDma * (kLead - 2)>();
-            rw = read_raw(raw8, i + 1);
-            if (mkb_last != 0xffffffffu) mask_v(vop, mkb_last);
-            mkb_last = mkb;
-        }
         if (mka != 0xffffffffu) mask_scores(sa0, sa1, mka);
         mfma_settle(tl[0].o);
-        pv_tile<DT, KV8>(vop, pb, tl[1]);  // zero at i = 0
+        pv_tile<DT>(vop, pb, tl[1]);  // zero at i = 0
         float lmx = sm_exponents(tl[0], sa0, sa1, l2, pr);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -598,7 +600,7 @@ __device__ inline void stream_range(const DecodeParams& p, const Range& r, const
         if (ballot(lmx > kMaxSlack)) sm_raise(tl[0], sa0, sa1, l2, pr);
         qk_tile<DT>(kop, qB[1], sb0, sb1);
         read_v(slot + kKvBytes, vop);
-        pa = sm_finish<DT, KV8>(tl[0], pr);
+        pa = sm_finish<DT>(tl[0], pr);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
@@ -606,14 +608,11 @@ __device__ inline void stream_range(const DecodeParams& p, const Range& r, const
             __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);  // VALU
         }
         settle<DT>(pa);
-        if constexpr (KV8) widen<DT>(smem + ((i + 1) % kNs) * kStageBytes, rw);
         lds_wait();
         // own share of step i + 1 landed (with a key split, fewer loads follow it near
         // the end)
-        if constexpr (!KV8) {
-            if (KS == 1 || i + kLead <= nsteps) wait_vmcnt<kDma * (kLead - 2)>();
-            else wait_vmcnt<0>();
-        }
+        if (KS == 1 || i + kLead <= nsteps) wait_vmcnt<kDma * (kLead - 2)>();
+        else wait_vmcnt<0>();
         wg_barrier();
         if (KS > 1 && i + kLead < nsteps) {
             // the loads of step i + kLead, into the slots of step i (free since the
@@ -626,11 +625,10 @@ __device__ inline void stream_range(const DecodeParams& p, const Range& r, const
         // ---- H2(i) (past the end, step i + 1 holds rows of zeros or what the slot
         // held before: K and S_A of the next stage need no branch, the last ones go
         // unused)
-        read_k(smem + ((st + KS) % kNs) * kStageBytes, kop);
-        if (KV8 && mka != 0xffffffffu) mask_v(vop, mka);
+        read_k(smem + ((st + KS) % kStages) * kStageBytes, kop);
         if (mkb != 0xffffffffu) mask_scores(sb0, sb1, mkb);
         mfma_settle(tl[1].o);
-        pv_tile<DT, KV8>(vop, pa, tl[0]);
+        pv_tile<DT>(vop, pa, tl[0]);
         lmx = sm_exponents(tl[1], sb0, sb1, l2, pr);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
@@ -640,26 +638,149 @@ __device__ inline void stream_range(const DecodeParams& p, const Range& r, const
         }
         if (ballot(lmx > kMaxSlack)) sm_raise(tl[1], sb0, sb1, l2, pr);
         qk_tile<DT>(kop, qB[0], sa0, sa1);
-        pb = sm_finish<DT, KV8>(tl[1], pr);
+        pb = sm_finish<DT>(tl[1], pr);
         // the loads of stage i + kAhead (into the slot of stage i - 1, free since
         // the barrier), their address arithmetic beside the MFMAs
-        if constexpr (KV8) issue_raw<P2>(p, r, pages, lds_addr(raw8), i + kLead, sa + (i + kLead) * kStep);
-        else if constexpr (KS == 1) issue_stage<KVM, P2>(p, r, pages, ring, i + kLead, sa + (i + kLead) * kStep);
+        if constexpr (KS == 1) issue_stage<KVM, P2>(p, r, pages, ring, i + kLead, sa + (i + kLead) * kStep);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
             __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);  // VALU
         }
         settle<DT>(pb);
-        if (KV8 && mka != 0xffffffffu) read_v(slot + kKvBytes, vop);  // whole again, for B
     }
     // P V of B's last stage
-    if (KV8 && mkb_last != 0xffffffffu) mask_v(vop, mkb_last);
     mfma_settle(tl[1].o);
-    pv_tile<DT, KV8>(vop, pb, tl[1]);
+    pv_tile<DT>(vop, pb, tl[1]);
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) mfma_settle(tl[t].o);
     wait_vmcnt<0>();  // the trailing zero-row stages land before the ring is reused
+    __syncthreads();
+}
+
+// The same loop over an 8-bit cache (KS = 1): stage i + 1 is widened in H1(i), complete
+// before the barrier after which K(i + 1) is read.  Two loops, one after the other in the
+// same pipeline: stages that both tiles see whole (no masks at all), then those from the
+// first that some tile sees in part -- the last ones of a causal chunk -- where scores are
+// masked and each tile's V operand too.  In one loop, the masked operand would cost the
+// common stages 32 registers, which there are not.
+template <int DT, bool P2>
+__device__ inline void stream_range8(const DecodeParams& p, const Range& r, const int* pages, unsigned char* smem,
+                                     int sa, int sbnd, int ntile, const int (&vis_t)[kTiles],
+                                     const u32x4 (&qB)[kTiles][4], Tile (&tl)[kTiles]) {
+    constexpr int kLead = lead<1>();
+    constexpr int kDma = kDmaPerStage;  // of a raw stage: rows and exponents
+    const uint32_t ring = lds_addr(smem);
+    const uint32_t raw = ring + kWideSlots * kStageBytes;
+    const int nsteps = (sbnd - sa + kStep - 1) / kStep;
+    const float l2 = p.l2scale;
+    const Off8 o8 = offsets8();
+    // stages that every tile of this wave sees whole
+    int seen = sbnd;
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+        if (t < ntile && vis_t[t] < seen) seen = vis_t[t];
+    const int nfull = r.pages_ok && seen > sa ? (seen - sa) / kStep : 0;
+#pragma unroll
+    for (int s = 0; s < kLead; ++s) issue_raw<P2>(p, r, pages, raw, s, sa + s * kStep, o8);
+    wait_vmcnt<kDma * (kLead - 1)>();  // own share of stage 0 landed
+    widen<DT>(ring, raw, 0, o8);
+    lds_wait();
+    wg_barrier();
+
+    KOp kop;
+    VOp vop;
+#pragma unroll
+    for (int cc = 0; cc < 8; ++cc) vop.v[cc] = u32x4{0u, 0u, 0u, 0u};  // the first P V adds 0 * 0
+    f32x4 sa0, sa1, sb0, sb1;
+    POperand pa = {}, pb = {};
+    read_k_at(ring + o8.k, kop);
+    qk_tile<DT>(kop, qB[0], sa0, sa1);
+    uint32_t mkb_last = 0xffffffffu;  // what B saw of the stage whose P V is still to come
+    uint32_t at = 0, next = kStageBytes;  // slots of stages i and i + 1
+
+    auto step = [&](auto masked, int i) {
+        constexpr bool kMask = decltype(masked)::value;
+        const int kb0 = sa + i * kStep;
+        uint32_t mka = 0xffffffffu, mkb = 0xffffffffu;
+        float pr[8];
+        // ---- H1(i)
+        if constexpr (kMask) {
+            const uint32_t okm = stage_mask<kKvPaged, P2, 1>(p, r, pages, sbnd, kb0);
+            mka = okm & token_mask(vis_t[0], kb0);
+            mkb = okm & token_mask(vis_t[1], kb0);
+            if (mka != 0xffffffffu) mask_scores(sa0, sa1, mka);
+            if (mkb_last != 0xffffffffu) mask_v(vop, mkb_last);
+            mkb_last = mkb;
+        }
+        mfma_settle(tl[0].o);
+        pv_tile<DT, true>(vop, pb, tl[1]);  // zero at i = 0
+        float lmx = sm_exponents(tl[0], sa0, sa1, l2, pr);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);  // VALU
+        }
+        if (ballot(lmx > kMaxSlack)) sm_raise(tl[0], sa0, sa1, l2, pr);
+        qk_tile<DT>(kop, qB[1], sb0, sb1);
+        read_v_at(ring + at + o8.v, vop);
+        pa = sm_finish<DT, true>(tl[0], pr);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS read
+            __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);  // VALU
+        }
+        settle<DT>(pa);
+        // own share of stage i + 1 landed: widened here, where K(i)'s registers are free
+        wait_vmcnt<kDma * (kLead - 2)>();
+        __builtin_amdgcn_sched_barrier(0);
+        widen<DT>(ring + next, raw, i + 1, o8);
+        lds_wait();
+        wg_barrier();
+        // ---- H2(i)
+        read_k_at(ring + next + o8.k, kop);
+        if constexpr (kMask) {
+            if (mkb != 0xffffffffu) mask_scores(sb0, sb1, mkb);
+            if (mka != 0xffffffffu) mask_v(vop, mka);
+        }
+        mfma_settle(tl[1].o);
+        pv_tile<DT, true>(vop, pa, tl[0]);
+        lmx = sm_exponents(tl[1], sb0, sb1, l2, pr);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS read
+            __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);  // VALU
+        }
+        if (ballot(lmx > kMaxSlack)) sm_raise(tl[1], sb0, sb1, l2, pr);
+        qk_tile<DT>(kop, qB[0], sa0, sa1);
+        pb = sm_finish<DT, true>(tl[1], pr);
+        issue_raw<P2>(p, r, pages, raw, i + kLead, sa + (i + kLead) * kStep, o8);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+            __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);  // VALU
+        }
+        settle<DT>(pb);
+        if constexpr (kMask) {
+            if (mka != 0xffffffffu) read_v_at(ring + at + o8.v, vop);  // whole again, for B
+        }
+        at = next;
+        next = next == (kWideSlots - 1) * kStageBytes ? 0u : next + kStageBytes;
+    };
+    int i = 0;
+#pragma unroll 1
+    for (; i < nfull; ++i) step(std::false_type{}, i);
+#pragma unroll 1
+    for (; i < nsteps; ++i) step(std::true_type{}, i);
+    // P V of B's last stage
+    if (mkb_last != 0xffffffffu) mask_v(vop, mkb_last);
+    mfma_settle(tl[1].o);
+    pv_tile<DT, true>(vop, pb, tl[1]);
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) mfma_settle(tl[t].o);
+    wait_vmcnt<0>();  // the trailing stages land before the ring is reused
     __syncthreads();
 }
 
@@ -813,7 +934,8 @@ __device__ void chunk_piece(const DecodeParams& p, unsigned char* smem, int* pag
                     read_q_tiles(qreg, ntile, qB);
                     __syncthreads();
                 }
-                stream_range<DT, KVM, P2, KS, KV8>(p, r, pages, smem, sa, sbnd, kg, vis_t, qB, tl);
+                if constexpr (KV8) stream_range8<DT, P2>(p, r, pages, smem, sa, sbnd, ntile, vis_t, qB, tl);
+                else stream_range<DT, KVM, P2, KS>(p, r, pages, smem, sa, sbnd, kg, vis_t, qB, tl);
             }
         }
         P += vis_blk;
