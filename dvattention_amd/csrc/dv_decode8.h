@@ -16,8 +16,9 @@
 //    rounding is the same with and without).
 //  * Precision: bf16 calls take one operand for Q and P, as the 16-bit decode does.  fp16
 //    calls take Q as it is against K in fp16, and P as a bf16 pair hi + lo (16 bits).
-//    fp32 calls take Q and P as three bf16 numbers each, which hold 24 bits: the products
-//    with exact K and V lose nothing that fp32 arithmetic keeps.
+//    fp32 calls take Q, its row scaled by a power of two, as an fp16 pair and P as three
+//    bf16 numbers, 24 bits either way: the products with exact K and V lose nothing that
+//    fp32 arithmetic keeps.
 #pragma once
 
 #include "dv_common.h"
@@ -37,16 +38,18 @@ constexpr int kLoads = 9;                       // direct-to-LDS loads per stage
 // Tokens of a row group at most: a wave holds NT query tiles (16 heads of a token each).
 constexpr int kMaxTok = 4;
 // Waves of one or two tiles fit two to a SIMD with two stages each in LDS, their
-// accumulators in VGPRs (as their file is compiled); those of four have the SIMD to
-// themselves, four stages, and accumulators in AGPRs.
-template <int NT> constexpr int kWavesPerCu = NT <= 2 ? 8 : 4;
-template <int NT> constexpr int kRing = kWavesPerCu<NT> == 8 ? 2 : 4;
-template <int NT> constexpr int kWaveLds = kRing<NT> * kStage + stream::kPc * 4;
+// accumulators in VGPRs (as their file is compiled); those of four, and of two in fp32
+// (their operands alone are 128 registers), have the SIMD to themselves, four stages, and
+// accumulators in AGPRs.
+constexpr int waves_per_cu(int dtype, int nt) { return nt == 1 || (nt == 2 && dtype != kF32) ? 8 : 4; }
+template <int DT, int NT> constexpr int kWavesPerCu = waves_per_cu(DT, NT);
+template <int DT, int NT> constexpr int kRing = kWavesPerCu<DT, NT> == 8 ? 2 : 4;
+template <int DT, int NT> constexpr int kWaveLds = kRing<DT, NT> * kStage + stream::kPc * 4;
 
 // MFMA operands of a query (or probability) value: 16-bit parts that sum to it.
-template <int DT> constexpr int kQParts = DT == kF32 ? 3 : 1;
+template <int DT> constexpr int kQParts = DT == kF32 ? 2 : 1;
 template <int DT> constexpr int kPParts = DT == kF32 ? 3 : DT == kF16 ? 2 : 1;
-template <int DT> constexpr int kKType = DT == kF16 ? kF16 : kBF16;
+template <int DT> constexpr int kKType = DT == kBF16 ? kBF16 : kF16;
 
 // Eight E4M3 bytes as four words of 16-bit pairs, exactly.
 template <int T16>
@@ -88,22 +91,12 @@ __device__ inline int swz_v(int row) { return ((row >> 1) & 3) | ((row >> 2) & 4
 // 2^(b - 127) of an exponent byte (0: zero).
 __device__ inline float power_of(uint32_t b) { return __uint_as_float(b << 23); }
 
-// This lane's byte offsets from a stage's row bases: load i moves rows 8i .. 8i + 7 (lane /
-// 8), whose swizzles repeat every other load (K) and every two (V).
-struct LaneOff {
-    uint32_t k[2], v[2];
-};
-__device__ inline LaneOff lane_offsets(const DecodeParams& p) {
+// This lane's byte offset from a stage's row bases: load i moves rows 8i .. 8i + 7 (lane /
+// 8); with i odd (K) or above 1 (V) the swizzle is the same but for bit 2: offset ^ 64.
+__device__ inline uint32_t lane_offset(const DecodeParams& p) {
     const int lane = threadIdx.x & 63;
     const int r = lane >> 3, c = lane & 7;
-    const uint32_t row = (uint32_t)r * ((uint32_t)p.Hkv * kRowB);
-    LaneOff o;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        o.k[i] = row + (uint32_t)((c ^ swz_k(8 * i + r)) * 16);
-        o.v[i] = row + (uint32_t)((c ^ swz_v(16 * i + r)) * 16);
-    }
-    return o;
+    return (uint32_t)r * ((uint32_t)p.Hkv * kRowB) + (uint32_t)((c ^ swz_k(r)) * 16);
 }
 
 // Issues the loads of the stage holding keys [l, l + 32) into the ring slot at LDS address
@@ -112,7 +105,7 @@ __device__ inline LaneOff lane_offsets(const DecodeParams& p) {
 // two pages, one for each half, so its row bases are scalar and no lane looks a row up
 // (32 ragged sequences: 9 + 140 instructions per stage instead of 9 + 250).
 template <bool P2, bool kAsk>
-__device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, const LaneOff& lo, const int* pc,
+__device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, uint32_t lo, const int* pc,
                                  uint32_t sbase, int l) {
     const int lane = threadIdx.x & 63;
     if constexpr (P2) {
@@ -131,8 +124,8 @@ __device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, c
                 for (int i = 0; i < 4; ++i) {
                     const unsigned long long r =
                         row[i >> 1] + (unsigned long long)((uint32_t)(i & 1) * ((uint32_t)p.Hkv << 10));
-                    dma16_kv(kb + r, lo.k[i & 1], sbase + (uint32_t)(i * 1024), vb + r, lo.v[i >> 1],
-                             sbase + (uint32_t)(kTile + i * 1024));
+                    dma16_kv(kb + r, (i & 1) ? lo ^ 64u : lo, sbase + (uint32_t)(i * 1024), vb + r,
+                             (i >> 1) ? lo ^ 64u : lo, sbase + (uint32_t)(kTile + i * 1024));
                 }
                 const uint32_t pg = (uint32_t)((lane & 16) ? pg1 : pg0);
                 dma1((lane < 32 ? p.ks : p.vs) + (pg * (uint32_t)p.Hkv + (uint32_t)v.hkv),
@@ -178,21 +171,14 @@ __device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, c
 }
 
 // A query row's 16-bit MFMA operands: lane (g, n) holds dims c * 32 + g * 8 .. + 8 of head n.
+// fp32: times 2^k, k such that the head's largest magnitude lies in [2^14, 2^15), as hi + lo:
+// hi is within 2^-12 of the element, lo within 2^-12 of what hi leaves (or 2^-25 of 2^15);
+// l2: softmax scale / ln 2, times 2^-k.
 template <int DT>
 struct QOp {
     u32x4 q[kQParts<DT>][4];
+    float l2;
 };
-
-// fp32: the three bf16 numbers that sum to x (each part rounds what the ones before left).
-__device__ inline void split3(float x, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-    const uint16_t h = Tr<kBF16>::fromf(x);
-    const float r = x - Tr<kBF16>::tof(h);
-    const uint16_t m = Tr<kBF16>::fromf(r);
-    const uint16_t l = Tr<kBF16>::fromf(r - Tr<kBF16>::tof(m));
-    hi = h;
-    mid = m;
-    lo = l;
-}
 
 // Eight consecutive elements as floats (16-byte aligned).
 template <int DT>
@@ -220,14 +206,22 @@ template <int DT>
 __device__ inline void rotated8(const typename Tr<DT>::raw* q, const float* cs, const float* sn, int R, int d0,
                                 bool wide, typename Tr<DT>::raw (&r)[8]) {
 #pragma clang fp contract(off)
-    if (!wide) {
-        rotate_run<DT, 8>(q, cs, sn, R, d0, r);
-        return;
-    }
+    const int half = R >> 1;
     float x[8];
     load_run8<DT>(q + d0, x);
-    if (d0 < R) {
-        const int half = R >> 1;
+    if (!wide) {  // element by element (static indices: the run stays in registers)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int d = d0 + i;
+            if (d < R) {
+                const bool first = d < half;
+                const int ci = first ? d : d - half;
+                const float o = Tr<DT>::tof(q[first ? d + half : ci]);
+                const float a = x[i] * cs[ci], b = o * sn[ci];
+                x[i] = first ? a - b : a + b;
+            }
+        }
+    } else if (d0 < R) {
         const bool first = d0 < half;
         const int ci = first ? d0 : d0 - half;
         float o[8], c[8], s[8];
@@ -264,22 +258,41 @@ __device__ inline void load_q(const DecodeParams& p, int row, int f, int hkv, QO
     const float *cs = p.cosv + co, *sn = p.sinv + co;
     const bool wide = (p.R & 15) == 0 &&
                       ((reinterpret_cast<uintptr_t>(p.cosv) | reinterpret_cast<uintptr_t>(p.sinv)) & 15) == 0;
+    o.l2 = p.l2scale;
+    if constexpr (DT == kF32) {
+        float x[4][8], amax = 0.0f;
 #pragma unroll
-    for (int cc = 0; cc < 4; ++cc) {
-        raw r[8];
-        compiler_fence();  // one run's loads at a time
-        rotated8<DT>(q, cs, sn, p.R, cc * 32 + g * 8, wide, r);
+        for (int cc = 0; cc < 4; ++cc) {
+            compiler_fence();  // one run's loads at a time
+            rotated8<DT>(q, cs, sn, p.R, cc * 32 + g * 8, wide, x[cc]);
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if constexpr (DT == kF32) {
-                uint32_t a[3], b[3];
-                split3(r[2 * t], a[0], a[1], a[2]);
-                split3(r[2 * t + 1], b[0], b[1], b[2]);
-#pragma unroll
-                for (int k = 0; k < 3; ++k) o.q[k][cc][t] = a[k] | (b[k] << 16);
-            } else {
-                o.q[0][cc][t] = (uint32_t)r[2 * t] | ((uint32_t)r[2 * t + 1] << 16);
+            for (int i = 0; i < 8; ++i) {
+                const float a = __builtin_fabsf(x[cc][i]);
+                amax = a < DV_INF && a > amax ? a : amax;
             }
+        }
+        amax = rows4_max(amax);
+        int k = 15 - __builtin_amdgcn_frexp_expf(amax);  // amax = m * 2^e, m in [0.5, 1); 0: e = 0
+        k = k < 100 ? k : 100;
+        o.l2 *= __builtin_amdgcn_ldexpf(1.0f, -k);
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const float a = __builtin_amdgcn_ldexpf(x[cc][2 * t], k), b = __builtin_amdgcn_ldexpf(x[cc][2 * t + 1], k);
+                const uint32_t hi = pack2<kF16>(a, b);
+                o.q[0][cc][t] = hi;
+                o.q[1][cc][t] = pack2<kF16>(a - Tr<kF16>::tof((uint16_t)(hi & 0xffffu)),
+                                            b - Tr<kF16>::tof((uint16_t)(hi >> 16)));
+            }
+    } else {
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+            raw r[8];
+            compiler_fence();
+            rotated8<DT>(q, cs, sn, p.R, cc * 32 + g * 8, wide, r);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) o.q[0][cc][t] = (uint32_t)r[2 * t] | ((uint32_t)r[2 * t + 1] << 16);
         }
     }
 }
@@ -327,32 +340,40 @@ struct State {
     float m, l;
 };
 
-// This lane's LDS offsets within a stage: K operand slice cc of row n (row 16 + n: 16 rows
-// further, same swizzle), V^T operand slice cc.
+// This lane's LDS offsets within a stage (128-byte aligned): K operand slice 0 of row n
+// (slice cc: ^ 32 cc; row 16 + n: 16 rows further, same swizzle), V^T operand slice 0
+// (slice cc: ^ 16 cc), exponents.
 struct ReadOff {
-    uint32_t k[4], v[8], s;
+    uint32_t k, v, s;
 };
 __device__ inline ReadOff read_offsets() {
     const int lane = threadIdx.x & 63;
     const int g = lane >> 4, n = lane & 15;
     ReadOff o;
-#pragma unroll
-    for (int cc = 0; cc < 4; ++cc)
-        o.k[cc] = (uint32_t)(n * kRowB + (((cc * 2 + (g >> 1)) ^ swz_k(n)) * 16) + (g & 1) * 8);
+    o.k = (uint32_t)(n * kRowB + (((g >> 1) ^ swz_k(n)) * 16) + (g & 1) * 8);
     // k = g * 8 + j <-> key (j / 4) * 16 + g * 4 + j % 4, as the scores' lanes hold them
     const int j = n >> 1;
     const int row = (j >> 2) * 16 + g * 4 + (j & 3);
-#pragma unroll
-    for (int cc = 0; cc < 8; ++cc) o.v[cc] = (uint32_t)(kTile + row * kRowB + ((cc ^ swz_v(row)) * 16) + (n & 1) * 8);
+    o.v = (uint32_t)(kTile + row * kRowB + swz_v(row) * 16 + (n & 1) * 8);
     o.s = (uint32_t)(2 * kTile + g * 16);
     return o;
 }
 
+// 2^(b - 127) of this lane's eight K (or, 128 bytes further, V) rows.
+__device__ inline void read_powers(uint32_t at, float (&f)[8]) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        const u32x4 a = lds_read16_at(at + (uint32_t)(kb * 64));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[kb * 4 + i] = power_of(a[i]);
+    }
+}
+
 // One stage for NT tiles: scores, softmax, O^T += V^T P^T.  okm: the stage's keys that hold
 // rows; mask[t]: those that tile t sees.
-template <int DT, int NT>
+template <int DT, int NT, bool kAcc>
 __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro, uint32_t okm,
-                               const uint32_t (&mask)[NT], const QOp<DT> (&q)[NT], float l2scale) {
+                               const uint32_t (&mask)[NT], const QOp<DT> (&q)[NT]) {
     f32x4 s[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -360,23 +381,15 @@ __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro
     for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
-            const u32x4 k = widen8<kKType<DT>>(lds_read8_at(slot + ro.k[cc] + (uint32_t)(kb * 16 * kRowB)));
+            const u32x4 k =
+                widen8<kKType<DT>>(lds_read8_at(((slot + ro.k) ^ (uint32_t)(cc * 32)) + (uint32_t)(kb * 16 * kRowB)));
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int j = 0; j < kQParts<DT>; ++j) s[t][kb] = Tr<kKType<DT>>::mma(k, q[t].q[j][cc], s[t][kb]);
         }
-    float ks[8], vs[8];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-        const u32x4 a = lds_read16_at(slot + ro.s + (uint32_t)(kb * 64));
-        const u32x4 b = lds_read16_at(slot + ro.s + (uint32_t)(128 + kb * 64));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            ks[kb * 4 + i] = power_of(a[i]);
-            vs[kb * 4 + i] = power_of(b[i]);
-        }
-    }
+    float ks[8];
+    read_powers(slot + ro.s, ks);
     POp<DT> pB[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -386,7 +399,9 @@ __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro
             s[t][1][i] *= ks[4 + i];
         }
         float pr[8];
-        softmax32<false>(st[t].o, st[t].m, st[t].l, s[t][0], s[t][1], mask[t], l2scale, pr);
+        softmax32<false>(st[t].o, st[t].m, st[t].l, s[t][0], s[t][1], mask[t], q[t].l2, pr);
+        float vs[8];
+        read_powers(slot + ro.s + 128, vs);
         pB[t] = p_scaled<DT>(pr, vs, st[t].l);
     }
     // a key that some tile sees and another does not takes part there with weight 0, which
@@ -400,7 +415,7 @@ __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int cc = 0; cc < 8; ++cc) {
-            const u32x4 v = widen8<kBF16>(lds_read_tr8_at(slot + ro.v[cc]));
+            const u32x4 v = widen8<kBF16>(lds_read_tr8_at((slot + ro.v) ^ (uint32_t)(cc * 16)));
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 const uint32_t mg = mask[t] >> (g * 4);
@@ -417,7 +432,7 @@ __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro
     } else {
 #pragma unroll
         for (int cc = 0; cc < 8; ++cc) {
-            const u32x4 v = widen8<kBF16>(lds_read_tr8_at(slot + ro.v[cc]));
+            const u32x4 v = widen8<kBF16>(lds_read_tr8_at((slot + ro.v) ^ (uint32_t)(cc * 16)));
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -426,8 +441,8 @@ __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        if constexpr (kWavesPerCu<NT> == 8) mfma_settle(st[t].o);
-        else mfma_settle_acc(st[t].o);
+        if constexpr (kAcc) mfma_settle_acc(st[t].o);
+        else mfma_settle(st[t].o);
     }
 }
 
@@ -484,27 +499,28 @@ __device__ inline long long group_visible(const DecodeParams& p, int rg) {
 }
 
 // One wave: KV head hkv over visible keys [v0, v1) of one row group.
-template <int DT, int QM, int RM, int NT, bool MV, bool P2>
+// NT tiles, of a launch whose groups hold up to GT tokens.
+template <int DT, int QM, int RM, int NT, int GT, bool MV, bool P2>
 __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds, int rg, int hkv, long long v0,
                                       long long v1, bool final_out, int slot, int wv, long long row_keys) {
-    constexpr int R = kRing<NT>;
+    constexpr int R = kRing<DT, GT>;
     const int lane = threadIdx.x & 63;
     const int g = lane >> 4, n = lane & 15;
     const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_addr(wlds));
     int* pc = reinterpret_cast<int*>(wlds + R * kStage);
     Group gr;
-    if constexpr (NT == 1) {
+    if constexpr (GT == 1) {
         gr.w = RM == kRowVarlen ? varlen_seq(p, rg) : rg / p.S;
         gr.lin = rg;
         gr.ntok = 1;
     } else {
-        gr = group_of<RM, NT>(p, rg);
+        gr = group_of<RM, GT>(p, rg);
         gr.w = uniform(gr.w);
         gr.lin = uniform(gr.lin);
         gr.ntok = uniform(gr.ntok);
     }
     const int w = gr.w;
-    const LaneOff lo = lane_offsets(p);
+    const uint32_t lo = lane_offset(p);
     const ReadOff ro = read_offsets();
 
     State st[NT];
@@ -552,7 +568,7 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
             for (int k = 0; k < R; ++k) m[k] = 0;
 #pragma unroll 1
             for (int k = 0; k < R && k < ns; ++k) {
-                const uint32_t x = issue<P2, (NT > 1)>(p, v, lo, pc, ring + (uint32_t)(k * kStage), sa + k * kStep);
+                const uint32_t x = issue<P2, (GT > 1)>(p, v, lo, pc, ring + (uint32_t)(k * kStage), sa + k * kStep);
 #pragma unroll
                 for (int j = 0; j < R; ++j) m[j] = j == k ? x : m[j];
             }
@@ -585,12 +601,12 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
                         mask[t] &= lim >= kStep ? 0xffffffffu : lim <= 0 ? 0u : (1u << lim) - 1u;
                     }
                 }
-                compute<DT, NT>(st, ring + (uint32_t)(cur * kStage), ro, m[0], mask, q, p.l2scale);
+                compute<DT, NT, kWavesPerCu<DT, GT> == 4>(st, ring + (uint32_t)(cur * kStage), ro, m[0], mask, q);
 #pragma unroll
                 for (int k = 0; k + 1 < R; ++k) m[k] = m[k + 1];
                 lds_wait();  // the slot's reads are complete before it is refilled
                 if (s + R < ns)
-                    m[R - 1] = issue<P2, (NT > 1)>(p, v, lo, pc, ring + (uint32_t)(cur * kStage), sa + (s + R) * kStep);
+                    m[R - 1] = issue<P2, (GT > 1)>(p, v, lo, pc, ring + (uint32_t)(cur * kStage), sa + (s + R) * kStep);
                 cur = cur + 1 == R ? 0 : cur + 1;
             }
             sa = sb;
@@ -598,7 +614,7 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
     };
     if constexpr (!MV) {
         if (v0 < v1) one_view(0, (int)row_keys, 0ll, 0ll);
-    } else if constexpr (NT == 1) {
+    } else if constexpr (GT == 1) {
         if (v0 < v1)
             for_views_blocks<kKvPaged, RM>(p, rg, v0, v1, [&](int f, int vis, long long P, long long off) {
                 one_view(f, uniform(vis), uniform(P), uniform(off));
@@ -606,7 +622,7 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
     } else {
         long long P = 0, off = 0;
         for (int f = 0; f < p.F && P < v1; ++f) {
-            const int vis = uniform(group_view_vis<RM, NT>(p, f, gr));
+            const int vis = uniform(group_view_vis<RM, GT>(p, f, gr));
             if (vis > 0 && P + vis > v0) one_view(f, vis, P, off);
             P += vis;
             off += p.fl[f];
@@ -641,7 +657,7 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
                                                              pack2<DT>(st[t].o[c][2] * scale, st[t].o[c][3] * scale)};
             }
         } else {
-            store_partial<DT>(p.part + (long long)slot * p.slot_floats, p.hpw * NT * kGqa, (wv * NT + t) * kGqa + n, g,
+            store_partial<DT>(p.part + (long long)slot * p.slot_floats, p.hpw * GT * kGqa, (wv * GT + t) * kGqa + n, g,
                               st[t].o, inv, row_lse(st[t].m, lt));
         }
     }
@@ -652,19 +668,26 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
 // MV: calls of several views (or none), whose pieces may start anywhere.  P2: pages of a
 // power of two of at least 16 rows (NT > 1: looked up, one kernel for all calls).
 template <int DT, int QM, int RM, int NT, bool MV, bool P2>
-__global__ __launch_bounds__((q8::kWavesPerCu<NT> * kWave)) void dv_decode8(const DecodeParams p) {
-    extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ long long s_scan[q8::kWavesPerCu<NT>];
+__global__ __launch_bounds__((q8::kWavesPerCu<DT, NT> * kWave)) void dv_decode8(const DecodeParams p) {
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((128u - (lds_addr(smem_raw) & 127u)) & 127u);  // (ReadOff)
+    __shared__ long long s_scan[q8::kWavesPerCu<DT, NT>];
     const int wv = uniform((int)(threadIdx.x >> 6));
     const int HPW = p.hpw;
-    long long* s_pref = reinterpret_cast<long long*>(smem + HPW * q8::kWaveLds<NT>);
-    unsigned char* wlds = smem + wv * q8::kWaveLds<NT>;
+    long long* s_pref = reinterpret_cast<long long*>(smem + HPW * q8::kWaveLds<DT, NT>);
+    unsigned char* wlds = smem + wv * q8::kWaveLds<DT, NT>;
     run_schedule<true, MV ? 1 : kStep, 1, NT == 1>(
         p, p.Hkv / HPW, s_pref, s_scan, [&](int row) { return q8::group_visible<RM, NT>(p, row); },
         [&](int row, int hg, long long v0, long long v1, bool fin, int slot, long long rk) {
-            if (wv < HPW)
-                q8::piece<DT, QM, RM, NT, MV, P2>(p, wlds, uniform(row), uniform(hg) * HPW + wv, uniform(v0),
-                                                  uniform(v1), uniform((int)fin) != 0, uniform(slot), wv, uniform(rk));
+            if (wv >= HPW) return;
+            const int h = uniform(hg) * HPW + wv;
+            // packed calls mix groups of one token with others
+            if (RM == kRowVarlen && NT == 2 && uniform(q8::group_of<RM, NT>(p, row).ntok) == 1)
+                q8::piece<DT, QM, RM, 1, NT, MV, P2>(p, wlds, uniform(row), h, uniform(v0), uniform(v1),
+                                                     uniform((int)fin) != 0, uniform(slot), wv, uniform(rk));
+            else
+                q8::piece<DT, QM, RM, NT, NT, MV, P2>(p, wlds, uniform(row), h, uniform(v0), uniform(v1),
+                                                      uniform((int)fin) != 0, uniform(slot), wv, uniform(rk));
         });
 }
 
@@ -699,7 +722,7 @@ hipError_t launch8_one(DecodeParams p, int device, long long cap, int cus, hipSt
     const void* kern = reinterpret_cast<const void*>(&dv_decode8<DT, QM, RM, NT, MV, P2>);
     // (up to 64 rows the schedule's sums stay in registers)
     auto lds_of = [](int hpw, int nrows) {
-        return (size_t)hpw * q8::kWaveLds<NT> + (nrows > kWave ? (size_t)(nrows + 1) * sizeof(long long) : 0);
+        return 128 + (size_t)hpw * q8::kWaveLds<DT, NT> + (nrows > kWave ? (size_t)(nrows + 1) * sizeof(long long) : 0);
     };
     static std::atomic<unsigned long long> attr_done{0};
     hipError_t e = once_per_device(attr_done, device, [&] {
@@ -710,7 +733,7 @@ hipError_t launch8_one(DecodeParams p, int device, long long cap, int cus, hipSt
     // workgroups that are all resident at once
     const size_t lds = lds_of(p.hpw, p.nrows);
     const int fit = (int)(160 * 1024 / (lds + 512));
-    const int most = q8::kWavesPerCu<NT> / p.hpw;
+    const int most = q8::kWavesPerCu<DT, NT> / p.hpw;
     const long long nwg = (long long)cus * (fit < most ? fit : most);
     p.nwg = (int)(nwg < cap ? nwg : cap < 1 ? 1 : cap);
     hipLaunchKernelGGL((dv_decode8<DT, QM, RM, NT, MV, P2>), dim3(p.nwg), dim3(p.hpw * kWave), lds, stream, p);
@@ -725,8 +748,8 @@ hipError_t launch8_one(DecodeParams p, int device, long long cap, int cus, hipSt
     }
 }
 
-// Calls of groups of four tokens (dv_decode8m.hip).
-hipError_t launch_decode8_four(int dtype, bool varlen, const DecodeParams& p, int device, long long cap, int cus,
+// Calls whose waves have a SIMD to themselves (dv_decode8m.hip).
+hipError_t launch_decode8_wide(int dtype, bool varlen, const DecodeParams& p, int device, long long cap, int cus,
                                hipStream_t stream);
 
 }  // namespace dv

@@ -19,14 +19,14 @@ hipError_t launch8_row(const DecodeParams& p, int device, long long cap, int cus
 template <int DT>
 hipError_t launch8(bool varlen, int nt, const DecodeParams& p, int device, long long cap, int cus,
                    hipStream_t stream) {
-    if (nt == 4) return launch_decode8_four(DT, varlen, p, device, cap, cus, stream);
+    if (q8::waves_per_cu(DT, nt) == 4) return launch_decode8_wide(DT, varlen, p, device, cap, cus, stream);
     if (nt == 1)
         return varlen ? launch8_row<DT, kQRotHalf, kRowVarlen>(p, device, cap, cus, stream)
                       : launch8_row<DT, kQRotFull, kRowWS>(p, device, cap, cus, stream);
-    if constexpr (DT == kF32)  // (16-bit varlen groups are of four tokens)
-        if (varlen) return launch8_one<DT, kQRotHalf, kRowVarlen, 2, true, true>(p, device, cap, cus, stream);
-    return varlen ? hipErrorInvalidValue
-                  : launch8_one<DT, kQRotFull, kRowWS, 2, true, true>(p, device, cap, cus, stream);
+    if constexpr (DT != kF32)
+        return varlen ? launch8_one<DT, kQRotHalf, kRowVarlen, 2, true, true>(p, device, cap, cus, stream)
+                      : launch8_one<DT, kQRotFull, kRowWS, 2, true, true>(p, device, cap, cus, stream);
+    return hipErrorInvalidValue;
 }
 
 // Workspace of a call: partial slots (of the workgroups, and one per segment), then the
@@ -48,8 +48,8 @@ Ws8 ws8(long long groups, int nt, int Hkv, int device) {
 // then lie side by side in memory as a workgroup reads them (32 sequences of 1k - 8k
 // tokens, 8 KV heads: 62.6 -> 60.6 us, 4 x 131072: 191 -> 184), unless the call is too
 // small to fill the chip so (one sequence of 3001 tokens: 11.0 us with four, 13.3).
-int pick_hpw8(long long groups, long long max_keys, int nt, int Hkv, int cus) {
-    if (Hkv % 8 == 0 && nt <= 2 && groups <= 1024 && groups * max_keys >= 256ll * cus) return 8;
+int pick_hpw8(int dtype, long long groups, long long max_keys, int nt, int Hkv, int cus) {
+    if (Hkv % 8 == 0 && q8::waves_per_cu(dtype, nt) == 8 && groups <= 1024 && groups * max_keys >= 256ll * cus) return 8;
     return pick_hpw(Hkv);
 }
 
@@ -67,7 +67,7 @@ hipError_t launch_decode8(int dtype, bool varlen, int nt, const DecodeParams& ba
     const Ws8 l = ws8(groups, nt, base.Hkv, device);
     const int cus = device_cu_count(device);
     DecodeParams p = base;
-    p.hpw = pick_hpw8(groups, max_keys_per_row, nt, p.Hkv, cus);
+    p.hpw = pick_hpw8(dtype, groups, max_keys_per_row, nt, p.Hkv, cus);
     const int nhg = p.Hkv / p.hpw;
     p.slot_floats = p.hpw * nt * kGqa * (kHeadDim + 1);
     p.part = reinterpret_cast<float*>(workspace);
@@ -97,10 +97,12 @@ hipError_t launch_decode8(int dtype, bool varlen, int nt, const DecodeParams& ba
 // other (K and V are read once for them): up to four, in fp32 two.  16-bit calls of more
 // go through the multi-query kernel, 16 tokens to a workgroup.  Packed calls of two or
 // more tokens per sequence are cut into row groups on the device; in 16-bit types those of
-// up to four tokens and those of more are two launches.
+// up to four tokens (two to a wave, whose kernel has eight waves to a CU: most are decodes of
+// one token) and those of more are two launches.
 namespace {
 
 constexpr int kGroupTok = 16;  // tokens of a table entry (dv_varlen_groups)
+constexpr int kFewTokens = 4;  // of an entry that the 16-bit multi-query kernel leaves to the decode kernel
 
 struct Plan8 {
     bool table;                // varlen row groups
@@ -119,8 +121,8 @@ Plan8 plan8(int dtype, bool varlen, int W, int S_or_T, int Hkv, int device) {
         q.table = true;
         q.groups = (long long)S_or_T / kGroupTok + W + 1;
         q.table_bytes = (size_t)q.groups * 16;
-        q.nt = dtype == kF32 ? 2 : 4;
-        q.sub = dtype == kF32 ? kGroupTok / 2 : 1;
+        q.nt = 2;
+        q.sub = (dtype == kF32 ? kGroupTok : kFewTokens) / 2;
         q.chunk = dtype != kF32;
     } else if (varlen) {
         q.nt = 1;
