@@ -248,6 +248,8 @@ struct Append8Params {
     int W, S, Hkv, R;
     int bs, nblocks;
     int tile;                 // tokens of a workgroup
+    int apart;                // tiles between those of workgroups in a row
+    int team;                 // waves that share a run of many rows
     int vec;                  // 1: rows, tables and strides allow 16-byte loads
 };
 

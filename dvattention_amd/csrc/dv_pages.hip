@@ -3,12 +3,17 @@
 //    from the sequences' lengths and a stack of free pages.
 //  * dv_kv_append8   -- new keys (rotated) and values rounded to E4M3 in their slots, one
 //    power-of-two scale per page and KV head.
+#include <type_traits>
+
 #include "dv_common.h"
 #include "dv_device.h"
 
 namespace dv {
 
 namespace {
+
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
+typedef __attribute__((ext_vector_type(2))) short i16x2;
 
 // ---- block tables ------------------------------------------------------------------
 //
@@ -227,85 +232,328 @@ __device__ inline float round_to(float f) {
     return Tr<DT>::tof(Tr<DT>::fromf(f));
 }
 
-// Eight elements of X as floats, 16 bytes at a time where `vec` says they are aligned.
+// fp16: magnitudes above 61440 are held as 61440 (the next E4M3 number, 65536, is none of
+// fp16); infinities are no E4M3 numbers and become NaN.
 template <int DT>
-__device__ inline void load8(const typename Tr<DT>::raw* x, bool vec, float (&f)[8]) {
-    using raw = typename Tr<DT>::raw;
-    raw r[8];
-    if (vec) {
-        constexpr int V = (int)sizeof(r) / 16;
-        u32x4 t[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) t[i] = ld16(reinterpret_cast<const unsigned char*>(x) + 16 * i);
-        __builtin_memcpy(r, t, sizeof(r));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r[i] = x[i];
+__device__ inline float storable(float x) {
+    const float a = __builtin_fabsf(x);
+    if constexpr (DT == kF16) {
+        if (a > 61440.0f && a < DV_INF) x = __builtin_copysignf(61440.0f, x);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Tr<DT>::tof(r[i]);
+    return a < DV_INF ? x : __builtin_nanf("");
 }
 
-// Dims [d0, d0 + 8) of token t's key (rotated as dv_kv_append does, PyTorch's rounding) or
-// value for head h, as the storage type holds them.
-template <int DT, int CDT, bool K>
-__device__ inline void load_row8(const Append8Params& p, int t, int h, int d0, float (&x)[8]) {
+// Eight elements that are held under an exponent that is too small, rounded again under one
+// larger by -down.
+__device__ inline void raise_row(unsigned char* at, int down) {
+    u32x2* row = reinterpret_cast<u32x2*>(at);
+    float y[8];
+    from_fp8(*row, y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_ldexpf(y[e], down);
+    *row = to_fp8(y);
+}
+
+// One element of a rotated key, evaluated as PyTorch does in the rows' type.
+template <int DT, int CDT>
+__device__ inline float turn(float v, float o, float c, float sn, bool first) {
 #pragma clang fp contract(off)
+    float a = v * c, b = o * (first ? -sn : sn);
+    if constexpr (DT != kF32 && CDT != kF32) {
+        a = round_to<DT>(a);
+        b = round_to<DT>(b);
+    }
+    return round_to<DT>(a + b);
+}
+
+// Dims d0 and d0 + 1 of token t's key (rotated) or value for head h.
+template <int DT, int CDT>
+__device__ inline void load_pair(const Append8Params& p, bool isk, int t, int h, int d0, float (&x)[2]) {
     using raw = typename Tr<DT>::raw;
     using craw = typename Tr<CDT>::raw;
     const int w = t / p.S, s = t - w * p.S;
-    const long long* st = K ? p.kst : p.vst;
-    const raw* row = reinterpret_cast<const raw*>(K ? p.k : p.v) + w * st[0] + h * st[1] + s * st[2];
-    load8<DT>(row + d0, p.vec, x);
-    if constexpr (K) {
-        if (d0 < p.R) {
-            constexpr bool kF32Math = DT == kF32 || CDT == kF32;
-            const int half = p.R >> 1;
-            const long long co = w * p.cs[0] + s * p.cs[1];
-            const craw* cr = reinterpret_cast<const craw*>(p.cosv) + co;
-            const craw* sr = reinterpret_cast<const craw*>(p.sinv) + co;
-            auto turn = [&](float v, float o, float c, float sn, bool first) {
-                float a = v * c, b = o * sn;
-                if constexpr (!kF32Math) {
-                    a = round_to<DT>(a);
-                    b = round_to<DT>(b);
-                }
-                return round_to<DT>(first ? a - b : a + b);
-            };
-            if ((half & 7) == 0) {  // the run lies in one half
-                const bool first = d0 < half;
-                float o[8], c[8], sn[8];
-                load8<DT>(row + (first ? d0 + half : d0 - half), p.vec, o);
-                load8<CDT>(cr + d0, p.vec, c);
-                load8<CDT>(sr + d0, p.vec, sn);
+    const long long* st = isk ? p.kst : p.vst;
+    const raw* row = reinterpret_cast<const raw*>(isk ? p.k : p.v) + w * st[0] + h * st[1] + s * st[2];
+    const long long co = w * p.cs[0] + s * p.cs[1];
+    const int half = p.R >> 1;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = turn(x[i], o[i], c[i], sn[i], first);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int d = d0 + i;
-                    if (d >= p.R) continue;
-                    const bool first = d < half;
-                    const float o = Tr<DT>::tof(row[first ? d + half : d - half]);
-                    x[i] = turn(x[i], o, Tr<CDT>::tof(cr[d]), Tr<CDT>::tof(sr[d]), first);
-                }
-            }
+    for (int i = 0; i < 2; ++i) {
+        const int d = d0 + i;
+        x[i] = Tr<DT>::tof(row[d]);
+        if (isk && d < p.R) {
+            const bool first = d < half;
+            x[i] = turn<DT, CDT>(x[i], Tr<DT>::tof(row[first ? d + half : d - half]),
+                                 Tr<CDT>::tof(reinterpret_cast<const craw*>(p.cosv)[co + d]),
+                                 Tr<CDT>::tof(reinterpret_cast<const craw*>(p.sinv)[co + d]), first);
         }
-    }
-    // fp16: magnitudes above 61440 are held as 61440 (the next E4M3 number, 65536, is
-    // none of fp16); infinities are no E4M3 numbers and become NaN
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = __builtin_fabsf(x[i]);
-        if constexpr (DT == kF16) {
-            if (a > 61440.0f && a < DV_INF) x[i] = __builtin_copysignf(61440.0f, x[i]);
-        }
-        if (!(a < DV_INF)) x[i] = __builtin_nanf("");
+        x[i] = storable<DT>(x[i]);
     }
 }
 
-constexpr int kAppWaves = 16;     // most waves of a workgroup
-constexpr int kAppRows = 16;      // rows of a page that a wave holds in registers: 4 passes of 4
+// Eight elements of a row as its type has them, in whole 16-byte words.
+template <int DT>
+struct Row8 {
+    static constexpr int kWords = (int)sizeof(typename Tr<DT>::raw) * 2;
+    uint32_t w[kWords];
+    __device__ inline void load(const unsigned char* base, uint32_t off) {
+#pragma unroll
+        for (int i = 0; i < kWords / 4; ++i) {
+            const u32x4 v = ld16(base + off + 16 * i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[4 * i + j] = v[j];
+        }
+    }
+    __device__ inline float at(int i) const {
+        if constexpr (DT == kF32) return __uint_as_float(w[i]);
+        else return Tr<DT>::tof((uint16_t)(w[i >> 1] >> (16 * (i & 1))));
+    }
+    // magnitudes, as integers of the type's width (which order like them), folded into m
+    __device__ inline void fold(uint32_t& m) const {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (DT == kF32) {
+                const uint32_t u = w[i] & 0x7fffffffu;
+                m = u > m ? u : m;
+            } else {
+                const u16x2 u = __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu);
+                m = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m), u));
+            }
+        }
+    }
+    // the same over finite ones; fp16: magnitudes above 61440 become that
+    __device__ inline void fold_finite(uint32_t& m) {
+        constexpr uint32_t kInf = DT == kF32 ? 0x7f800000u : DT == kF16 ? 0x7c00u : 0x7f80u;
+        constexpr int kPer = DT == kF32 ? 1 : 2, kBits = 32 / kPer;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i)
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                uint32_t u = (w[i] >> (kBits * j)) & (DT == kF32 ? 0x7fffffffu : 0x7fffu);
+                if constexpr (DT == kF16) {
+                    if (u > 0x7b80u && u < kInf) {
+                        w[i] = (w[i] & ~(0x7fffu << (kBits * j))) | (0x7b80u << (kBits * j));
+                        u = 0x7b80u;
+                    }
+                }
+                m = u < kInf && u > m ? u : m;
+            }
+    }
+    // E4M3 bytes of the elements times 2^(127 - b), ties to even: magnitudes are at most
+    // 448 then, infinities and NaN become NaN
+    __device__ inline u32x2 bytes(int b) const {
+        if constexpr (DT == kF32) {
+            const float f = __uint_as_float((uint32_t)(254 - b) << 23);
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(w[e]) * f;
+            return to_fp8(y);
+        } else {
+            const float f = __uint_as_float((uint32_t)b << 23);  // (these divide)
+            u32x2 r;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                i16x2 o = {0, 0};
+                if constexpr (DT == kBF16) {
+                    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, __builtin_bit_cast(bf16x2, w[2 * i]), f, false);
+                    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(o, __builtin_bit_cast(bf16x2, w[2 * i + 1]), f, true);
+                } else {
+                    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, __builtin_bit_cast(f16x2, w[2 * i]), f, false);
+                    o = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(o, __builtin_bit_cast(f16x2, w[2 * i + 1]), f, true);
+                }
+                r[i] = __builtin_bit_cast(uint32_t, o);
+            }
+            return r;
+        }
+    }
+};
+
+// The largest magnitude that fold() may find without a look at single elements, and a
+// folded magnitude as a float.
+template <int DT>
+__device__ inline bool beyond(uint32_t m) {
+    if constexpr (DT == kF32) return m > 0x7f7fffffu;
+    const uint32_t k = DT == kF16 ? 0x7b80u : 0x7f7fu;
+    return (m & 0xffffu) > k || (m >> 16) > k;
+}
+
+// x rotated where `rot`: o holds the elements half a rotation away, c and sn the angles.
+template <int DT, int CDT>
+__device__ inline void rotate8(Row8<DT>& x, const Row8<DT>& o, const Row8<CDT>& c, const Row8<CDT>& sn, bool first,
+                               bool rot) {
+#pragma clang fp contract(off)
+    if constexpr (DT == kF32) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t y = __float_as_uint(turn<DT, CDT>(x.at(i), o.at(i), c.at(i), sn.at(i), first));
+            x.w[i] = rot ? y : x.w[i];
+        }
+    } else if constexpr (DT == kF16 && CDT == kF16) {
+        // products and sum in their own type: what rounding the exact products, and the
+        // sum in 24 bits, to 11 bits gives as well
+        const uint32_t flip = first ? 0x80008000u : 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f16x2 a = __builtin_bit_cast(f16x2, x.w[i]) * __builtin_bit_cast(f16x2, c.w[i]);
+            const f16x2 b = __builtin_bit_cast(f16x2, o.w[i]) * __builtin_bit_cast(f16x2, sn.w[i] ^ flip);
+            const uint32_t y = __builtin_bit_cast(uint32_t, a + b);
+            x.w[i] = rot ? y : x.w[i];
+        }
+    } else {
+        using T2 = std::conditional_t<DT == kBF16, bf16x2, f16x2>;
+        using T1 = std::conditional_t<DT == kBF16, __bf16, _Float16>;
+        const uint32_t flip = first ? 0x80000000u : 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float a[2], b[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                a[j] = x.at(2 * i + j) * c.at(2 * i + j);
+                b[j] = o.at(2 * i + j) * __uint_as_float(__float_as_uint(sn.at(2 * i + j)) ^ flip);
+            }
+            if constexpr (CDT != kF32) {
+                const T2 ra = {(T1)a[0], (T1)a[1]}, rb = {(T1)b[0], (T1)b[1]};
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    a[j] = (float)ra[j];
+                    b[j] = (float)rb[j];
+                }
+            }
+            const T2 y = {(T1)(a[0] + b[0]), (T1)(a[1] + b[1])};
+            x.w[i] = rot ? __builtin_bit_cast(uint32_t, y) : x.w[i];
+        }
+    }
+}
+
+// The exponent byte of a page with the byte `old` after rows of magnitude m (see fold) were
+// written, row 0 among them where `first_row`.
+template <int DT>
+__device__ inline int exponent_after(uint32_t m, bool first_row, int old) {
+    if constexpr (DT != kF32) m = (m & 0xffffu) > (m >> 16) ? m & 0xffffu : m >> 16;
+    const float amax = DT == kF32 ? __uint_as_float(m) : Tr<DT>::tof((typename Tr<DT>::raw)m);
+    const int want = exponent_of(amax);
+    return first_row || old == 255 || want > old ? want : old;
+}
+
+constexpr int kAppRows = 16;      // most rows of a page that a wave holds in registers: 4 times 4
+
+// Tokens that have their pages to themselves, rows and angles in whole 16-byte words, 16
+// lanes a row.  kPass > 0: the run's rows [row0, row0 + n) of one KV head, kPass * 4 at
+// once, without a branch (those behind the run's end repeat its last row).  kPass = 0: one
+// row of four KV heads from h on.  cache, sc: the page's bytes and exponents of head h.
+// `team` waves share a run, the caller being the rank-th of them: s_max has their largest
+// magnitudes, and all waves of the workgroup come here (store: false where only for that).
+template <int DT, int CDT, bool kTurn, int kPass>
+__device__ inline void write_run(const Append8Params& p, bool isk, int t, int row0, int n, int h, int lane,
+                                 unsigned char* cache, unsigned char* sc, int team = 1, int rank = 0,
+                                 uint32_t* s_max = nullptr, bool store = true) {
+    constexpr bool kHeads = kPass == 0;
+    constexpr int kQ = kHeads ? 1 : kPass, kRows = 4 * kQ;
+    constexpr uint32_t kEs = sizeof(typename Tr<DT>::raw), kCs = sizeof(typename Tr<CDT>::raw);
+    asm("" : "+v"(lane));  // (else lane offsets are held in registers over all units)
+    const int g = lane >> 4, d0 = (lane & 15) * 8;
+    const long long rstride = (long long)p.Hkv << 7;
+    // (a head behind the last one repeats the last)
+    const int hg = kHeads ? (h + g < p.Hkv ? g : p.Hkv - 1 - h) : 0;
+    const int old = sc[hg];
+    const int w = t / p.S, sq = t - w * p.S;
+    const long long* st = isk ? p.kst : p.vst;
+    const unsigned char* src = reinterpret_cast<const unsigned char*>(isk ? p.k : p.v) +
+                               (w * st[0] + h * st[1] + sq * st[2]) * (long long)kEs;
+    const unsigned char* ac = reinterpret_cast<const unsigned char*>(p.cosv);
+    const unsigned char* as = reinterpret_cast<const unsigned char*>(p.sinv);
+    const long long ao = (w * p.cs[0] + sq * p.cs[1]) * (long long)kCs;
+    const int half = p.R >> 1;
+    const bool rot = kTurn && d0 < p.R, first = d0 < half;
+    // byte offsets of a lane's row and of its angles; rows are less than 2^27 bytes apart
+    const uint32_t rs = (uint32_t)((kHeads ? st[1] : st[2]) * kEs), cs = (uint32_t)(p.cs[1] * kCs);
+    const uint32_t lx = d0 * kEs, lo = (rot ? first ? d0 + half : d0 - half : d0) * kEs, lc = (rot ? d0 : 0) * kCs;
+    Row8<DT> x[kQ];
+    auto load_block = [&](int rb) {
+        Row8<DT> o[kQ];
+        Row8<CDT> c[kQ], sn[kQ];
+        const unsigned char* at = src + rb * (long long)rs;
+        const unsigned char* atc = ac + ao + rb * (long long)cs;
+        const unsigned char* ats = as + ao + rb * (long long)cs;
+        const int last = n - 1 - rb;
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+            const uint32_t r = kHeads ? hg : q * 4 + g < last ? q * 4 + g : last;
+            x[q].load(at, r * rs + lx);
+            if constexpr (kTurn) {
+                const uint32_t ro = kHeads ? lc : r * cs + lc;
+                o[q].load(at, r * rs + lo);
+                c[q].load(atc, ro);
+                sn[q].load(ats, ro);
+            }
+        }
+        uint32_t m = 0;
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+            if constexpr (kTurn) rotate8<DT, CDT>(x[q], o[q], c[q], sn[q], first, rot);
+            x[q].fold(m);
+        }
+        if (ballot(beyond<DT>(m))) {  // rare
+            m = 0;
+#pragma unroll
+            for (int q = 0; q < kQ; ++q) x[q].fold_finite(m);
+        }
+        return m;
+    };
+    auto larger = [](uint32_t a, uint32_t b) {
+        if constexpr (DT == kF32) return a > b ? a : b;
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                      __builtin_bit_cast(u16x2, b)));
+    };
+    uint32_t m = 0;
+    const int rb0 = rank * kRows, rstep = team * kRows;
+    if constexpr (kHeads) m = load_block(0);
+    else
+        for (int rb = rb0; rb < n; rb += rstep) m = larger(m, load_block(rb));
+#pragma unroll
+    for (int d = 1; d < (kHeads ? 16 : kWave); d <<= 1) m = larger(m, (uint32_t)__shfl_xor((int)m, d, kWave));
+    if (team > 1) {
+        if (lane == 0) s_max[rank] = m;
+        __syncthreads();
+        m = 0;
+        for (int i = 0; i < team; ++i) m = larger(m, s_max[i]);
+        if (!store) return;
+    }
+    const int b = exponent_after<DT>(m, row0 == 0, old);
+    const bool mine = !kHeads || hg == g;
+    const bool raise = b > old && row0 != 0 && old != 255;
+    if constexpr (kHeads) {
+        if (ballot(raise)) {
+            for (int r = 0; r < p.bs; ++r)
+                if (raise && mine && r != row0) raise_row(cache + r * rstride + (g << 7) + d0, old - b);
+        }
+    } else if (raise) {
+        for (int r = rank * 4 + g; r < p.bs; r += team * 4)
+            if (r < row0 || r >= row0 + n) raise_row(cache + r * rstride + d0, old - b);
+    }
+    const uint32_t rnext = kHeads ? 128u : (uint32_t)rstride;
+    auto store_block = [&](int rb) {
+#pragma unroll
+        for (int q = 0; q < kQ; ++q) {
+            const uint32_t r = q * 4 + g;
+            const u32x2 y = x[q].bytes(b);
+            if (kHeads ? mine : (int)r < n - rb)
+                *reinterpret_cast<u32x2*>(cache + (row0 + rb) * rstride + (r * rnext + d0)) = y;
+        }
+    };
+    if (kHeads || n <= rstep) {
+        store_block(rb0);
+    } else {
+        for (int rb = rb0; rb < n; rb += rstep) {
+            load_block(rb);
+            store_block(rb);
+        }
+    }
+    if ((lane & (kHeads ? 15 : 63)) == 0 && rank == 0 && mine && b != old) sc[hg] = (unsigned char)b;
+}
+
+constexpr int kAppWaves = 8;      // most waves of a workgroup
+constexpr int kAppTile = 32;      // most tokens of a workgroup
+constexpr int kAppScan = 8;       // slots that a thread compares at a time
 
 }  // namespace
 
@@ -317,147 +565,181 @@ constexpr int kAppRows = 16;      // rows of a page that a wave holds in registe
 // few bytes beside the rows), and where other tokens of the page exist -- a page in
 // several runs, a slot named twice -- the first token's workgroup writes them all, the
 // last token of a slot winning.
+//
+// Bound by its chain of dependent reads while the call is small: slots (the tile's and
+// those compared, read together), then rows, angles and exponents together.
 template <int DT, int CDT>
-__global__ __launch_bounds__(kAppWaves * kWave) void dv_kv_append8(const Append8Params p, int T) {
-    __shared__ int s_run[64];      // first tokens of the runs
-    __shared__ int s_nrun;
-    __shared__ int s_other[64];    // 1: the run's page has tokens outside it; 2: earlier ones
+__global__ __launch_bounds__(kAppWaves * kWave, DT == kF32 || CDT == kF32 ? 2 : 4)
+void dv_kv_append8(const Append8Params p, int T) {
+    __shared__ uint32_t s_max[2][kAppWaves];
+    __shared__ int s_other[kAppTile];  // 1: the run's page has tokens outside it; 2: earlier ones
     const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), nthreads = blockDim.x;
     const long long nslots = (long long)p.nblocks * p.bs;
-    const int t0 = blockIdx.x * p.tile;
-    auto slot_at = [&](int t) {
-        const long long s = p.slots[t];
-        return s >= 0 && s < nslots ? s : -1;
-    };
-    // 1. runs of the tile (at most 64 tokens: one wave)
-    if (wv == 0) {
-        const int t = t0 + lane;
-        bool start = false;
-        if (lane < p.tile && t < T) {
-            const long long s = slot_at(t);
-            const long long before = t > 0 ? slot_at(t - 1) : -1;
-            start = s >= 0 && (before < 0 || s != before + 1 || s % p.bs == 0);
-        }
-        const uint64_t m = ballot(start);
-        if (start) s_run[__builtin_popcountll(m & ((1ull << lane) - 1ull))] = t;
-        if (lane == 0) s_nrun = __builtin_popcountll(m);
-        s_other[lane] = 0;
+    const bool small = nslots <= 0xffffffffll;
+    auto row_of = [&](long long s) { return small ? (int)((uint32_t)s % (uint32_t)p.bs) : (int)(s % p.bs); };
+    // workgroups in a row take tiles a page apart: runs recur at that distance, and
+    // workgroups go round the XCDs and CUs, some of which would else find runs only
+    const int groups = (int)gridDim.x / p.apart;
+    const int t0 = ((int)blockIdx.x % groups * p.apart + (int)blockIdx.x / groups) * p.tile;
+    if (t0 >= T) return;
+    // lane i of each wave: the slot of token t0 - 1 + i
+    long long win = -1;
+    {
+        const int t = t0 - 1 + lane;
+        if (t >= 0 && t < T) win = p.slots[t];
     }
+    long long sl[kAppScan];
+    auto load_scan = [&](int c) {
+#pragma unroll
+        for (int j = 0; j < kAppScan; ++j) {
+            const int u = c + j * nthreads + tid;
+            sl[j] = p.slots[u < T ? u : T - 1];
+        }
+    };
+    load_scan(0);
+    if (tid < kAppTile) s_other[tid] = 0;
     __syncthreads();
-    const int nrun = s_nrun;
+    // 1. runs of the tile.  more: bit i: lane i's token goes on with lane i - 1's run.
+    const bool in = win >= 0 && win < nslots;
+    const int wrow = in ? row_of(win) : 0;
+    const bool head = p.S < T && (t0 - 1 + lane) % p.S == 0;  // runs end with a sequence's tokens
+    const long long prev = __shfl_up(win, 1, kWave);
+    const uint64_t more = ballot(in && lane > 0 && prev == win - 1 && wrow != 0 && !head);
+    uint64_t starts = ballot(in && lane > 0 && lane <= p.tile) & ~more;
+    const int nrun = __builtin_popcountll(starts);
     if (nrun == 0) return;
-    auto run_of = [&](int i, int& t, long long& base, int& row0, int& n) {
-        t = s_run[i];
-        const long long s = p.slots[t];
-        row0 = (int)(s % p.bs);
+    auto run_at = [&](int l, int& t, long long& base, int& row0, int& n) {
+        t = t0 - 1 + l;
+        row0 = __builtin_amdgcn_readlane(wrow, l);
+        const long long s = ((long long)__builtin_amdgcn_readlane((int)(win >> 32), l) << 32) |
+                            (uint32_t)__builtin_amdgcn_readlane((int)win, l);
         base = s - row0;
-        n = 0;
-        const int most = p.bs - row0 < T - t ? p.bs - row0 : T - t;
-        while (n < most) {  // consecutive slots, 64 at a time
+        const uint64_t stop = l < 63 ? ~more >> (l + 1) : 0;  // (zeros come in behind lane 63)
+        n = 1 + (stop ? __builtin_ctzll(stop) : 63 - l);
+        if (l + n < 64) return;
+        // the window's end: on by what memory says, 64 tokens at a time
+        const int here = p.S - t % p.S;
+        const int most = p.bs - row0 < here ? p.bs - row0 : here;
+        while (n < most) {
             const int k = n + lane;
-            const uint64_t b = ballot(k < most && p.slots[t + (k < most ? k : 0)] == s + k);
-            const int good = b == ~0ull ? 64 : __builtin_ctzll(~b);
+            const uint64_t bm = ballot(k < most && p.slots[t + (k < most ? k : 0)] == s + k);
+            const int good = bm == ~0ull ? 64 : __builtin_ctzll(~bm);
             n += good;
             if (good < 64) break;
         }
     };
     // 2. tokens of the runs' pages elsewhere in the call
-    for (int i = 0; i < nrun; ++i) {
-        int t, row0, n;
-        long long base;
-        run_of(i, t, base, row0, n);
-        int found = 0;
-        for (int u = tid; u < T; u += nthreads)
-            if ((unsigned long long)(p.slots[u] - base) < (unsigned long long)p.bs && (u < t || u >= t + n))
-                found |= u < t ? 2 : 1;
-        if (found) atomicOr(&s_other[i], found);
+    for (int c = 0; c < T; c += kAppScan * nthreads) {
+        if (c > 0) load_scan(c);
+        uint64_t left = starts;
+        for (int i = 0; i < nrun; ++i) {
+            int t, row0, n, found = 0;
+            long long base;
+            run_at(__builtin_ctzll(left), t, base, row0, n);
+            left &= left - 1;
+#pragma unroll
+            for (int j = 0; j < kAppScan; ++j) {
+                const int u = c + j * nthreads + tid;
+                const bool same = (unsigned long long)(sl[j] - base) < (unsigned long long)p.bs;
+                if (same && u < T && (u < t || u >= t + n)) found |= u < t ? 2 : 1;
+            }
+            if (found) atomicOr(&s_other[i], found);
+        }
     }
     __syncthreads();
-    // 3. units
-    const int g = lane >> 4, d0 = (lane & 15) * 8;
-    const int nwaves = nthreads >> 6;
-    const int units = nrun * p.Hkv * 2;
-    for (int u = blockIdx.y * nwaves + wv; u < units; u += gridDim.y * nwaves) {
-        const int i = u / (2 * p.Hkv), hk = u - i * 2 * p.Hkv;
-        const int h = hk >> 1;
-        const bool isk = (hk & 1) == 0;
+    // 3. units: K or V of a run, of one KV head, or of four heads where the run is a token
+    const int nwaves = (nthreads >> 6) * (int)gridDim.y;
+    int next = (int)blockIdx.y * (nthreads >> 6) + wv;  // this wave's unit, counted from the run's first
+    int turn = 0;  // which of s_max: a wave may be a unit behind
+    for (int i = 0; i < nrun; ++i, starts &= starts - 1) {
         const int other = s_other[i];
         if (other & 2) continue;  // the page's first token lies in an earlier run
         int t, row0, n;
         long long base;
-        run_of(i, t, base, row0, n);
-        const int page = (int)(base / p.bs);
-        unsigned char* cache = (isk ? p.kc : p.vc) + ((base * p.Hkv + h) << 7);
-        const long long rstride = (long long)p.Hkv << 7;
-        unsigned char* sc = (isk ? p.ks : p.vs) + (long long)page * p.Hkv + h;
-        const int old = *sc;
-        // rows [r0, r1) of the page may have a token; tok(r): the one written there (-1: none)
-        const int r0 = other ? 0 : row0, r1 = other ? p.bs : row0 + n;
-        auto tok = [&](int r) {
-            if (!other) return r >= row0 && r < row0 + n ? t + r - row0 : -1;
-            int last = -1;
-            for (int k = t; k < T; ++k)
-                if (p.slots[k] == base + r) last = k;
-            return last;
-        };
-        float x[kAppRows / 4][8];
-        int rt[kAppRows / 4];
-        auto load_block = [&](int rb) {
-#pragma unroll
-            for (int q = 0; q < kAppRows / 4; ++q) {
-                const int r = rb + q * 4 + g;
-                rt[q] = r < r1 ? tok(r) : -1;
-                const int tt = rt[q] >= 0 ? rt[q] : t;
-                if (isk) load_row8<DT, CDT, true>(p, tt, h, d0, x[q]);
-                else load_row8<DT, CDT, false>(p, tt, h, d0, x[q]);
+        run_at(__builtin_ctzll(starts), t, base, row0, n);
+        const bool fast = !other && p.vec, heads = fast && n == 1;
+        const int per_kv = heads ? (p.Hkv + 3) >> 2 : p.Hkv;
+        // a run of many rows is shared by `team` waves, which wait for one another: every
+        // wave goes through the same number of units then
+        const int team = fast && n > kAppRows ? p.team : 1;
+        const int rank = wv % team, ahead = team > 1 ? wv / team : 0;
+        const int stride = nwaves / team;
+        int u0 = team > 1 ? (int)blockIdx.y * ((nthreads >> 6) / team) : next;
+        for (; u0 < 2 * per_kv; u0 += stride) {
+            const bool store = u0 + ahead < 2 * per_kv;
+            const int u = store ? u0 + ahead : u0;
+            const bool isk = u < per_kv;
+            const int h = (isk ? u : u - per_kv) * (heads ? 4 : 1);
+            const int page = small ? (int)((uint32_t)base / (uint32_t)p.bs) : (int)(base / p.bs);
+            unsigned char* cache = (isk ? p.kc : p.vc) + ((base * p.Hkv + h) << 7);
+            const long long rstride = (long long)p.Hkv << 7;
+            unsigned char* sc = (isk ? p.ks : p.vs) + (long long)page * p.Hkv + h;
+            if (fast) {
+                // (without a rotation there are no angles to read)
+                const bool turns = isk && p.R > 0;
+                if (heads) {
+                    if (turns) write_run<DT, CDT, true, 0>(p, isk, t, row0, n, h, lane, cache, sc);
+                    else write_run<DT, CDT, false, 0>(p, isk, t, row0, n, h, lane, cache, sc);
+                } else {
+                    uint32_t* sm = s_max[turn] + wv - rank;
+                    turn ^= team > 1;
+                    if (turns)
+                        write_run<DT, CDT, true, 4>(p, isk, t, row0, n, h, lane, cache, sc, team, rank, sm, store);
+                    else
+                        write_run<DT, CDT, false, 4>(p, isk, t, row0, n, h, lane, cache, sc, team, rank, sm, store);
+                }
+                continue;
             }
-        };
-        float amax = 0.0f;
-        bool first_row = false;
-        for (int rb = r0; rb < r1; rb += kAppRows) {
-            load_block(rb);
+            // The general form: a row at a time, two elements a lane, read again to be written.
+            // Rows [r0, r1) of the page may have a token; tok(r): the one written there (-1: none).
+            const int r0 = other ? 0 : row0, r1 = other ? p.bs : row0 + n;
+            auto tok = [&](int r) {
+                if (!other) return r >= row0 && r < row0 + n ? t + r - row0 : -1;
+                int last = -1;
+                for (int k = t; k < T; k += kWave) {
+                    const uint64_t at = ballot(k + lane < T && p.slots[k + lane < T ? k + lane : t] == base + r);
+                    if (at) last = k + 63 - __builtin_clzll(at);
+                }
+                return last;
+            };
+            float x[2];
+            const int old = *sc;
+            float amax = 0.0f;
+            for (int r = r0; r < r1; ++r) {
+                const int rt = tok(r);
+                if (rt < 0) continue;
+                load_pair<DT, CDT>(p, isk, rt, h, 2 * lane, x);
 #pragma unroll
-            for (int q = 0; q < kAppRows / 4; ++q) {
-                first_row |= rt[q] >= 0 && rb + q * 4 + g == 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float a = __builtin_fabsf(x[q][e]);
-                    amax = rt[q] >= 0 && a > amax ? a : amax;  // (NaN compares false)
+                for (int e = 0; e < 2; ++e) {
+                    const float a = __builtin_fabsf(x[e]);
+                    amax = a > amax ? a : amax;  // (NaN compares false)
                 }
             }
-        }
 #pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d, kWave));
-        const bool fresh = ballot(first_row) != 0 || old == 255;
-        const int want = exponent_of(amax);
-        const int b = fresh || want > old ? want : old;
-        if (!fresh && b > old) {
-            // rows held under the smaller exponent
-            for (int rb = 0; rb < p.bs; rb += 4) {
-                const int r = rb + g;
-                if (r < p.bs && tok(r) < 0) {
-                    u32x2* row = reinterpret_cast<u32x2*>(cache + r * rstride + d0);
-                    float y[8];
-                    from_fp8(*row, y);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_ldexpf(y[e], old - b);
-                    *row = to_fp8(y);
+            for (int d = 1; d < kWave; d <<= 1) amax = fmaxf(amax, __shfl_xor(amax, d, kWave));
+            const bool fresh = tok(0) >= 0 || old == 255;
+            const int want = exponent_of(amax);
+            const int b = fresh || want > old ? want : old;
+            const bool raise = !fresh && b > old;
+            for (int r = raise ? 0 : r0; r < (raise ? p.bs : r1); ++r) {
+                const int rt = tok(r);
+                uint16_t* to = reinterpret_cast<uint16_t*>(cache + r * rstride) + lane;
+                if (rt >= 0) {
+                    load_pair<DT, CDT>(p, isk, rt, h, 2 * lane, x);
+                    x[0] = __builtin_amdgcn_ldexpf(x[0], 127 - b);
+                    x[1] = __builtin_amdgcn_ldexpf(x[1], 127 - b);
+                } else if (raise) {
+                    const f32x2 y = __builtin_amdgcn_cvt_pk_f32_fp8((int)*to, false);
+                    x[0] = __builtin_amdgcn_ldexpf(y[0], old - b);
+                    x[1] = __builtin_amdgcn_ldexpf(y[1], old - b);
+                } else {
+                    continue;
                 }
+                *to = (uint16_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
             }
+            if (lane == 0 && b != old) *sc = (unsigned char)b;
         }
-        for (int rb = r0; rb < r1; rb += kAppRows) {
-            if (r1 - r0 > kAppRows) load_block(rb);
-#pragma unroll
-            for (int q = 0; q < kAppRows / 4; ++q) {
-                const int r = rb + q * 4 + g;
-                if (rt[q] < 0) continue;
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_ldexpf(x[q][e], 127 - b);
-                *reinterpret_cast<u32x2*>(cache + r * rstride + d0) = to_fp8(y);
-            }
-        }
-        if (lane == 0 && b != old) *sc = (unsigned char)b;
+        if (team == 1) next = u0 - 2 * per_kv;
     }
 }
 
@@ -466,12 +748,22 @@ namespace {
 template <int DT, int CDT>
 hipError_t append8_go(Append8Params p, hipStream_t stream) {
     const long long T = (long long)p.W * p.S;
-    // a token per workgroup while there are few (their pages are found and written side by
-    // side), then about a page of tokens
-    p.tile = T <= 512 ? 1 : p.bs < 16 ? 16 : p.bs < 64 ? p.bs : 64;
+    // as many workgroups as the device holds at a time: a token each while there are few
+    p.tile = (int)((T + 511) / 512 < kAppTile ? (T + 511) / 512 : kAppTile);
+    // waves that share a long run: one for each kAppRows rows of a page
+    p.team = 1;
+    while (p.team < kAppWaves && p.team * kAppRows < p.bs) p.team *= 2;
     const int units = 2 * p.Hkv;
-    const int waves = units < kAppWaves ? units : kAppWaves;
-    const dim3 grid((unsigned)((T + p.tile - 1) / p.tile), (unsigned)((units + waves - 1) / waves));
+    const int waves = units * p.team < kAppWaves ? units * p.team : kAppWaves;
+    const int teams = waves / p.team;
+    const long long tiles = (T + p.tile - 1) / p.tile;
+    // the heads of long runs are spread over workgroups where few have a run
+    const long long busy = T / (p.tile > p.bs ? p.tile : p.bs) + 1;
+    long long split = (units + teams - 1) / teams;
+    if (split > 512 / busy) split = 512 / busy > 1 ? 512 / busy : 1;
+    const long long apart = (p.bs + p.tile - 1) / p.tile;
+    p.apart = (int)(apart < tiles ? apart : tiles);
+    const dim3 grid((unsigned)((tiles + p.apart - 1) / p.apart * p.apart), (unsigned)split);
     hipLaunchKernelGGL((dv_kv_append8<DT, CDT>), grid, dim3(waves * kWave), 0, stream, p, (int)T);
     return hipGetLastError();
 }
@@ -480,11 +772,23 @@ hipError_t append8_go(Append8Params p, hipStream_t stream) {
 
 hipError_t launch_kv_append8(int dtype, int rope_dtype, const Append8Params& base, hipStream_t stream) {
     Append8Params p = base;
+    if (p.S == 1) {  // one row of tokens
+        p.S = p.W;
+        p.W = 1;
+        p.kst[2] = p.kst[0];
+        p.vst[2] = p.vst[0];
+        p.cs[1] = p.cs[0];
+    }
     const int es = dtype == kF32 ? 4 : 2, cs = rope_dtype == kF32 ? 4 : 2;
     auto al = [](const void* q) { return ((uintptr_t)q & 15) == 0; };
-    bool vec = al(p.k) && al(p.v) && al(p.cosv) && al(p.sinv);
-    for (int i = 0; i < 3; ++i) vec = vec && p.kst[i] * es % 16 == 0 && p.vst[i] * es % 16 == 0;
-    for (int i = 0; i < 2; ++i) vec = vec && p.cs[i] * cs % 16 == 0;
+    auto step = [](long long n, int bytes, bool near) {
+        return n * bytes % 16 == 0 && (!near || (n >= 0 && n * bytes < (1ll << 27)));
+    };
+    bool vec = al(p.k) && al(p.v);
+    for (int i = 0; i < 3; ++i) vec = vec && step(p.kst[i], es, i > 0) && step(p.vst[i], es, i > 0);
+    // (the elements half a rotation away start at whole words: half of R is eight or a multiple)
+    if (p.R > 0)
+        vec = vec && p.R % 16 == 0 && al(p.cosv) && al(p.sinv) && step(p.cs[0], cs, false) && step(p.cs[1], cs, true);
     p.vec = vec;
     const bool f32rope = rope_dtype == kF32;
     switch (dtype) {
