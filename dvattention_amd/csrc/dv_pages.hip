@@ -77,11 +77,13 @@ __device__ inline void place_token(const TablesParams& p, const int* cu, const i
 __global__ __launch_bounds__(kTabThreads) void dv_block_tables(const TablesParams p) {
     extern __shared__ __align__(16) int s_tab[];
     __shared__ long long s_part[kTabWaves];
+    __shared__ int s_gone[kTabThreads];  // ended sequences with pages
+    __shared__ int s_ngone;
     int* s_cu = s_tab;                 // [W + 1]
     int* s_start = s_cu + p.W + 1;     // [W] length before the step (0: ended), then the start
     int* s_off = s_start + p.W;        // [W] first stack entry given back, then pages needed before w
     int* s_got = s_off + p.W;          // [W] pages given back, then pages taken
-    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int tid = threadIdx.x;
     const int W = p.W;
     long long room = (long long)p.maxB * p.bs;
     room = room < 0x7fffffffll ? room : 0x7fffffffll;  // positions are 32-bit
@@ -113,12 +115,37 @@ __global__ __launch_bounds__(kTabThreads) void dv_block_tables(const TablesParam
         g_at += s_got[w];
     }
     __syncthreads();
-    // 2. ended sequences' pages go on the stack, a wave per sequence
+    // 2. ended sequences' pages go on the stack: eight sequences at a time by all threads
     if (gone_all > 0) {
-        for (int w = wv; w < W; w += kTabWaves) {
-            const int g = s_got[w], at = s_off[w];
-            for (int b = lane; b < g; b += kWave)
-                if (at + b < p.nblocks) p.stack[at + b] = p.bt[(long long)w * p.maxB + b];
+        for (int k = 0; k < per; ++k) {
+            if (tid == 0) s_ngone = 0;
+            __syncthreads();
+            const int w = w0 + k;
+            if (w < w1 && s_got[w] > 0) s_gone[atomicAdd(&s_ngone, 1)] = w;  // (in any order)
+            __syncthreads();
+            const int ngone = s_ngone;
+            for (int i = 0; i < ngone; i += 8) {
+                int most = 0;
+                for (int j = 0; j < 8; ++j) {
+                    const int g = i + j < ngone ? s_got[s_gone[i + j]] : 0;
+                    most = g > most ? g : most;
+                }
+                for (int b = tid; b < most; b += kTabThreads) {
+                    int page[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int v = s_gone[i + j < ngone ? i + j : i];
+                        page[j] = b < s_got[v] ? p.bt[(long long)v * p.maxB + b] : 0;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int v = s_gone[i + j < ngone ? i + j : i];
+                        const int at = s_off[v];
+                        if (i + j < ngone && b < s_got[v] && at < p.nblocks - b) p.stack[at + b] = page[j];
+                    }
+                }
+            }
+            __syncthreads();
         }
     }
     const long long have = count + gone_all < p.nblocks ? count + gone_all : p.nblocks;
@@ -164,13 +191,19 @@ __global__ __launch_bounds__(kTabThreads) void dv_block_tables(const TablesParam
         p.starts[w] = ok ? len : -1;
         p.lengths_out[w] = len < 0 ? 0 : ok ? len + nw : len;
     }
-    // 4. the pages themselves, from the top of the stack down
-    for (int w = wv; w < W; w += kTabWaves) {
-        const int got = s_got[w];
-        if (got <= 0) continue;
-        const int held = pages_of(s_start[w], p.bs);
-        for (int j = lane; j < got; j += kWave)
-            p.bt[(long long)w * p.maxB + held + j] = p.stack[have - 1 - s_off[w] - j];
+    // 4. the pages themselves, from the top of the stack down, a thread each: the page
+    // before which e others are needed goes to the last sequence that starts at or before e
+    const int pages = (int)(need_all < have ? need_all : have);
+    for (int e = tid; e < pages; e += kTabThreads) {
+        int lo = 0, hi = W - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (s_off[mid] <= e) lo = mid;
+            else hi = mid - 1;
+        }
+        const int j = e - s_off[lo];
+        if (j < s_got[lo])
+            p.bt[(long long)lo * p.maxB + pages_of(s_start[lo], p.bs) + j] = p.stack[have - 1 - e];
     }
     if (p.T > kTabTokens) return;
     __syncthreads();
