@@ -68,7 +68,8 @@ hipError_t launch_chunk8(int dtype, bool varlen, const DecodeParams& base, long 
     for (long long g0 = 0; g0 < groups; g0 += kMaxRows) {
         p.row_begin = (int)g0;
         p.nrows = (int)(groups - g0 < kMaxRows ? groups - g0 : kMaxRows);
-        const long long cap = ((long long)p.nrows * p.Hkv * max_keys_per_group + p.min_keys - 1) / p.min_keys;
+        const long long cap =
+            ((long long)p.nrows * p.Hkv * (max_keys_per_group + p.piece_cost) + p.min_keys - 1) / p.min_keys;
         if (dtype == kBF16)
             e = varlen ? chunk::launch8<kBF16, kQRotHalf, kRowVarlen>(p, device, cus, cap, stream)
                        : chunk::launch8<kBF16, kQRotFull, kRowWS>(p, device, cus, cap, stream);

@@ -6,9 +6,8 @@
 //  * One wave owns one KV head and its 16 query heads of one row over a range of the
 //    row's keys; up to four such waves (KV heads) make a workgroup.
 //  * A stage is 32 keys: 4 KiB of K, 4 KiB of V and the 64 exponent bytes of its rows,
-//    moved by nine direct-to-LDS loads into a ring of four stages private to the wave,
-//    three of them in flight beside the one computed.  The exponents travel with their
-//    rows, so pages of any size may end inside a stage.
+//    moved by nine direct-to-LDS loads into a ring of two stages private to the wave.  The
+//    exponents travel with their rows, so pages of any size may end inside a stage.
 //  * K bytes are widened to the 16-bit MFMA operand (every E4M3 number is one of bf16 and
 //    of fp16): S^T = K Q^T on 16x16x32 MFMA, and the page's 2^(b - 127) multiplies the
 //    fp32 score.  V^T comes from the transposing 8-bit LDS read, widened to bf16, and V's
@@ -35,16 +34,14 @@ constexpr int kScaleB = 64 * 4;                 // exponent bytes of 32 K rows, 
 constexpr int kStage = 2 * kTile + kScaleB;
 constexpr int kLoads = 9;                       // direct-to-LDS loads per stage
 
-// Tokens of a row group at most: a wave holds NT query tiles (16 heads of a token each).
-constexpr int kMaxTok = 4;
-// Waves of one or two tiles fit two to a SIMD with two stages each in LDS, their
-// accumulators in VGPRs (as their file is compiled); those of four, and of two in fp32
-// (their operands alone are 128 registers), have the SIMD to themselves, four stages, and
-// accumulators in AGPRs.
-constexpr int waves_per_cu(int dtype, int nt) { return nt == 1 || (nt == 2 && dtype != kF32) ? 8 : 4; }
-template <int DT, int NT> constexpr int kWavesPerCu = waves_per_cu(DT, NT);
-template <int DT, int NT> constexpr int kRing = kWavesPerCu<DT, NT> == 8 ? 2 : 4;
-template <int DT, int NT> constexpr int kWaveLds = kRing<DT, NT> * kStage + stream::kPc * 4;
+// A wave holds NT query tiles (16 heads of a token each), one or, in 16-bit types, two;
+// two waves to a SIMD, with two stages each in LDS and accumulators in VGPRs (as the
+// kernels' file is compiled).  fp32 with two tiles (whose operands alone are 128
+// registers) had the SIMD to itself: 100 MB of cache took 39 us for two tokens, where rows
+// of one token take 17.5 us each.
+constexpr int kWaves = 8;                       // per CU
+constexpr int kRing = 2;
+constexpr int kWaveLds = kRing * kStage + stream::kPc * 4;
 
 // MFMA operands of a query (or probability) value: 16-bit parts that sum to it.
 template <int DT> constexpr int kQParts = DT == kF32 ? 2 : 1;
@@ -371,7 +368,7 @@ __device__ inline void read_powers(uint32_t at, float (&f)[8]) {
 
 // One stage for NT tiles: scores, softmax, O^T += V^T P^T.  okm: the stage's keys that hold
 // rows; mask[t]: those that tile t sees.
-template <int DT, int NT, bool kAcc>
+template <int DT, int NT>
 __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro, uint32_t okm,
                                const uint32_t (&mask)[NT], const QOp<DT> (&q)[NT]) {
     f32x4 s[NT][2];
@@ -440,10 +437,7 @@ __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro
         }
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        if constexpr (kAcc) mfma_settle_acc(st[t].o);
-        else mfma_settle(st[t].o);
-    }
+    for (int t = 0; t < NT; ++t) mfma_settle(st[t].o);
 }
 
 // A row group: ntok tokens of sequence w, the first being row `lin` of the token axis.
@@ -503,7 +497,7 @@ __device__ inline long long group_visible(const DecodeParams& p, int rg) {
 template <int DT, int QM, int RM, int NT, int GT, bool MV, bool P2>
 __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds, int rg, int hkv, long long v0,
                                       long long v1, bool final_out, int slot, int wv, long long row_keys) {
-    constexpr int R = kRing<DT, GT>;
+    constexpr int R = kRing;
     const int lane = threadIdx.x & 63;
     const int g = lane >> 4, n = lane & 15;
     const uint32_t ring = __builtin_amdgcn_readfirstlane(lds_addr(wlds));
@@ -589,8 +583,6 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
             for (int s = 0; s < ns; ++s) {
                 // stage s landed: at most the R - 1 after it may be in flight
                 if (s + R <= ns) wait_vmcnt<(R - 1) * kLoads>();
-                else if (R > 3 && s + 2 < ns) wait_vmcnt<2 * kLoads>();
-                else if (R > 2 && s + 1 < ns) wait_vmcnt<kLoads>();
                 else wait_vmcnt<0>();
                 uint32_t mask[NT];
 #pragma unroll
@@ -601,7 +593,7 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
                         mask[t] &= lim >= kStep ? 0xffffffffu : lim <= 0 ? 0u : (1u << lim) - 1u;
                     }
                 }
-                compute<DT, NT, kWavesPerCu<DT, GT> == 4>(st, ring + (uint32_t)(cur * kStage), ro, m[0], mask, q);
+                compute<DT, NT>(st, ring + (uint32_t)(cur * kStage), ro, m[0], mask, q);
 #pragma unroll
                 for (int k = 0; k + 1 < R; ++k) m[k] = m[k + 1];
                 lds_wait();  // the slot's reads are complete before it is refilled
@@ -668,14 +660,14 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
 // MV: calls of several views (or none), whose pieces may start anywhere.  P2: pages of a
 // power of two of at least 16 rows (NT > 1: looked up, one kernel for all calls).
 template <int DT, int QM, int RM, int NT, bool MV, bool P2>
-__global__ __launch_bounds__((q8::kWavesPerCu<DT, NT> * kWave)) void dv_decode8(const DecodeParams p) {
+__global__ __launch_bounds__(q8::kWaves * kWave) void dv_decode8(const DecodeParams p) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((128u - (lds_addr(smem_raw) & 127u)) & 127u);  // (ReadOff)
-    __shared__ long long s_scan[q8::kWavesPerCu<DT, NT>];
+    __shared__ long long s_scan[q8::kWaves];
     const int wv = uniform((int)(threadIdx.x >> 6));
     const int HPW = p.hpw;
-    long long* s_pref = reinterpret_cast<long long*>(smem + HPW * q8::kWaveLds<DT, NT>);
-    unsigned char* wlds = smem + wv * q8::kWaveLds<DT, NT>;
+    long long* s_pref = reinterpret_cast<long long*>(smem + HPW * q8::kWaveLds);
+    unsigned char* wlds = smem + wv * q8::kWaveLds;
     run_schedule<true, MV ? 1 : kStep, 1, NT == 1>(
         p, p.Hkv / HPW, s_pref, s_scan, [&](int row) { return q8::group_visible<RM, NT>(p, row); },
         [&](int row, int hg, long long v0, long long v1, bool fin, int slot, long long rk) {
@@ -722,7 +714,7 @@ hipError_t launch8_one(DecodeParams p, int device, long long cap, int cus, hipSt
     const void* kern = reinterpret_cast<const void*>(&dv_decode8<DT, QM, RM, NT, MV, P2>);
     // (up to 64 rows the schedule's sums stay in registers)
     auto lds_of = [](int hpw, int nrows) {
-        return 128 + (size_t)hpw * q8::kWaveLds<DT, NT> + (nrows > kWave ? (size_t)(nrows + 1) * sizeof(long long) : 0);
+        return 128 + (size_t)hpw * q8::kWaveLds + (nrows > kWave ? (size_t)(nrows + 1) * sizeof(long long) : 0);
     };
     static std::atomic<unsigned long long> attr_done{0};
     hipError_t e = once_per_device(attr_done, device, [&] {
@@ -733,7 +725,7 @@ hipError_t launch8_one(DecodeParams p, int device, long long cap, int cus, hipSt
     // workgroups that are all resident at once
     const size_t lds = lds_of(p.hpw, p.nrows);
     const int fit = (int)(160 * 1024 / (lds + 512));
-    const int most = q8::kWavesPerCu<DT, NT> / p.hpw;
+    const int most = q8::kWaves / p.hpw;
     const long long nwg = (long long)cus * (fit < most ? fit : most);
     p.nwg = (int)(nwg < cap ? nwg : cap < 1 ? 1 : cap);
     hipLaunchKernelGGL((dv_decode8<DT, QM, RM, NT, MV, P2>), dim3(p.nwg), dim3(p.hpw * kWave), lds, stream, p);
@@ -747,9 +739,5 @@ hipError_t launch8_one(DecodeParams p, int device, long long cap, int cus, hipSt
         return hipGetLastError();
     }
 }
-
-// Calls whose waves have a SIMD to themselves (dv_decode8m.hip).
-hipError_t launch_decode8_wide(int dtype, bool varlen, const DecodeParams& p, int device, long long cap, int cus,
-                               hipStream_t stream);
 
 }  // namespace dv

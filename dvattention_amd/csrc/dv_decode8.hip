@@ -19,7 +19,6 @@ hipError_t launch8_row(const DecodeParams& p, int device, long long cap, int cus
 template <int DT>
 hipError_t launch8(bool varlen, int nt, const DecodeParams& p, int device, long long cap, int cus,
                    hipStream_t stream) {
-    if (q8::waves_per_cu(DT, nt) == 4) return launch_decode8_wide(DT, varlen, p, device, cap, cus, stream);
     if (nt == 1)
         return varlen ? launch8_row<DT, kQRotHalf, kRowVarlen>(p, device, cap, cus, stream)
                       : launch8_row<DT, kQRotFull, kRowWS>(p, device, cap, cus, stream);
@@ -44,12 +43,12 @@ Ws8 ws8(long long groups, int nt, int Hkv, int device) {
     return w;
 }
 
-// KV heads (waves) per workgroup: eight where a CU's waves allow it, whose rows of a token
+// KV heads (waves) per workgroup: eight where there are as many, whose rows of a token
 // then lie side by side in memory as a workgroup reads them (32 sequences of 1k - 8k
 // tokens, 8 KV heads: 62.6 -> 60.6 us, 4 x 131072: 191 -> 184), unless the call is too
 // small to fill the chip so (one sequence of 3001 tokens: 11.0 us with four, 13.3).
-int pick_hpw8(int dtype, long long groups, long long max_keys, int nt, int Hkv, int cus) {
-    if (Hkv % 8 == 0 && q8::waves_per_cu(dtype, nt) == 8 && groups <= 1024 && groups * max_keys >= 256ll * cus) return 8;
+int pick_hpw8(long long groups, long long max_keys, int Hkv, int cus) {
+    if (Hkv % 8 == 0 && groups <= 1024 && groups * max_keys >= 256ll * cus) return 8;
     return pick_hpw(Hkv);
 }
 
@@ -67,7 +66,7 @@ hipError_t launch_decode8(int dtype, bool varlen, int nt, const DecodeParams& ba
     const Ws8 l = ws8(groups, nt, base.Hkv, device);
     const int cus = device_cu_count(device);
     DecodeParams p = base;
-    p.hpw = pick_hpw8(dtype, groups, max_keys_per_row, nt, p.Hkv, cus);
+    p.hpw = pick_hpw8(groups, max_keys_per_row, p.Hkv, cus);
     const int nhg = p.Hkv / p.hpw;
     p.slot_floats = p.hpw * nt * kGqa * (kHeadDim + 1);
     p.part = reinterpret_cast<float*>(workspace);
@@ -93,16 +92,21 @@ hipError_t launch_decode8(int dtype, bool varlen, int nt, const DecodeParams& ba
 
 // ---- which kernels a call takes --------------------------------------------------------
 //
-// A wave of the decode kernels holds as many tokens of a sequence as it can beside each
-// other (K and V are read once for them): up to four, in fp32 two.  16-bit calls of more
-// go through the multi-query kernel, 16 tokens to a workgroup.  Packed calls of two or
-// more tokens per sequence are cut into row groups on the device; in 16-bit types those of
-// up to four tokens (two to a wave, whose kernel has eight waves to a CU: most are decodes of
-// one token) and those of more are two launches.
+// A wave of the decode kernels holds a token or, in 16-bit types, up to two tokens of a
+// sequence beside each other (K and V are read once for them).  16-bit calls of
+// few tokens are cut into such pairs, which read the cache once each; those of more go
+// through the multi-query kernel, 16 tokens to a workgroup.  24 sequences of 4096 keys, 4
+// KV heads, us as pairs and in the multi-query kernel:
+//   bf16: 4 tokens 73, 93;   6 tokens 94, 101;   8 tokens 117, 107
+//   fp16: 4 tokens 78, 99;   6 tokens 101, 138;  8 tokens 124, 140;  16 tokens 204, 152
+// (Four tokens to a wave, which has the SIMD to itself then: 93 us for 4.)  Packed calls of
+// two or more tokens per sequence are cut into row groups on the device; in 16-bit types
+// those of up to four tokens and those of more are two launches.
 namespace {
 
 constexpr int kGroupTok = 16;  // tokens of a table entry (dv_varlen_groups)
 constexpr int kFewTokens = 4;  // of an entry that the 16-bit multi-query kernel leaves to the decode kernel
+constexpr int few_tokens(int dtype) { return dtype == kBF16 ? 6 : 8; }  // the same of a [W, S] call's sequence
 
 struct Plan8 {
     bool table;                // varlen row groups
@@ -117,18 +121,21 @@ Plan8 plan8(int dtype, bool varlen, int W, int S_or_T, int Hkv, int device) {
     Plan8 q = {};
     const int S = varlen ? 1 : S_or_T;
     q.sub = 1;
-    if (varlen && use_varlen_chunk(dtype, S_or_T, W)) {
+    if (dtype == kF32) {
+        q.nt = 1;
+        q.groups = varlen ? S_or_T : (long long)W * S;
+    } else if (varlen && use_varlen_chunk(dtype, S_or_T, W)) {
         q.table = true;
         q.groups = (long long)S_or_T / kGroupTok + W + 1;
         q.table_bytes = (size_t)q.groups * 16;
         q.nt = 2;
-        q.sub = (dtype == kF32 ? kGroupTok : kFewTokens) / 2;
-        q.chunk = dtype != kF32;
+        q.sub = kFewTokens / 2;
+        q.chunk = true;
     } else if (varlen) {
         q.nt = 1;
         q.groups = S_or_T;
-    } else if (dtype == kF32 || S <= 4) {
-        q.nt = S <= 2 ? S : dtype == kF32 ? 2 : 4;
+    } else if (S <= few_tokens(dtype)) {
+        q.nt = S < 2 ? S : 2;
         q.groups = (long long)W * ((S + q.nt - 1) / q.nt);
     } else {
         q.chunk = true;
