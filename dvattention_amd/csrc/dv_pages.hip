@@ -21,7 +21,10 @@ typedef __attribute__((ext_vector_type(2))) short i16x2;
 // sequences give back (which come first, so that this step can hand them out again), and
 // the pages that the others need.  One workgroup of sixteen waves: a step of some
 // hundred sequences is bound by the latency of its few dependent reads (lengths, table
-// entries, stack entries), not by bytes.
+// entries, stack entries) and its scans, not by bytes.  64 sequences, one token each: 7.5
+// us; 512 of up to 32000 tokens, 24 of which end and 32 of which add up to 512 tokens:
+// 16.6 us (22 with a wave per sequence for the pages), and 3.9 for the places of its 8000
+// tokens.
 constexpr int kTabThreads = 1024;
 constexpr int kTabWaves = kTabThreads / kWave;
 // Tokens that the table workgroup still places itself; with more, a second launch places
@@ -600,7 +603,13 @@ constexpr int kAppScan = 8;       // slots that a thread compares at a time
 // last token of a slot winning.
 //
 // Bound by its chain of dependent reads while the call is small: slots (the tile's and
-// those compared, read together), then rows, angles and exponents together.
+// those compared, read together), then rows, angles and exponents together.  32 single
+// tokens, 8 KV heads: 6 us; 548 tokens of decodes and prompts, 4 KV heads, pages of 24: 9 us
+// (138 with a page of tokens to a workgroup, whose decodes went one after the other).
+// Large calls are bound by VALU issue and the chain, 2 rounds of units a wave, and near the
+// end by HBM: 8188 tokens of four prompts, 8 KV heads, 54 MB: 25 us cold, 17 warm (3.2
+// TB/s), 55 with branches around the loads, which waited for each.  The comparisons grow
+// with the square of the call: 32768 tokens take 64 us, of which about 20 are those.
 template <int DT, int CDT>
 __global__ __launch_bounds__(kAppWaves * kWave, DT == kF32 || CDT == kF32 ? 2 : 4)
 void dv_kv_append8(const Append8Params p, int T) {
@@ -812,6 +821,8 @@ hipError_t launch_kv_append8(int dtype, int rope_dtype, const Append8Params& bas
         p.vst[2] = p.vst[0];
         p.cs[1] = p.cs[0];
     }
+    if (p.W == 1) p.kst[0] = p.vst[0] = p.cs[0] = 0;  // (strides of a single index say nothing)
+    if (p.Hkv == 1) p.kst[1] = p.vst[1] = 0;
     const int es = dtype == kF32 ? 4 : 2, cs = rope_dtype == kF32 ? 4 : 2;
     auto al = [](const void* q) { return ((uintptr_t)q & 15) == 0; };
     auto step = [](long long n, int bytes, bool near) {

@@ -2,8 +2,9 @@
 64-bit restatement in oracle/cache8_oracle.py.
 
 Tables and appended bytes have to be equal.  The attention's tolerances are bounds.  A
-float32 score sums E exact products of K and Q (fp32 calls: three of them per element,
-the parts of Q, whose last remainder is below 2^-24 of q), so it is off by at most e =
+float32 score sums E exact products of K and Q (fp32 calls: two of them per element, the
+parts of Q, whose last remainder is below 2^-24 of q and 2^-39 of the head's largest; three
+are counted), so it is off by at most e =
 (m E + 8) * 2^-24 * sum |q_e k_e| * |scale| with m = 3 for fp32 and 1 else, and a softmax
 weight by a factor exp(2 e); a sum over n keys adds (m n + 16) * 2^-24.  To that come, times
 the sum of weight * |v|: for bf16 the weights' rounding twice (the normaliser sums the
