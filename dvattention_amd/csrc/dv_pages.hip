@@ -590,6 +590,7 @@ __device__ inline void write_run(const Append8Params& p, bool isk, int t, int ro
 constexpr int kAppWaves = 8;      // most waves of a workgroup
 constexpr int kAppTile = 32;      // most tokens of a workgroup
 constexpr int kAppScan = 8;       // slots that a thread compares at a time
+constexpr int kAppMap = 1024;     // rows of a page whose last tokens are listed
 
 }  // namespace
 
@@ -614,6 +615,7 @@ template <int DT, int CDT>
 __global__ __launch_bounds__(kAppWaves * kWave, DT == kF32 || CDT == kF32 ? 2 : 4)
 void dv_kv_append8(const Append8Params p, int T) {
     __shared__ uint32_t s_max[2][kAppWaves];
+    __shared__ int s_tok[kAppMap];
     __shared__ int s_other[kAppTile];  // 1: the run's page has tokens outside it; 2: earlier ones
     const int tid = threadIdx.x, lane = tid & 63, wv = uniform(tid >> 6), nthreads = blockDim.x;
     const long long nslots = (long long)p.nblocks * p.bs;
@@ -682,7 +684,7 @@ void dv_kv_append8(const Append8Params p, int T) {
 #pragma unroll
             for (int j = 0; j < kAppScan; ++j) {
                 const int u = c + j * nthreads + tid;
-                const bool same = (unsigned long long)(sl[j] - base) < (unsigned long long)p.bs;
+                const bool same = (unsigned long long)sl[j] - (unsigned long long)base < (unsigned long long)p.bs;
                 if (same && u < T && (u < t || u >= t + n)) found |= u < t ? 2 : 1;
             }
             if (found) atomicOr(&s_other[i], found);
@@ -699,6 +701,16 @@ void dv_kv_append8(const Append8Params p, int T) {
         int t, row0, n;
         long long base;
         run_at(__builtin_ctzll(starts), t, base, row0, n);
+        if (other) {  // the last token of each row (a maximum: the same in any order)
+            __syncthreads();  // an earlier run's list is done with
+            for (int r = tid; r < kAppMap; r += nthreads) s_tok[r] = -1;
+            __syncthreads();
+            for (int k = t + tid; k < T; k += nthreads) {
+                const unsigned long long r = (unsigned long long)p.slots[k] - (unsigned long long)base;
+                if (r < (unsigned long long)p.bs && r < (unsigned long long)kAppMap) atomicMax(&s_tok[r], k);
+            }
+            __syncthreads();
+        }
         const bool fast = !other && p.vec, heads = fast && n == 1;
         const int per_kv = heads ? (p.Hkv + 3) >> 2 : p.Hkv;
         // a run of many rows is shared by `team` waves, which wait for one another: every
@@ -737,6 +749,7 @@ void dv_kv_append8(const Append8Params p, int T) {
             const int r0 = other ? 0 : row0, r1 = other ? p.bs : row0 + n;
             auto tok = [&](int r) {
                 if (!other) return r >= row0 && r < row0 + n ? t + r - row0 : -1;
+                if (r < kAppMap) return uniform(s_tok[r]);
                 int last = -1;
                 for (int k = t; k < T; k += kWave) {
                     const uint64_t at = ballot(k + lane < T && p.slots[k + lane < T ? k + lane : t] == base + r);

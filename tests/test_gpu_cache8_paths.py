@@ -62,6 +62,17 @@ def test_append_single_tokens(dv, gpu, dtype):
         check_append(dv, gpu, d, (torch.randperm(W + 2, generator=g)[:W] * bs + row)[:, None])
 
 
+@pytest.mark.parametrize("bs,P", [(48, 20), (1500, 3)])
+def test_append_slots_of_any_order_in_long_pages(dv, gpu, bs, P):
+    """Several runs and single tokens in each page, rows named twice, rows behind the 1024th."""
+    g = torch.Generator().manual_seed(bs)
+    T = 1300
+    d = append_case(g, torch.bfloat16, torch.bfloat16, 1, 3, T, P, bs, 64, size=20.0)
+    check_append(dv, gpu, d, torch.randint(-5, P * bs, (1, T), generator=g))
+    slots = torch.cat([torch.arange(100) + int(x) for x in torch.randint(0, P * bs - 100, (13,), generator=g)])
+    check_append(dv, gpu, d, slots[None])
+
+
 def test_append_runs_across_sequences(dv, gpu):
     """The last slots of a sequence and the first of the next are consecutive, in one page."""
     g = torch.Generator().manual_seed(5)
