@@ -110,10 +110,12 @@ template <bool P2, bool kAsk>
 __device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, uint32_t lo, const int* pc,
                                  uint32_t sbase, int l) {
     const int lane = threadIdx.x & 63;
+    // (positions are 31 bits: rows of views that start behind that are absent)
+    const uint32_t pos0 = (uint32_t)v.off + (uint32_t)l;
+    const bool whole = l + kStep <= v.b && pos0 <= 0x7fffffffu - (uint32_t)(kStep - 1);
     if constexpr (P2) {
-        const int pos0 = v.off + l;
-        if ((!kAsk || p.bs_shift >= 4) && l + kStep <= v.b && stream::full_stage_in_cache(pos0, p.bs_shift, v.lp0)) {
-            const uint32_t pos = (uint32_t)pos0, in = (1u << p.bs_shift) - 1u;
+        if ((!kAsk || p.bs_shift >= 4) && whole && stream::full_stage_in_cache((int)pos0, p.bs_shift, v.lp0)) {
+            const uint32_t pos = pos0, in = (1u << p.bs_shift) - 1u;
             const int pg0 = uniform(pc[(int)(pos >> p.bs_shift) - v.lp0]);
             const int pg1 = uniform(pc[(int)((pos + 16) >> p.bs_shift) - v.lp0]);
             if (pg0 >= 0 && pg1 >= 0) {
@@ -137,9 +139,45 @@ __device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, u
         }
     }
     const int ol = opaque_tid() & 63;  // (lane-dependent values are computed here, not held)
+    // Pages of 16 rows or more: 32 visible keys lie in at most three, whose bases are scalar;
+    // a lane picks its row's.
+    if (p.bs >= 16 && p.bs < (1 << 28) && whole) {
+        uint32_t q, r;
+        page_split(p, pos0, q, r);
+        const int at = uniform((int)q) - v.lp0, r0 = uniform((int)r);
+        const int more = (r0 + kStep - 1 >= p.bs ? 1 : 0) + (r0 + kStep - 1 >= 2 * p.bs ? 1 : 0);
+        if (at >= 0 && at + more < stream::kPc) {
+            int pg[3];
+#pragma unroll
+            for (int j = 0; j < 3; ++j) pg[j] = uniform(pc[at + (j < more ? j : more)]);
+            if (pg[0] >= 0 && pg[1] >= 0 && pg[2] >= 0) {
+                uint32_t base[3];  // of key 0, as if its page held all keys
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    base[j] = ((uint32_t)(pg[j] - j) * (uint32_t)p.bs + (uint32_t)r0) * (uint32_t)p.Hkv + (uint32_t)v.hkv;
+                const int t1 = p.bs - r0, t2 = 2 * p.bs - r0;  // first keys of the second and third page
+                auto pick = [&](int k, uint32_t a, uint32_t b, uint32_t c) { return k >= t1 ? k >= t2 ? c : b : a; };
+                const uint32_t lrow = (uint32_t)(ol >> 3) * (uint32_t)p.Hkv;
+                // piece of a row; the swizzle of other loads' rows differs in bit 2 (lane_offset)
+                const uint32_t piece = (uint32_t)(((ol & 7) ^ swz_k(ol >> 3)) * 16);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t row = pick(i * 8 + (ol >> 3), base[0], base[1], base[2]) + lrow +
+                                         (uint32_t)(i * 8) * (uint32_t)p.Hkv;
+                    const unsigned long long off = (unsigned long long)row * kRowB;
+                    dma16(v.k + (off | ((i & 1) ? piece ^ 64u : piece)), sbase + (uint32_t)(i * 1024));
+                    dma16(v.v + (off | ((i >> 1) ? piece ^ 64u : piece)), sbase + (uint32_t)(kTile + i * 1024));
+                }
+                const uint32_t page = pick(ol & 31, (uint32_t)pg[0], (uint32_t)pg[1], (uint32_t)pg[2]);
+                dma1((ol < 32 ? p.ks : p.vs) + (page * (uint32_t)p.Hkv + (uint32_t)v.hkv),
+                     sbase + (uint32_t)(2 * kTile));
+                return 0xffffffffu;
+            }
+        }
+    }
     // page and in-page offset of the row of key l + k, or page -1
     auto find = [&](int k, uint32_t& r) {
-        const int pos = v.off + l + k;
+        const int pos = (int)(pos0 + (uint32_t)k);
         uint32_t q;
         page_split(p, (uint32_t)(pos > 0 ? pos : 0), q, r);
         const uint32_t idx = q - (uint32_t)v.lp0;
@@ -539,7 +577,7 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
         v.hkv = hkv;
         v.k = reinterpret_cast<const unsigned char*>(p.kc);
         v.v = reinterpret_cast<const unsigned char*>(p.vc);
-        v.off = (int)off;
+        v.off = (int)(off < 0x7fffffffll ? off : 0x7fffffffll);
         int vis_t[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -555,9 +593,12 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
             const int sb = (long long)l1 - sa > span ? (int)(sa + span) : l1;
             v.b = sb;
             uint32_t lpa, lpz, r;
-            const int pa = v.off + sa, pz = v.off + sb - 1;
-            page_split(p, pa > 0 ? (uint32_t)pa : 0u, lpa, r);
-            page_split(p, pz > 0 ? (uint32_t)pz : 0u, lpz, r);
+            auto at = [&](long long l) {
+                const long long pos = v.off + l;
+                return pos < 0 ? 0u : pos < 0x7fffffffll ? (uint32_t)pos : 0x7fffffffu;
+            };
+            page_split(p, at(sa), lpa, r);
+            page_split(p, at(sb - 1ll), lpz, r);
             v.lp0 = (int)lpa;
             stream::fill_pages(p, p.bt + (long long)w * p.maxB, pc, (int)(lpz - lpa) + 1,
                                [&](int i) { return lpa + (uint32_t)i; });
