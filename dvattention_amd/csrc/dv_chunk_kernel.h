@@ -883,8 +883,12 @@ __device__ void chunk_piece(const DecodeParams& p, unsigned char* smem, int* pag
             vis_t[t] = t < ntile ? v : 0;
         }
         const int vis_blk = p.F == 1 ? (int)row_keys : uniform(group_view_vis<KVM, RM>(p, f, gr));
-        const long long a = v0 > P ? v0 : P;
-        const long long bnd = v1 < P + vis_blk ? v1 : P + vis_blk;
+        long long a = v0 > P ? v0 : P;
+        long long bnd = v1 < P + vis_blk ? v1 : P + vis_blk;
+        if constexpr (KV8) {  // rows at positions outside 31 bits are absent (issue_raw counts in 32)
+            a = a > P - off ? a : P - off;
+            bnd = bnd < P - off + 0x80000000ll ? bnd : P - off + 0x80000000ll;
+        }
         if (a < bnd) {
             const int la = (int)(a - P), lb = (int)(bnd - P);
             Range r;

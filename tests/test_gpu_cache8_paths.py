@@ -194,3 +194,32 @@ def test_sdpa_captured_and_on_two_streams(dv, gpu, dtype, S):
             got += [both() for _ in range(3)]
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for x in got for a, b in zip(x, want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("S", [1, 2, 20])
+@pytest.mark.parametrize("bs", [1, 16, 24])
+def test_sdpa_views_behind_all_positions(dv, gpu, dtype, S, bs):
+    """A view that starts behind what a position can count has no rows; nor have the first rows
+    of one behind a negative length."""
+    d = case(dtype, 2, 1, S, [60, 5, 40], bs, 32, seed=S)
+    d["locations"][0], d["locations"][1], d["locations"][2] = 59, -1, 39
+    alone = {**d, "fragment_lengths": torch.tensor([60, 0, 0], dtype=torch.int32)}
+    want = CO.sdpa(SCALE, **alone)
+    for lens in ([60, 2147483647, 40], [60, 2147483647 - 61, 40]):
+        d["fragment_lengths"] = torch.tensor(lens, dtype=torch.int32)
+        compare(dv.dvattn_paged_sdpa_q8(scale=SCALE, **to(gpu, d)), dtype, 60, *want)
+        v, w, s = packed(d, 2, S, [S, S])
+        vd = to(gpu, v)
+        out = dv.dvattn_varlen_paged_sdpa_q8(scale=SCALE, cu_seqlens_k=vd["cu_seqlens_q"], **vd)
+        compare(out, dtype, 60, *(x[w, :, s] for x in want))
+    # two such views: positions behind 2^32
+    d["fragment_lengths"] = torch.tensor([60, 2147483647, 2147483647, 40], dtype=torch.int32)
+    loc = d["locations"]
+    d.update({n: torch.cat([d[n], d[n][:1]]) for n in ("cosines", "sines")},
+             locations=torch.stack([loc[0], loc[1], loc[1], loc[2]]))
+    compare(dv.dvattn_paged_sdpa_q8(scale=SCALE, **to(gpu, d)), dtype, 60, *want)
+    few = case(dtype, 2, 1, S, [-7, 40], bs, 32, seed=S)
+    few["locations"][0], few["locations"][1] = -1, 30
+    dv.dvattn_paged_sdpa_q8(scale=SCALE, **to(gpu, few))
+    torch.cuda.synchronize()
