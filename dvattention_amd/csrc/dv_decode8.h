@@ -106,7 +106,7 @@ __device__ inline uint32_t lane_offset(const DecodeParams& p) {
 // least 16 rows): a stage of 32 visible keys that starts at a multiple of 16 lies in at most
 // two pages, one for each half, so its row bases are scalar and no lane looks a row up
 // (32 ragged sequences: 9 + 140 instructions per stage instead of 9 + 250).
-template <bool P2, bool kAsk>
+template <bool P2, bool kAsk, bool kAny>
 __device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, uint32_t lo, const int* pc,
                                  uint32_t sbase, int l) {
     const int lane = threadIdx.x & 63;
@@ -140,8 +140,8 @@ __device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, u
     }
     const int ol = opaque_tid() & 63;  // (lane-dependent values are computed here, not held)
     // Pages of 16 rows or more: 32 visible keys lie in at most three, whose bases are scalar;
-    // a lane picks its row's.
-    if (p.bs >= 16 && p.bs < (1 << 28) && whole) {
+    // a lane picks its row's.  (kAny: stages that the first form does not take are common.)
+    if (kAny && p.bs >= 16 && p.bs < (1 << 28) && whole) {
         uint32_t q, r;
         page_split(p, pos0, q, r);
         const int at = uniform((int)q) - v.lp0, r0 = uniform((int)r);
@@ -154,7 +154,8 @@ __device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, u
                 uint32_t base[3];  // of key 0, as if its page held all keys
 #pragma unroll
                 for (int j = 0; j < 3; ++j)
-                    base[j] = ((uint32_t)(pg[j] - j) * (uint32_t)p.bs + (uint32_t)r0) * (uint32_t)p.Hkv + (uint32_t)v.hkv;
+                    base[j] = ((uint32_t)(pg[j] - j) * (uint32_t)p.bs + (uint32_t)r0) * (uint32_t)p.Hkv +
+                              (uint32_t)v.hkv;
                 const int t1 = p.bs - r0, t2 = 2 * p.bs - r0;  // first keys of the second and third page
                 auto pick = [&](int k, uint32_t a, uint32_t b, uint32_t c) { return k >= t1 ? k >= t2 ? c : b : a; };
                 const uint32_t lrow = (uint32_t)(ol >> 3) * (uint32_t)p.Hkv;
@@ -278,8 +279,26 @@ __device__ inline void rotated8(const typename Tr<DT>::raw* q, const float* cs, 
     for (int i = 0; i < 8; ++i) r[i] = Tr<DT>::fromf(x[i]);
 }
 
-template <int DT, int QM, int RM>
+// A run's operands as loaded: the run, the one it pairs with, cos and sin.
+template <int DT>
+struct QRun {
+    static constexpr int kWords = (int)sizeof(typename Tr<DT>::raw) / 2;  // 16-byte words of eight elements
+    u32x4 x[kWords], o[kWords];
+    f32x4 c[2], s[2];
+    __device__ static inline float at(const u32x4 (&w)[kWords], int i) {
+        if constexpr (DT == kF32) return __uint_as_float(w[i >> 2][i & 3]);
+        else return Tr<DT>::tof((uint16_t)(w[0][i >> 1] >> (16 * (i & 1))));
+    }
+};
+
+// The rotated query of token `row` in view f, a wave's 16 heads.  kAhead: the loads of all four
+// runs are in flight at once, 96 registers; else a run at a time.  Kernels of two tokens to
+// a wave take the first (24 sequences x 4 tokens, R = 128: 61.8 -> 57.0 us; decodes beside
+// prompt chunks 182 -> 176); rows of one token wait for their stages longer than for the
+// runs (batch and long decodes the same, fp32 69 -> 72).
+template <int DT, int QM, int RM, bool kAhead>
 __device__ inline void load_q(const DecodeParams& p, int row, int f, int hkv, QOp<DT>& o) {
+#pragma clang fp contract(off)
     using raw = typename Tr<DT>::raw;
     // (addresses from an opaque lane: computed here, not held in registers from the start)
     const int lane = opaque_tid() & 63;
@@ -298,19 +317,56 @@ __device__ inline void load_q(const DecodeParams& p, int row, int f, int hkv, QO
     const float *cs = p.cosv + co, *sn = p.sinv + co;
     const bool wide = (p.R & 15) == 0 &&
                       ((reinterpret_cast<uintptr_t>(p.cosv) | reinterpret_cast<uintptr_t>(p.sinv)) & 15) == 0;
-    o.l2 = p.l2scale;
-    if constexpr (DT == kF32) {
-        float x[4][8], amax = 0.0f;
+    raw r[4][8];
+    if (kAhead && wide && p.R > 0) {
+        const int half = p.R >> 1;
+        QRun<DT> u[4];
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {  // (lanes behind the rotation load their own run and the first angles)
+            const int d0 = cc * 32 + g * 8;
+            const bool rot = d0 < p.R, first = d0 < half;
+            const int od = rot ? first ? d0 + half : d0 - half : d0, ci = rot ? first ? d0 : d0 - half : 0;
+#pragma unroll
+            for (int i = 0; i < QRun<DT>::kWords; ++i) {
+                u[cc].x[i] = ld16(reinterpret_cast<const unsigned char*>(q + d0) + 16 * i);
+                u[cc].o[i] = ld16(reinterpret_cast<const unsigned char*>(q + od) + 16 * i);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                u[cc].c[i] = ld16f(cs + ci + 4 * i);
+                u[cc].s[i] = ld16f(sn + ci + 4 * i);
+            }
+        }
+        compiler_fence();
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc) {
+            const int d0 = cc * 32 + g * 8;
+            const bool rot = d0 < p.R, first = d0 < half;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float x = QRun<DT>::at(u[cc].x, i);
+                const float a = x * u[cc].c[i >> 2][i & 3], b = QRun<DT>::at(u[cc].o, i) * u[cc].s[i >> 2][i & 3];
+                const float y = first ? a - b : a + b;
+                r[cc][i] = Tr<DT>::fromf(rot ? y : x);
+            }
+        }
+    } else {
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc) {
             compiler_fence();  // one run's loads at a time
-            rotated8<DT>(q, cs, sn, p.R, cc * 32 + g * 8, wide, x[cc]);
+            rotated8<DT>(q, cs, sn, p.R, cc * 32 + g * 8, wide, r[cc]);
+        }
+    }
+    o.l2 = p.l2scale;
+    if constexpr (DT == kF32) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float a = __builtin_fabsf(x[cc][i]);
+                const float a = __builtin_fabsf(r[cc][i]);
                 amax = a < DV_INF && a > amax ? a : amax;
             }
-        }
         amax = rows4_max(amax);
         int k = 15 - __builtin_amdgcn_frexp_expf(amax);  // amax = m * 2^e, m in [0.5, 1); 0: e = 0
         k = k < 100 ? k : 100;
@@ -319,7 +375,8 @@ __device__ inline void load_q(const DecodeParams& p, int row, int f, int hkv, QO
         for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                const float a = __builtin_amdgcn_ldexpf(x[cc][2 * t], k), b = __builtin_amdgcn_ldexpf(x[cc][2 * t + 1], k);
+                const float a = __builtin_amdgcn_ldexpf(r[cc][2 * t], k);
+                const float b = __builtin_amdgcn_ldexpf(r[cc][2 * t + 1], k);
                 const uint32_t hi = pack2<kF16>(a, b);
                 o.q[0][cc][t] = hi;
                 o.q[1][cc][t] = pack2<kF16>(a - Tr<kF16>::tof((uint16_t)(hi & 0xffffu)),
@@ -327,13 +384,9 @@ __device__ inline void load_q(const DecodeParams& p, int row, int f, int hkv, QO
             }
     } else {
 #pragma unroll
-        for (int cc = 0; cc < 4; ++cc) {
-            raw r[8];
-            compiler_fence();
-            rotated8<DT>(q, cs, sn, p.R, cc * 32 + g * 8, wide, r);
+        for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) o.q[0][cc][t] = (uint32_t)r[2 * t] | ((uint32_t)r[2 * t + 1] << 16);
-        }
+            for (int t = 0; t < 4; ++t) o.q[0][cc][t] = (uint32_t)r[cc][2 * t] | ((uint32_t)r[cc][2 * t + 1] << 16);
     }
 }
 
@@ -603,12 +656,15 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
             stream::fill_pages(p, p.bt + (long long)w * p.maxB, pc, (int)(lpz - lpa) + 1,
                                [&](int i) { return lpa + (uint32_t)i; });
             const int ns = (sb - sa + kStep - 1) / kStep;
+            auto load_stage = [&](int at, int l) {
+                return issue<P2, (GT > 1), (MV || !P2)>(p, v, lo, pc, ring + (uint32_t)(at * kStage), l);
+            };
             uint32_t m[R];  // masks of the stages in flight, the one computed next first
 #pragma unroll
             for (int k = 0; k < R; ++k) m[k] = 0;
 #pragma unroll 1
             for (int k = 0; k < R && k < ns; ++k) {
-                const uint32_t x = issue<P2, (GT > 1)>(p, v, lo, pc, ring + (uint32_t)(k * kStage), sa + k * kStep);
+                const uint32_t x = load_stage(k, sa + k * kStep);
 #pragma unroll
                 for (int j = 0; j < R; ++j) m[j] = j == k ? x : m[j];
             }
@@ -616,7 +672,7 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     compiler_fence();
-                    load_q<DT, QM, RM>(p, gr.lin + (t < gr.ntok ? t : 0), f, hkv, q[t]);
+                    load_q<DT, QM, RM, (GT > 1)>(p, gr.lin + (t < gr.ntok ? t : 0), f, hkv, q[t]);
                     // settled here: a load still pending at the loop would make the compiler
                     // wait for all vector memory in every step
 #pragma unroll
@@ -644,7 +700,7 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
                 for (int k = 0; k + 1 < R; ++k) m[k] = m[k + 1];
                 lds_wait();  // the slot's reads are complete before it is refilled
                 if (s + R < ns)
-                    m[R - 1] = issue<P2, (GT > 1)>(p, v, lo, pc, ring + (uint32_t)(cur * kStage), sa + (s + R) * kStep);
+                    m[R - 1] = load_stage(cur, sa + (s + R) * kStep);
                 cur = cur + 1 == R ? 0 : cur + 1;
             }
             sa = sb;
