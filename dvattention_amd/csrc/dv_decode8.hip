@@ -97,11 +97,11 @@ hipError_t launch_decode8(int dtype, bool varlen, int nt, const DecodeParams& ba
 // few tokens are cut into such pairs, which read the cache once each; those of more go
 // through the multi-query kernel, 16 tokens to a workgroup.  24 sequences of 4096 keys, 4
 // KV heads, us as pairs and in the multi-query kernel:
-//   bf16: 4 tokens 73, 93;   6 tokens 94, 101;   8 tokens 117, 107
-//   fp16: 4 tokens 78, 99;   6 tokens 101, 138;  8 tokens 124, 140;  16 tokens 204, 152
-// (Four tokens to a wave, which has the SIMD to itself then: 93 us for 4.)  Packed calls of
-// two or more tokens per sequence are cut into row groups on the device; in 16-bit types
-// those of up to four tokens and those of more are two launches.
+//   bf16: 4 tokens 72, 97;   6 tokens 91, 100;   8 tokens 110, 103
+//   fp16: 4 tokens 81, 136;  6 tokens 102, 137;  8 tokens 126, 140;  10 tokens 146, 144
+// (Four tokens to a wave, which has the SIMD to itself then: 93 us for 4 in bf16.)  Packed 16-bit
+// calls of two or more tokens per sequence are cut into row groups on the device; those of up
+// to four tokens and those of more are two launches.
 namespace {
 
 constexpr int kGroupTok = 16;  // tokens of a table entry (dv_varlen_groups)
