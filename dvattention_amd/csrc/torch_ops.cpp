@@ -1061,8 +1061,11 @@ void dvattn_paged_kv_append_q8_op(at::Tensor& k_cache, at::Tensor& v_cache, at::
                 ": cosines and sines must have the same strides");
     const int64_t R = cosines.size(2);
     TORCH_CHECK(R <= E && R % 2 == 0, op, ": rotary dim ", R, " must be even and <= E=", E);
-    at::assert_no_overlap(k_cache, keys);
-    at::assert_no_overlap(v_cache, values);
+    const at::Tensor* held[] = {&k_cache, &v_cache, &k_scales, &v_scales};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = i + 1; j < 4; ++j) at::assert_no_overlap(*held[i], *held[j]);
+        for (int j = 0; j < 5; ++j) at::assert_no_overlap(*held[i], *all[j]);
+    }
     c10::hip::HIPGuardMasqueradingAsCUDA guard(k_cache.device());
     dvattn_shape s{};
     s.W = as_int(W, "W");

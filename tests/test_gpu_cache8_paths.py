@@ -82,6 +82,18 @@ def test_append_runs_across_sequences(dv, gpu):
         check_append(dv, gpu, d, 4 + torch.arange(W * S).reshape(W, S))
 
 
+def test_append_refuses_overlapping_caches(dv, gpu):
+    """Caches or scales that share a part of their memory."""
+    d = to(gpu, append_case(torch.Generator().manual_seed(1), torch.bfloat16, torch.bfloat16, 1, 2, 5, 4, 16, 64))
+    slots = torch.arange(5, device=gpu)[None]
+    rows, bytes_ = torch.zeros(5, 16, 2, 128, dtype=torch.uint8, device=gpu), torch.zeros(5, 2, dtype=torch.uint8,
+                                                                                        device=gpu)
+    for bad in (dict(k_cache=rows[:4], v_cache=rows[1:]), dict(k_scales=bytes_[:4], v_scales=bytes_[1:])):
+        x = {**d, **bad}
+        with pytest.raises(RuntimeError):
+            dv.dvattn_paged_kv_append_q8(x["keys"], x["values"], slots, x["cos"], x["sin"], *(x[n] for n in CACHE))
+
+
 # ---------------------------------------------------------------------------
 # Attention.
 @pytest.mark.parametrize("dtype", DTYPES)
