@@ -151,16 +151,15 @@ hipError_t launch(const DecodeParams& p, int ks, int device, int cus, long long 
 // bf16, one sequence of 3001 keys, 8 KV heads 29.7 / 30.8 / 32.7 -> 26.2 / 27.1 /
 // 29.1 us; fp16, 32 x 4608 keys 224 / 223 / 234 -> 112 / 114 / 153; contiguous fp16,
 // 16 x 4096 keys 119 / 120 / 122 -> 60 / 63 / 84; 64 x 60-100 keys, bf16 50.1 /
-// 52.5 / 58.7 -> 45.1 / 47.0 / 51.6.  A split step with no visible key must leave no
-// trace in the softmax, which -inf scores only do for a positive scale.  Short views
+// 52.5 / 58.7 -> 45.1 / 47.0 / 51.6.  Short views
 // gain nothing (each one's queries are staged for all sets, and a piece ends with the
 // sets' combination), so a call is split from 48 keys per view on, as far as the host
 // knows them (paged: what the block tables hold), and a contiguous one of 5 - 8
 // tokens in several views from 128 on: without the split / with it, 8 KV heads, 6 x 30
 // contiguous keys, 2 tokens 68 / 76 us, paged 96 / 99; 12 x 90 contiguous, 8 tokens 62
 // / 67; 6 x 60 paged, 2 / 8 tokens 65 / 62, 70 / 62; 6 x 150 contiguous, 8 tokens 51 / 50.
-int key_split(float l2scale, int ntok, long long keys, int F, bool contig) {
-    if (!(l2scale > 0.0f) || ntok > 8) return 1;
+int key_split(int ntok, long long keys, int F, bool contig) {
+    if (ntok > 8) return 1;
     const int ks = ntok > kFewTok ? 2 : 4;
     const long long per_view = contig && ks == 2 && F > 1 ? kSplitContig2Keys : kSplitMinKeys;
     return keys < per_view * F ? 1 : ks;
@@ -213,6 +212,7 @@ hipError_t launch_groups(int dtype, int qmode, int kvmode, DecodeParams p, long 
     // split; 30 per mille measured best on configuration 5
     static const int skew = env_per_mille("DVATTN_CHUNK_SKEW_PM", 30);
     p.skew_pm = skew;
+    chunk::fold_scale(p);
     for (long long g0 = 0; g0 < groups_total; g0 += kMaxRows) {
         p.row_begin = (int)g0;
         p.nrows = (int)(groups_total - g0 < kMaxRows ? groups_total - g0 : kMaxRows);
@@ -264,8 +264,7 @@ hipError_t launch_chunk(int dtype, int qmode, int kvmode, const DecodeParams& ba
     const ChunkWs l = chunk_ws(groups, base.Hkv, device, false);
     if (ws_bytes < l.total) return hipErrorInvalidValue;
     const int ks = dtype == kF32 ? 1
-                                 : chunk::key_split(base.l2scale, base.S, max_keys_per_group, base.F,
-                                                    kvmode == kKvContig);
+                                 : chunk::key_split(base.S, max_keys_per_group, base.F, kvmode == kKvContig);
     return launch_groups<kRowWS>(dtype, qmode, kvmode, base, groups, max_keys_per_group, ks, l, workspace, stream);
 }
 

@@ -65,6 +65,7 @@ hipError_t launch_chunk8(int dtype, bool varlen, const DecodeParams& base, long 
     p.piece_cost = chunk::kPieceCost;
     p.min_keys = 256;
     p.skew_pm = 30;  // as the 16-bit launches
+    chunk::fold_scale(p);
     for (long long g0 = 0; g0 < groups; g0 += kMaxRows) {
         p.row_begin = (int)g0;
         p.nrows = (int)(groups - g0 < kMaxRows ? groups - g0 : kMaxRows);

@@ -269,6 +269,12 @@ __device__ inline void stage_q_tiles(const DecodeParams& p, unsigned char* qreg,
     }
     wait_vmcnt<0>();
     compiler_fence();
+    if (p.qsign) {  // a negative scale (fold_scale); the rotation keeps the sign
+        for (int t = 0; t < ntile; ++t)
+            for (int i = kg * (4 / KS); i < (kg + 1) * (4 / KS); ++i)
+                *reinterpret_cast<u32x4*>(qreg + t * 4096 + i * 1024 + lane * 16) ^= p.qsign;
+        compiler_fence();
+    }
     if (rot) {
         constexpr int kLanes = 4 * KS;  // lanes per head
         const int hn = kg * (kGqa / KS) + lane / kLanes, q = lane % kLanes;
@@ -438,7 +444,7 @@ __device__ inline void mask_v(VOp& v, uint32_t mask) {
 
 // Scores of invisible keys set to -inf (mask bit k = key k; lane (g, n) holds
 // keys g*4 + i and 16 + g*4 + i): a partially visible stage only, so full
-// stages spend nothing on masks.
+// stages spend nothing on masks.  They are scaled later, by a positive number (fold_scale).
 __device__ inline void mask_scores(f32x4& s0, f32x4& s1, uint32_t mask) {
     const int lane = threadIdx.x & 63;
     const uint32_t mg = mask >> ((lane >> 4) * 4);
@@ -557,7 +563,7 @@ __device__ inline void stream_range(const DecodeParams& p, const Range& r, const
     constexpr int kDma = kDmaPerStage * KS;  // loads per wave and step
     const uint32_t ring = lds_addr(smem);
     const int nsteps = (sbnd - sa + KS * kStep - 1) / (KS * kStep);
-    const float l2 = p.l2scale;
+    const float l2 = p.loop_scale;
     // prologue: steps 0 .. kLead-1.  Past the end, KS = 1 issues rows of zeros; with a
     // key split such steps issue nothing (a view of 30 keys would pay for the
     // addresses of 12 stages and not 4: 2 tokens, 4 sequences, six such views, 8 KV
@@ -678,7 +684,7 @@ __device__ inline void stream_range8(const DecodeParams& p, const Range& r, cons
     const uint32_t ring = lds_addr(smem);
     const uint32_t raw = ring + kWideSlots * kStageBytes;
     const int nsteps = (sbnd - sa + kStep - 1) / kStep;
-    const float l2 = p.l2scale;
+    const float l2 = p.loop_scale;
     const Off8 o8 = offsets8();
     // stages that every tile of this wave sees whole
     int seen = sbnd;
@@ -1011,13 +1017,13 @@ __global__ __launch_bounds__(kThreads) void dv_chunk(const DecodeParams p) {
     } else {
         // the schedule counts units, even for a group without the split, odd with it
         // (one unit more than its keys': both sides of a cut round down alike, so it
-        // never makes a key); a split needs a positive scale (key_split)
+        // never makes a key)
         run_schedule<false, 1, kLongKeyCost>(
                      p, NHG, s_pref, s_scan,
                      [&](int rg) {
                          const long long v = group_visible<KVM, RM>(p, rg);
-                         const bool split = p.l2scale > 0.0f && group_of<RM>(p, rg).ntok <= kFewTok &&
-                                            v >= (long long)kSplitVarlenKeys * p.F;
+                         const bool split =
+                             group_of<RM>(p, rg).ntok <= kFewTok && v >= (long long)kSplitVarlenKeys * p.F;
                          return split ? v * kShortKeyCost + 1 : v * kLongKeyCost;
                      },
                      [&](int rg, int hg, long long v0, long long v1, bool fin, int slot, long long rk) {
@@ -1033,6 +1039,14 @@ __global__ __launch_bounds__(kThreads) void dv_chunk(const DecodeParams p) {
                                                                  uniform(slot), uniform(rk / kLongKeyCost));
                      });
     }
+}
+
+// The scale as the stage loops take it: positive, its sign in the queries' (exact), so that a
+// hidden score of -inf stays one when it is scaled.  Zero becomes the smallest float, 2^-149:
+// a finite score then adds less than 2^-21 to an exponent.
+inline void fold_scale(DecodeParams& p) {
+    p.qsign = p.l2scale < 0.0f ? 0x80008000u : 0u;
+    p.loop_scale = p.l2scale == 0.0f ? __FLT_DENORM_MIN__ : __builtin_fabsf(p.l2scale);
 }
 
 template <bool KV8 = false>

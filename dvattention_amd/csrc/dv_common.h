@@ -86,6 +86,9 @@ struct DecodeParams {
     const unsigned char* ks;
     const unsigned char* vs;
     int sub;              // varlen groups of several tokens: blocks that a table entry is cut into
+    // the 16-bit multi-query kernel's scale and query signs (fold_scale in dv_chunk_kernel.h)
+    float loop_scale;
+    uint32_t qsign;
 };
 
 // Single-launch path for short contiguous views (dv_small.hip): one workgroup

@@ -44,6 +44,7 @@
  *   - Key l of view f is visible to a query iff 0 <= l <= locations[f, row]
  *     and l < fragment_lengths[f]; one softmax over all visible keys of all
  *     views; fp32 accumulation; a query row with no visible key outputs zeros.
+ *     scale may be negative, or zero (all visible keys weigh the same).
  *   - Paged views are laid out back to back in each sequence's logical token
  *     stream: view f starts at sum_{g<f} fragment_lengths[g]; logical position
  *     p lives in page block_tables[w, p / block_size], row p % block_size of a
