@@ -233,6 +233,16 @@ __device__ inline bool store_pages(const DecodeParams& p, int* pages, uint32_t l
     return ok;
 }
 
+// Keys of a sub-range whose pages (of bs rows) fit the page cache wherever in a page it
+// starts, at most 2^30, and the end of the sub-range of [sa, lb) that starts at sa: the
+// product is compared before it is formed (pages may have up to 2^31 - 1 rows), and no sum
+// passes lb.
+__host__ __device__ inline int subrange_keys(int bs) {
+    constexpr int kMost = 1 << 30, kPages = kPageCap - 2;
+    return bs <= kMost / kPages ? kPages * bs : kMost;
+}
+__host__ __device__ inline int subrange_end(int sa, int lb, int span) { return lb - sa > span ? sa + span : lb; }
+
 // Tokens of the largest row group of a launch (the token blocks of its merge).
 template <int RM>
 inline int max_group_tokens(const DecodeParams& p) {

@@ -252,10 +252,9 @@ __device__ void chunk32_piece(const DecodeParams& p, unsigned char* smem, int* p
                 r.L = fd.L;
             }
             const int la = (int)(a - P), lb = (int)(bnd - P);
-            const int span = KVM == kKvPaged ? (p.bs_shift >= 0 ? (kPageCap - 2) << p.bs_shift : (kPageCap - 2) * p.bs)
-                                             : (1 << 30);
-            for (int sa = la; sa < lb; sa += span) {
-                const int sbnd = sa + span < lb ? sa + span : lb;
+            const int span = KVM == kKvPaged ? subrange_keys(p.bs) : 1 << 30;
+            for (int sa = la, sbnd; sa < lb; sa = sbnd) {
+                sbnd = subrange_end(sa, lb, span);
                 r.b = sbnd;
                 r.pages_ok = true;
                 if (KVM == kKvPaged) {

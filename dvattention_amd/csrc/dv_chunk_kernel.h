@@ -69,11 +69,13 @@ constexpr int kRawBytes = kWaves * kRawWave;
 template <bool KV8> constexpr int kLdsRing = KV8 ? kWideSlots * kStageBytes + kRawStages * kRawBytes : kRingBytes;
 
 // Per-lane constants of the loop, held in a register each (what derives from them is
-// computed where it is used): the LDS offsets of this lane's K and V^T operands in a slot
-// and of its widened piece, and 16 * lane.
+// computed where it is used, as is 16 * lane: a register more and fp16 calls read query
+// operands back from memory in every stage): the LDS offsets of this lane's K and V^T operands
+// in a slot and of its widened piece.
 struct Off8 {
-    uint32_t k, v, w, lane16;
+    uint32_t k, v, w;
 };
+__device__ inline uint32_t lane_times_16() { return (uint32_t)(opaque_tid() & 63) * 16; }
 __device__ inline Off8 offsets8() {
     const int lane = threadIdx.x & 63, wv = uniform((int)(threadIdx.x >> 6));
     const int g = lane >> 4, n = lane & 15;
@@ -83,8 +85,7 @@ __device__ inline Off8 offsets8() {
     o.k = (uint32_t)(n * 256 + 16 * (g ^ (n & 3)) + 64 * (n >> 2));
     o.v = (uint32_t)(kKvBytes + k0 * 256 + 16 * ((n & 3) >> 1) + (n & 1) * 8 + 32 * (k0 & 7));
     o.w = (uint32_t)((wv < 4 ? 0 : kKvBytes) + kl * 256 + (wv < 4 ? swz_k(kl, piece) : swz_v(kl, piece)) * 16);
-    o.lane16 = (uint32_t)lane * 16;
-    asm volatile("" : "+v"(o.k), "+v"(o.v), "+v"(o.w), "+v"(o.lane16));
+    asm volatile("" : "+v"(o.k), "+v"(o.v), "+v"(o.w));
     return o;
 }
 
@@ -92,10 +93,11 @@ __device__ inline Off8 offsets8() {
 // (wave % 4) + lane / 8, 16-byte piece lane % 8.
 template <bool P2>
 __device__ inline void issue_raw(const DecodeParams& p, const Range& r, const int* pages, uint32_t raw, int st,
-                                 int kb0, const Off8& o) {
+                                 int kb0) {
     const int wv = uniform((int)(threadIdx.x >> 6));
     const uint32_t base = raw + (uint32_t)((st % kRawStages) * kRawBytes + wv * kRawWave);
-    const int lrow = (int)(o.lane16 >> 7);
+    const uint32_t lane16 = lane_times_16();
+    const int lrow = (int)(lane16 >> 7);
     const int l = kb0 + (wv & 3) * 8 + lrow;
     const uint32_t pos = (uint32_t)(r.off + kb0 + (wv & 3) * 8) + (uint32_t)lrow;
     uint32_t lp, rr;
@@ -113,7 +115,7 @@ __device__ inline void issue_raw(const DecodeParams& p, const Range& r, const in
     const int pg = pages[idx < (uint32_t)kPageCap ? idx : (uint32_t)(kPageCap - 1)];
     const bool ok = l < r.b && idx < (uint32_t)kPageCap && pg >= 0;
     const uint32_t h = ((uint32_t)pg * (uint32_t)p.bs + rr) * (uint32_t)p.Hkv + (uint32_t)r.hkv;
-    const unsigned char* a = (ok ? c + ((unsigned long long)h << 7) : zrow) + (o.lane16 & 127u);
+    const unsigned char* a = (ok ? c + ((unsigned long long)h << 7) : zrow) + (lane16 & 127u);
     const unsigned char* s = ok ? e + ((uint32_t)pg * (uint32_t)p.Hkv + (uint32_t)r.hkv) : zrow;
     dma16(a, __builtin_amdgcn_readfirstlane(base));
     dma1(s, __builtin_amdgcn_readfirstlane(base + 64 * 16));
@@ -127,8 +129,9 @@ __device__ inline void widen(uint32_t slot, uint32_t raw, int st, const Off8& o)
     const int wv = uniform((int)(threadIdx.x >> 6));
     const uint32_t base = raw + (uint32_t)((st % kRawStages) * kRawBytes + wv * kRawWave);
     typedef __attribute__((address_space(3))) const uint32_t lds_u32;
-    u32x4 x = lds_read16_at(base + o.lane16);
-    const uint32_t e = *(lds_u32*)(uintptr_t)(base + 64 * 16 + (o.lane16 >> 2));
+    const uint32_t lane16 = lane_times_16();
+    u32x4 x = lds_read16_at(base + lane16);
+    const uint32_t e = *(lds_u32*)(uintptr_t)(base + 64 * 16 + (lane16 >> 2));
     if (ballot(e == 0)) {  // an exponent of 0: a page of zeros (or no page)
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = e ? x[i] : 0u;
@@ -693,7 +696,7 @@ __device__ inline void stream_range8(const DecodeParams& p, const Range& r, cons
         if (t < ntile && vis_t[t] < seen) seen = vis_t[t];
     const int nfull = r.pages_ok && seen > sa ? (seen - sa) / kStep : 0;
 #pragma unroll
-    for (int s = 0; s < kLead; ++s) issue_raw<P2>(p, r, pages, raw, s, sa + s * kStep, o8);
+    for (int s = 0; s < kLead; ++s) issue_raw<P2>(p, r, pages, raw, s, sa + s * kStep);
     wait_vmcnt<kDma * (kLead - 1)>();  // own share of stage 0 landed
     widen<DT>(ring, raw, 0, o8);
     lds_wait();
@@ -767,7 +770,7 @@ __device__ inline void stream_range8(const DecodeParams& p, const Range& r, cons
         if (ballot(lmx > kMaxSlack)) sm_raise(tl[1], sb0, sb1, l2, pr);
         qk_tile<DT>(kop, qB[0], sa0, sa1);
         pb = sm_finish<DT, true>(tl[1], pr);
-        issue_raw<P2>(p, r, pages, raw, i + kLead, sa + (i + kLead) * kStep, o8);
+        issue_raw<P2>(p, r, pages, raw, i + kLead, sa + (i + kLead) * kStep);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
@@ -916,10 +919,9 @@ __device__ void chunk_piece(const DecodeParams& p, unsigned char* smem, int* pag
             }
             u32x4 qB[kTiles][4] = {};
             // sub-ranges whose page ids fit the LDS page cache
-            const int span = KVM == kKvPaged ? (p.bs_shift >= 0 ? (kPageCap - 2) << p.bs_shift : (kPageCap - 2) * p.bs)
-                                             : (1 << 30);
-            for (int sa = la; sa < lb; sa += span) {
-                const int sbnd = sa + span < lb ? sa + span : lb;
+            const int span = KVM == kKvPaged ? subrange_keys(p.bs) : 1 << 30;
+            for (int sa = la, sbnd; sa < lb; sa = sbnd) {
+                sbnd = subrange_end(sa, lb, span);
                 r.b = sbnd;
                 int pg[kPageIt];
                 uint32_t lpl = 0;
