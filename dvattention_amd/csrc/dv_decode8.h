@@ -90,7 +90,7 @@ __device__ inline u32x2 lds_read_tr8_at(uint32_t addr) {
 __device__ inline int swz_k(int row) { return (row >> 1) & 7; }
 __device__ inline int swz_v(int row) { return ((row >> 1) & 3) | ((row >> 2) & 4); }
 
-// 2^(b - 127) of an exponent byte (0: zero).
+// 2^(b - 127) of an exponent byte (0 and 255: settle_row).
 __device__ inline float power_of(uint32_t b) { return __uint_as_float(b << 23); }
 
 // This lane's byte offset from a stage's row bases: load i moves rows 8i .. 8i + 7 (lane /
@@ -462,27 +462,56 @@ __device__ inline void read_powers(uint32_t at, float (&f)[8]) {
     }
 }
 
+// Exponents that are no power of two to multiply with: 0, an empty page, whose elements are
+// zeros whatever its bytes are, and 255, no number.  A stage that has such rows among its keys
+// gets them rewritten, as zeros or NaN under 2^0: so a NaN byte does not survive the first,
+// and the weight 0 of a key that another tile sees stays 0 times the second (0 times infinity
+// would be NaN).  e: the exponent of this lane's row: K row `lane`, V row lane - 32.
+__device__ inline uint32_t exponent_at(uint32_t slot) {
+    typedef __attribute__((address_space(3))) const uint32_t lds_w;
+    return *(lds_w*)(uintptr_t)(slot + (uint32_t)(2 * kTile) + (uint32_t)(opaque_tid() & 63) * 4);
+}
+__device__ inline void settle_row(uint32_t slot, uint32_t e) {
+    typedef __attribute__((address_space(3))) uint32_t lds_w;
+    typedef __attribute__((address_space(3))) u32x4 lds_w4;
+    const uint32_t lane = (uint32_t)(opaque_tid() & 63);
+    if (e - 1u >= 254u) {
+        const uint32_t x = e ? 0x7f7f7f7fu : 0u;
+#pragma unroll
+        for (int i = 0; i < kRowB / 16; ++i)
+            *(lds_w4*)(uintptr_t)(slot + lane * kRowB + (uint32_t)(i * 16)) = u32x4{x, x, x, x};
+        *(lds_w*)(uintptr_t)(slot + (uint32_t)(2 * kTile) + lane * 4) = 127u;
+    }
+    compiler_fence();
+}
+
 // One stage for NT tiles: scores, softmax, O^T += V^T P^T.  okm: the stage's keys that hold
 // rows; mask[t]: those that tile t sees.
 template <int DT, int NT>
 __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro, uint32_t okm,
                                const uint32_t (&mask)[NT], const QOp<DT> (&q)[NT]) {
     f32x4 s[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int cc = 0; cc < 4; ++cc)
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const u32x4 k =
-                widen8<kKType<DT>>(lds_read8_at(((slot + ro.k) ^ (uint32_t)(cc * 32)) + (uint32_t)(kb * 16 * kRowB)));
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int j = 0; j < kQParts<DT>; ++j) s[t][kb] = Tr<kKType<DT>>::mma(k, q[t].q[j][cc], s[t][kb]);
-        }
     float ks[8];
-    read_powers(slot + ro.s, ks);
+    uint32_t e = exponent_at(slot);
+    while (true) {  // (twice where rows are rewritten; before the scores, the look at e would be waited for)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int cc = 0; cc < 4; ++cc)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const u32x4 k = widen8<kKType<DT>>(
+                    lds_read8_at(((slot + ro.k) ^ (uint32_t)(cc * 32)) + (uint32_t)(kb * 16 * kRowB)));
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int j = 0; j < kQParts<DT>; ++j) s[t][kb] = Tr<kKType<DT>>::mma(k, q[t].q[j][cc], s[t][kb]);
+            }
+        read_powers(slot + ro.s, ks);
+        if (!(ballot(e - 1u >= 254u) & (((uint64_t)okm << 32) | okm))) break;
+        settle_row(slot, e);
+        e = 127u;
+    }
     POp<DT> pB[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {

@@ -279,14 +279,14 @@ __device__ inline float storable(float x) {
     return a < DV_INF ? x : __builtin_nanf("");
 }
 
-// Eight elements that are held under an exponent that is too small, rounded again under one
-// larger by -down.
-__device__ inline void raise_row(unsigned char* at, int down) {
+// Eight elements that are held under the exponent byte `old`, which is too small, rounded
+// again under b (0: an empty page, which holds zeros whatever its bytes are).
+__device__ inline void raise_row(unsigned char* at, int old, int b) {
     u32x2* row = reinterpret_cast<u32x2*>(at);
     float y[8];
     from_fp8(*row, y);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_ldexpf(y[e], down);
+    for (int e = 0; e < 8; ++e) y[e] = old ? __builtin_amdgcn_ldexpf(y[e], old - b) : 0.0f;
     *row = to_fp8(y);
 }
 
@@ -560,11 +560,11 @@ __device__ inline void write_run(const Append8Params& p, bool isk, int t, int ro
     if constexpr (kHeads) {
         if (ballot(raise)) {
             for (int r = 0; r < p.bs; ++r)
-                if (raise && mine && r != row0) raise_row(cache + r * rstride + (g << 7) + d0, old - b);
+                if (raise && mine && r != row0) raise_row(cache + r * rstride + (g << 7) + d0, old, b);
         }
     } else if (raise) {
         for (int r = rank * 4 + g; r < p.bs; r += team * 4)
-            if (r < row0 || r >= row0 + n) raise_row(cache + r * rstride + d0, old - b);
+            if (r < row0 || r >= row0 + n) raise_row(cache + r * rstride + d0, old, b);
     }
     const uint32_t rnext = kHeads ? 128u : (uint32_t)rstride;
     auto store_block = [&](int rb) {
@@ -785,8 +785,8 @@ void dv_kv_append8(const Append8Params p, int T) {
                     x[1] = __builtin_amdgcn_ldexpf(x[1], 127 - b);
                 } else if (raise) {
                     const f32x2 y = __builtin_amdgcn_cvt_pk_f32_fp8((int)*to, false);
-                    x[0] = __builtin_amdgcn_ldexpf(y[0], old - b);
-                    x[1] = __builtin_amdgcn_ldexpf(y[1], old - b);
+                    x[0] = old ? __builtin_amdgcn_ldexpf(y[0], old - b) : 0.0f;
+                    x[1] = old ? __builtin_amdgcn_ldexpf(y[1], old - b) : 0.0f;
                 } else {
                     continue;
                 }

@@ -435,7 +435,8 @@ DVATTN_API dvattn_status dvattn_block_tables(int* cu_seqlens, int* starts, int* 
  * k_cache [num_blocks,block_size,Hkv,E], v_cache [num_blocks,block_size,Hkv,Ev] hold OCP E4M3
  * bytes and k_scales, v_scales [num_blocks,Hkv] an exponent byte b (E8M0) for each page
  * and KV head: an element is byte * 2^(b - 127).  b = 0 is an empty page (its elements count
- * as zeros), so caches and scales cleared to zero are a valid cache; b = 255 is no number.
+ * as zeros, whatever its bytes are), so scales cleared to zero make a valid cache; b = 255 is
+ * no number: the elements are NaN to the tokens that see them.
  *
  * dvattn_paged_kv_append_q8 rounds new tokens to that form.  Token (w, s) is written to
  * slots[w,s] i64 (slot = page * block_size + row; negative or past the cache: not

@@ -119,7 +119,8 @@ def append(k_cache, v_cache, k_scales, v_scales, slots, keys, values, cos, sin):
                 if 0 not in rows and old != 255:
                     if b > old:
                         rest = [r for r in range(bs) if r not in rows]
-                        v = values_of(new[page, rest, h]).numpy() * 2.0 ** (old - b)
+                        v = values_of(new[page, rest, h]).numpy()
+                        v = v * 2.0 ** (old - b) if old else np.zeros_like(v)
                         new[page, rest, h] = bytes_of(e4m3(v))
                     b = max(b, old)
                 b8[page, h] = b
@@ -129,11 +130,10 @@ def append(k_cache, v_cache, k_scales, v_scales, slots, keys, values, cos, sin):
 
 
 def dequantised(cache, scales):
-    """float64 [P,bs,Hkv,E]."""
-    b = scales.view(torch.uint8).double()
-    f = torch.where(b == 0, 0.0, torch.exp2(b - 127))
-    f = torch.where(b == 255, math.nan, f)
-    return values_of(cache) * f[:, None, :, None]
+    """float64 [P,bs,Hkv,E]; the elements of an empty page (0) are zeros whatever its bytes are."""
+    b = scales.view(torch.uint8).double()[:, None, :, None]
+    f = torch.where(b == 255, math.nan, torch.exp2(b - 127))
+    return torch.where(b == 0, 0.0, values_of(cache) * f)
 
 
 def sdpa(scale, locations, queries, cosines, sines, fragment_lengths, k_cache, v_cache, k_scales, v_scales,
