@@ -378,7 +378,7 @@ struct Row8 {
     // 448 then, infinities and NaN become NaN
     __device__ inline u32x2 bytes(int b) const {
         if constexpr (DT == kF32) {
-            const float f = __uint_as_float((uint32_t)(254 - b) << 23);
+            const float f = __uint_as_float(b < 254 ? (uint32_t)(254 - b) << 23 : 0x400000u);  // (2^-127 is subnormal)
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(w[e]) * f;

@@ -2,11 +2,13 @@
 exponents that are no number, empty pages, the largest and smallest ones, views that begin at
 negative positions.  Oracle and tolerances: test_gpu_cache8.py.
 """
+import math
+
 import pytest
 import torch
 
 from oracle import cache8_oracle as CO
-from test_gpu_cache8 import (CACHE, DTYPES, SCALE, case, check, compare, dv,  # noqa: F401
+from test_gpu_cache8 import (CACHE, DTYPES, SCALE, append_case, case, check, check_append, compare, dv,  # noqa: F401
                              packed, to)
 
 pytestmark = pytest.mark.gpu
@@ -90,3 +92,33 @@ def test_sdpa_view_at_a_negative_position(dv, gpu, dtype, S, bs, neg, n):  # noq
     vd = to(gpu, v)
     out = dv.dvattn_varlen_paged_sdpa_q8(scale=SCALE, cu_seqlens_k=vd["cu_seqlens_q"], **vd)
     compare(out, dtype, n, *(x[w, :, s] for x in want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("old", [0, 1, 5, 250, 253, 254])
+@pytest.mark.parametrize("Hkv,T,bs,R", [(1, 1, 16, 0), (2, 1, 16, 32), (5, 9, 16, 0), (2, 40, 48, 64), (1, 9, 16, 20)])
+def test_append_under_every_exponent(dv, gpu, dtype, old, Hkv, T, bs, R):  # noqa: F811
+    """Rows behind row 0 of a page whose exponent is the largest or the smallest there is, of
+    the type's largest and smallest numbers and ordinary ones; what an empty page (0) holds
+    counts as zeros."""
+    g = torch.Generator().manual_seed(old + T)
+    for size in (1.0, 2.0 ** -120 if dtype != torch.float16 else 2.0 ** -13, float(torch.finfo(dtype).max) / 2.0 ** 7):
+        d = append_case(g, dtype, dtype, 1, Hkv, T, 3, bs, R)
+        for x in ("keys", "values"):
+            d[x] = (d[x].double().clamp(-60, 60) * size).to(dtype)
+        d["k_scales"][:], d["v_scales"][:] = old, old
+        if old == 0:
+            for x in ("k_cache", "v_cache"):
+                d[x].view(torch.uint8)[1, :, 0, 5] = 0x7f
+        check_append(dv, gpu, d, bs + 3 + torch.arange(T)[None])
+
+
+def test_append_exponents_from_finite_numbers(dv, gpu):  # noqa: F811
+    """Infinities and NaN beside ordinary numbers leave the page's exponent to those."""
+    g = torch.Generator().manual_seed(2)
+    for dtype in DTYPES:
+        d = append_case(g, dtype, dtype, 1, 2, 30, 3, 16, 0)
+        for t, x in ((2, math.inf), (3, math.nan), (20, -math.inf)):
+            d["keys"][0, 0, t, 7], d["values"][0, 1, t, 9] = x, x
+        got = check_append(dv, gpu, d, 16 + torch.arange(30)[None])
+        assert got[2].view(torch.uint8)[1:].max() < 140
