@@ -246,7 +246,7 @@ constexpr float kMaxSlack = 8.0f;
 template <bool kSum = true>
 __device__ inline void softmax32(f32x4 (&o)[8], float& m, float& l, const f32x4& s0, const f32x4& s1,
                                  uint32_t mask, float l2scale, float (&pr)[8]) {
-    const bool full = mask == 0xffffffffu && l2scale > 0.0f;
+    bool full = mask == 0xffffffffu && l2scale > 0.0f;
     bool exact = true;  // wave-uniform
     float mx;           // the row's scaled max, on the exact path
     if (full) {
@@ -260,11 +260,17 @@ __device__ inline void softmax32(f32x4 (&o)[8], float& m, float& l, const f32x4&
             fmaxf(fmaxf(fmaxf(pr[0], pr[1]), fmaxf(pr[2], pr[3])), fmaxf(fmaxf(pr[4], pr[5]), fmaxf(pr[6], pr[7])));
         exact = ballot(lmx > kMaxSlack) != 0;
         // max of the raw scores, scaled once
-        if (exact)
+        if (exact) {
             mx = rows4_max(fmaxf(fmaxf(fmaxf(s0[0], s0[1]), fmaxf(s0[2], s0[3])),
                                  fmaxf(fmaxf(s1[0], s1[1]), fmaxf(s1[2], s1[3])))) *
                  l2scale;
-    } else {
+            // The running max is a rounded product: from 2^24 on an exact one may exceed it by
+            // whole units (by 2^25 for scores around 2^50), and 2 to that power be infinite.
+            // There exponents come from rounded products too, as on the masked path.
+            full = ballot(__builtin_fabsf(fmaxf(m, mx)) >= 0x1p24f) == 0;
+        }
+    }
+    if (!full) {
         // bit g*4 + i (+16) of the mask: the per-lane shift sits behind an empty
         // asm so the eight bit masks are not precomputed and held in registers
         uint32_t mg = mask >> (((opaque_tid() & 63) >> 4) * 4);
