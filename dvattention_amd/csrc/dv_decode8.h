@@ -214,12 +214,21 @@ __device__ inline uint32_t issue(const DecodeParams& p, const stream::View& v, u
 // A query row's 16-bit MFMA operands: lane (g, n) holds dims c * 32 + g * 8 .. + 8 of head n.
 // fp32: times 2^k, k such that the head's largest magnitude lies in [2^14, 2^15), as hi + lo:
 // hi is within 2^-12 of the element, lo within 2^-12 of what hi leaves (or 2^-25 of 2^15);
-// l2: softmax scale / ln 2, times 2^-k.
+// bias: k + 127.
 template <int DT>
 struct QOp {
     u32x4 q[kQParts<DT>][4];
-    float l2;
+    int bias;
 };
+
+// A score from the product with K's bytes and its row's exponent byte.  fp32: 2^-k with it in
+// one step, so that neither leaves the floats where their product does not (one VALU
+// instruction and an integer subtraction, as the multiplication by 2^(b - 127) takes).
+template <int DT>
+__device__ inline float score(float x, uint32_t e, const QOp<DT>& q) {
+    if constexpr (DT == kF32) return __builtin_amdgcn_ldexpf(x, (int)e - q.bias);
+    else return x * power_of(e);
+}
 
 // Eight consecutive elements as floats (16-byte aligned).
 template <int DT>
@@ -357,7 +366,6 @@ __device__ inline void load_q(const DecodeParams& p, int row, int f, int hkv, QO
             rotated8<DT>(q, cs, sn, p.R, cc * 32 + g * 8, wide, r[cc]);
         }
     }
-    o.l2 = p.l2scale;
     if constexpr (DT == kF32) {
         float amax = 0.0f;
 #pragma unroll
@@ -370,7 +378,7 @@ __device__ inline void load_q(const DecodeParams& p, int row, int f, int hkv, QO
         amax = rows4_max(amax);
         int k = 15 - __builtin_amdgcn_frexp_expf(amax);  // amax = m * 2^e, m in [0.5, 1); 0: e = 0
         k = k < 100 ? k : 100;
-        o.l2 *= __builtin_amdgcn_ldexpf(1.0f, -k);
+        o.bias = k + 127;
 #pragma unroll
         for (int cc = 0; cc < 4; ++cc)
 #pragma unroll
@@ -398,7 +406,7 @@ struct POp {
 };
 
 template <int DT>
-__device__ inline POp<DT> p_scaled(const float (&pr)[8], const float (&vs)[8], float& l) {
+__device__ inline POp<DT> p_scaled(const float (&pr)[8], const uint32_t (&vs)[8], float& l) {
     POp<DT> o;
     if constexpr (DT == kBF16) {
         // the normaliser sums the rounded weights, as p_operands does
@@ -414,7 +422,7 @@ __device__ inline POp<DT> p_scaled(const float (&pr)[8], const float (&vs)[8], f
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        float a = pr[2 * i] * vs[2 * i], b = pr[2 * i + 1] * vs[2 * i + 1];
+        float a = pr[2 * i] * power_of(vs[2 * i]), b = pr[2 * i + 1] * power_of(vs[2 * i + 1]);
 #pragma unroll
         for (int k = 0; k < kPParts<DT>; ++k) {
             const uint32_t w = pack2<kBF16>(a, b);
@@ -452,13 +460,13 @@ __device__ inline ReadOff read_offsets() {
     return o;
 }
 
-// 2^(b - 127) of this lane's eight K (or, 128 bytes further, V) rows.
-__device__ inline void read_powers(uint32_t at, float (&f)[8]) {
+// Exponent bytes of this lane's eight K (or, 128 bytes further, V) rows.
+__device__ inline void read_exponents(uint32_t at, uint32_t (&e)[8]) {
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
         const u32x4 a = lds_read16_at(at + (uint32_t)(kb * 64));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) f[kb * 4 + i] = power_of(a[i]);
+        for (int i = 0; i < 4; ++i) e[kb * 4 + i] = a[i];
     }
 }
 
@@ -489,9 +497,9 @@ __device__ inline void settle_row(uint32_t slot, uint32_t e) {
 // rows; mask[t]: those that tile t sees.
 template <int DT, int NT>
 __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro, uint32_t okm,
-                               const uint32_t (&mask)[NT], const QOp<DT> (&q)[NT]) {
+                               const uint32_t (&mask)[NT], const QOp<DT> (&q)[NT], float l2scale) {
     f32x4 s[NT][2];
-    float ks[8];
+    uint32_t ks[8];
     uint32_t e = exponent_at(slot);
     while (true) {  // (twice where rows are rewritten; before the scores, the look at e would be waited for)
 #pragma unroll
@@ -507,7 +515,7 @@ __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro
 #pragma unroll
                     for (int j = 0; j < kQParts<DT>; ++j) s[t][kb] = Tr<kKType<DT>>::mma(k, q[t].q[j][cc], s[t][kb]);
             }
-        read_powers(slot + ro.s, ks);
+        read_exponents(slot + ro.s, ks);
         if (!(ballot(e - 1u >= 254u) & (((uint64_t)okm << 32) | okm))) break;
         settle_row(slot, e);
         e = 127u;
@@ -517,13 +525,13 @@ __device__ inline void compute(State (&st)[NT], uint32_t slot, const ReadOff& ro
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            s[t][0][i] *= ks[i];
-            s[t][1][i] *= ks[4 + i];
+            s[t][0][i] = score<DT>(s[t][0][i], ks[i], q[t]);
+            s[t][1][i] = score<DT>(s[t][1][i], ks[4 + i], q[t]);
         }
         float pr[8];
-        softmax32<false>(st[t].o, st[t].m, st[t].l, s[t][0], s[t][1], mask[t], q[t].l2, pr);
-        float vs[8];
-        read_powers(slot + ro.s + 128, vs);
+        softmax32<false>(st[t].o, st[t].m, st[t].l, s[t][0], s[t][1], mask[t], l2scale, pr);
+        uint32_t vs[8];
+        read_exponents(slot + ro.s + 128, vs);
         pB[t] = p_scaled<DT>(pr, vs, st[t].l);
     }
     // a key that some tile sees and another does not takes part there with weight 0, which
@@ -724,7 +732,7 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
                         mask[t] &= lim >= kStep ? 0xffffffffu : lim <= 0 ? 0u : (1u << lim) - 1u;
                     }
                 }
-                compute<DT, NT>(st, ring + (uint32_t)(cur * kStage), ro, m[0], mask, q);
+                compute<DT, NT>(st, ring + (uint32_t)(cur * kStage), ro, m[0], mask, q, p.l2scale);
 #pragma unroll
                 for (int k = 0; k + 1 < R; ++k) m[k] = m[k + 1];
                 lds_wait();  // the slot's reads are complete before it is refilled

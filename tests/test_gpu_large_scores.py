@@ -107,3 +107,19 @@ def test_attention_over_8_bits(dv, gpu, dtype, up, scale, S, b):  # noqa: F811
     assert torch.equal(dv.dvattn_paged_sdpa_q8(scale=scale, **x).cpu(), want)
     p, flat = packed(x, want)
     assert torch.equal(dv.dvattn_varlen_paged_sdpa_q8(scale=scale, **p).cpu(), flat)
+
+
+@pytest.mark.parametrize("up,b", [(-30, 237), (-60, 244), (-100, 240), (-2, 230), (40, 190), (100, 100), (110, 60)])
+@pytest.mark.parametrize("S", [1, 3, 20])
+def test_float32_queries_and_keys_of_other_sizes(dv, gpu, up, b, S):  # noqa: F811
+    """Queries of 2^up against keys under the exponent b: no score leaves the floats, whatever
+    the sizes of the two are."""
+    d, want, _ = make(torch.float32, 3, S, up, seed=S)
+    for n in ("k", "v"):
+        d[n + "_cache"] = d[n + "_cache"].to(torch.float8_e4m3fn)
+        d[n + "_scales"] = torch.full((d["k_cache"].shape[0], Hkv), b if n == "k" else 127, dtype=torch.uint8)
+    x = to(gpu, d)
+    scale = 2.0 ** (147 - up - b)  # the largest scores around 2^36
+    assert torch.equal(dv.dvattn_paged_sdpa_q8(scale=scale, **x).cpu(), want)
+    p, flat = packed(x, want)
+    assert torch.equal(dv.dvattn_varlen_paged_sdpa_q8(scale=scale, **p).cpu(), flat)
