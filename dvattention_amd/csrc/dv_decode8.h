@@ -667,7 +667,8 @@ __device__ __forceinline__ void piece(const DecodeParams& p, unsigned char* wlds
         v.hkv = hkv;
         v.k = reinterpret_cast<const unsigned char*>(p.kc);
         v.v = reinterpret_cast<const unsigned char*>(p.vc);
-        v.off = (int)(off < 0x80000000ll ? off : -0x80000000ll);  // (all positions below 0: absent)
+        // (past 31 bits on either side: all positions below 0, absent)
+        v.off = (int)(off < 0x80000000ll && off >= -0x80000000ll ? off : -0x80000000ll);
         int vis_t[NT];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {

@@ -95,6 +95,25 @@ def test_sdpa_view_at_a_negative_position(dv, gpu, dtype, S, bs, neg, n):  # noq
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("S", [1, 2, 4, 20])
+def test_sdpa_view_far_before_all_positions(dv, gpu, dtype, S):  # noqa: F811
+    """Negative lengths that add up to -2^32: the view behind them has no rows, wherever its
+    positions lie modulo 2^32."""
+    d = case(dtype, 2, 1, S, [40, 0, 0, 40], 16, 64, seed=S)
+    d["locations"][0], d["locations"][3] = 30, 39
+    d["fragment_lengths"][0] = 40
+    d["fragment_lengths"][1:3] = -2 ** 31
+    want = CO.sdpa(SCALE, **d)
+    alone = CO.sdpa(SCALE, **{**d, "fragment_lengths": torch.tensor([40, 0, 0, 0], dtype=torch.int32)})
+    assert torch.equal(want[0], alone[0])
+    compare(dv.dvattn_paged_sdpa_q8(scale=SCALE, **to(gpu, d)), dtype, 40, *want)
+    v, w, s = packed(d, 2, S, [S, max(1, S // 2)])
+    vd = to(gpu, v)
+    out = dv.dvattn_varlen_paged_sdpa_q8(scale=SCALE, cu_seqlens_k=vd["cu_seqlens_q"], **vd)
+    compare(out, dtype, 40, *(x[w, :, s] for x in want))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("old", [0, 1, 5, 250, 253, 254])
 @pytest.mark.parametrize("Hkv,T,bs,R", [(1, 1, 16, 0), (2, 1, 16, 32), (5, 9, 16, 0), (2, 40, 48, 64), (1, 9, 16, 20)])
 def test_append_under_every_exponent(dv, gpu, dtype, old, Hkv, T, bs, R):  # noqa: F811
