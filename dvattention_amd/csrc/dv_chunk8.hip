@@ -6,6 +6,8 @@
 namespace dv {
 namespace chunk {
 
+static_assert(kTokBlk == kGroupTokens && kFewTok == kFewGroupTokens, "groups of a packed call's two launches");
+
 template <int DT, int QM, bool P2, int RM>
 hipError_t launch8(DecodeParams p, int device, int cus, long long cap, hipStream_t stream) {
     static std::atomic<unsigned long long> attr_done{0};

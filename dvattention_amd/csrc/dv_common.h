@@ -333,9 +333,12 @@ hipError_t launch_key_mass(int dtype, const MassParams& p, void* workspace, hipS
 hipError_t launch_block_tables(const TablesParams& p, hipStream_t stream);
 hipError_t launch_kv_append8(int dtype, int rope_dtype, const Append8Params& p, hipStream_t stream);
 
-// Attention over an 8-bit cache (dv_decode8.hip: a wave per KV head and up to four tokens;
+// Attention over an 8-bit cache (dv_decode8.hip: a wave per KV head and up to two tokens;
 // dv_chunk8.hip: workgroups of 16 tokens): workspace of a [W, S] call and of T packed
-// tokens, and the launches.
+// tokens, and the launches.  Both launches of a packed call divide its row groups by these
+// (dv_chunk.h, asserted in dv_chunk8.hip):
+constexpr int kGroupTokens = 16;    // most tokens of a row group
+constexpr int kFewGroupTokens = 4;  // of a group that the multi-query kernel leaves to the decode kernel
 size_t sdpa8_workspace_bytes(int dtype, bool varlen, int W, int S_or_T, int Hkv, int device);
 hipError_t launch_sdpa8(int dtype, bool varlen, const DecodeParams& base, long long max_keys_per_row, void* workspace,
                         size_t ws_bytes, hipStream_t stream);

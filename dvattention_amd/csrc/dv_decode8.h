@@ -1,10 +1,10 @@
 // gfx950 decode attention with fused query RoPE over a paged cache held in 8 bits:
 // E4M3 bytes [num_blocks, block_size, Hkv, 128] and one exponent byte b per page and KV
-// head, so that a cached element is byte * 2^(b - 127) (b = 0: zero).  Rows, views,
+// head, so that a cached element is byte * 2^(b - 127) (b = 0: zero, 255: NaN).  Rows, views,
 // rotation, work split and merge are the 16-bit decode's (dv_decode.hip).
 //
 //  * One wave owns one KV head and its 16 query heads of one row over a range of the
-//    row's keys; up to four such waves (KV heads) make a workgroup.
+//    row's keys; up to eight such waves (KV heads, pick_hpw8) make a workgroup.
 //  * A stage is 32 keys: 4 KiB of K, 4 KiB of V and the 64 exponent bytes of its rows,
 //    moved by nine direct-to-LDS loads into a ring of two stages private to the wave.  The
 //    exponents travel with their rows, so pages of any size may end inside a stage.
@@ -13,11 +13,13 @@
 //    fp32 score.  V^T comes from the transposing 8-bit LDS read, widened to bf16, and V's
 //    2^(b - 127) multiplies the probability before it is rounded (a power of two: the
 //    rounding is the same with and without).
-//  * Precision: bf16 calls take one operand for Q and P, as the 16-bit decode does.  fp16
+//  * Precision: bf16 calls take one operand for Q and P, as the 16-bit decode does, and
+//    hold partial results as fp16 under a power of two per row (store_partial).  fp16
 //    calls take Q as it is against K in fp16, and P as a bf16 pair hi + lo (16 bits).
 //    fp32 calls take Q, its row scaled by a power of two, as an fp16 pair and P as three
 //    bf16 numbers, 24 bits either way: the products with exact K and V lose nothing that
-//    fp32 arithmetic keeps.
+//    fp32 arithmetic keeps (V under exponents below 18 aside, whose weights' last part
+//    leaves bf16).
 //
 // Bound by HBM on long caches and by starts on short ones: 4 x 131072 keys of 8 KV heads
 // in fp16, 1.07 GB, 169 us (6.4 TB/s; reads alone reach 6.9); 32 ragged sequences of 1k -
@@ -43,7 +45,9 @@ constexpr int kLoads = 9;                       // direct-to-LDS loads per stage
 // two waves to a SIMD, with two stages each in LDS and accumulators in VGPRs (as the
 // kernels' file is compiled).  fp32 with two tiles (whose operands alone are 128
 // registers) had the SIMD to itself: 100 MB of cache took 39 us for two tokens, where rows
-// of one token take 17.5 us each.
+// of one token take 17.5 us each.  (A launch's schedule lies in LDS too, 8 bytes a row above
+// 64 rows: from 688 rows on -- 112 / 304 / 1456 with 1 / 2 / 8 KV heads to a workgroup, 4 in
+// most calls -- fewer than eight waves fit a CU.)
 constexpr int kWaves = 8;                       // per CU
 constexpr int kRing = 2;
 constexpr int kWaveLds = kRing * kStage + stream::kPc * 4;

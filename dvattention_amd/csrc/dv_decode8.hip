@@ -104,8 +104,6 @@ hipError_t launch_decode8(int dtype, bool varlen, int nt, const DecodeParams& ba
 // to four tokens and those of more are two launches.
 namespace {
 
-constexpr int kGroupTok = 16;  // tokens of a table entry (dv_varlen_groups)
-constexpr int kFewTokens = 4;  // of an entry that the 16-bit multi-query kernel leaves to the decode kernel
 constexpr int few_tokens(int dtype) { return dtype == kBF16 ? 6 : 8; }  // the same of a [W, S] call's sequence
 
 struct Plan8 {
@@ -126,10 +124,10 @@ Plan8 plan8(int dtype, bool varlen, int W, int S_or_T, int Hkv, int device) {
         q.groups = varlen ? S_or_T : (long long)W * S;
     } else if (varlen && use_varlen_chunk(dtype, S_or_T, W)) {
         q.table = true;
-        q.groups = (long long)S_or_T / kGroupTok + W + 1;
+        q.groups = (long long)S_or_T / kGroupTokens + W + 1;
         q.table_bytes = (size_t)q.groups * 16;
         q.nt = 2;
-        q.sub = kFewTokens / 2;
+        q.sub = kFewGroupTokens / 2;
         q.chunk = true;
     } else if (varlen) {
         q.nt = 1;
@@ -139,7 +137,7 @@ Plan8 plan8(int dtype, bool varlen, int W, int S_or_T, int Hkv, int device) {
         q.groups = (long long)W * ((S + q.nt - 1) / q.nt);
     } else {
         q.chunk = true;
-        q.groups = (long long)W * ((S + kGroupTok - 1) / kGroupTok);
+        q.groups = (long long)W * ((S + kGroupTokens - 1) / kGroupTokens);
     }
     // (one after the other, both kernels of a table use the same bytes)
     size_t a = q.nt ? decode8_workspace_bytes(q.groups * q.sub, q.nt, Hkv, device) : 0;

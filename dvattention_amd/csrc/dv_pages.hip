@@ -83,7 +83,7 @@ __global__ __launch_bounds__(kTabThreads) void dv_block_tables(const TablesParam
     __shared__ int s_gone[kTabThreads];  // ended sequences with pages
     __shared__ int s_ngone;
     int* s_cu = s_tab;                 // [W + 1]
-    int* s_start = s_cu + p.W + 1;     // [W] length before the step (0: ended), then the start
+    int* s_start = s_cu + p.W + 1;     // [W] length before the step (-1: ended), then the start
     int* s_off = s_start + p.W;        // [W] first stack entry given back, then pages needed before w
     int* s_got = s_off + p.W;          // [W] pages given back, then pages taken
     const int tid = threadIdx.x;
