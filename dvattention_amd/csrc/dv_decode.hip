@@ -270,7 +270,7 @@ __device__ void process_piece(const DecodeParams& p, unsigned char* vt, int row,
         }
     } else {
         store_partial<DT>(p.part + (long long)slot * p.slot_floats, p.hpw * kGqa, wv * kGqa + n, g, st.o, inv,
-                          lt > 0.0f ? st.m + log2f(lt) : -DV_INF);
+                          row_lse(st.m, lt));
     }
 }
 
@@ -697,7 +697,7 @@ __device__ void piece(const DecodeParams& p, unsigned char* wlds, int row, int h
         }
     } else {
         store_partial<DT>(p.part + (long long)slot * p.slot_floats, p.hpw * kGqa, wv * kGqa + n, g, st.o, inv,
-                          lt > 0.0f ? st.m + log2f(lt) : -DV_INF);
+                          row_lse(st.m, lt));
     }
 }
 
@@ -784,25 +784,22 @@ __global__ __launch_bounds__(kMergeWaves * kWave) void dv_merge(const DecodePara
         ww[w] = s_part[w - 1][1][t];
         M = fmaxf(M, mw[w]);
     }
-    float v[8];
-    if (M == -DV_INF) {  // no piece has a visible key
+    // without a visible key in any piece all weights and sums are 0; a NaN that a quarter
+    // without a maximum left in its sums stays
+    const float Mz = M == -DV_INF ? 0.0f : M;
+    float v[8], sc[kMergeWaves], tw = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    } else {
-        float sc[kMergeWaves], tw = 0.0f;
+    for (int w = 0; w < kMergeWaves; ++w) {
+        sc[w] = exp2f(mw[w] - Mz);  // a quarter without visible keys (-inf) -> 0
+        tw += ww[w] * sc[w];
+    }
+    const float inv = tw > 0.0f ? 1.0f / tw : 0.0f;
 #pragma unroll
-        for (int w = 0; w < kMergeWaves; ++w) {
-            sc[w] = exp2f(mw[w] - M);  // a quarter without visible keys (-inf) -> 0
-            tw += ww[w] * sc[w];
-        }
-        const float inv = tw > 0.0f ? 1.0f / tw : 0.0f;
+    for (int e = 0; e < 8; ++e) {
+        float a = acc[0][e] * sc[0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float a = acc[0][e] * sc[0];
-#pragma unroll
-            for (int w = 1; w < kMergeWaves; ++w) a += s_part[w - 1][2 + e][t] * sc[w];
-            v[e] = a * inv;
-        }
+        for (int w = 1; w < kMergeWaves; ++w) a += s_part[w - 1][2 + e][t] * sc[w];
+        v[e] = a * inv;
     }
     store_run8<DT>(o, v);
 }

@@ -46,8 +46,8 @@ constexpr int kLoads = 9;                       // direct-to-LDS loads per stage
 // kernels' file is compiled).  fp32 with two tiles (whose operands alone are 128
 // registers) had the SIMD to itself: 100 MB of cache took 39 us for two tokens, where rows
 // of one token take 17.5 us each.  (A launch's schedule lies in LDS too, 8 bytes a row above
-// 64 rows: from 688 rows on -- 112 / 304 / 1456 with 1 / 2 / 8 KV heads to a workgroup, 4 in
-// most calls -- fewer than eight waves fit a CU.)
+// 64 rows: from 688 rows on, 112 / 304 with one / two KV heads to a workgroup, fewer than
+// eight waves fit a CU.)
 constexpr int kWaves = 8;                       // per CU
 constexpr int kRing = 2;
 constexpr int kWaveLds = kRing * kStage + stream::kPc * 4;

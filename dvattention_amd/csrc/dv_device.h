@@ -502,7 +502,8 @@ constexpr int kMergeBatchLong = 16;
 // d[q]: the base-2-LSE-weighted sum of the pieces' normalised outputs
 // (paged_kernel_v21.cuh:325-364), with B pieces' loads in flight per round
 // (merge_runs: B = kMergeBatch up to kMergeBatch pieces, else kMergeBatchLong).
-// res[q][e] = merged value of dim d[q] + e; 0 when no piece has a visible key.
+// res[q][e] = merged value of dim d[q] + e; 0 when no piece has a visible key, NaN
+// when some piece has a NaN log-sum-exp (row_lse).
 // The result depends on the pieces and on B (the running max is raised once
 // per round).
 // merge_acc_b: the accumulation -- the running base-2 max m_out, the weight
@@ -539,10 +540,15 @@ __device__ inline void merge_acc_b(const float* part, long long slot_floats, int
             }
         }
         float bm = m;
+        bool nan = false;  // a maximum passes over NaN
 #pragma unroll
-        for (int i = 0; i < B; ++i) bm = fmaxf(bm, lse[i]);
-        if (bm == -DV_INF) continue;
-        const float sc = exp2f(m - bm);  // m == -inf -> 0
+        for (int i = 0; i < B; ++i) {
+            bm = fmaxf(bm, lse[i]);
+            nan |= lse[i] != lse[i];
+        }
+        if (bm == -DV_INF && !nan) continue;
+        const float bz = bm == -DV_INF ? 0.0f : bm;
+        const float sc = exp2f(m - bz);  // m == -inf -> 0
         wsum *= sc;
 #pragma unroll
         for (int q = 0; q < NQ; ++q)
@@ -550,7 +556,7 @@ __device__ inline void merge_acc_b(const float* part, long long slot_floats, int
             for (int e = 0; e < 8; ++e) acc[q][e] *= sc;
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-            const float wgt = exp2f(lse[i] - bm);  // empty piece (-inf) -> 0
+            const float wgt = exp2f(lse[i] - bz);  // empty piece (-inf) -> 0, a NaN score -> NaN
             wsum += wgt;
             if constexpr (kHalfPartials<DT>) {
                 const float w = __builtin_amdgcn_ldexpf(wgt, -kx[i]);
