@@ -338,10 +338,14 @@ __global__ __launch_bounds__(256) void dv_small(const SmallParams sp) {
     float L = 0.0f, o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = 0.0f;
-    if (M != -DV_INF) {
+    bool nan = false;  // a maximum passes over NaN
+#pragma unroll
+    for (int k = 0; k < kWaves; ++k) nan |= sm.l[k][h] != sm.l[k][h];
+    if (M != -DV_INF || nan) {
+        const float Mz = M == -DV_INF ? 0.0f : M;
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) {
-            const float e = __builtin_amdgcn_exp2f(sm.m[k][h] - M);  // wave without visible keys: 0
+            const float e = __builtin_amdgcn_exp2f(sm.m[k][h] - Mz);  // wave without visible keys: 0
             L += e * sm.l[k][h];
             const f32x4 a = *reinterpret_cast<const f32x4*>(&sm.o[k][h][d0]);
             const f32x4 c = *reinterpret_cast<const f32x4*>(&sm.o[k][h][d0 + 4]);
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(256) void dv_small(const SmallParams sp) {
     }
     float* slot = sp.part + ((long long)item * sp.chunks + ci) * kSlot;
     store8<kF32>(slot + h * kHeadDim + d0, o, inv);
-    if ((tid & 15) == 0) slot[kGqa * kHeadDim + h] = L > 0.0f ? M + log2f(L) : -DV_INF;
+    if ((tid & 15) == 0) slot[kGqa * kHeadDim + h] = row_lse(M, L);
     // every thread's partial stores complete before the barrier; the agent-scope
     // release of wave 0 then writes the workgroup's partial back from this XCD's
     // L2, and the flag is raised after it.  The sequentially consistent fence
@@ -405,16 +409,21 @@ __global__ __launch_bounds__(256) void dv_small(const SmallParams sp) {
             v1[i] = ld16f(sl + h * kHeadDim + d0 + 4);
         }
         float bm = m;
+        bool any_nan = false;
 #pragma unroll
-        for (int i = 0; i < kMergeBatch; ++i) bm = fmaxf(bm, lse[i]);
-        if (bm == -DV_INF) continue;
-        const float scl = __builtin_amdgcn_exp2f(m - bm);  // m == -inf -> 0
+        for (int i = 0; i < kMergeBatch; ++i) {
+            bm = fmaxf(bm, lse[i]);
+            any_nan |= lse[i] != lse[i];
+        }
+        if (bm == -DV_INF && !any_nan) continue;
+        const float bz = bm == -DV_INF ? 0.0f : bm;
+        const float scl = __builtin_amdgcn_exp2f(m - bz);  // m == -inf -> 0
         wsum *= scl;
 #pragma unroll
         for (int e = 0; e < 8; ++e) acc8[e] *= scl;
 #pragma unroll
         for (int i = 0; i < kMergeBatch; ++i) {
-            const float wgt = __builtin_amdgcn_exp2f(lse[i] - bm);  // empty chunk (-inf) -> 0
+            const float wgt = __builtin_amdgcn_exp2f(lse[i] - bz);  // empty chunk (-inf) -> 0, a NaN score -> NaN
             wsum += wgt;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {

@@ -67,3 +67,26 @@ def test_nan_in_every_piece(dv, gpu, dtype, q8, S, n, where, part):  # noqa: F81
         rest[1, 32:48] = False
         assert out[rest].isfinite().all()
     assert torch.equal(one(scale=SCALE, **d)[rest], before[rest])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("S", [1, 3, 9, 20])
+@pytest.mark.parametrize("lens", [[16], [60], [40, 700], [3000]])
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("step", [1, 5])
+def test_nan_in_contiguous_views(dv, gpu, dtype, S, lens, where, step):  # noqa: F811
+    """Every row, or every fifth, of every view of KV head 2 of sequence 1."""
+    g = torch.Generator(device=gpu).manual_seed(S)
+    F = len(lens)
+    q = torch.randn(F, 2, 16 * Hkv, S, E, generator=g, device=gpu).to(dtype)
+    views = {x: [torch.randn(2, Hkv, n, E, generator=g, device=gpu).to(dtype) for n in lens] for x in "kv"}
+    loc = torch.stack([torch.full((2, S), n - 1, dtype=torch.int32, device=gpu) for n in lens])
+    fl = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    before = dv.dvattn_sdpa(q, loc, views["k"], views["v"], SCALE, fl)
+    for x in views[where]:
+        x[1, 2, ::step] = math.nan
+    out = dv.dvattn_sdpa(q, loc, views["k"], views["v"], SCALE, fl)
+    assert out[1, 32:48].isnan().all()
+    rest = torch.ones(2, 16 * Hkv, dtype=torch.bool, device=gpu)
+    rest[1, 32:48] = False
+    assert torch.equal(out[rest], before[rest])
