@@ -23,8 +23,8 @@
 //
 // Bound by HBM on long caches and by starts on short ones: 4 x 131072 keys of 8 KV heads
 // in fp16, 1.07 GB, 169 us (6.4 TB/s; reads alone reach 6.9); 32 ragged sequences of 1k -
-// 8k keys in bf16, 320 MB, 60 us (5.3); one sequence of 3001 keys 10.5; 96 fp32 rows over 73
-// MB 63, half of it VALU issue and MFMAs (24 of a stage's 40 are P's three parts).
+// 8k keys in bf16, 320 MB, 60 us (5.3); one sequence of 3001 keys 10.8; 96 fp32 rows over 73
+// MB 65, half of it VALU issue and MFMAs (24 of a stage's 40 are P's three parts).
 #pragma once
 
 #include "dv_common.h"

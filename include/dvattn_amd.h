@@ -466,9 +466,11 @@ DVATTN_API dvattn_status dvattn_paged_kv_append_q8(int dtype, int rope_dtype, vo
  * caches' bytes and their scales.  dtype is that of queries and out; every element of a
  * cache is exact in the products, queries are rounded to dtype after their rotation,
  * and weights to bf16 in bf16 calls (fp16 calls carry 16 bits of them, fp32 calls
- * 24).  But fp16 calls of more than eight tokens per sequence, and packed sequences of more
- * than four, take keys as fp16 numbers, whose magnitudes end at 65504 and whose spacing at
- * 2^-24: caches that an fp16 append wrote hold no larger ones. */
+ * 24).  bf16 calls hold a split row's partial results as fp16 under a power of two per
+ * row, within 2^-11 of its largest element.  But fp16 calls of more than eight tokens per
+ * sequence, and packed sequences of more than four, take keys as fp16 numbers, whose
+ * magnitudes end at 65504 and whose spacing at 2^-24: caches that an fp16 append wrote hold no
+ * larger ones. */
 DVATTN_API size_t dvattn_paged_sdpa_q8_workspace_size(int dtype, const dvattn_shape* shape, int device);
 DVATTN_API dvattn_status dvattn_paged_sdpa_q8(int dtype, void* out, float scale, const int* locations,
                                    const void* queries, const float* cosines, const float* sines,
